@@ -304,6 +304,27 @@ int qlm_matmul_i8_t_whole_config(const float* x, int ldx, const float* norm_w, f
                                  int tiles, int grid, int k_slices, void* work,
                                  size_t work_bytes, void* stream);
 
+/* The matmul with the activations in 8 bits too (no counterpart in the
+ * reference): y[m, n] = x_scales[m] * s_rows[n] * sum_k x[m, k] * q[n, k],
+ * int8 x [M, ldx] with one scale a row (qlm_add_rms_norm_q8, or
+ * qlm_quantize_q8_f32 with group K), int8 weights with one scale a row:
+ * tile-major q_tiles (qlm_mx_swizzle with group K) and s_rows as quantised
+ * ([2N] for SwiGLU: gate rows, then up rows). On the int8 matrix cores; the
+ * sums are exact in int32 and rounded to fp32 once, so the result differs
+ * from the exact one by a few fp32 roundings only, in every form. epilogue
+ * 0: y = result; 1: y += result; 2: SwiGLU, y = silu(gate) * up (N outputs).
+ * Any M >= 1 and N, K a multiple of 64 below 2^17; x and q_tiles 16-byte
+ * aligned, ldx a multiple of 16 below 2^23; y of any stride and alignment,
+ * its columns past N left as they are. work: device scratch of
+ * qlm_matmul_a8_workspace_bytes(M, N, K, epilogue) bytes (0: may be NULL),
+ * 16-byte aligned, no initial contents needed; calls sharing it must be
+ * ordered on one stream. The size never falls with M: a workspace for the
+ * most rows serves every call of fewer. */
+size_t qlm_matmul_a8_workspace_bytes(int M, int N, int K, int epilogue);
+int qlm_matmul_a8(const int8_t* x, int ldx, const float* x_scales, const int8_t* q_tiles,
+                  const float* s_rows, float* y, int ldy, int M, int N, int K, int epilogue,
+                  void* work, size_t work_bytes, void* stream);
+
 /* Fused forms used by the decode step (same arithmetic as the unfused
  * reference sequence, one launch instead of two or three):
  *   _rmsnorm: x is first replaced by rms_norm(x, norm_w, eps) (zero-centred
@@ -329,6 +350,20 @@ int qlm_rms_norm(const float* x, const float* w, float* y, int rows, int n, floa
 /* math::add_rms_norm (math_ops.cpp:1133-1172): res += delta; y = rms_norm(res). */
 int qlm_add_rms_norm(float* res, const float* delta, const float* w, float* y, int rows, int n,
                      float eps, void* stream);
+/* math::add_rms_norm with an output in 8 bits, the input rows of
+ * qlm_matmul_a8 (no counterpart in the reference, whose activations stay
+ * fp32): r = x + delta (delta NULL: r = x), y = r / sqrt(mean(r^2) + eps) *
+ * (1 + w), scales[row] = max|y| / 127 (1 for a row of zeros), q = y / scale
+ * rounded to the nearest whole number, ties to even. Statistics and quotient are held in 64
+ * bits, so the bytes are those of the exact quotient. sum (may be NULL;
+ * needs delta) receives r; it may be x or delta itself with the same row
+ * stride, and overlaps neither otherwise. A row with a value that is not
+ * finite gets scale NaN and bytes 0: its products come out NaN. x [rows,
+ * ldx], delta [rows, ldd], sum [rows, lds] fp32, q [rows, ldq]; any n and
+ * alignment; rows at most 2^21; columns past n are left as they are. */
+int qlm_add_rms_norm_q8(const float* x, int ldx, const float* delta, int ldd, const float* w,
+                        float eps, float* sum, int lds, int8_t* q, int ldq, float* scales,
+                        int rows, int n, void* stream);
 /* math::silu_mul (math_ops.cpp:1122-1129): a = a/(1+exp(-a)) * b. */
 int qlm_silu_mul(float* a, const float* b, int n, void* stream);
 
@@ -509,6 +544,26 @@ int qlm_attention_decode_noalloc(const float* q, const void* k_cache, const void
  * of logits [B, ldl] over n entries. idx is [B] int32. */
 int qlm_argmax(const float* logits, int ldl, int n, int B, int* idx, void* work, void* stream);
 size_t qlm_argmax_workspace_bytes(int B, int n);
+
+/* ---- log probabilities of tokens (no counterpart in the reference) ----------
+ * For each row of logits [rows, ldl] over n tokens, with p = softmax:
+ *   id_logprobs[row, j] = log p(ids[row, j]), ids [rows, n_ids] int32 (n_ids 0:
+ *     none; an id outside 0..n-1 gets NaN and is not read);
+ *   entropy[row] = -sum p log p (NULL: not wanted);
+ *   top_ids, top_logprobs [rows, top]: the `top` most likely tokens, larger
+ *     logit first and equal logits by the lower id (top 0: none).
+ * A logit of -inf is a masked token: probability 0, log probability -inf,
+ * after every other token. A row with NaN, with +inf or with nothing but -inf
+ * has no distribution: its log probabilities and entropy are NaN; its top_ids
+ * still follow the logits, NaN counted as -inf. fp32, sums relative to the
+ * running maximum, in an order that depends only on rows and n. top <= 64 and
+ * top <= n; n at most 2^21, rows at most 2^23. work: device scratch of
+ * qlm_token_logprobs_workspace_bytes(rows, n, top) bytes, 16-byte aligned, no
+ * initial contents needed; calls sharing it must be ordered on one stream. */
+size_t qlm_token_logprobs_workspace_bytes(int rows, int n, int top);
+int qlm_token_logprobs(const float* logits, int ldl, int n, int rows, const int* ids, int n_ids,
+                       float* id_logprobs, float* entropy, int top, int* top_ids,
+                       float* top_logprobs, void* work, size_t work_bytes, void* stream);
 
 /* ---- A14/A15: device-resident greedy loop ------------------------------------
  * The CLI's decode loop (main.cpp:659-676) with the token stream kept on the

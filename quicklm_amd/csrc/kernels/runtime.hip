@@ -38,10 +38,13 @@ hipError_t qlm_load_deltanet();
 hipError_t qlm_load_deltanet_chunk();
 hipError_t qlm_load_elementwise();
 hipError_t qlm_load_gemm();
+hipError_t qlm_load_gemm_a8();
 hipError_t qlm_load_gemm_mx();
 hipError_t qlm_load_gemm_t();
 hipError_t qlm_load_gemm_w();
 hipError_t qlm_load_gemv();
+hipError_t qlm_load_logprobs();
+hipError_t qlm_load_norm_q8();
 hipError_t qlm_load_quant();
 
 // Selects the device and loads every kernel file's code object on it, so no
@@ -49,7 +52,10 @@ hipError_t qlm_load_quant();
 extern "C" int qlm_set_device(int device) {
     hipError_t e = hipSetDevice(device);
     if (e != hipSuccess) return qlm_status(e);
-    for (hipError_t (*load)() : {qlm_load_attention, qlm_load_deltanet, qlm_load_deltanet_chunk, qlm_load_elementwise, qlm_load_gemm, qlm_load_gemm_mx, qlm_load_gemm_t, qlm_load_gemm_w, qlm_load_gemv, qlm_load_quant}) {
+    for (hipError_t (*load)() :
+         {qlm_load_attention, qlm_load_deltanet, qlm_load_deltanet_chunk, qlm_load_elementwise,
+          qlm_load_gemm, qlm_load_gemm_a8, qlm_load_gemm_mx, qlm_load_gemm_t, qlm_load_gemm_w,
+          qlm_load_gemv, qlm_load_logprobs, qlm_load_norm_q8, qlm_load_quant}) {
         e = load();
         if (e != hipSuccess) return qlm_status(e);
     }

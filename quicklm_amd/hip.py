@@ -72,6 +72,8 @@ _SIGS = {
                            _vp]),
     "qlm_matmul_i8_tm": (_i, [_vp, _i, _vp, _f, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _sz,
                               _vp]),
+    "qlm_matmul_a8_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "qlm_matmul_a8": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "qlm_gemv_i8_config": (_i, [_vp, _vp, _f, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "qlm_gemv_i8_mx_config": (_i, [_vp, _vp, _f, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i,
                                    _vp]),
@@ -101,6 +103,7 @@ _SIGS = {
                                         _vp]),
     "qlm_rms_norm": (_i, [_vp, _vp, _vp, _i, _i, _f, _vp]),
     "qlm_add_rms_norm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _vp]),
+    "qlm_add_rms_norm_q8": (_i, [_vp, _i, _vp, _i, _vp, _f, _vp, _i, _vp, _i, _vp, _i, _i, _vp]),
     "qlm_silu_mul": (_i, [_vp, _vp, _i, _vp]),
     "qlm_rope_neox": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "qlm_conv1d_update": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _vp]),
@@ -122,6 +125,8 @@ _SIGS = {
     "qlm_attention_decode_noalloc": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp]),
     "qlm_argmax": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
     "qlm_argmax_workspace_bytes": (_sz, [_i, _i]),
+    "qlm_token_logprobs": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
+    "qlm_token_logprobs_workspace_bytes": (_sz, [_i, _i, _i]),
     "qlm_greedy_advance": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp]),
     "qlm_lm_head_greedy_workspace_bytes": (_sz, []),
     "qlm_lm_head_greedy": (_i, [_vp, _vp, _f, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _vp,
