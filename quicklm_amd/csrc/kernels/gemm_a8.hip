@@ -15,11 +15,17 @@
 // waves of a workgroup split K over one 16-row weight tile.
 // More rows, k_a8_tile: both operands staged through LDS.
 
+#ifdef A8_TUNE
+#include <stdio.h>
+#include <stdlib.h>
+#endif
+
 #include "common.hpp"
 
 namespace {
 
 enum { EPI_STORE = 0, EPI_RESID = 1, EPI_SWIGLU = 2 };
+enum { OUT_PART = 3 };  // beside the epilogues: a slice's sums, joined by k_a8_join
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -31,202 +37,614 @@ struct A8Args {
     float* y;
     long long ldx, ldy;
     int M, N, K;
-    int tiles;  // 16-row weight tiles (of a half, for SwiGLU)
+    int tiles;    // 16-row weight tiles (of a half, for SwiGLU)
+    int t_first;  // the launch's first output tile
+    int gx, gy, blocks, per_xcd;  // column and row blocks, all (slices too), a XCD's share
+    int* part;                    // the slices' sums [slice][M][halves][16 tiles]
+    int bslice;                   // 64-column blocks a slice (even), all of them: one slice
 };
 
-// Four neighbouring outputs n .. n + 3 of row m.
-template <int EPI>
-__device__ __forceinline__ void put4(const A8Args& a, int m, int n, v4i s0, v4i s1) {
-    if (m >= a.M || n >= a.N) return;
-    const float sx = a.sx[m];
-    float* dst = a.y + (size_t)m * a.ldy + n;
-    const bool whole = n + 4 <= a.N;
-    f32x4u w0{0, 0, 0, 0}, w1{0, 0, 0, 0}, old{0, 0, 0, 0}, v;
-    if (whole) {
-        w0 = *reinterpret_cast<const f32x4u*>(a.sw + n);
-        if constexpr (EPI == EPI_SWIGLU) w1 = *reinterpret_cast<const f32x4u*>(a.sw + a.N + n);
-        if constexpr (EPI == EPI_RESID) old = *reinterpret_cast<const f32x4u*>(dst);
-    } else {
+// Scales of four neighbouring channels (those past the last are copies of it).
+__device__ __forceinline__ f32x4u load_scales(const float* sw, int n, int N) {
+    if (n + 4 <= N) return *reinterpret_cast<const f32x4u*>(sw + n);
+    f32x4u v;
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
-            if (n + i < a.N) {
-                w0[i] = a.sw[n + i];
-                if constexpr (EPI == EPI_SWIGLU) w1[i] = a.sw[a.N + n + i];
-                if constexpr (EPI == EPI_RESID) old[i] = dst[i];
-            }
-    }
+    for (int i = 0; i < 4; ++i) v[i] = sw[min(n + i, N - 1)];
+    return v;
+}
+
+// g / (1 + exp(-g)) in a third of the instructions of expf and a division:
+// exp2 of the product with log2 e, whose rounding error is put back, and a
+// reciprocal with one Newton step; off by 3 + 1 + 1 + 1 roundings at most (the
+// exponential, the sum, the reciprocal, the product). The epilogue of a
+// 2048 x 9728 SwiGLU took 10 us of a round's 40 with the library's.
+__device__ __forceinline__ float silu_fast(float g) {
+    constexpr float kLog2e = 1.44269502e0f, kRest = 1.92596303e-8f, kLn2 = 0.693147182f;
+    const float hi = g * -kLog2e;
+    const float lo = fmaf(g, -kLog2e, -hi) - g * kRest;
+    float e = __builtin_amdgcn_exp2f(hi);
+    // past the range of fp32 the result is 0; 1 / 3e38 is still not a NaN
+    e = fminf(fmaf(e * kLn2, lo, e), 3e38f);
+    const float d = 1.0f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    return g * r;
+}
+
+// Four results of one row from their sums (SwiGLU: gate and up sums).
+template <int EPI>
+__device__ __forceinline__ f32x4u scaled(v4i s0, v4i s1, float sx, f32x4u w0, f32x4u w1) {
+    f32x4u v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float p = (float)s0[i] * sx * w0[i];
-        if constexpr (EPI == EPI_SWIGLU)
-            v[i] = silu_f(p) * ((float)s1[i] * sx * w1[i]);
-        else if constexpr (EPI == EPI_RESID)
-            v[i] = old[i] + p;
-        else
-            v[i] = p;
+        v[i] = EPI == EPI_SWIGLU ? silu_fast(p) * ((float)s1[i] * sx * w1[i]) : p;
     }
-    if (whole) {
-        *reinterpret_cast<f32x4u*>(dst) = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 3; ++i)
-            if (n + i < a.N) dst[i] = v[i];
-    }
+    return v;
 }
 
-// MT 16-row tiles of x against one weight tile (SwiGLU: the gate tile and its
-// up tile) a workgroup; NW waves take the 64-column blocks in turn and add
-// their sums in LDS (integers: in any order).
-template <int EPI, int MT, int NW>
-__global__ __launch_bounds__(NW * QLM_WAVE) void k_a8_stream(A8Args a) {
-    constexpr int H = EPI == EPI_SWIGLU ? 2 : 1;
-    constexpr int U = 4;
-    __shared__ int sums[H * MT * 256];
-    const int lane = threadIdx.x & (QLM_WAVE - 1), wave = threadIdx.x / QLM_WAVE;
-    for (int i = threadIdx.x; i < H * MT * 256; i += NW * QLM_WAVE) sums[i] = 0;
-    __syncthreads();
-    const int nblk = a.K >> 6, tile = blockIdx.x;
+// Stores (EPI_RESID: adds) the first `left` of four results.
+template <int EPI>
+__device__ __forceinline__ void put(float* dst, f32x4u v, int left) {
+    if (left >= 4) {
+        if constexpr (EPI == EPI_RESID) v += *reinterpret_cast<const f32x4u*>(dst);
+        *reinterpret_cast<f32x4u*>(dst) = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+        if (i < left) dst[i] = EPI == EPI_RESID ? dst[i] + v[i] : v[i];
+}
+
+// MT 16-row tiles of x against NT weight tiles (SwiGLU: NT gate tiles and
+// their up tiles) a workgroup. NW waves take the 64-column blocks of K in
+// turn, straight from memory into registers, U blocks of a wave in flight, and
+// add their sums in LDS (integers: in any order).
+template <int EPI, int MT, int NT, int NW, int U, int P>
+__global__ __launch_bounds__(NW* QLM_WAVE) void k_a8_stream(A8Args a) {
+    constexpr int H = EPI == EPI_SWIGLU ? 2 : 1, F = H * NT;
+    __shared__ int sums[F * MT * 256];
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
+    const int nblk = a.K >> 6, t0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
     const int8_t* xr[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
-        xr[t] = a.x + (size_t)min(16 * t + (lane & 15), a.M - 1) * a.ldx + (lane >> 4) * 16;
-    const v4i* wq[H];
+        xr[t] = a.x + (size_t)min(m0 + 16 * t + (lane & 15), a.M - 1) * a.ldx + (lane >> 4) * 16;
+    const v4i* wq[F];
 #pragma unroll
-    for (int h = 0; h < H; ++h)
-        wq[h] = reinterpret_cast<const v4i*>(a.q) +
-                ((size_t)h * a.tiles + tile) * nblk * QLM_WAVE + lane;
-    v4i acc[H][MT];
+    for (int f = 0; f < F; ++f)
+        wq[f] = reinterpret_cast<const v4i*>(a.q) +
+                ((size_t)(f / NT) * a.tiles + min(t0 + f % NT, a.tiles - 1)) * nblk * QLM_WAVE +
+                lane;
+    v4i acc[F][MT];
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+    for (int f = 0; f < F; ++f)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[h][t] = v4i{0, 0, 0, 0};
-    for (int b = wave; b < nblk; b += NW * U) {
-        v4i w[U][H], x[U][MT];
+        for (int t = 0; t < MT; ++t) acc[f][t] = v4i{0, 0, 0, 0};
+    v4i w[U][F], x[U][MT];
+    auto load = [&](int u, int b) {  // blocks past the last are copies of it
+        b = min(b, nblk - 1);
+#pragma unroll
+        for (int f = 0; f < F; ++f) w[u][f] = wq[f][(size_t)b * QLM_WAVE];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            x[u][t] = *reinterpret_cast<const v4i*>(xr[t] + (size_t)b * 64);
+    };
+    auto multiply = [&](int u, int b) {
+        if (b >= nblk) return;
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[f][t] =
+                    __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][f], x[u][t], acc[f][t], 0, 0, 0);
+    };
+    // slot u's block, b0 the wave's first of this round
+    auto at = [&](int b0, int u) { return b0 + u / P * (NW * P) + u % P; };
+    constexpr int ROUND = U * NW;
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(u, at(wave * P, u));
+    for (int i = threadIdx.x; i < F * MT * 256; i += NW * QLM_WAVE) sums[i] = 0;
+    __syncthreads();
+    int b = wave * P;
+    for (; b + ROUND < nblk; b += ROUND)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int bu = b + u * NW, bc = min(bu, nblk - 1);
-#pragma unroll
-            for (int h = 0; h < H; ++h) w[u][h] = wq[h][(size_t)bc * QLM_WAVE];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                x[u][t] = *reinterpret_cast<const v4i*>(xr[t] + (size_t)bc * 64);
-                if (bu >= nblk) x[u][t] = v4i{0, 0, 0, 0};
-            }
+            multiply(u, at(b, u));
+            load(u, at(b + ROUND, u));
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-                    acc[h][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][h], x[u][t],
-                                                                     acc[h][t], 0, 0, 0);
-    }
+    for (int u = 0; u < U; ++u) multiply(u, at(b, u));
     // lane l holds outputs n = 4 (l >> 4) + i of row m = l & 15
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+    for (int f = 0; f < F; ++f)
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                atomicAdd(&sums[((h * MT + t) * 4 + i) * QLM_WAVE + lane], acc[h][t][i]);
+                atomicAdd(&sums[((f * MT + t) * 4 + i) * QLM_WAVE + lane], acc[f][t][i]);
     __syncthreads();
-    if (wave < MT) {
+    for (int p = wave; p < NT * MT; p += NW) {
+        const int f = p / MT, t = p % MT;
         v4i s[2];
 #pragma unroll
-        for (int h = 0; h < H; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                s[h][i] = sums[((h * MT + wave) * 4 + i) * QLM_WAVE + lane];
-        if constexpr (H == 1) s[1] = s[0];
-        put4<EPI>(a, 16 * wave + (lane & 15), 16 * tile + 4 * (lane >> 4), s[0], s[1]);
+                s[h][i] = sums[(((f + (h & (H - 1)) * NT) * MT + t) * 4 + i) * QLM_WAVE + lane];
+        const int m = m0 + 16 * t + (lane & 15), n = 16 * (t0 + f) + 4 * (lane >> 4);
+        if (m < a.M && n < a.N) {
+            const f32x4u w0 = load_scales(a.sw, n, a.N);
+            const f32x4u w1 = H == 2 ? load_scales(a.sw + a.N, n, a.N) : w0;
+            put<EPI>(a.y + (size_t)m * a.ldy + n, scaled<EPI>(s[0], s[1], a.sx[m], w0, w1),
+                     a.N - n);
+        }
     }
+}
+
+// Buffer descriptor of a uniform base: a load then takes a lane's 32-bit
+// offset and a scalar one, no vector arithmetic on addresses. Reads past
+// `bytes` return 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, unsigned bytes) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0, (int)bytes, 0x00027000);
+}
+
+// 16 bytes a lane straight into LDS, lane after lane from `to` (uniform).
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, char* to, int lane_off,
+                                            int uniform_off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16,
+                                             lane_off, uniform_off, 0, 0);
+}
+
+// acc += w . x. IN_A: the sums in accumulator registers, tied by hand.
+template <bool IN_A>
+__device__ __forceinline__ void mma(v4i& acc, v4i w, v4i x) {
+    if constexpr (IN_A)
+        asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
+    else
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, acc, 0, 0, 0);
 }
 
 // BM = 16 WM FM rows of x and BN = 16 WN FN weight rows a workgroup, WM x WN
 // waves of FM x FN fragments each.
-template <int EPI, int WM, int WN, int FM, int FN>
-__global__ __launch_bounds__(WM * WN * QLM_WAVE) void k_a8_tile(A8Args a) {
-    constexpr int NW = WM * WN, BF = WN * FN, AF = WM * FM;  // fragments a stage
-    constexpr bool SW = EPI == EPI_SWIGLU;
+//
+// LDS holds WD blocks (64 columns) of weight fragments and XU units (128
+// columns) of x. A load of x takes 8 rows x 128 columns, whole cache lines:
+// loads of 16 rows x 64 columns, the fragments themselves, took half as long
+// again. Row r's 16-byte piece p lies at r * 128 + (p ^ (r & 7)) * 16 of its
+// 8-row group, so that the 8 lanes of an LDS access meet every bank once.
+template <int EPI, bool SW, int WM, int WN, int FM, int FN, int WD, int XU, int OCC>
+__global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
+    constexpr int NW = WM * WN, BF = WN * FN, AF = WM * FM;  // fragments of a block
     constexpr int OF = SW ? FN / 2 : FN;  // output fragments of a wave
-    __shared__ __attribute__((aligned(16))) v4i smem[(AF + BF) * QLM_WAVE];
-    const int lane = threadIdx.x & (QLM_WAVE - 1), wave = threadIdx.x / QLM_WAVE;
+    constexpr int LX = AF / NW, LW = BF / NW, L = LX + LW;  // a wave's loads a block
+    static_assert(AF % NW == 0 && BF % NW == 0 && FN % 2 == 0 && FN / 2 <= FM, "tile shape");
+    constexpr int XUNIT = AF * 2048, WBLK = BF * 1024, W0 = XU * XUNIT;
+    __shared__ __attribute__((aligned(1024))) char smem[XU * XUNIT + WD * WBLK];
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
     const int wm = wave / WN, wn = wave % WN;
-    const int nblk = a.K >> 6;
-    const int m0 = blockIdx.y * AF * 16, t0 = blockIdx.x * WN * OF;
-    // staged fragment f: rows of x, then weight tiles in the waves' order
-    auto src = [&](int f) -> const int8_t* {
-        if (f < AF)
-            return a.x + (size_t)min(m0 + 16 * f + (lane & 15), a.M - 1) * a.ldx +
-                   (lane >> 4) * 16;
-        const int g = f - AF, w = g / FN, j = g % FN;
-        const int h = SW ? j / OF : 0;
-        const int t = min(t0 + w * OF + (SW ? j % OF : j), a.tiles - 1);
-        return a.q + ((size_t)(h * a.tiles + t) * nblk * QLM_WAVE + lane) * 16;
-    };
-    constexpr int L = (AF + BF + NW - 1) / NW;
-    const int8_t* from[L];
+    // Workgroups go to the 8 XCDs in turn: XCD i takes the i-th eighth of the
+    // blocks, in bands of BAND row blocks (column by column inside a band).
+    constexpr int BAND = 4;
+    int t = (int)(blockIdx.x & 7) * a.per_xcd + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= a.per_xcd || t >= a.blocks) return;
+    const int slice = t / (a.gx * a.gy);
+    t -= slice * a.gx * a.gy;
+    const int band = t / (BAND * a.gx);
+    const int bh = min(BAND, a.gy - BAND * band);
+    t -= band * BAND * a.gx;
+    const int m0 = (BAND * band + t % bh) * AF * 16;
+    const int t0 = a.t_first + (t / bh) * WN * OF;  // first output tile
+    // this slice's blocks of K
+    const int b0 = slice * a.bslice, kblk = a.K >> 6, nblk = min(kblk - b0, a.bslice);
+
+    // x: the unit's 8-row groups, LX of each half of them a wave. Rows past the
+    // last are copies of it; where K ends in the middle of a unit, so are the
+    // pieces past it (of those before), and none of them is multiplied.
+    const int rows = min(a.M - m0, AF * 16);
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(
+        a.x + (size_t)m0 * a.ldx + b0 * 64, (unsigned)(rows - 1) * (unsigned)a.ldx + a.K - b0 * 64);
+    const int piece = (lane & 7) ^ (lane >> 3);
+    const int past = piece >= 4 ? 64 : 0;
+    int xoff[LX], xstep[LX];  // first half of the groups, and on to the second
 #pragma unroll
-    for (int l = 0; l < L; ++l) from[l] = src(min(wave + l * NW, AF + BF - 1));
+    for (int l = 0; l < LX; ++l) {
+        const int r = 8 * (wave * LX + l) + (lane >> 3);
+        xoff[l] = min(r, rows - 1) * (int)a.ldx + piece * 16;
+        xstep[l] = min(r + 8 * AF, rows - 1) * (int)a.ldx + piece * 16 - xoff[l];
+    }
+    // weights: staged fragments in the waves' order (gate tiles, up tiles)
+    __amdgpu_buffer_rsrc_t rw[LW];
+#pragma unroll
+    for (int l = 0; l < LW; ++l) {
+        const int f = wave * LW + l, w = f / FN, j = f % FN, h = SW ? j / OF : 0;
+        const int tl = min(t0 + w * OF + (SW ? j % OF : j), a.tiles - 1);
+        rw[l] = make_rsrc(a.q + (((size_t)h * a.tiles + tl) * kblk + b0) * 1024,
+                          (unsigned)nblk * 1024);
+    }
+    const int woff = lane * 16;
+    const int last_unit = (nblk - 1) >> 1;
+    // load l of half unit `half` of x into unit slot `slot`, of block b's weights
+    auto fetch_x1 = [&](int l, int half, int slot) {
+        const int h = half & 1, u = min(half >> 1, last_unit);
+        const int back = u == last_unit && (nblk & 1) ? past : 0;
+        load_to_lds(rx, smem + slot * XUNIT + (h * AF + wave * LX + l) * 1024,
+                    xoff[l] + (xstep[l] & -h) - back, u * 128);
+    };
+    auto fetch_w1 = [&](int l, int b, int slot) {
+        load_to_lds(rw[l], smem + W0 + slot * WBLK + (wave * LW + l) * 1024, woff,
+                    min(b, nblk - 1) * 1024);
+    };
+    auto fetch_x = [&](int half, int slot) {
+#pragma unroll
+        for (int l = 0; l < LX; ++l) fetch_x1(l, half, slot);
+    };
     v4i acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+
+    // fragment i of x: row r = lane & 15, piece lane >> 4 of the block's half
+    const int xl = ((wm * FM * 2) + ((lane & 15) >> 3)) * 1024 + (lane & 7) * 128 +
+                   ((lane >> 4) ^ (lane & 7)) * 16;
+    auto read_x = [&](int at, int i) {
+        return *reinterpret_cast<const v4i*>(smem + at + i * 2048);
+    };
+    auto read_w = [&](int at, int j) {
+        return *reinterpret_cast<const v4i*>(smem + at + j * 1024);
+    };
+    const int wl = W0 + wn * FN * 1024 + lane * 16;
+
+    // A wave's fragments of block b sit in one set of registers. Its columns
+    // are multiplied in two halves; a register is read anew, for block b + 1,
+    // as soon as its last product is issued:
+    //   first half   the upper columns' weights of block b
+    //   barrier b    block b is read by everyone, block b + 1 has arrived
+    //   second half  the lower columns' weights and x of block b + 1
+    // so every read has half a block of products to return. Weights of block
+    // b + WD and half a unit of x are requested after barrier b, spread over a
+    // block's length: a burst of them holds up the products behind it.
+    constexpr int HN = FN / 2;
+    constexpr bool IN_A = FM * FN > 32;
+    constexpr int XH = 2 * XU - 1;  // iteration b requests x's half unit b + XH
+    // iterations whose requests may be under way when block b + 1 is needed
+    constexpr int AHEAD = (WD - 1 < 2 * XU - 3 ? WD - 1 : 2 * XU - 3) - 1;
+    static_assert(AHEAD >= 0, "ring depths");
+    constexpr int L1 = L / 4;  // a block's requests in its second half; the others follow it
+    v4i x[FM], w[FN];
+#pragma unroll
+    for (int h = 0; h < XH - WD; ++h) fetch_x(h, (h >> 1) % XU);
+#pragma unroll
+    for (int b = -WD; b < 0; ++b)
+#pragma unroll
+        for (int l = 0; l < (b < -1 ? L : L1); ++l) {
+            if (l < LW)
+                fetch_w1(l, b + WD, b + WD);
+            else if (b + XH >= 0)
+                fetch_x1(l - LW, b + XH, ((b + XH) >> 1) % XU);
+        }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L * AHEAD) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {  // in the order of the second half below
+        if (2 * i < HN) w[2 * i] = read_w(wl, 2 * i);
+        if (2 * i + 1 < HN) w[2 * i + 1] = read_w(wl, 2 * i + 1);
+        x[i] = read_x(xl, i);
+    }
+    int ws = 0;               // slot of block b's weights
+    int xs = 0;               // slot of block b's unit of x
+    int xf = (XH >> 1) % XU;  // slot of half unit b + XH
+    int ws0 = WD - 1, xf0 = ((XH - 1) >> 1) % XU;  // those that block b - 1 requests into
+    // the zeros are written before the first product reads them
+    if constexpr (IN_A) asm volatile("s_nop 7" ::: "memory");
+#pragma unroll 1
     for (int b = 0; b < nblk; ++b) {
-        v4i in[L];
+        auto request = [&](int l, int b0) {
+            if (l < LW)
+                fetch_w1(l, b0 + WD, ws0);
+            else
+                fetch_x1(l - LW, b0 + XH, xf0);
+        };
+        int wa = wl + ws * WBLK;
 #pragma unroll
-        for (int l = 0; l < L; ++l)
-            in[l] = *reinterpret_cast<const v4i*>(
-                from[l] + (size_t)b * (wave + l * NW < AF ? 64 : 1024));
-        __syncthreads();
+        for (int i = 0; i < FM; ++i) {
 #pragma unroll
-        for (int l = 0; l < L; ++l)
-            if (wave + l * NW < AF + BF) smem[(wave + l * NW) * QLM_WAVE + lane] = in[l];
-        __syncthreads();
-        v4i x[FM], w[FN];
+            for (int j = 0; j < HN; ++j) mma<IN_A>(acc[i][j], w[j], x[i]);
+            if (i < HN) w[HN + i] = read_w(wa, HN + i);
 #pragma unroll
-        for (int i = 0; i < FM; ++i) x[i] = smem[(wm * FM + i) * QLM_WAVE + lane];
+            for (int l = L1 + i * (L - L1) / FM; l < L1 + (i + 1) * (L - L1) / FM; ++l)
+                request(l, b - 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(L * AHEAD) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        ws0 = ws;
+        xf0 = xf;
+        if ((b + XH) & 1) xf = xf + 1 == XU ? 0 : xf + 1;
+        ws = ws + 1 == WD ? 0 : ws + 1;
+        if (b & 1) xs = xs + 1 == XU ? 0 : xs + 1;
+        wa = wl + ws * WBLK;
+        const int xa = (xl ^ (((b + 1) & 1) << 6)) + xs * XUNIT;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) w[j] = smem[(AF + wn * FN + j) * QLM_WAVE + lane];
+        for (int i = 0; i < FM; ++i) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
+            for (int j = 0; j < HN; ++j) mma<IN_A>(acc[i][HN + j], w[HN + j], x[i]);
+            if (2 * i < HN) w[2 * i] = read_w(wa, 2 * i);
+            if (2 * i + 1 < HN) w[2 * i + 1] = read_w(wa, 2 * i + 1);
+            x[i] = read_x(xa, i);
+#pragma unroll
+            for (int l = i * L1 / FM; l < (i + 1) * L1 / FM; ++l) request(l, b);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // nothing lands after the end, and the last products are written
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+    const int ml = m0 + wm * FM * 16 + (lane & 15);
+    const int nl = (t0 + wn * OF) * 16 + 4 * (lane >> 4);
+    if constexpr (EPI == OUT_PART) {
+        const int ldp = 16 * a.tiles, H = SW ? 2 : 1;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            int* p = a.part + ((size_t)slice * a.M + ml + 16 * i) * H * ldp + nl;
 #pragma unroll
             for (int j = 0; j < FN; ++j)
-                acc[i][j] =
-                    __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+                if (ml + 16 * i < a.M && nl + 16 * (j % OF) < ldp)
+                    *reinterpret_cast<v4i*>(p + (j / OF) * ldp + 16 * (j % OF)) = acc[i][j];
+        }
+        return;
     }
+    // every scale is requested before the first output is formed
+    float sx[FM];
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < FM; ++i) sx[i] = a.sx[min(ml + 16 * i, a.M - 1)];
+    f32x4u s0[OF], s1[OF];
 #pragma unroll
-        for (int j = 0; j < OF; ++j)
-            put4<EPI>(a, m0 + (wm * FM + i) * 16 + (lane & 15),
-                      (t0 + wn * OF + j) * 16 + 4 * (lane >> 4), acc[i][j],
-                      acc[i][SW ? j + OF : j]);
+    for (int j = 0; j < OF; ++j) {
+        s0[j] = load_scales(a.sw, nl + 16 * j, a.N);
+        if constexpr (SW) s1[j] = load_scales(a.sw + a.N, nl + 16 * j, a.N);
+    }
+    // inside the matrix, and with every block of a full launch but the last
+    // ones, nothing of a store is conditional
+    const bool inside = m0 + AF * 16 <= a.M && (t0 + WN * OF) * 16 <= a.N;
+    float* y = a.y + (size_t)ml * a.ldy + nl;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        f32x4u old[OF];
+        if constexpr (EPI == EPI_RESID) {
+            if (inside) {
+#pragma unroll
+                for (int j = 0; j < OF; ++j)
+                    old[j] = *reinterpret_cast<const f32x4u*>(y + 16 * j);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < OF; ++j) {
+            const f32x4u v = scaled<EPI>(acc[i][j], acc[i][SW ? j + OF : j], sx[i], s0[j],
+                                         SW ? s1[j] : s0[j]);
+            if (inside)
+                *reinterpret_cast<f32x4u*>(y + 16 * j) = EPI == EPI_RESID ? old[j] + v : v;
+            else if (ml + 16 * i < a.M)
+                put<EPI>(y + 16 * j, v, a.N - (nl + 16 * j));
+        }
+        y += 16 * a.ldy;
+    }
+}
+
+// The slices' sums of four neighbouring outputs a thread, in 32-bit integers
+// (order does not matter), then the epilogue.
+constexpr int kJoinThreads = 256;
+template <int EPI>
+__global__ __launch_bounds__(kJoinThreads) void k_a8_join(A8Args a, int slices) {
+    constexpr int H = EPI == EPI_SWIGLU ? 2 : 1;
+    const int q4 = 4 * a.tiles;  // groups of four of a row
+    const long long i = (long long)blockIdx.x * kJoinThreads + threadIdx.x;
+    if (i >= (long long)a.M * q4) return;
+    const int m = (int)(i / q4), n = 4 * (int)(i - (long long)m * q4);
+    const int ldp = 16 * a.tiles;
+    const int* p = a.part + (size_t)m * H * ldp + n;
+    const size_t step = (size_t)a.M * H * ldp;
+    v4i s[2] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
+    constexpr int U = 4;  // slices in flight
+    for (int k = 0; k < slices; k += U) {
+        v4i v[U][H];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                v[u][h] = *reinterpret_cast<const v4i*>(p + min(k + u, slices - 1) * step + h * ldp);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                if (k + u < slices) s[h] += v[u][h];
+    }
+    if (n >= a.N) return;
+    const f32x4u w0 = load_scales(a.sw, n, a.N);
+    const f32x4u w1 = H == 2 ? load_scales(a.sw + a.N, n, a.N) : w0;
+    put<EPI>(a.y + (size_t)m * a.ldy + n, scaled<EPI>(s[0], s[1], a.sx[m], w0, w1), a.N - n);
+}
+
+// The streaming form of a call: 16-row tiles of x and weight tiles a
+// workgroup. More weight tiles a workgroup read x fewer times, where enough
+// workgroups are left.
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+struct StreamShape {
+    int mt, nt;
+    bool longk;
+};
+StreamShape stream_shape(int M, int tiles, int kblk, int halves) {
+    const bool longk = kblk > 64;
+    if (M <= 16) return {1, M > 1 && tiles * halves >= 4096 ? 2 : 1, longk};
+    if (M <= 32) return {2, tiles * halves >= 1024 ? 4 : 1, longk};
+    const int groups = (M + 63) / 64;
+    if (M <= 48 || (M > 64 && (M + 47) / 48 * 48 < groups * 64)) return {3, 2, longk};
+    if (M > 64 && M <= 80) return {5, 2, longk};
+    return {4, tiles * halves * groups >= 1024 ? 4 : 1, longk};
+}
+
+// How a call runs. Times in us, measured on an MI355X with operands cold in
+// the caches; kblk 64-column blocks of K.
+enum { K_STREAM = 0, K_T128 = 1, K_T256 = 2 };
+struct Plan {
+    int kind;            // of the first `cols` column blocks of its tile width;
+    int cols;            // the others run as 128 x 128 tiles (K_T256 only)
+    int slices, bslice;  // of K, and 64-column blocks in each (K_T128 only)
+};
+
+constexpr int kSliceMinRows = 32, kSliceMinBlocks = 8, kSliceMost = 8, kSliceTiles = 256;
+
+// 128 x 128 tiles, two workgroups a CU: alone on its CU a workgroup takes
+// 0.28 a block, beside another 0.5 to 0.6.
+double cost128(int n, int kblk) {
+    if (n <= 512) return 5 + (n <= 256 ? 0.28 : 0.5) * kblk;
+    return ceil_div(n, 512) * (6 + 0.6 * kblk);
+}
+// 256 x 256 tiles, one workgroup a CU: 0.58 a block while the other CUs idle,
+// 0.7 with all of them.
+double cost256(int n, int kblk) {
+    return n < 192 ? 14 + 0.58 * kblk : ceil_div(n, 256) * (10 + 0.7 * kblk);
+}
+
+Plan plan_of(int M, int N, int K, int epilogue) {
+    const int halves = epilogue == EPI_SWIGLU ? 2 : 1, kblk = K / 64;
+    const int tiles = ceil_div(N, 16);
+    Plan best{K_STREAM, 0, 1, kblk};
+    double least = 1e30;
+    const int gx1 = ceil_div(tiles, 8 / halves), gy1 = ceil_div(M, 128);
+    const int gx2 = ceil_div(tiles, 16 / halves), gy2 = ceil_div(M, 256);
+    auto offer = [&](double us, Plan p) {
+        if (us < least) least = us, best = p;
+    };
+    // Few rows: the L2 feeds a CU of the streaming form with about 36 KB a us
+    // of x and weights, and a workgroup reads all of both for its tiles.
+    {
+        const StreamShape f = stream_shape(M, tiles, kblk, halves);
+        const long long groups = (long long)ceil_div(tiles, f.nt) * ceil_div(M, 16 * f.mt);
+        const double kb = K * 16.0 * (f.mt + f.nt * halves) / 1024;
+        offer(2.5 + (groups <= 256 ? 1.0 : groups / 256.0) * kb / 36, best);
+    }
+    if (M > kSliceMinRows) {
+        for (int s = 1; s <= kSliceMost; s *= 2) {
+            if (s > 1 && (gx1 * gy1 * s > kSliceTiles || kblk < kSliceMinBlocks * s)) break;
+            // the slices' sums are written and read back, 4 MB a us
+            const double join = s == 1 ? 0 : 3 + 8e-6 * s * M * halves * N / 4;
+            const int bs = s == 1 ? kblk : ceil_div(ceil_div(kblk, s), 2) * 2;
+            offer(cost128(gx1 * gy1 * s, bs) + join, Plan{K_T128, gx1, ceil_div(kblk, bs), bs});
+        }
+    }
+    if (M > 128) {
+        offer(cost256(gx2 * gy2, kblk), Plan{K_T256, gx2, 1, kblk});
+        // full rounds of 256 tiles, and the columns left over as smaller ones
+        const int full = gx2 * gy2 / 256 * 256 / gy2;
+        if (full > 0 && full < gx2)
+            offer(cost256(full * gy2, kblk) + cost128((gx1 - 2 * full) * gy1, kblk),
+                  Plan{K_T256, full, 1, kblk});
+    }
+#ifdef A8_TUNE
+    if (getenv("A8K")) {
+        best = Plan{atoi(getenv("A8K")), 1 << 20, 1, kblk};
+        if (getenv("A8S") && atoi(getenv("A8S")) > 1) {
+            best.bslice = ceil_div(ceil_div(kblk, atoi(getenv("A8S"))), 2) * 2;
+            best.slices = ceil_div(kblk, best.bslice);
+        }
+    }
+#endif
+    return best;
+}
+
+// Bytes that a sliced call writes of its workspace.
+size_t part_bytes(const Plan& p, int M, int N, int epilogue) {
+    return (size_t)p.slices * M * (epilogue == EPI_SWIGLU ? 2 : 1) * (ceil_div(N, 16) * 16) * 4;
+}
+
+// Column blocks [first, last) of the tile width.
+template <int EPI, int WM, int WN, int FM, int FN, int WD, int XU, int OCC>
+void launch_tile(A8Args a, const Plan& p, int first, int last, hipStream_t st) {
+    constexpr bool SW = EPI == EPI_SWIGLU;
+    constexpr int OT = WN * (SW ? FN / 2 : FN);
+    a.t_first = first * OT;
+    a.gx = min(last, ceil_div(a.tiles, OT)) - first;
+    a.gy = ceil_div(a.M, 16 * WM * FM);
+    a.blocks = a.gx * a.gy * p.slices;
+    a.per_xcd = ceil_div(a.blocks, 8);
+    a.bslice = p.bslice;
+    const dim3 grid(8 * a.per_xcd), threads(WM * WN * QLM_WAVE);
+    if (p.slices == 1) {
+        hipLaunchKernelGGL((k_a8_tile<EPI, SW, WM, WN, FM, FN, WD, XU, OCC>), grid, threads, 0, st,
+                           a);
+        return;
+    }
+    hipLaunchKernelGGL((k_a8_tile<OUT_PART, SW, WM, WN, FM, FN, WD, XU, OCC>), grid, threads, 0, st,
+                       a);
+    const long long groups = (long long)a.M * 4 * a.tiles;
+    hipLaunchKernelGGL((k_a8_join<EPI>), dim3((unsigned)((groups + kJoinThreads - 1) / kJoinThreads)),
+                       dim3(kJoinThreads), 0, st, a, p.slices);
+}
+
+template <int EPI, int MT, int NT, int NW, int U, int P>
+void launch_stream(const A8Args& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_a8_stream<EPI, MT, NT, NW, U, P>),
+                       dim3(ceil_div(a.tiles, NT), ceil_div(a.M, 16 * MT)), dim3(NW * QLM_WAVE), 0,
+                       st, a);
 }
 
 template <int EPI>
-void launch(const A8Args& a, hipStream_t st) {
-    constexpr int NW = 8;
-    if (a.M <= 16) {
-        hipLaunchKernelGGL((k_a8_stream<EPI, 1, NW>), dim3(a.tiles), dim3(NW * QLM_WAVE), 0, st, a);
-    } else if (a.M <= 32) {
-        hipLaunchKernelGGL((k_a8_stream<EPI, 2, NW>), dim3(a.tiles), dim3(NW * QLM_WAVE), 0, st, a);
-    } else if (a.M <= 64) {
-        hipLaunchKernelGGL((k_a8_stream<EPI, 4, NW>), dim3(a.tiles), dim3(NW * QLM_WAVE), 0, st, a);
-    } else {
-        constexpr int ot = EPI == EPI_SWIGLU ? 4 : 8;
-        hipLaunchKernelGGL((k_a8_tile<EPI, 2, 2, 4, 4>),
-                           dim3((a.tiles + ot - 1) / ot, (a.M + 127) / 128), dim3(256), 0, st, a);
+void launch(const A8Args& a, const Plan& p, hipStream_t st) {
+    constexpr int ALL = 1 << 30;
+    if (p.kind == K_T256) {
+        launch_tile<EPI, 2, 4, 8, 4, 4, 3, 2>(a, p, 0, p.cols, st);
+        if (p.cols < ceil_div(a.tiles, EPI == EPI_SWIGLU ? 8 : 16))
+            launch_tile<EPI, 2, 2, 4, 4, 4, 3, 2>(a, p, 2 * p.cols, ALL, st);
+        return;
     }
+    if (p.kind == K_T128) {
+        launch_tile<EPI, 2, 2, 4, 4, 4, 3, 2>(a, p, 0, ALL, st);
+        return;
+    }
+#ifdef A8_TUNE
+    if (getenv("A8M")) {
+        const int mt = atoi(getenv("A8M")), nt = atoi(getenv("A8N")), nw = atoi(getenv("A8W")),
+                  u = atoi(getenv("A8U")), pz = atoi(getenv("A8P"));
+#define TRY(m, n, w, uu, pp)                                  \
+    if (mt == m && nt == n && nw == w && u == uu && pz == pp) \
+        return launch_stream<EPI, m, n, w, uu, pp>(a, st);
+#include "tune_shapes.inc"
+    }
+#endif
+    const StreamShape f = stream_shape(a.M, a.tiles, a.K / 64, EPI == EPI_SWIGLU ? 2 : 1);
+    if (f.mt == 1 && f.nt == 2) return launch_stream<EPI, 1, 2, 8, 5, 1>(a, st);
+    if (f.mt == 1 && f.longk) return launch_stream<EPI, 1, 1, 16, 5, 1>(a, st);
+    if (f.mt == 1) return launch_stream<EPI, 1, 1, 5, 4, 2>(a, st);
+    if (f.mt == 2 && f.nt == 4) return launch_stream<EPI, 2, 4, 8, 2, 2>(a, st);
+    if (f.mt == 2 && f.longk) return launch_stream<EPI, 2, 1, 8, 5, 1>(a, st);
+    if (f.mt == 2) return launch_stream<EPI, 2, 1, 5, 4, 2>(a, st);
+    if (f.mt == 3) return launch_stream<EPI, 3, 2, 8, 2, 2>(a, st);
+    if (f.mt == 5) return launch_stream<EPI, 5, 2, 8, 2, 1>(a, st);
+    if (f.nt == 4) return launch_stream<EPI, 4, 4, 8, 2, 2>(a, st);
+    launch_stream<EPI, 4, 1, 8, 2, 2>(a, st);
 }
 
 }  // namespace
 
 extern "C" size_t qlm_matmul_a8_workspace_bytes(int M, int N, int K, int epilogue) {
-    (void)M, (void)N, (void)K, (void)epilogue;
-    return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K % 64 != 0 || epilogue < EPI_STORE || epilogue > EPI_SWIGLU)
+        return 0;
+    // Slices are cut for at most 256 tiles of 128 x 128 sums in all, at most 8
+    // of a call: a bound that never falls with M.
+    if (M <= kSliceMinRows || K / 64 < 2 * kSliceMinBlocks) return 0;
+    const size_t sums = (size_t)M * (epilogue == EPI_SWIGLU ? 2 : 1) * ((N + 15) / 16 * 16);
+    const size_t most = (size_t)kSliceTiles * 128 * 128;
+    return 4 * (kSliceMost * sums < most ? kSliceMost * sums : most);
 }
 
 extern "C" int qlm_matmul_a8(const int8_t* x, int ldx, const float* x_scales,
@@ -238,16 +656,30 @@ extern "C" int qlm_matmul_a8(const int8_t* x, int ldx, const float* x_scales,
     if (epilogue < EPI_STORE || epilogue > EPI_SWIGLU || ldx < K || ldy < N) return QLM_ERR_ARG;
     if (K % 64 != 0 || K >= 1 << 17 || ldx % 16 != 0 || ldx >= 1 << 23) return QLM_ERR_SHAPE;
     if (((uintptr_t)x | (uintptr_t)q_tiles | (uintptr_t)work) & 15u) return QLM_ERR_SHAPE;
+    const Plan p = plan_of(M, N, K, epilogue);
     const size_t need = qlm_matmul_a8_workspace_bytes(M, N, K, epilogue);
     if (need && (!work || work_bytes < need)) return QLM_ERR_ARG;
-    const A8Args a{x, x_scales, q_tiles, s_rows, y, ldx, ldy, M, N, K, (N + 15) / 16};
+    if (p.slices > 1 && part_bytes(p, M, N, epilogue) > work_bytes) return QLM_ERR_ARG;
+    A8Args a{};
+    a.x = x;
+    a.sx = x_scales;
+    a.q = q_tiles;
+    a.sw = s_rows;
+    a.y = y;
+    a.ldx = ldx;
+    a.ldy = ldy;
+    a.M = M;
+    a.N = N;
+    a.K = K;
+    a.tiles = (N + 15) / 16;
+    a.part = static_cast<int*>(work);
     hipStream_t st = as_stream(stream);
     if (epilogue == EPI_SWIGLU)
-        launch<EPI_SWIGLU>(a, st);
+        launch<EPI_SWIGLU>(a, p, st);
     else if (epilogue == EPI_RESID)
-        launch<EPI_RESID>(a, st);
+        launch<EPI_RESID>(a, p, st);
     else
-        launch<EPI_STORE>(a, st);
+        launch<EPI_STORE>(a, p, st);
     return qlm_launch_status();
 }
 
@@ -255,5 +687,5 @@ extern "C" int qlm_matmul_a8(const int8_t* x, int ldx, const float* x_scales,
 // otherwise loads it at the first launch of one of its kernels.
 hipError_t qlm_load_gemm_a8() {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>((k_a8_stream<EPI_STORE, 1, 8>)));
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(k_a8_join<EPI_STORE>));
 }
