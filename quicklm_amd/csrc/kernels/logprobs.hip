@@ -19,14 +19,17 @@
 // the GPU; otherwise slices leave (M, z, u) and their maxima to
 // k_logprob_finish. Bound by the one read of the logits.
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;   // of a workgroup that reads a row or a slice
 constexpr int kWaves = kThreads / QLM_WAVE;
+constexpr int kFinishWaves = 8;   // of a workgroup that finishes a sliced row
 constexpr int kChunk = 4 * QLM_WAVE;  // logits of a chunk: a vector of four a lane
 constexpr int kUnroll = 4;            // chunks a wave keeps in flight
 constexpr int kMaxTop = 64;
@@ -67,10 +70,15 @@ struct LpArgs {
     int* maxima;  // [rows, nchunk], orders of the chunks' maxima, likewise
 };
 
-// A lane's four logits of chunk c (-inf past the row's end).
+// A lane's four logits of chunk c (-inf past the row's end). STREAM: not kept
+// in the caches, which read 2047 rows of 151936 in 213 us instead of 235.
+template <bool STREAM = false>
 __device__ __forceinline__ f32x4u load_chunk(const float* row, int n, int c) {
     const int i = c * kChunk + 4 * (int)(threadIdx.x & (QLM_WAVE - 1));
-    if (i + 4 <= n) return *reinterpret_cast<const f32x4u*>(row + i);
+    if (i + 4 <= n) {
+        const f32x4u* p = reinterpret_cast<const f32x4u*>(row + i);
+        return STREAM ? __builtin_nontemporal_load(p) : *p;
+    }
     f32x4u v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = i + j < n ? row[i + j] : -INFINITY;
@@ -98,7 +106,7 @@ __device__ __forceinline__ Part stream_row(const float* lr, int n, int c0, int c
         f32x4u v[kUnroll];
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j)
-            v[j] = load_chunk(lr, n, min(c + j * kWaves, c1 - 1));
+            v[j] = load_chunk<true>(lr, n, min(c + j * kWaves, c1 - 1));
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) {
             const int cj = c + j * kWaves;
@@ -137,235 +145,305 @@ __device__ __forceinline__ Part stream_row(const float* lr, int n, int c0, int c
 }
 
 struct TopShared {
-    int red[kWaves];
-    int nsel, ncand;
+    int red[kFinishWaves];
+    int nsel, lo;  // chunks named, and their threshold
     int sel[kMaxTop + kSlack];
     int same[kMaxTop + kSlack];
-    int cand_o[kCand];
-    int cand_i[kCand];
+    long long cand[kCand];  // order of the logit, then what is left of 2^32 - 1 by the id
 };
 
-// Sum of an int over the workgroup, for every thread.
-__device__ __forceinline__ int block_count(int v, int* red) {
-    __syncthreads();
-    if ((threadIdx.x & (QLM_WAVE - 1)) == 0) red[threadIdx.x / QLM_WAVE] = v;
-    __syncthreads();
-    int t = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) t += red[w];
-    return t;
+// Sum, minimum and maximum of an int over the wave, for every lane.
+template <typename Op>
+__device__ __forceinline__ int wave_reduce(int v, Op op) {
+    auto dpp = [](int x, auto ctrl) {
+        return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false);
+    };
+    v = op(v, dpp(v, std::integral_constant<int, kDppXor1>{}));
+    v = op(v, dpp(v, std::integral_constant<int, kDppXor2>{}));
+    v = op(v, dpp(v, std::integral_constant<int, kDppHalfMirror>{}));
+    v = op(v, dpp(v, std::integral_constant<int, kDppMirror>{}));
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op((int)s[0], (int)s[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_amdgcn_readfirstlane(op((int)t[0], (int)t[1]));
+}
+__device__ __forceinline__ int wave_sum_i(int v) {
+    return wave_reduce(v, [](int a, int b) { return a + b; });
 }
 
-// The first `top` tokens of a row by (logit, then lower id). `mx`: the orders
-// of the row's chunk maxima in LDS, `most` the largest of them. CPW: chunks a
-// wave can hold, kWaves CPW >= top + kSlack. Called by the whole workgroup.
-// emit(rank, id, logit).
-template <int CPW, typename Emit>
-__device__ void select_top(const float* row, int n, int nchunk, int top, const int* mx, int most,
-                           TopShared& sh, Emit emit) {
+// The threshold over a row's chunk maxima and the chunks that reach it, in
+// order, by one wave. at(c): order of chunk c's maximum.
+template <typename At>
+__device__ __forceinline__ void name_chunks(int nchunk, int top, At at, TopShared& sh) {
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    const unsigned long long below = (1ull << lane) - 1;
+    // count(>= lo) >= top, as near to top as the slack, unless maxima tie
+    int lo, hi, above = 0, named = nchunk;  // count(>= hi) = above < top
+    auto bisect = [&](int least, int most, auto count) {
+        lo = wave_reduce(least, [](int a, int b) { return min(a, b); });
+        hi = wave_reduce(most, [](int a, int b) { return max(a, b); }) + 1;
+        // first whether all but a few are equal (a masked row's chunks)
+        for (int m = lo + 1; hi - (long long)lo > 1 && named > top + kSlack; m = mid_of(lo, hi)) {
+            const int cnt = count(m);
+            if (cnt >= top) {
+                lo = m;
+                named = cnt;
+            } else {
+                hi = m;
+                above = cnt;
+            }
+        }
+    };
+    int listed = 0, left = 0;
+    auto list = [&](int c, int o) {
+        const bool over = c < nchunk && o > lo, same = c < nchunk && o == lo;
+        const unsigned long long bs = __ballot(same);
+        const bool take = over || (same && (int)__popcll(bs & below) < left);
+        const unsigned long long bt = __ballot(take);
+        if (take) sh.sel[listed + (int)__popcll(bt & below)] = c;
+        listed += (int)__popcll(bt);
+        left -= min(left, (int)__popcll(bs));
+    };
+    if (nchunk <= kRegMax * QLM_WAVE) {  // the maxima in registers
+        int o[kRegMax], least = INT32_MAX, most = INT32_MIN;
+#pragma unroll
+        for (int j = 0; j < kRegMax; ++j) {
+            o[j] = INT32_MIN;
+            if (j * QLM_WAVE + lane < nchunk) o[j] = at(j * QLM_WAVE + lane);
+        }
+#pragma unroll
+        for (int j = 0; j < kRegMax; ++j) {
+            most = max(most, o[j]);
+            if (j * QLM_WAVE + lane < nchunk) least = min(least, o[j]);
+        }
+        bisect(least, most, [&](int m) {
+            int cnt = 0;
+#pragma unroll
+            for (int j = 0; j < kRegMax; ++j) cnt += o[j] >= m;
+            return wave_sum_i(cnt);
+        });
+        left = named > top + kSlack ? top - above : INT32_MAX;
+#pragma unroll
+        for (int j = 0; j < kRegMax; ++j)
+            if (j * QLM_WAVE < nchunk) list(j * QLM_WAVE + lane, o[j]);
+    } else {
+        int least = INT32_MAX, most = INT32_MIN;
+        for (int c = lane; c < nchunk; c += QLM_WAVE) {
+            const int o = at(c);
+            least = min(least, o);
+            most = max(most, o);
+        }
+        bisect(least, most, [&](int m) {
+            int cnt = 0;
+            for (int c = lane; c < nchunk; c += QLM_WAVE) cnt += at(c) >= m;
+            return wave_sum_i(cnt);
+        });
+        left = named > top + kSlack ? top - above : INT32_MAX;
+        for (int c0 = 0; c0 < nchunk; c0 += QLM_WAVE)
+            list(c0 + lane, at(min(c0 + lane, nchunk - 1)));
+    }
+    if (lane == 0) {
+        sh.nsel = listed;
+        sh.lo = lo;
+    }
+}
+
+// The first `top` tokens of a row by (logit, then lower id), the chunks that
+// hold them named in `sh` (or all, where there are no more than `top`), `most`
+// the order of its largest logit. CPW: chunks a wave can hold, NW CPW >= top + kSlack. Called by the whole
+// workgroup. emit(rank, id, order of the logit).
+template <int CPW, int NW, typename Emit>
+__device__ __forceinline__ void select_top(const float* row, int n, int nchunk, int top, int most,
+                                           TopShared& sh, Emit emit) {
     const int lane = threadIdx.x & (QLM_WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
     const unsigned long long below = (1ull << lane) - 1;
     const bool listed = nchunk > top;
-    // Every wave finds the same threshold `lo` over the chunk maxima:
-    // count(>= lo) >= top, and as near to top as the slack, unless maxima tie.
-    int lo = kLowest, spare = 0x7fffffff;  // spare: chunks equal to lo that are taken
-    if (listed) {
-        int hi = most + 1, above = 0, named = nchunk;  // count(>= hi) = above < top
-        auto bisect = [&](auto count) {
-            while (hi - (long long)lo > 1 && named > top + kSlack) {
-                const int m = mid_of(lo, hi);
-                const int cnt = count(m);
-                if (cnt >= top) {
-                    lo = m;
-                    named = cnt;
-                } else {
-                    hi = m;
-                    above = cnt;
-                }
-            }
-        };
-        if (nchunk <= kRegMax * QLM_WAVE) {
-            int o[kRegMax];
-#pragma unroll
-            for (int j = 0; j < kRegMax; ++j) {
-                o[j] = INT32_MIN;
-                if (j * QLM_WAVE < nchunk && j * QLM_WAVE + lane < nchunk)
-                    o[j] = mx[j * QLM_WAVE + lane];
-            }
-            bisect([&](int m) {
-                int cnt = 0;
-#pragma unroll
-                for (int j = 0; j < kRegMax; ++j)
-                    if (j * QLM_WAVE < nchunk) cnt += (int)__popcll(__ballot(o[j] >= m));
-                return cnt;
-            });
-        } else {
-            bisect([&](int m) {
-                int cnt = 0;
-                for (int c = lane; c < nchunk + lane; c += QLM_WAVE)
-                    cnt += (int)__popcll(__ballot(c < nchunk && mx[min(c, nchunk - 1)] >= m));
-                return cnt;
-            });
-        }
-        if (named > top + kSlack) spare = top - above;
-    }
-    // The chunks, in order, into LDS (wave 0).
-    if (threadIdx.x == 0) sh.ncand = 0;
-    if (listed && wave == 0) {
-        int at = 0, left = spare;
-        for (int c0 = 0; c0 < nchunk; c0 += QLM_WAVE) {
-            const int c = c0 + lane;
-            const int o = mx[min(c, nchunk - 1)];
-            const bool over = c < nchunk && o > lo, same = c < nchunk && o == lo;
-            const unsigned long long bs = __ballot(same);
-            const bool take = over || (same && (int)__popcll(bs & below) < left);
-            const unsigned long long bt = __ballot(take);
-            if (take) sh.sel[at + (int)__popcll(bt & below)] = c;
-            at += (int)__popcll(bt);
-            left -= min(left, (int)__popcll(bs));
-        }
-        if (lane == 0) sh.nsel = at;
-    }
-    __syncthreads();
     const int nsel = listed ? sh.nsel : nchunk;
-    // The chunks' logits, chunk `wave + j kWaves` of the list in v[j], all
+    // The chunks' logits, chunk `wave + j NW` of the list in o[j], all
     // requested before the first is used; what lies past the row is below all.
     int o[CPW][4], at[CPW];
     {
         f32x4u v[CPW];
 #pragma unroll
         for (int j = 0; j < CPW; ++j) {
-            const int s = wave + j * kWaves;
+            const int s = wave + j * NW;
             if (s < nsel) {
                 const int c = listed ? __builtin_amdgcn_readfirstlane(sh.sel[s]) : s;
-                at[j] = c * kChunk + 4 * lane;
+                at[j] = c * kChunk;
                 v[j] = load_chunk(row, n, c);
             }
         }
 #pragma unroll
         for (int j = 0; j < CPW; ++j)
-            if (wave + j * kWaves < nsel)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    o[j][k] = at[j] + k < n ? order_of(v[j][k]) : INT32_MIN;
+            for (int k = 0; k < 4; ++k) {
+                o[j][k] = INT32_MIN;
+                if (wave + j * NW < nsel && at[j] + 4 * lane + k < n)
+                    o[j][k] = order_of(v[j][k]);
+            }
     }
+    // a count over the workgroup, its own share left in `mine`
+    auto total = [&](int c) {
+        c = wave_sum_i(c);
+        __syncthreads();
+        if (lane == 0) sh.red[wave] = c;
+        __syncthreads();
+        int t = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) t += sh.red[w];
+        return t;
+    };
+    // how many logits reach `from`
     auto count_from = [&](int from) {
-        int cnt = 0;
+        int c = 0;
 #pragma unroll
         for (int j = 0; j < CPW; ++j)
-            if (wave + j * kWaves < nsel)
+            if (wave + j * NW < nsel)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) cnt += (int)__popcll(__ballot(o[j][k] >= from));
-        return block_count(cnt, sh.red);
+                for (int k = 0; k < 4; ++k) c += o[j][k] >= from;
+        return total(c);
     };
-    auto gather = [&](int from) {
-#pragma unroll
-        for (int j = 0; j < CPW; ++j)
-            if (wave + j * kWaves < nsel)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool in = o[j][k] >= from;
-                    const unsigned long long b = __ballot(in);
-                    if (b == 0) continue;
-                    int base = 0;
-                    if (lane == 0) base = atomicAdd(&sh.ncand, (int)__popcll(b));
-                    base = __builtin_amdgcn_readfirstlane(base) + (int)__popcll(b & below);
-                    if (in && base < kCand) {
-                        sh.cand_o[base] = o[j][k];
-                        sh.cand_i[base] = at[j] + k;
-                    }
-                }
-    };
-    int from = lo, cnt = count_from(lo);
+    int from = listed ? sh.lo : kLowest, cnt = count_from(from);
     bool tied = false;
     if (cnt > kCand) {
-        // bisect over the logits: count(>= from) >= top, <= kCand
-        int hi = most + 1;
-        while (hi - (long long)from > 1 && cnt > kCand) {
-            const int m = mid_of(from, hi);
-            const int k = count_from(m);
-            if (k >= top) {
-                from = m;
-                cnt = k;
-            } else {
-                hi = m;
+        // Logits equal to `from` may be many (masked ones): fewer than `top`
+        // above it leave only those, in order. Otherwise bisect: first over
+        // the threads' largest logits (at least as many logits reach what
+        // `top` of them reach, and hardly more), then, where that was not
+        // enough, over the logits: count(>= from) >= top, <= kCand.
+        int k = count_from(from + 1);
+        if (k >= top) {
+            from += 1;
+            cnt = k;
+            int mine = INT32_MIN;
+#pragma unroll
+            for (int j = 0; j < CPW; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mine = max(mine, o[j][i]);
+            int hi = most + 1, reach = total(mine >= from);
+            if (reach >= top) {
+                while (hi - (long long)from > 1 && reach > 2 * top) {
+                    const int m = mid_of(from, hi);
+                    k = total(mine >= m);
+                    if (k >= top) {
+                        from = m;
+                        reach = k;
+                    } else {
+                        hi = m;
+                    }
+                }
+                cnt = count_from(from);
+                hi = most + 1;
+            }
+            while (hi - (long long)from > 1 && cnt > kCand) {
+                const int m = mid_of(from, hi);
+                k = count_from(m);
+                if (k >= top) {
+                    from = m;
+                    cnt = k;
+                } else {
+                    hi = m;
+                }
             }
         }
         tied = cnt > kCand;
+        cnt = count_from(tied ? from + 1 : from);  // the waves' shares again
     }
-    gather(tied ? from + 1 : from);  // tied: fewer than `top` lie above
-    if (tied) {
-        // those equal to it follow in the order of their ids: places by the
-        // counts of the chunks before, then of the lanes before
+    // candidates, this wave's behind those of the waves before it
+    int place = 0;
+    for (int w = 0; w < wave; ++w) place += sh.red[w];
+    auto take = [&](bool in, int order, int id, int p) {
+        if (in) sh.cand[p] = ((long long)order << 32) | (unsigned)(0x7fffffff - id);
+    };
+    {
+        const int least = tied ? from + 1 : from;
 #pragma unroll
         for (int j = 0; j < CPW; ++j)
-            if (wave + j * kWaves < nsel) {
-                int c = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) c += (int)__popcll(__ballot(o[j][k] == from));
-                if (lane == 0) sh.same[wave + j * kWaves] = c;
-            }
-        __syncthreads();
-        const int over = sh.ncand;
-        __syncthreads();
-        int before = 0, s0 = 0;
-#pragma unroll
-        for (int j = 0; j < CPW; ++j)
-            if (wave + j * kWaves < nsel) {
-                for (; s0 < wave + j * kWaves; ++s0) before += sh.same[s0];
-                if (over + before >= top) continue;
-                unsigned long long b[4];
-                int place = over + before;
+            if (wave + j * NW < nsel)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    b[k] = __ballot(o[j][k] == from);
-                    place += (int)__popcll(b[k] & below);
+                    const bool in = o[j][k] >= least;
+                    const unsigned long long b = __ballot(in);
+                    take(in, o[j][k], at[j] + 4 * lane + k, place + (int)__popcll(b & below));
+                    place += (int)__popcll(b);
                 }
+    }
+    if (tied) {
+        // those equal to `from` follow in the order of their ids: places by
+        // the counts of the chunks before, then of the lanes before
+#pragma unroll
+        for (int j = 0; j < CPW; ++j)
+            if (wave + j * NW < nsel) {
+                int c = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) c += o[j][k] == from;
+                c = wave_sum_i(c);
+                if (lane == 0) sh.same[wave + j * NW] = c;
+            }
+        __syncthreads();
+        int before = cnt, s0 = 0;
+#pragma unroll
+        for (int j = 0; j < CPW; ++j)
+            if (wave + j * NW < nsel) {
+                for (; s0 < wave + j * NW && before < top; ++s0) before += sh.same[s0];
+                if (before >= top) continue;
+                int p = before;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (o[j][k] == from) {
-                        if (place < top) {
-                            sh.cand_o[place] = from;
-                            sh.cand_i[place] = at[j] + k;
-                        }
-                        ++place;
-                    }
+                    p += (int)__popcll(__ballot(o[j][k] == from) & below);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = o[j][k] == from;
+                    take(in && p < top, from, at[j] + 4 * lane + k, p);
+                    p += in;
+                }
             }
         cnt = top;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < cnt; i += kThreads) {
-        const int oi = sh.cand_o[i], id = sh.cand_i[i];
+    // ranks: four lanes a candidate, each against a quarter of the others
+    for (int i0 = 0; i0 < cnt; i0 += NW * QLM_WAVE / 4) {
+        const int i = i0 + (int)threadIdx.x / 4;
+        const long long key = sh.cand[min(i, cnt - 1)];
         int rank = 0;
-        for (int j = 0; j < cnt; ++j) {
-            const int oj = sh.cand_o[j];
-            rank += oj > oi || (oj == oi && sh.cand_i[j] < id);
-        }
-        if (rank < top) emit(rank, id, row[id]);
+#pragma unroll 8
+        for (int j = threadIdx.x & 3; j < cnt; j += 4) rank += sh.cand[j] > key;
+        rank += __shfl_xor(rank, 1, QLM_WAVE);
+        rank += __shfl_xor(rank, 2, QLM_WAVE);
+        if ((threadIdx.x & 3) == 0 && i < cnt && rank < top)
+            emit(rank, 0x7fffffff - (int)(key & 0x7fffffff), (int)(key >> 32));
     }
 }
 
-// What is wanted of a row whose (M, z, u) is p; `mx` as select_top's.
-template <int CPW>
-__device__ __forceinline__ void finish_row(const LpArgs& a, int row, Part p, const int* mx,
-                                           TopShared& sh) {
+// What is wanted of a row whose (M, z, u) is p. The last wave does the sums'
+// part while the first names the chunks; at(c): order of chunk c's maximum.
+template <int CPW, int NW, typename At>
+__device__ __forceinline__ void finish_row(const LpArgs& a, int row, Part p, TopShared& sh,
+                                           At at) {
     const float* lr = a.logits + (size_t)row * a.ldl;
-    const int most = order_of(p.m);
+    const int wave = threadIdx.x / QLM_WAVE, lane = threadIdx.x & (QLM_WAVE - 1);
     // no distribution: every logit masked, a NaN, or +inf among them
-    if (!(p.z > 0.0f)) p.z = NAN;
-    const float lz = logf(p.z);
-    if (a.entropy && threadIdx.x == 0) a.entropy[row] = lz - p.u / p.z;
-    for (int j = threadIdx.x; j < a.n_ids; j += kThreads) {
-        const int id = a.ids[(size_t)row * a.n_ids + j];
-        // an id outside the row is not read
-        a.id_lp[(size_t)row * a.n_ids + j] = id >= 0 && id < a.n ? (lr[id] - p.m) - lz : NAN;
+    const float z = p.z > 0.0f ? p.z : NAN;
+    const float lz = logf(z);
+    if (wave == NW - 1) {
+        if (a.entropy && lane == 0) a.entropy[row] = lz - p.u / z;
+        for (int j = lane; j < a.n_ids; j += QLM_WAVE) {
+            const int id = a.ids[(size_t)row * a.n_ids + j];
+            // an id outside the row is not read
+            a.id_lp[(size_t)row * a.n_ids + j] =
+                id >= 0 && id < a.n ? (lr[id] - p.m) - lz : NAN;
+        }
     }
-    if constexpr (CPW > 0)
-        select_top<CPW>(lr, a.n, a.nchunk, a.top, mx, most, sh, [&](int rank, int id, float v) {
+    if constexpr (CPW > 0) {
+        if (wave == 0 && a.nchunk > a.top) name_chunks(a.nchunk, a.top, at, sh);
+        __syncthreads();
+        select_top<CPW, NW>(lr, a.n, a.nchunk, a.top, order_of(p.m), sh, [&](int rank, int id, int order) {
+            const float v = __int_as_float(order < 0 ? order ^ 0x7fffffff : order);
             a.top_ids[(size_t)row * a.top + rank] = id;
             a.top_lp[(size_t)row * a.top + rank] = (v - p.m) - lz;
         });
+    }
 }
 
 // CPW 0: no alternatives. WHOLE: a workgroup a row, finished at once.
@@ -387,32 +465,28 @@ __global__ __launch_bounds__(kThreads) void k_logprob(LpArgs a) {
             maxima[c] = o;
     });
     if constexpr (WHOLE)
-        finish_row<CPW>(a, row, p, mx, sh);
+        finish_row<CPW, kWaves>(a, row, p, sh, [&](int c) { return mx[c]; });
     else if (threadIdx.x == 0)
         a.part[(size_t)row * a.slices + slice] = p;
 }
 
 template <int CPW>
-__global__ __launch_bounds__(kThreads) void k_logprob_finish(LpArgs a) {
-    extern __shared__ int mx[];
+__global__ __launch_bounds__(kFinishWaves* QLM_WAVE) void k_logprob_finish(LpArgs a) {
     __shared__ TopShared sh;
     const int row = blockIdx.x, lane = threadIdx.x & (QLM_WAVE - 1);
-    if (CPW > 0)
-        for (int c = threadIdx.x; c < a.nchunk; c += kThreads)
-            mx[c] = a.maxima[(size_t)row * a.nchunk + c];
     // the slices joined over the lanes, alike in every wave
     const Part* parts = a.part + (size_t)row * a.slices;
     Part p{-INFINITY, 0.0f, 0.0f};
     for (int s = lane; s < a.slices; s += QLM_WAVE) p = join(p, parts[s]);
-#pragma unroll
     for (int m = QLM_WAVE / 2; m >= 1; m >>= 1)
-        p = join(p, Part{__shfl_down(p.m, m, QLM_WAVE), __shfl_down(p.z, m, QLM_WAVE),
-                         __shfl_down(p.u, m, QLM_WAVE)});
+        if (m < a.slices)
+            p = join(p, Part{__shfl_down(p.m, m, QLM_WAVE), __shfl_down(p.z, m, QLM_WAVE),
+                             __shfl_down(p.u, m, QLM_WAVE)});
     p.m = __shfl(p.m, 0, QLM_WAVE);
     p.z = __shfl(p.z, 0, QLM_WAVE);
     p.u = __shfl(p.u, 0, QLM_WAVE);
-    __syncthreads();
-    finish_row<CPW>(a, row, p, mx, sh);
+    const int* maxima = a.maxima + (size_t)row * a.nchunk;
+    finish_row<CPW, kFinishWaves>(a, row, p, sh, [&](int c) { return maxima[c]; });
 }
 
 // Whether rows are finished by the workgroups that read them. Many
@@ -420,16 +494,17 @@ __global__ __launch_bounds__(kThreads) void k_logprob_finish(LpArgs a) {
 bool whole(int slices, int top) { return slices == 1 && top + kSlack <= 8 * kWaves; }
 
 template <int CPW>
-void launch(const LpArgs& a, hipStream_t st) {
+void launch_whole(const LpArgs& a, hipStream_t st) {
     const size_t lds = CPW > 0 ? (size_t)a.nchunk * sizeof(int) : 0;
-    if constexpr (CPW <= 8)
-        if (whole(a.slices, a.top)) {
-            hipLaunchKernelGGL((k_logprob<CPW, true>), dim3(a.rows), dim3(kThreads), lds, st, a);
-            return;
-        }
+    hipLaunchKernelGGL((k_logprob<CPW, true>), dim3(a.rows), dim3(kThreads), lds, st, a);
+}
+
+template <int CPW>
+void launch_sliced(const LpArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_logprob<CPW, false>), dim3((unsigned)(a.slices * a.rows)),
                        dim3(kThreads), 0, st, a);
-    hipLaunchKernelGGL((k_logprob_finish<CPW>), dim3(a.rows), dim3(kThreads), lds, st, a);
+    hipLaunchKernelGGL((k_logprob_finish<CPW>), dim3(a.rows), dim3(kFinishWaves * QLM_WAVE), 0, st,
+                       a);
 }
 
 int chunks_of(int n) { return (n + kChunk - 1) / kChunk; }
@@ -438,7 +513,7 @@ int chunks_of(int n) { return (n + kChunk - 1) / kChunk; }
 // wave's loads in flight.
 int slices_of(int rows, int n) {
     const int most = (chunks_of(n) + kWaves * kUnroll - 1) / (kWaves * kUnroll);
-    const int want = rows >= 1024 ? 1 : 2048 / rows;
+    const int want = rows >= 768 ? 1 : 2048 / rows;
     return want < most ? want : most;
 }
 
@@ -483,15 +558,16 @@ extern "C" int qlm_token_logprobs(const float* logits, int ldl, int n, int rows,
     a.maxima = reinterpret_cast<int*>(static_cast<char*>(work) +
                                       round16((size_t)rows * a.slices * sizeof(Part)));
     hipStream_t st = as_stream(stream);
-    // chunks a wave holds: top + kSlack of them over kWaves
-    if (top == 0)
-        launch<0>(a, st);
+    // chunks a wave holds: top + kSlack of them over the waves
+    constexpr int kFinish = (kMaxTop + kSlack + kFinishWaves - 1) / kFinishWaves;
+    if (!whole(a.slices, top))
+        top ? launch_sliced<kFinish>(a, st) : launch_sliced<0>(a, st);
+    else if (top == 0)
+        launch_whole<0>(a, st);
     else if (top + kSlack <= 4 * kWaves)
-        launch<4>(a, st);
-    else if (top + kSlack <= 8 * kWaves)
-        launch<8>(a, st);
+        launch_whole<4>(a, st);
     else
-        launch<(kMaxTop + kSlack) / kWaves>(a, st);
+        launch_whole<8>(a, st);
     return qlm_launch_status();
 }
 
