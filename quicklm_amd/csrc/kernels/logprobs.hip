@@ -29,9 +29,12 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kThreads = 256;   // of a workgroup that reads a row or a slice
 constexpr int kWaves = kThreads / QLM_WAVE;
-constexpr int kFinishWaves = 8;   // of a workgroup that finishes a sliced row
+constexpr int kFinishWaves = 8;  // of a workgroup that finishes a sliced row
+constexpr int kMostWaves = 16;   // of a workgroup that reads one of few short rows
 constexpr int kChunk = 4 * QLM_WAVE;  // logits of a chunk: a vector of four a lane
-constexpr int kUnroll = 4;            // chunks a wave keeps in flight
+// Chunks a wave keeps in flight: many where one workgroup reads a long row
+// (2047 x 151936 211 us with 8, 221 with 4), few where slices are many.
+constexpr int kLongUnroll = 8, kShortUnroll = 4, kSliceUnroll = 2;
 constexpr int kMaxTop = 64;
 constexpr int kSlack = 8;             // chunks beyond k that a threshold may name
 constexpr int kCand = 512;            // logits that are ranked by counting
@@ -70,12 +73,13 @@ struct LpArgs {
     int* maxima;  // [rows, nchunk], orders of the chunks' maxima, likewise
 };
 
-// A lane's four logits of chunk c (-inf past the row's end). STREAM: not kept
-// in the caches, which read 2047 rows of 151936 in 213 us instead of 235.
+// A lane's four logits of chunk c (-inf past the row's end). c is uniform: a
+// branch by lane would wait for the load inside it. STREAM: not kept in the
+// caches, which read 2047 rows of 151936 in 213 us instead of 235.
 template <bool STREAM = false>
 __device__ __forceinline__ f32x4u load_chunk(const float* row, int n, int c) {
     const int i = c * kChunk + 4 * (int)(threadIdx.x & (QLM_WAVE - 1));
-    if (i + 4 <= n) {
+    if ((c + 1) * kChunk <= n) {
         const f32x4u* p = reinterpret_cast<const f32x4u*>(row + i);
         return STREAM ? __builtin_nontemporal_load(p) : *p;
     }
@@ -92,24 +96,36 @@ __device__ __forceinline__ int order_of(float v) {
     const int b = __float_as_int(v + 0.0f);
     return v != v ? kLowest : b < 0 ? b ^ 0x7fffffff : b;
 }
-// Between lo and hi, lo < mid < hi, where hi - lo > 1.
-__device__ __forceinline__ int mid_of(int lo, int hi) { return (lo & hi) + ((lo ^ hi) >> 1); }
+__device__ __forceinline__ float value_of(int o) {
+    return __int_as_float(o < 0 ? o ^ 0x7fffffff : o);
+}
+// A place to cut the orders lo .. hi, lo < cut < hi, where hi - lo > 1: the
+// middle of the values and the middle of the orders in turn. Values are cut in
+// a few steps where they lie near each other; the orders end any other case.
+__device__ __forceinline__ int cut_of(int lo, int hi, int step) {
+    const int mid = (lo & hi) + ((lo ^ hi) >> 1);
+    if (step & 1) return mid;
+    const float v = 0.5f * value_of(lo) + 0.5f * value_of(hi);
+    const int o = order_of(v);
+    return v == v && o > lo && o < hi ? o : mid;
+}
 
-// The workgroup's share of a row: chunks c0 .. c1 - 1, joined over the waves
-// into every thread's result. keep(c, order of chunk c's maximum), by one lane.
-template <typename Keep>
-__device__ __forceinline__ Part stream_row(const float* lr, int n, int c0, int c1, Part* parts,
+// The workgroup's share of a row: chunks c0 .. c1 - 1, a part each of the NW
+// waves. keep(c, order of chunk c's maximum), by one lane.
+template <int NW, int U, typename Keep>
+__device__ __forceinline__ void stream_row(const float* lr, int n, int c0, int c1, Part* parts,
                                            bool want_max, Keep keep) {
-    const int lane = threadIdx.x & (QLM_WAVE - 1), wave = threadIdx.x / QLM_WAVE;
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
     Part p{-INFINITY, 0.0f, 0.0f};
-    for (int c = c0 + wave; c < c1; c += kWaves * kUnroll) {
-        f32x4u v[kUnroll];
+    for (int c = c0 + wave; c < c1; c += NW * U) {
+        f32x4u v[U];
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
-            v[j] = load_chunk<true>(lr, n, min(c + j * kWaves, c1 - 1));
+        for (int j = 0; j < U; ++j)
+            if (c + j * NW < c1) v[j] = load_chunk<true>(lr, n, c + j * NW);
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
-            const int cj = c + j * kWaves;
+        for (int j = 0; j < U; ++j) {
+            const int cj = c + j * NW;
             if (cj >= c1) break;
             const float mx = wave_max(fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
             if (want_max && lane == 0) keep(cj, order_of(mx));
@@ -138,14 +154,23 @@ __device__ __forceinline__ Part stream_row(const float* lr, int n, int c0, int c
     p.u = wave_sum(p.u);
     if (lane == 0) parts[wave] = p;
     __syncthreads();
-    p = parts[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) p = join(p, parts[w]);
-    return p;
+}
+
+// `count` parts joined over the lanes of a wave, in one order; for every lane.
+__device__ __forceinline__ Part join_parts(const Part* parts, int count) {
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    Part p{-INFINITY, 0.0f, 0.0f};
+    for (int s = lane; s < count; s += QLM_WAVE) p = s < QLM_WAVE ? parts[s] : join(p, parts[s]);
+    for (int m = QLM_WAVE / 2; m >= 1; m >>= 1)
+        if (m < count)
+            p = join(p, Part{__shfl_down(p.m, m, QLM_WAVE), __shfl_down(p.z, m, QLM_WAVE),
+                             __shfl_down(p.u, m, QLM_WAVE)});
+    return Part{__shfl(p.m, 0, QLM_WAVE), __shfl(p.z, 0, QLM_WAVE), __shfl(p.u, 0, QLM_WAVE)};
 }
 
 struct TopShared {
-    int red[kFinishWaves];
+    float m, lz;  // the row's largest logit and log z
+    int red[kMostWaves];
     int nsel, lo;  // chunks named, and their threshold
     int sel[kMaxTop + kSlack];
     int same[kMaxTop + kSlack];
@@ -183,7 +208,8 @@ __device__ __forceinline__ void name_chunks(int nchunk, int top, At at, TopShare
         lo = wave_reduce(least, [](int a, int b) { return min(a, b); });
         hi = wave_reduce(most, [](int a, int b) { return max(a, b); }) + 1;
         // first whether all but a few are equal (a masked row's chunks)
-        for (int m = lo + 1; hi - (long long)lo > 1 && named > top + kSlack; m = mid_of(lo, hi)) {
+        for (int m = lo + 1, step = 0; hi - (long long)lo > 1 && named > top + kSlack;
+             m = cut_of(lo, hi, step++)) {
             const int cnt = count(m);
             if (cnt >= top) {
                 lo = m;
@@ -219,7 +245,8 @@ __device__ __forceinline__ void name_chunks(int nchunk, int top, At at, TopShare
         bisect(least, most, [&](int m) {
             int cnt = 0;
 #pragma unroll
-            for (int j = 0; j < kRegMax; ++j) cnt += o[j] >= m;
+            for (int j = 0; j < kRegMax; ++j)
+                if (j * QLM_WAVE < nchunk) cnt += o[j] >= m;
             return wave_sum_i(cnt);
         });
         left = named > top + kSlack ? top - above : INT32_MAX;
@@ -306,7 +333,9 @@ __device__ __forceinline__ void select_top(const float* row, int n, int nchunk, 
     };
     int from = listed ? sh.lo : kLowest, cnt = count_from(from);
     bool tied = false;
-    if (cnt > kCand) {
+    // (ranking many more than `top` costs more than cutting them: 1271 x 5675
+    // with 20 alternatives 35 us where any 512 were ranked)
+    if (cnt > max(128, 3 * top)) {
         // Logits equal to `from` may be many (masked ones): fewer than `top`
         // above it leave only those, in order. Otherwise bisect: first over
         // the threads' largest logits (at least as many logits reach what
@@ -323,8 +352,17 @@ __device__ __forceinline__ void select_top(const float* row, int n, int nchunk, 
                 for (int i = 0; i < 4; ++i) mine = max(mine, o[j][i]);
             int hi = most + 1, reach = total(mine >= from);
             if (reach >= top) {
-                while (hi - (long long)from > 1 && reach > 2 * top) {
-                    const int m = mid_of(from, hi);
+                // from what every thread that has logits reaches
+                const int least = wave_reduce(mine >= from ? mine : INT32_MAX,
+                                              [](int a, int b) { return min(a, b); });
+                __syncthreads();
+                if (lane == 0) sh.red[wave] = least;
+                __syncthreads();
+                from = sh.red[0];
+#pragma unroll
+                for (int w = 1; w < NW; ++w) from = min(from, sh.red[w]);
+                for (int step = 0; hi - (long long)from > 1 && reach > 2 * top; ++step) {
+                    const int m = cut_of(from, hi, step);
                     k = total(mine >= m);
                     if (k >= top) {
                         from = m;
@@ -336,8 +374,8 @@ __device__ __forceinline__ void select_top(const float* row, int n, int nchunk, 
                 cnt = count_from(from);
                 hi = most + 1;
             }
-            while (hi - (long long)from > 1 && cnt > kCand) {
-                const int m = mid_of(from, hi);
+            for (int step = 0; hi - (long long)from > 1 && cnt > kCand; ++step) {
+                const int m = cut_of(from, hi, step);
                 k = count_from(m);
                 if (k >= top) {
                     from = m;
@@ -365,6 +403,7 @@ __device__ __forceinline__ void select_top(const float* row, int n, int nchunk, 
                 for (int k = 0; k < 4; ++k) {
                     const bool in = o[j][k] >= least;
                     const unsigned long long b = __ballot(in);
+                    if (b == 0) continue;
                     take(in, o[j][k], at[j] + 4 * lane + k, place + (int)__popcll(b & below));
                     place += (int)__popcll(b);
                 }
@@ -416,18 +455,24 @@ __device__ __forceinline__ void select_top(const float* row, int n, int nchunk, 
     }
 }
 
-// What is wanted of a row whose (M, z, u) is p. The last wave does the sums'
-// part while the first names the chunks; at(c): order of chunk c's maximum.
+// What is wanted of a row. The last wave joins the `count` parts and does
+// what needs nothing but sums while the first names the chunks; at(c): order of
+// chunk c's maximum.
 template <int CPW, int NW, typename At>
-__device__ __forceinline__ void finish_row(const LpArgs& a, int row, Part p, TopShared& sh,
-                                           At at) {
+__device__ __forceinline__ void finish_row(const LpArgs& a, int row, const Part* parts, int count,
+                                           TopShared& sh, At at) {
     const float* lr = a.logits + (size_t)row * a.ldl;
     const int wave = threadIdx.x / QLM_WAVE, lane = threadIdx.x & (QLM_WAVE - 1);
-    // no distribution: every logit masked, a NaN, or +inf among them
-    const float z = p.z > 0.0f ? p.z : NAN;
-    const float lz = logf(z);
     if (wave == NW - 1) {
-        if (a.entropy && lane == 0) a.entropy[row] = lz - p.u / z;
+        const Part p = join_parts(parts, count);
+        // no distribution: every logit masked, a NaN, or +inf among them
+        const float z = p.z > 0.0f ? p.z : NAN;
+        const float lz = logf(z);
+        if (lane == 0) {
+            sh.m = p.m;
+            sh.lz = lz;
+            if (a.entropy) a.entropy[row] = lz - p.u / z;
+        }
         for (int j = lane; j < a.n_ids; j += QLM_WAVE) {
             const int id = a.ids[(size_t)row * a.n_ids + j];
             // an id outside the row is not read
@@ -438,19 +483,20 @@ __device__ __forceinline__ void finish_row(const LpArgs& a, int row, Part p, Top
     if constexpr (CPW > 0) {
         if (wave == 0 && a.nchunk > a.top) name_chunks(a.nchunk, a.top, at, sh);
         __syncthreads();
-        select_top<CPW, NW>(lr, a.n, a.nchunk, a.top, order_of(p.m), sh, [&](int rank, int id, int order) {
-            const float v = __int_as_float(order < 0 ? order ^ 0x7fffffff : order);
-            a.top_ids[(size_t)row * a.top + rank] = id;
-            a.top_lp[(size_t)row * a.top + rank] = (v - p.m) - lz;
-        });
+        const float m = sh.m, lz = sh.lz;
+        select_top<CPW, NW>(lr, a.n, a.nchunk, a.top, order_of(m), sh,
+                            [&](int rank, int id, int order) {
+                                a.top_ids[(size_t)row * a.top + rank] = id;
+                                a.top_lp[(size_t)row * a.top + rank] = (value_of(order) - m) - lz;
+                            });
     }
 }
 
 // CPW 0: no alternatives. WHOLE: a workgroup a row, finished at once.
-template <int CPW, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void k_logprob(LpArgs a) {
+template <int CPW, int NW, bool WHOLE>
+__global__ __launch_bounds__(NW* QLM_WAVE) void k_logprob(LpArgs a) {
     extern __shared__ int mx[];
-    __shared__ Part parts[kWaves];
+    __shared__ Part parts[NW];
     __shared__ TopShared sh;
     const int row = WHOLE ? blockIdx.x : blockIdx.x / a.slices;
     const int slice = WHOLE ? 0 : blockIdx.x - row * a.slices;
@@ -458,50 +504,39 @@ __global__ __launch_bounds__(kThreads) void k_logprob(LpArgs a) {
     const int per = (a.nchunk + a.slices - 1) / a.slices;
     const int c0 = slice * per, c1 = min(a.nchunk, c0 + per);
     int* maxima = a.maxima + (size_t)row * a.nchunk;
-    const Part p = stream_row(lr, a.n, c0, c1, parts, CPW > 0, [&](int c, int o) {
+    constexpr int U = !WHOLE ? kSliceUnroll : NW == kMostWaves ? kShortUnroll : kLongUnroll;
+    stream_row<NW, U>(lr, a.n, c0, c1, parts, CPW > 0, [&](int c, int o) {
         if constexpr (WHOLE)
             mx[c] = o;
         else
             maxima[c] = o;
     });
-    if constexpr (WHOLE)
-        finish_row<CPW, kWaves>(a, row, p, sh, [&](int c) { return mx[c]; });
-    else if (threadIdx.x == 0)
-        a.part[(size_t)row * a.slices + slice] = p;
+    if constexpr (WHOLE) {
+        finish_row<CPW, NW>(a, row, parts, NW, sh, [&](int c) { return mx[c]; });
+    } else if (threadIdx.x < QLM_WAVE) {
+        const Part p = join_parts(parts, NW);
+        if (threadIdx.x == 0) a.part[(size_t)row * a.slices + slice] = p;
+    }
 }
 
 template <int CPW>
 __global__ __launch_bounds__(kFinishWaves* QLM_WAVE) void k_logprob_finish(LpArgs a) {
     __shared__ TopShared sh;
-    const int row = blockIdx.x, lane = threadIdx.x & (QLM_WAVE - 1);
-    // the slices joined over the lanes, alike in every wave
-    const Part* parts = a.part + (size_t)row * a.slices;
-    Part p{-INFINITY, 0.0f, 0.0f};
-    for (int s = lane; s < a.slices; s += QLM_WAVE) p = join(p, parts[s]);
-    for (int m = QLM_WAVE / 2; m >= 1; m >>= 1)
-        if (m < a.slices)
-            p = join(p, Part{__shfl_down(p.m, m, QLM_WAVE), __shfl_down(p.z, m, QLM_WAVE),
-                             __shfl_down(p.u, m, QLM_WAVE)});
-    p.m = __shfl(p.m, 0, QLM_WAVE);
-    p.z = __shfl(p.z, 0, QLM_WAVE);
-    p.u = __shfl(p.u, 0, QLM_WAVE);
+    const int row = blockIdx.x;
     const int* maxima = a.maxima + (size_t)row * a.nchunk;
-    finish_row<CPW, kFinishWaves>(a, row, p, sh, [&](int c) { return maxima[c]; });
+    finish_row<CPW, kFinishWaves>(a, row, a.part + (size_t)row * a.slices, a.slices, sh,
+                                  [&](int c) { return maxima[c]; });
 }
 
-// Whether rows are finished by the workgroups that read them. Many
-// alternatives take registers that would leave too few of them on a CU.
-bool whole(int slices, int top) { return slices == 1 && top + kSlack <= 8 * kWaves; }
-
-template <int CPW>
+template <int CPW, int NW>
 void launch_whole(const LpArgs& a, hipStream_t st) {
     const size_t lds = CPW > 0 ? (size_t)a.nchunk * sizeof(int) : 0;
-    hipLaunchKernelGGL((k_logprob<CPW, true>), dim3(a.rows), dim3(kThreads), lds, st, a);
+    hipLaunchKernelGGL((k_logprob<CPW, NW, true>), dim3(a.rows), dim3(NW * QLM_WAVE), lds, st, a);
 }
 
 template <int CPW>
 void launch_sliced(const LpArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_logprob<CPW, false>), dim3((unsigned)(a.slices * a.rows)),
+    hipLaunchKernelGGL((k_logprob<CPW, kWaves, false>), dim3((unsigned)(a.slices * a.rows)),
                        dim3(kThreads), 0, st, a);
     hipLaunchKernelGGL((k_logprob_finish<CPW>), dim3(a.rows), dim3(kFinishWaves * QLM_WAVE), 0, st,
                        a);
@@ -509,12 +544,27 @@ void launch_sliced(const LpArgs& a, hipStream_t st) {
 
 int chunks_of(int n) { return (n + kChunk - 1) / kChunk; }
 
-// Workgroups a row: enough in all to fill the GPU, each with work for every
-// wave's loads in flight.
+// Waves of the workgroup that reads a whole row, 0: rows are sliced. Few short
+// rows need no second launch (38 x 6839 11 us sliced, 9 whole); many rows fill
+// the GPU with small workgroups. The sums' order goes by this and slices_of alone.
+int whole_waves(int rows, int n) {
+    if (rows >= 768 || chunks_of(n) <= 4 * kWaves) return kWaves;
+    return rows <= 256 && chunks_of(n) <= 4 * kMostWaves ? kMostWaves : 0;
+}
+
+// Workgroups a row otherwise: enough in all to fill the GPU, each with work for
+// every wave's loads in flight.
 int slices_of(int rows, int n) {
-    const int most = (chunks_of(n) + kWaves * kUnroll - 1) / (kWaves * kUnroll);
-    const int want = rows >= 768 ? 1 : 2048 / rows;
+    if (whole_waves(rows, n)) return 1;
+    const int most = (chunks_of(n) + kWaves * kSliceUnroll - 1) / (kWaves * kSliceUnroll);
+    const int want = 2048 / rows;
     return want < most ? want : most;
+}
+
+// Whether rows are finished by the workgroups that read them: with few waves
+// many alternatives take registers that would leave too few of them on a CU.
+bool finished(int waves, int top) {
+    return waves == kMostWaves || (waves == kWaves && top + kSlack <= 8 * kWaves);
 }
 
 size_t round16(size_t b) { return (b + 15) / 16 * 16; }
@@ -523,8 +573,8 @@ size_t round16(size_t b) { return (b + 15) / 16 * 16; }
 
 extern "C" size_t qlm_token_logprobs_workspace_bytes(int rows, int n, int top) {
     if (rows <= 0 || n <= 0 || n > kMaxVocab || top < 0) return 0;
+    if (finished(whole_waves(rows, n), top)) return 16;
     const int slices = slices_of(rows, n);
-    if (whole(slices, top)) return 16;
     return round16((size_t)rows * slices * sizeof(Part)) +
            (top ? (size_t)rows * chunks_of(n) * sizeof(int) : 0);
 }
@@ -560,14 +610,18 @@ extern "C" int qlm_token_logprobs(const float* logits, int ldl, int n, int rows,
     hipStream_t st = as_stream(stream);
     // chunks a wave holds: top + kSlack of them over the waves
     constexpr int kFinish = (kMaxTop + kSlack + kFinishWaves - 1) / kFinishWaves;
-    if (!whole(a.slices, top))
+    constexpr int kShort = (kMaxTop + kSlack + kMostWaves - 1) / kMostWaves;
+    const int waves = whole_waves(rows, n);
+    if (!finished(waves, top))
         top ? launch_sliced<kFinish>(a, st) : launch_sliced<0>(a, st);
+    else if (waves == kMostWaves)
+        top ? launch_whole<kShort, kMostWaves>(a, st) : launch_whole<0, kMostWaves>(a, st);
     else if (top == 0)
-        launch_whole<0>(a, st);
+        launch_whole<0, kWaves>(a, st);
     else if (top + kSlack <= 4 * kWaves)
-        launch_whole<4>(a, st);
+        launch_whole<4, kWaves>(a, st);
     else
-        launch_whole<8>(a, st);
+        launch_whole<8, kWaves>(a, st);
     return qlm_launch_status();
 }
 
@@ -575,5 +629,5 @@ extern "C" int qlm_token_logprobs(const float* logits, int ldl, int n, int rows,
 // otherwise loads it at the first launch of one of its kernels.
 hipError_t qlm_load_logprobs() {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(k_logprob<0, true>));
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(k_logprob<0, kWaves, true>));
 }
