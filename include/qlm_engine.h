@@ -89,6 +89,17 @@ int qlm_engine_forward_greedy(void* handle, int token, int pos, int* next);
 int qlm_engine_forward_batch(void* handle, const int* tokens, int n, int pos, int* argmax,
                              float* logits);
 
+/* No counterpart in the reference: forward_batch with the log probabilities
+ * taken on the device instead of the logits copied out, for scoring a text or
+ * showing alternatives. logprobs [n]: row i's log p(tokens[i + 1] | ..
+ * tokens[i]), NaN for the last row, which nothing follows; entropy [n]: of each
+ * row's distribution over the next token; top_ids, top_logprobs [n, top]: its
+ * `top` most likely tokens (0..QLM_TOKEN_LOGPROBS_MAX_TOP), in qlm_token_logprobs'
+ * order. Host arrays; logprobs and entropy may be NULL, and the others where
+ * top is 0. The states advance as in forward_batch. */
+int qlm_engine_score(void* handle, const int* tokens, int n, int pos, int top, float* logprobs,
+                     float* entropy, int* top_ids, float* top_logprobs);
+
 /* The CLI's turn loop (main.cpp:455-690) over token ids, with
  * SpeculativeDecoder (speculative.cpp:1-222) when draft is non-NULL: target
  * and draft are engine handles (kept alive by the caller; the draft is

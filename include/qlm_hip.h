@@ -556,10 +556,12 @@ size_t qlm_argmax_workspace_bytes(int B, int n);
  * after every other token. A row with NaN, with +inf or with nothing but -inf
  * has no distribution: its log probabilities and entropy are NaN; its top_ids
  * still follow the logits, NaN counted as -inf. fp32, sums relative to the
- * running maximum, in an order that depends only on rows and n. top <= 64 and
- * top <= n; n at most 2^21, rows at most 2^23. work: device scratch of
+ * running maximum, in an order that depends only on rows and n; a log
+ * probability below the fp32 range is -inf. top <= QLM_TOKEN_LOGPROBS_MAX_TOP
+ * and top <= n; n at most 2^21, rows at most 2^23. work: device scratch of
  * qlm_token_logprobs_workspace_bytes(rows, n, top) bytes, 16-byte aligned, no
  * initial contents needed; calls sharing it must be ordered on one stream. */
+#define QLM_TOKEN_LOGPROBS_MAX_TOP 64
 size_t qlm_token_logprobs_workspace_bytes(int rows, int n, int top);
 int qlm_token_logprobs(const float* logits, int ldl, int n, int rows, const int* ids, int n_ids,
                        float* id_logprobs, float* entropy, int top, int* top_ids,

@@ -139,6 +139,13 @@ int qlm_engine_forward_batch(void* handle, const int* tokens, int n, int pos, in
     return guarded([&] { M(handle)->forward_batch(tokens, n, pos, argmax, logits); });
 }
 
+int qlm_engine_score(void* handle, const int* tokens, int n, int pos, int top, float* logprobs,
+                     float* entropy, int* top_ids, float* top_logprobs) {
+    return guarded([&] {
+        M(handle)->score(tokens, n, pos, top, logprobs, entropy, top_ids, top_logprobs);
+    });
+}
+
 int qlm_session_create(void* target, void* draft, int draft_tokens, int eos_id, int im_end_id,
                        int kv_reuse, void** session) {
     return guarded([&] {

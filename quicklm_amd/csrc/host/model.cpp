@@ -632,7 +632,7 @@ void DecoderModel::prefill(int b, int n, bool chunked_deltanet) {
 }
 
 void DecoderModel::run_rows(int b, int first, int count, bool chunked_deltanet, int* lm_idx,
-                            float* logits_host) {
+                            float* logits_host, const ScoreRows* score) {
     if (count <= 0) return;
     const int chunk = std::min(count, kPrefillChunk);
     ensure_prefill_buffers(chunk);
@@ -699,7 +699,7 @@ void DecoderModel::run_rows(int b, int first, int count, bool chunked_deltanet, 
             math::matmul_swiglu_rmsnorm(hx, post_ln, eps, w.gate_up.view(), act);
             math::matmul_residual(act, w.down.view(), hx);
         }
-        if (!lm_idx && !logits_host) continue;
+        if (!lm_idx && !logits_host && !score) continue;
         // final norm + lm_head + greedy pick of these rows (model.cpp:246-255),
         // kLmRows rows at a time
         Tensor fn({H}, final_norm_.get<float>());
@@ -713,6 +713,7 @@ void DecoderModel::run_rows(int b, int first, int count, bool chunked_deltanet, 
                 check(qlm_argmax(lm_pf_.get<float>(), V, V, m, lm_idx + row, lm_pf_work_.get(),
                                  stream_),
                       "argmax");
+            if (score) score_logits(lm_pf_.get<float>(), *score, row, m);
             if (logits_host)
                 check(qlm_memcpy_d2h(logits_host + row * V, lm_pf_.get(),
                                      (size_t)m * V * sizeof(float), stream_),
@@ -798,6 +799,69 @@ void DecoderModel::forward_batch(const int* toks, int n, int pos, int* argmax, f
     if (argmax)
         check(qlm_memcpy_d2h(argmax, lm_pf_idx_.get(), (size_t)n * sizeof(int), stream_),
               "download");
+    check(qlm_stream_sync(stream_), "sync");
+}
+
+// Rows row .. row + rows - 1 of a score() call from their logits.
+void DecoderModel::score_logits(const float* logits, const ScoreRows& s, size_t row, int rows) {
+    const int V = cfg_.vocab_size;
+    check(qlm_token_logprobs(logits, V, V, rows, s.ids + row, 1, s.lp + row, s.entropy + row, s.top,
+                             s.top ? s.top_ids + row * s.top : nullptr,
+                             s.top ? s.top_lp + row * s.top : nullptr, score_work_.get(),
+                             score_work_.bytes(), stream_),
+          "log probabilities");
+}
+
+void DecoderModel::score(const int* toks, int n, int pos, int top, float* logprobs,
+                         float* entropy, int* top_ids, float* top_logprobs) {
+    if (n <= 0) return;
+    if (!toks) throw std::runtime_error("score: null tokens");
+    if (pos < 0 || pos + n > max_seq_)
+        throw std::runtime_error("context length exceeded max_seq_len (" + std::to_string(max_seq_) +
+                                 ")");
+    const int V = cfg_.vocab_size;
+    for (int i = 0; i < n; ++i)
+        if (toks[i] < 0 || toks[i] >= V) throw std::runtime_error("score: token id out of range");
+    const size_t work = qlm_token_logprobs_workspace_bytes(1, V, top);
+    if (top < 0 || top > std::min(V, QLM_TOKEN_LOGPROBS_MAX_TOP) || work == 0)
+        throw std::runtime_error("score: top out of range");
+    if (top > 0 && (!top_ids || !top_logprobs)) throw std::runtime_error("score: null output");
+    // one buffer: next tokens, log probabilities, entropies, alternatives
+    const size_t N = (size_t)n;
+    const size_t words = N * (3 + 2 * (size_t)top);
+    if (score_.bytes() < 4 * words) score_.alloc(4 * words);
+    size_t wb = 0;  // any number of rows up to a pass's
+    for (int m = 1; m <= std::min(n, kLmRows); ++m)
+        wb = std::max(wb, qlm_token_logprobs_workspace_bytes(m, V, top));
+    if (score_work_.bytes() < wb) score_work_.alloc(wb);
+    ScoreRows s;
+    s.ids = score_.get<int>();
+    s.lp = score_.get<float>() + N;
+    s.entropy = s.lp + N;
+    s.top = top;
+    s.top_ids = score_.get<int>() + 3 * N;
+    s.top_lp = score_.get<float>() + 3 * N + N * top;
+    std::vector<int> next(toks + 1, toks + n);
+    next.push_back(-1);
+    check(qlm_memcpy_h2d(s.ids, next.data(), N * sizeof(int), stream_), "upload");
+    if (n == 1) {  // a plain forward, as forward_batch
+        forward_greedy(toks[0], pos);
+        score_logits(logits_.get<float>(), s, 0, 1);
+    } else {
+        if (!lm_pf_) {
+            lm_pf_.alloc((size_t)kLmRows * V * sizeof(float));
+            lm_pf_work_.alloc(qlm_argmax_workspace_bytes(kLmRows, V));
+        }
+        check(qlm_memcpy_h2d(tokens_.get<int>() + pos, toks, N * sizeof(int), stream_), "upload");
+        run_rows(0, pos, n, n > kRowsMax, nullptr, nullptr, &s);
+    }
+    auto out = [&](void* dst, const void* src, size_t count) {
+        if (dst && count) check(qlm_memcpy_d2h(dst, src, 4 * count, stream_), "download");
+    };
+    out(logprobs, s.lp, N);
+    out(entropy, s.entropy, N);
+    out(top_ids, s.top_ids, N * top);
+    out(top_logprobs, s.top_lp, N * top);
     check(qlm_stream_sync(stream_), "sync");
 }
 

@@ -115,6 +115,14 @@ class DecoderModel : public GreedyModel {
     // arrays [n] / [n, vocab]) the final norm and lm_head run over every row.
     // n == 1 is a decode step, as in the reference.
     void forward_batch(const int* tokens, int n, int pos, int* argmax, float* logits);
+    // forward_batch with every row's log probabilities taken on the device
+    // instead of its logits copied out: logprobs[i] = log p(tokens[i + 1] |
+    // .. tokens[i]), NaN for the last row (host arrays [n]; each output may be
+    // null), the entropy of each row's distribution, and its `top` most likely
+    // next tokens with their log probabilities ([n, top]). The states advance
+    // as in forward_batch.
+    void score(const int* tokens, int n, int pos, int top, float* logprobs, float* entropy,
+               int* top_ids, float* top_logprobs);
     void forward_batch_greedy(const int* tokens, int n, int pos, int* argmax) override {
         forward_batch(tokens, n, pos, argmax, nullptr);
     }
@@ -163,9 +171,19 @@ class DecoderModel : public GreedyModel {
     // rows first..first+count-1 of sequence b's tokens through every layer;
     // with lm_rows, each pass's rows also get the final norm, lm_head and a
     // greedy pick (stored at lm_idx[row - first], device) and, with
-    // logits_host, their logits copied out
+    // logits_host or score, their logits
+    // copied out, or scored (`score`: device arrays of count rows)
+    struct ScoreRows {
+        int* ids;      // next tokens, -1: none
+        float* lp;     // [count]
+        float* entropy;
+        int top;
+        int* top_ids;  // [count, top]
+        float* top_lp;
+    };
     void run_rows(int b, int first, int count, bool chunked_deltanet, int* lm_idx = nullptr,
-                  float* logits_host = nullptr);
+                  float* logits_host = nullptr, const ScoreRows* score = nullptr);
+    void score_logits(const float* logits, const ScoreRows& s, size_t row, int rows);
     void ensure_prefill_buffers(int rows);
     size_t matmul_workspace(int M) const;
     void embed_current(int B);
@@ -216,6 +234,7 @@ class DecoderModel : public GreedyModel {
     std::vector<DeviceBuffer> conv_snap_, dn_snap_;
     bool have_snapshot_ = false;
     DeviceBuffer lm_pf_, lm_pf_idx_, lm_pf_work_;
+    DeviceBuffer score_, score_work_;  // outputs of score() and its kernels' workspace
 
     std::map<std::pair<int, int>, void*> graphs_;
     int run_B_ = 0, run_n_ = 0, run_steps_ = 0;

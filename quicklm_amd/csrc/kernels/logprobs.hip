@@ -35,7 +35,7 @@ constexpr int kChunk = 4 * QLM_WAVE;  // logits of a chunk: a vector of four a l
 // Chunks a wave keeps in flight: many where one workgroup reads a long row
 // (2047 x 151936 211 us with 8, 221 with 4), few where slices are many.
 constexpr int kLongUnroll = 8, kShortUnroll = 4, kSliceUnroll = 2;
-constexpr int kMaxTop = 64;
+constexpr int kMaxTop = QLM_TOKEN_LOGPROBS_MAX_TOP;
 constexpr int kSlack = 8;             // chunks beyond k that a threshold may name
 constexpr int kCand = 512;            // logits that are ranked by counting
 constexpr int kMaxVocab = 1 << 21;    // chunk maxima of a row fit 32 KB of LDS

@@ -40,6 +40,7 @@ def lib() -> C.CDLL:
         L.qlm_engine_restore.argtypes = [_vp]
         L.qlm_engine_forward_greedy.argtypes = [_vp, _i, _i, C.POINTER(_i)]
         L.qlm_engine_forward_batch.argtypes = [_vp, _vp, _i, _i, _vp, _vp]
+        L.qlm_engine_score.argtypes = [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]
         L.qlm_session_create.argtypes = [_vp, _vp, _i, _i, _i, _i, C.POINTER(_vp)]
         L.qlm_session_free.argtypes = [_vp]
         L.qlm_session_reset.argtypes = [_vp]
@@ -159,6 +160,18 @@ class Engine:
                                               None if am is None else am.ctypes.data,
                                               None if lg is None else lg.ctypes.data))
         return am, lg
+
+    def score(self, tokens, pos: int = 0, top: int = 0):
+        """tokens at positions pos.. through every layer at once; returns
+        (logprobs [n]: log p of the token after each, NaN for the last one;
+        entropy [n]; top_ids [n, top]; top_logprobs [n, top])."""
+        t = np.ascontiguousarray(tokens, np.int32).ravel()
+        lp, ent = np.empty(t.size, np.float32), np.empty(t.size, np.float32)
+        ti, tl = np.empty((t.size, max(top, 0)), np.int32), np.empty((t.size, max(top, 0)),
+                                                                     np.float32)
+        _check(lib().qlm_engine_score(self.h, t.ctypes.data, t.size, pos, top, lp.ctypes.data,
+                                      ent.ctypes.data, ti.ctypes.data, tl.ctypes.data))
+        return lp, ent, ti, tl
 
     def kernels_per_step(self) -> int:
         return int(lib().qlm_engine_kernels_per_step(self.h))

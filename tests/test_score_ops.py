@@ -105,3 +105,11 @@ def test_token_logprobs_workspace():
         assert 0 < L.qlm_token_logprobs_workspace_bytes(rows, n, 0) <= b
     for bad in [(0, 5, 1), (1, 0, 1), (1, 5, -1), (1, (1 << 21) + 1, 1), (-1, 5, 1)]:
         assert L.qlm_token_logprobs_workspace_bytes(*bad) == 0
+
+
+def test_engine_score_refuses_a_null_handle():
+    from quicklm_amd import engine
+
+    L = engine.lib()
+    assert L.qlm_engine_score(None, None, 0, 0, 0, None, None, None, None) == 1
+    assert b"null engine handle" in L.qlm_engine_last_error()
