@@ -20,6 +20,8 @@
 #include <stdlib.h>
 #endif
 
+#include <algorithm>
+
 #include "common.hpp"
 
 namespace {
@@ -96,66 +98,118 @@ __device__ __forceinline__ void put(float* dst, f32x4u v, int left) {
         if (i < left) dst[i] = EPI == EPI_RESID ? dst[i] + v[i] : v[i];
 }
 
+// Buffer descriptor of a uniform base: a load then takes a lane's 32-bit
+// offset and a scalar one, no vector arithmetic on addresses. Reads past
+// `bytes` return 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, unsigned bytes) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0, (int)bytes, 0x00027000);
+}
+
+// 16 bytes a lane straight into LDS, lane after lane from `to` (uniform).
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, char* to, int lane_off,
+                                            int uniform_off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16,
+                                             lane_off, uniform_off, 0, 0);
+}
+
 // MT 16-row tiles of x against NT weight tiles (SwiGLU: NT gate tiles and
-// their up tiles) a workgroup. NW waves take the 64-column blocks of K in
-// turn, straight from memory into registers, U blocks of a wave in flight, and
-// add their sums in LDS (integers: in any order).
-template <int EPI, int MT, int NT, int NW, int U, int P>
+// their up tiles) a workgroup. NW waves take units of two 64-column blocks of K
+// in turn, each through a ring of D units of its own in LDS, so nothing waits
+// for another wave before the end, when the sums are added in LDS (integers:
+// in any order). Loads go straight to LDS in whole cache lines: a lane's 16
+// bytes of a row of x straight into the matrix instruction's registers put
+// neighbouring lanes on different rows, which the L1 serves four times slower
+// (64 x 2560 x 9728 24 us).
+template <int EPI, int MT, int NT, int NW, int D>
 __global__ __launch_bounds__(NW* QLM_WAVE) void k_a8_stream(A8Args a) {
     constexpr int H = EPI == EPI_SWIGLU ? 2 : 1, F = H * NT;
-    __shared__ int sums[F * MT * 256];
+    constexpr int UNIT = (MT + F) * 2048, L = 2 * (MT + F);  // a unit's bytes and loads
+    static_assert(F * MT * 1024 <= NW * D * UNIT, "the sums take the rings' place");
+    __shared__ __attribute__((aligned(1024))) char smem[NW * D * UNIT];
     const int lane = threadIdx.x & (QLM_WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
     const int nblk = a.K >> 6, t0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
-    const int8_t* xr[MT];
+    const int nunit = (nblk + 1) >> 1, units = (nunit - wave + NW - 1) / NW;  // of this wave
+
+    // x: 8 rows x 128 columns a load, row r's 16-byte piece p at
+    // r * 128 + (p ^ (r & 7)) * 16 of its 8-row group. Rows past the last are
+    // copies of it, and so are pieces past K (of those before), never multiplied.
+    const int rows = min(a.M - m0, 16 * MT);
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x + (size_t)m0 * a.ldx,
+                                                (unsigned)(rows - 1) * (unsigned)a.ldx + a.K);
+    const int piece = (lane & 7) ^ (lane >> 3);
+    const int past = piece >= 4 ? 64 : 0;
+    int xoff[2 * MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-        xr[t] = a.x + (size_t)min(m0 + 16 * t + (lane & 15), a.M - 1) * a.ldx + (lane >> 4) * 16;
-    const v4i* wq[F];
+    for (int g = 0; g < 2 * MT; ++g)
+        xoff[g] = min(8 * g + (lane >> 3), rows - 1) * (int)a.ldx + piece * 16;
+    __amdgpu_buffer_rsrc_t rw[F];
 #pragma unroll
     for (int f = 0; f < F; ++f)
-        wq[f] = reinterpret_cast<const v4i*>(a.q) +
-                ((size_t)(f / NT) * a.tiles + min(t0 + f % NT, a.tiles - 1)) * nblk * QLM_WAVE +
-                lane;
+        rw[f] = make_rsrc(a.q + ((size_t)(f / NT) * a.tiles + min(t0 + f % NT, a.tiles - 1)) *
+                                    nblk * 1024,
+                          (unsigned)nblk * 1024);
+    char* ring = smem + wave * (D * UNIT);
+    auto fetch = [&](int i) {  // the wave's unit i
+        const int u = wave + i * NW;
+        char* to = ring + (i % D) * UNIT;
+        const int back = 2 * u + 1 >= nblk ? past : 0;
+        const int b1 = min(2 * u + 1, nblk - 1);
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            load_to_lds(rw[f], to + f * 2048, lane * 16, u * 2048);
+            load_to_lds(rw[f], to + f * 2048 + 1024, lane * 16, b1 * 1024);
+        }
+#pragma unroll
+        for (int g = 0; g < 2 * MT; ++g)
+            load_to_lds(rx, to + F * 2048 + g * 1024, xoff[g] - back, u * 128);
+    };
     v4i acc[F][MT];
 #pragma unroll
     for (int f = 0; f < F; ++f)
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[f][t] = v4i{0, 0, 0, 0};
-    v4i w[U][F], x[U][MT];
-    auto load = [&](int u, int b) {  // blocks past the last are copies of it
-        b = min(b, nblk - 1);
 #pragma unroll
-        for (int f = 0; f < F; ++f) w[u][f] = wq[f][(size_t)b * QLM_WAVE];
+    for (int i = 0; i < D; ++i)
+        if (i < units) fetch(i);
+    const int xl = F * 2048 + ((lane & 15) >> 3) * 1024 + (lane & 7) * 128 +
+                   ((lane >> 4) ^ (lane & 7)) * 16;
+#pragma unroll 1
+    for (int i = 0; i < units; ++i) {
+        if (units - i >= D)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L * (D - 1)) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const char* at = ring + (i % D) * UNIT;
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-            x[u][t] = *reinterpret_cast<const v4i*>(xr[t] + (size_t)b * 64);
-    };
-    auto multiply = [&](int u, int b) {
-        if (b >= nblk) return;
+        for (int h = 0; h < 2; ++h) {
+            if (h && 2 * (wave + i * NW) + 1 >= nblk) break;
+            v4i w[F], x[MT];
 #pragma unroll
-        for (int f = 0; f < F; ++f)
+            for (int f = 0; f < F; ++f)
+                w[f] = *reinterpret_cast<const v4i*>(at + f * 2048 + h * 1024 + lane * 16);
 #pragma unroll
             for (int t = 0; t < MT; ++t)
-                acc[f][t] =
-                    __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][f], x[u][t], acc[f][t], 0, 0, 0);
-    };
-    // slot u's block, b0 the wave's first of this round
-    auto at = [&](int b0, int u) { return b0 + u / P * (NW * P) + u % P; };
-    constexpr int ROUND = U * NW;
+                x[t] = *reinterpret_cast<const v4i*>(at + (xl ^ (h << 6)) + t * 2048);
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(u, at(wave * P, u));
+            for (int f = 0; f < F; ++f)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    acc[f][t] =
+                        __builtin_amdgcn_mfma_i32_16x16x64_i8(w[f], x[t], acc[f][t], 0, 0, 0);
+        }
+        // the unit is read: its place takes the unit after the ring's last
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + D < units) fetch(i + D);
+    }
+    int* sums = reinterpret_cast<int*>(smem);
+    __syncthreads();  // every ring is read
     for (int i = threadIdx.x; i < F * MT * 256; i += NW * QLM_WAVE) sums[i] = 0;
     __syncthreads();
-    int b = wave * P;
-    for (; b + ROUND < nblk; b += ROUND)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            multiply(u, at(b, u));
-            load(u, at(b + ROUND, u));
-        }
-#pragma unroll
-    for (int u = 0; u < U; ++u) multiply(u, at(b, u));
     // lane l holds outputs n = 4 (l >> 4) + i of row m = l & 15
 #pragma unroll
     for (int f = 0; f < F; ++f)
@@ -181,24 +235,6 @@ __global__ __launch_bounds__(NW* QLM_WAVE) void k_a8_stream(A8Args a) {
                      a.N - n);
         }
     }
-}
-
-// Buffer descriptor of a uniform base: a load then takes a lane's 32-bit
-// offset and a scalar one, no vector arithmetic on addresses. Reads past
-// `bytes` return 0.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, unsigned bytes) {
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc(
-        reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0, (int)bytes, 0x00027000);
-}
-
-// 16 bytes a lane straight into LDS, lane after lane from `to` (uniform).
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, char* to, int lane_off,
-                                            int uniform_off) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16,
-                                             lane_off, uniform_off, 0, 0);
 }
 
 // acc += w . x. IN_A: the sums in accumulator registers, tied by hand.
@@ -412,30 +448,38 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
         s0[j] = load_scales(a.sw, nl + 16 * j, a.N);
         if constexpr (SW) s1[j] = load_scales(a.sw + a.N, nl + 16 * j, a.N);
     }
-    // inside the matrix, and with every block of a full launch but the last
-    // ones, nothing of a store is conditional
+    // inside the matrix nothing of a load or store is conditional; what is added
+    // to is requested half the rows at a time (row by row each waits in turn:
+    // 2862 x 3428 x 2048 47 us)
     const bool inside = m0 + AF * 16 <= a.M && (t0 + WN * OF) * 16 <= a.N;
-    float* y = a.y + (size_t)ml * a.ldy + nl;
+    constexpr int G = FM / 2;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        f32x4u old[OF];
+    for (int g = 0; g < FM; g += G) {
+        f32x4u old[G][OF];
+        float* y = a.y + (size_t)(ml + 16 * g) * a.ldy + nl;
         if constexpr (EPI == EPI_RESID) {
             if (inside) {
 #pragma unroll
-                for (int j = 0; j < OF; ++j)
-                    old[j] = *reinterpret_cast<const f32x4u*>(y + 16 * j);
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int j = 0; j < OF; ++j)
+                        old[i][j] =
+                            *reinterpret_cast<const f32x4u*>(y + 16 * i * a.ldy + 16 * j);
             }
         }
 #pragma unroll
-        for (int j = 0; j < OF; ++j) {
-            const f32x4u v = scaled<EPI>(acc[i][j], acc[i][SW ? j + OF : j], sx[i], s0[j],
-                                         SW ? s1[j] : s0[j]);
-            if (inside)
-                *reinterpret_cast<f32x4u*>(y + 16 * j) = EPI == EPI_RESID ? old[j] + v : v;
-            else if (ml + 16 * i < a.M)
-                put<EPI>(y + 16 * j, v, a.N - (nl + 16 * j));
+        for (int i = 0; i < G; ++i) {
+#pragma unroll
+            for (int j = 0; j < OF; ++j) {
+                const f32x4u v = scaled<EPI>(acc[g + i][j], acc[g + i][SW ? j + OF : j], sx[g + i],
+                                             s0[j], SW ? s1[j] : s0[j]);
+                if (inside)
+                    *reinterpret_cast<f32x4u*>(y + 16 * j) = EPI == EPI_RESID ? old[i][j] + v : v;
+                else if (ml + 16 * (g + i) < a.M)
+                    put<EPI>(y + 16 * j, v, a.N - (nl + 16 * j));
+            }
+            y += 16 * a.ldy;
         }
-        y += 16 * a.ldy;
     }
 }
 
@@ -473,23 +517,48 @@ __global__ __launch_bounds__(kJoinThreads) void k_a8_join(A8Args a, int slices) 
     put<EPI>(a.y + (size_t)m * a.ldy + n, scaled<EPI>(s[0], s[1], a.sx[m], w0, w1), a.N - n);
 }
 
-// The streaming form of a call: 16-row tiles of x and weight tiles a
-// workgroup. More weight tiles a workgroup read x fewer times, where enough
-// workgroups are left.
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// A streaming form: 16-row tiles of x and weight tiles a workgroup, its waves
+// and the units of their rings; its time by the plan's reckoning.
 struct StreamShape {
-    int mt, nt;
-    bool longk;
+    int mt, nt, waves, depth;
+    double us;
 };
-StreamShape stream_shape(int M, int tiles, int kblk, int halves) {
-    const bool longk = kblk > 64;
-    if (M <= 16) return {1, M > 1 && tiles * halves >= 4096 ? 2 : 1, longk};
-    if (M <= 32) return {2, tiles * halves >= 1024 ? 4 : 1, longk};
-    const int groups = (M + 63) / 64;
-    if (M <= 48 || (M > 64 && (M + 47) / 48 * 48 < groups * 64)) return {3, 2, longk};
-    if (M > 64 && M <= 80) return {5, 2, longk};
-    return {4, tiles * halves * groups >= 1024 ? 4 : 1, longk};
+
+// The form of a call. A workgroup reads all of its rows of x and weights, and a
+// CU takes in 62 KB a us of them, whoever shares it; beyond one workgroup a CU,
+// those whose rings fill the LDS also wait for each other. Measured on an
+// MI355X with operands cold (2560 x 2560 weights, us): 64 rows 5.9 in groups of
+// 16, 5.5 in one of 64; 128 rows 7.2 in groups of 64 x 2 tiles, 9.1 of 16; 400
+// rows 11.4 in groups of 48 x 2 tiles, 13.8 of 64 x 2, 20 of 16.
+StreamShape stream_shape(int M, int tiles, int K, int halves) {
+    // Long rows of tiles: workgroups that share a CU (16 x 2 x 9728 x 2560:
+    // 11.9 us with 4 waves, 14.6 with 8), and with thousands of tiles two of
+    // them a workgroup, to read x half as often (16 x 151936 x 2560: 75, 80).
+    const bool many = tiles * halves > 512, most = M > 1 && tiles * halves >= 4096;
+    StreamShape best{0, 0, 0, 0, 1e30};
+    auto offer = [&](int mt, int nt, int waves, int depth) {
+        const double groups = (double)ceil_div(tiles, nt) * ceil_div(M, 16 * mt);
+        const double kb = K * 16.0 * (mt + nt * halves) / 1024;
+        const bool shares = waves * depth * (mt + nt * halves) * 2 <= 40;  // KB of LDS
+        const double rounds = groups <= 256 ? 1 : groups / 256 + (shares ? 0 : 0.4);
+        // (a workgroup's own start and end, and its outputs' way to memory)
+        const double us = 2.6 + rounds * kb / (halves > 1 ? 48 : 62) + 1.2 * (rounds - 1) +
+                          2e-7 * 4 * M * tiles * 16;
+        if (us < best.us) best = {mt, nt, waves, depth, us};
+    };
+    if (most && M <= 32) {
+        M <= 16 ? offer(1, 2, 4, 2) : offer(2, 2, 2, 2);
+        return best;
+    }
+    offer(1, 1, many ? 4 : 8, 2);
+    if (M > 16) offer(2, 1, many ? 4 : 8, 2);
+    if (M > 32) offer(3, 1, 4, many ? 1 : 2);
+    if (M > 48) offer(4, 1, many ? 2 : 4, 2);
+    if (M > 64) offer(3, 2, 4, 1);
+    if (M > 64 && halves == 1) offer(4, 2, 8, 1);
+    return best;
 }
 
 // How a call runs. Times in us, measured on an MI355X with operands cold in
@@ -525,21 +594,14 @@ Plan plan_of(int M, int N, int K, int epilogue) {
     auto offer = [&](double us, Plan p) {
         if (us < least) least = us, best = p;
     };
-    // Few rows: the L2 feeds a CU of the streaming form with about 36 KB a us
-    // of x and weights, and a workgroup reads all of both for its tiles.
-    {
-        const StreamShape f = stream_shape(M, tiles, kblk, halves);
-        const long long groups = (long long)ceil_div(tiles, f.nt) * ceil_div(M, 16 * f.mt);
-        const double kb = K * 16.0 * (f.mt + f.nt * halves) / 1024;
-        offer(2.5 + (groups <= 256 ? 1.0 : groups / 256.0) * kb / 36, best);
-    }
+    offer(stream_shape(M, tiles, K, halves).us, best);
     if (M > kSliceMinRows) {
         for (int s = 1; s <= kSliceMost; s *= 2) {
             if (s > 1 && (gx1 * gy1 * s > kSliceTiles || kblk < kSliceMinBlocks * s)) break;
             // the slices' sums are written and read back, 4 MB a us
             const double join = s == 1 ? 0 : 3 + 8e-6 * s * M * halves * N / 4;
             const int bs = s == 1 ? kblk : ceil_div(ceil_div(kblk, s), 2) * 2;
-            offer(cost128(gx1 * gy1 * s, bs) + join, Plan{K_T128, gx1, ceil_div(kblk, bs), bs});
+            offer(cost128(gx1 * gy1 * s, bs) + join + 1e-7 * 4 * M * N, Plan{K_T128, gx1, ceil_div(kblk, bs), bs});
         }
     }
     if (M > 128) {
@@ -591,9 +653,9 @@ void launch_tile(A8Args a, const Plan& p, int first, int last, hipStream_t st) {
                        dim3(kJoinThreads), 0, st, a, p.slices);
 }
 
-template <int EPI, int MT, int NT, int NW, int U, int P>
+template <int EPI, int MT, int NT, int NW, int D>
 void launch_stream(const A8Args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_a8_stream<EPI, MT, NT, NW, U, P>),
+    hipLaunchKernelGGL((k_a8_stream<EPI, MT, NT, NW, D>),
                        dim3(ceil_div(a.tiles, NT), ceil_div(a.M, 16 * MT)), dim3(NW * QLM_WAVE), 0,
                        st, a);
 }
@@ -614,24 +676,29 @@ void launch(const A8Args& a, const Plan& p, hipStream_t st) {
 #ifdef A8_TUNE
     if (getenv("A8M")) {
         const int mt = atoi(getenv("A8M")), nt = atoi(getenv("A8N")), nw = atoi(getenv("A8W")),
-                  u = atoi(getenv("A8U")), pz = atoi(getenv("A8P"));
-#define TRY(m, n, w, uu, pp)                                  \
-    if (mt == m && nt == n && nw == w && u == uu && pz == pp) \
-        return launch_stream<EPI, m, n, w, uu, pp>(a, st);
+                  dd = atoi(getenv("A8D"));
+#define TRY(m, n, w, d)                          \
+    if (mt == m && nt == n && nw == w && dd == d) \
+        return launch_stream<EPI, m, n, w, d>(a, st);
 #include "tune_shapes.inc"
     }
 #endif
-    const StreamShape f = stream_shape(a.M, a.tiles, a.K / 64, EPI == EPI_SWIGLU ? 2 : 1);
-    if (f.mt == 1 && f.nt == 2) return launch_stream<EPI, 1, 2, 8, 5, 1>(a, st);
-    if (f.mt == 1 && f.longk) return launch_stream<EPI, 1, 1, 16, 5, 1>(a, st);
-    if (f.mt == 1) return launch_stream<EPI, 1, 1, 5, 4, 2>(a, st);
-    if (f.mt == 2 && f.nt == 4) return launch_stream<EPI, 2, 4, 8, 2, 2>(a, st);
-    if (f.mt == 2 && f.longk) return launch_stream<EPI, 2, 1, 8, 5, 1>(a, st);
-    if (f.mt == 2) return launch_stream<EPI, 2, 1, 5, 4, 2>(a, st);
-    if (f.mt == 3) return launch_stream<EPI, 3, 2, 8, 2, 2>(a, st);
-    if (f.mt == 5) return launch_stream<EPI, 5, 2, 8, 2, 1>(a, st);
-    if (f.nt == 4) return launch_stream<EPI, 4, 4, 8, 2, 2>(a, st);
-    launch_stream<EPI, 4, 1, 8, 2, 2>(a, st);
+    const StreamShape f = stream_shape(a.M, a.tiles, a.K, EPI == EPI_SWIGLU ? 2 : 1);
+    if (f.mt == 1 && f.nt == 2) return launch_stream<EPI, 1, 2, 4, 2>(a, st);
+    if (f.mt == 1 && f.waves == 8) return launch_stream<EPI, 1, 1, 8, 2>(a, st);
+    if (f.mt == 1) return launch_stream<EPI, 1, 1, 4, 2>(a, st);
+    if (f.mt == 2 && f.nt == 2) return launch_stream<EPI, 2, 2, 2, 2>(a, st);
+    if (f.mt == 2 && f.waves == 8) return launch_stream<EPI, 2, 1, 8, 2>(a, st);
+    if (f.mt == 2) return launch_stream<EPI, 2, 1, 4, 2>(a, st);
+    if (f.mt == 3 && f.nt == 2) return launch_stream<EPI, 3, 2, 4, 1>(a, st);
+    if (f.mt == 3 && f.depth == 2) return launch_stream<EPI, 3, 1, 4, 2>(a, st);
+    if (f.mt == 3) return launch_stream<EPI, 3, 1, 4, 1>(a, st);
+    if (f.nt == 2) {  // (not SwiGLU: see stream_shape)
+        if constexpr (EPI != EPI_SWIGLU) launch_stream<EPI, 4, 2, 8, 1>(a, st);
+        return;
+    }
+    if (f.waves == 4) return launch_stream<EPI, 4, 1, 4, 2>(a, st);
+    launch_stream<EPI, 4, 1, 2, 2>(a, st);
 }
 
 }  // namespace
