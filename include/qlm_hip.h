@@ -313,7 +313,7 @@ int qlm_matmul_i8_t_whole_config(const float* x, int ldx, const float* norm_w, f
  * sums are exact in int32 and rounded to fp32 once, so the result differs
  * from the exact one by a few fp32 roundings only, in every form. epilogue
  * 0: y = result; 1: y += result; 2: SwiGLU, y = silu(gate) * up (N outputs).
- * Any M >= 1 and N, K a multiple of 64 below 2^17; x and q_tiles 16-byte
+ * M below 2^20, N below 2^23, K a multiple of 64 below 2^17; x and q_tiles 16-byte
  * aligned, ldx a multiple of 16 below 2^23; y of any stride and alignment,
  * its columns past N left as they are. work: device scratch of
  * qlm_matmul_a8_workspace_bytes(M, N, K, epilogue) bytes (0: may be NULL),
@@ -558,7 +558,7 @@ size_t qlm_argmax_workspace_bytes(int B, int n);
  * still follow the logits, NaN counted as -inf. fp32, sums relative to the
  * running maximum, in an order that depends only on rows and n; a log
  * probability below the fp32 range is -inf. top <= QLM_TOKEN_LOGPROBS_MAX_TOP
- * and top <= n; n at most 2^21, rows at most 2^23. work: device scratch of
+ * and top <= n; n at most 2^21, rows at most 2^22. work: device scratch of
  * qlm_token_logprobs_workspace_bytes(rows, n, top) bytes, 16-byte aligned, no
  * initial contents needed; calls sharing it must be ordered on one stream. */
 #define QLM_TOKEN_LOGPROBS_MAX_TOP 64

@@ -11,14 +11,17 @@
 // of x puts them that way. The weights are the first operand: a lane of the
 // result then holds four neighbouring outputs of one row of x.
 //
-// Few rows (M <= 64), k_a8_stream: bound by the stream of the weights; the
-// waves of a workgroup split K over one 16-row weight tile.
-// More rows, k_a8_tile: both operands staged through LDS.
-
-#ifdef A8_TUNE
-#include <stdio.h>
-#include <stdlib.h>
-#endif
+// Three forms, taken by what each is reckoned to cost (plan_of):
+//   k_a8_stream  few workgroups' worth of tiles: bound by the way of the bytes
+//                to the CUs; every wave streams its share of K by itself.
+//   k_a8_tile    as 128 x 128 tiles, two workgroups a CU, K in slices if they
+//                are few: bound by the bytes' way too.
+//   k_a8_tile    as 256 x 256 tiles: bound by the matrix cores.
+// Measured on an MI355X, operands cold in the caches, us (and the larger of
+// the bytes' time at 4.75 TB/s and the products' at 2134 TOP/s): 1 x 9728 x
+// 2560 SwiGLU 11.5 (10.5), 16 x 2560 x 9728 9.1 (5.4), 1000 x 2560 x 2560 18.7
+// (6.1), 2048 x 9728 x 2560 SwiGLU 107 to 116 from card to card (96), 4096 x
+// 12288 x 4096 178 to 190 (193).
 
 #include <algorithm>
 
@@ -237,13 +240,8 @@ __global__ __launch_bounds__(NW* QLM_WAVE) void k_a8_stream(A8Args a) {
     }
 }
 
-// acc += w . x. IN_A: the sums in accumulator registers, tied by hand.
-template <bool IN_A>
 __device__ __forceinline__ void mma(v4i& acc, v4i w, v4i x) {
-    if constexpr (IN_A)
-        asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
-    else
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, acc, 0, 0, 0);
 }
 
 // BM = 16 WM FM rows of x and BN = 16 WN FN weight rows a workgroup, WM x WN
@@ -254,8 +252,8 @@ __device__ __forceinline__ void mma(v4i& acc, v4i w, v4i x) {
 // loads of 16 rows x 64 columns, the fragments themselves, took half as long
 // again. Row r's 16-byte piece p lies at r * 128 + (p ^ (r & 7)) * 16 of its
 // 8-row group, so that the 8 lanes of an LDS access meet every bank once.
-template <int EPI, bool SW, int WM, int WN, int FM, int FN, int WD, int XU, int OCC>
-__global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
+template <int EPI, bool SW, int WM, int WN, int FM, int FN, int WD, int XU>
+__global__ __launch_bounds__(WM* WN* QLM_WAVE, 2) void k_a8_tile(A8Args a) {
     constexpr int NW = WM * WN, BF = WN * FN, AF = WM * FM;  // fragments of a block
     constexpr int OF = SW ? FN / 2 : FN;  // output fragments of a wave
     constexpr int LX = AF / NW, LW = BF / NW, L = LX + LW;  // a wave's loads a block
@@ -269,7 +267,7 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
     // blocks, in bands of BAND row blocks (column by column inside a band).
     constexpr int BAND = 4;
     int t = (int)(blockIdx.x & 7) * a.per_xcd + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= a.per_xcd || t >= a.blocks) return;
+    if (t >= a.blocks) return;
     const int slice = t / (a.gx * a.gy);
     t -= slice * a.gx * a.gy;
     const int band = t / (BAND * a.gx);
@@ -348,7 +346,6 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
     // b + WD and half a unit of x are requested after barrier b, spread over a
     // block's length: a burst of them holds up the products behind it.
     constexpr int HN = FN / 2;
-    constexpr bool IN_A = FM * FN > 32;
     constexpr int XH = 2 * XU - 1;  // iteration b requests x's half unit b + XH
     // iterations whose requests may be under way when block b + 1 is needed
     constexpr int AHEAD = (WD - 1 < 2 * XU - 3 ? WD - 1 : 2 * XU - 3) - 1;
@@ -379,8 +376,6 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
     int xs = 0;               // slot of block b's unit of x
     int xf = (XH >> 1) % XU;  // slot of half unit b + XH
     int ws0 = WD - 1, xf0 = ((XH - 1) >> 1) % XU;  // those that block b - 1 requests into
-    // the zeros are written before the first product reads them
-    if constexpr (IN_A) asm volatile("s_nop 7" ::: "memory");
 #pragma unroll 1
     for (int b = 0; b < nblk; ++b) {
         auto request = [&](int l, int b0) {
@@ -393,7 +388,7 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
-            for (int j = 0; j < HN; ++j) mma<IN_A>(acc[i][j], w[j], x[i]);
+            for (int j = 0; j < HN; ++j) mma(acc[i][j], w[j], x[i]);
             if (i < HN) w[HN + i] = read_w(wa, HN + i);
 #pragma unroll
             for (int l = L1 + i * (L - L1) / FM; l < L1 + (i + 1) * (L - L1) / FM; ++l)
@@ -413,7 +408,7 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
-            for (int j = 0; j < HN; ++j) mma<IN_A>(acc[i][HN + j], w[HN + j], x[i]);
+            for (int j = 0; j < HN; ++j) mma(acc[i][HN + j], w[HN + j], x[i]);
             if (2 * i < HN) w[2 * i] = read_w(wa, 2 * i);
             if (2 * i + 1 < HN) w[2 * i + 1] = read_w(wa, 2 * i + 1);
             x[i] = read_x(xa, i);
@@ -422,8 +417,7 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, OCC) void k_a8_tile(A8Args a) {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // nothing lands after the end, and the last products are written
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands after the end
     const int ml = m0 + wm * FM * 16 + (lane & 15);
     const int nl = (t0 + wn * OF) * 16 + 4 * (lane >> 4);
     if constexpr (EPI == OUT_PART) {
@@ -570,18 +564,25 @@ struct Plan {
     int slices, bslice;  // of K, and 64-column blocks in each (K_T128 only)
 };
 
+constexpr int kMaxRows = 1 << 20, kMaxOutputs = 1 << 23;  // tile numbers fit 32 bits
 constexpr int kSliceMinRows = 32, kSliceMinBlocks = 8, kSliceMost = 8, kSliceTiles = 256;
 
 // 128 x 128 tiles, two workgroups a CU: alone on its CU a workgroup takes
-// 0.28 a block, beside another 0.5 to 0.6.
+// 0.275 a block, beside another twice as long; after the first 512 tiles the
+// CUs are no longer in step. (Its 16 KB a block come in at 60 KB a us, as in
+// the streaming form. Eight waves a workgroup, four on every other block, gain
+// a tenth with the GPU half empty and lose a fifth with it full; deeper rings
+// and a wave that touches the lines ahead gain nothing.)
 double cost128(int n, int kblk) {
-    if (n <= 512) return 5 + (n <= 256 ? 0.28 : 0.5) * kblk;
-    return ceil_div(n, 512) * (6 + 0.6 * kblk);
+    const int full = n / 512, rest = n % 512;
+    const double round = 9.5 + 0.57 * kblk;
+    if (rest <= 256) return full * round + (rest ? 6.5 + 0.275 * kblk : 0);
+    return full * round + (full ? rest / 512.0 * round : rest <= 384 ? 9 + 0.5 * kblk : round);
 }
-// 256 x 256 tiles, one workgroup a CU: 0.58 a block while the other CUs idle,
-// 0.7 with all of them.
+// 256 x 256 tiles, one workgroup a CU: 0.51 a block while the other CUs idle,
+// 0.64 with all of them.
 double cost256(int n, int kblk) {
-    return n < 192 ? 14 + 0.58 * kblk : ceil_div(n, 256) * (10 + 0.7 * kblk);
+    return ceil_div(n, 256) * (16.5 + (0.5 + 0.14 * std::min(1.0, n / 256.0)) * kblk);
 }
 
 Plan plan_of(int M, int N, int K, int epilogue) {
@@ -598,10 +599,10 @@ Plan plan_of(int M, int N, int K, int epilogue) {
     if (M > kSliceMinRows) {
         for (int s = 1; s <= kSliceMost; s *= 2) {
             if (s > 1 && (gx1 * gy1 * s > kSliceTiles || kblk < kSliceMinBlocks * s)) break;
-            // the slices' sums are written and read back, 4 MB a us
-            const double join = s == 1 ? 0 : 3 + 8e-6 * s * M * halves * N / 4;
+            // the slices' sums are written and read back, 3.3 MB a us
+            const double join = s == 1 ? 0 : 2.5 + 1.2e-6 * s * M * halves * N;
             const int bs = s == 1 ? kblk : ceil_div(ceil_div(kblk, s), 2) * 2;
-            offer(cost128(gx1 * gy1 * s, bs) + join + 1e-7 * 4 * M * N, Plan{K_T128, gx1, ceil_div(kblk, bs), bs});
+            offer(cost128(gx1 * gy1 * s, bs) + join, Plan{K_T128, gx1, ceil_div(kblk, bs), bs});
         }
     }
     if (M > 128) {
@@ -612,15 +613,6 @@ Plan plan_of(int M, int N, int K, int epilogue) {
             offer(cost256(full * gy2, kblk) + cost128((gx1 - 2 * full) * gy1, kblk),
                   Plan{K_T256, full, 1, kblk});
     }
-#ifdef A8_TUNE
-    if (getenv("A8K")) {
-        best = Plan{atoi(getenv("A8K")), 1 << 20, 1, kblk};
-        if (getenv("A8S") && atoi(getenv("A8S")) > 1) {
-            best.bslice = ceil_div(ceil_div(kblk, atoi(getenv("A8S"))), 2) * 2;
-            best.slices = ceil_div(kblk, best.bslice);
-        }
-    }
-#endif
     return best;
 }
 
@@ -629,28 +621,29 @@ size_t part_bytes(const Plan& p, int M, int N, int epilogue) {
     return (size_t)p.slices * M * (epilogue == EPI_SWIGLU ? 2 : 1) * (ceil_div(N, 16) * 16) * 4;
 }
 
-// Column blocks [first, last) of the tile width.
-template <int EPI, int WM, int WN, int FM, int FN, int WD, int XU, int OCC>
+// Column blocks [first, last) of tiles of 256 x 256 (BIG) or 128 x 128.
+template <int EPI, bool BIG>
 void launch_tile(A8Args a, const Plan& p, int first, int last, hipStream_t st) {
     constexpr bool SW = EPI == EPI_SWIGLU;
-    constexpr int OT = WN * (SW ? FN / 2 : FN);
+    constexpr int SIDE = BIG ? 256 : 128, OT = SIDE / 16 / (SW ? 2 : 1);
     a.t_first = first * OT;
-    a.gx = min(last, ceil_div(a.tiles, OT)) - first;
-    a.gy = ceil_div(a.M, 16 * WM * FM);
+    a.gx = std::min(last, ceil_div(a.tiles, OT)) - first;
+    a.gy = ceil_div(a.M, SIDE);
     a.blocks = a.gx * a.gy * p.slices;
     a.per_xcd = ceil_div(a.blocks, 8);
     a.bslice = p.bslice;
-    const dim3 grid(8 * a.per_xcd), threads(WM * WN * QLM_WAVE);
-    if (p.slices == 1) {
-        hipLaunchKernelGGL((k_a8_tile<EPI, SW, WM, WN, FM, FN, WD, XU, OCC>), grid, threads, 0, st,
-                           a);
-        return;
+    const dim3 grid(8 * a.per_xcd), threads((BIG ? 8 : 4) * QLM_WAVE);
+    if constexpr (BIG) {
+        hipLaunchKernelGGL((k_a8_tile<EPI, SW, 2, 4, 8, 4, 4, 3>), grid, threads, 0, st, a);
+    } else if (p.slices == 1) {
+        hipLaunchKernelGGL((k_a8_tile<EPI, SW, 2, 2, 4, 4, 4, 3>), grid, threads, 0, st, a);
+    } else {
+        hipLaunchKernelGGL((k_a8_tile<OUT_PART, SW, 2, 2, 4, 4, 4, 3>), grid, threads, 0, st, a);
+        const long long groups = (long long)a.M * 4 * a.tiles;
+        hipLaunchKernelGGL((k_a8_join<EPI>),
+                           dim3((unsigned)((groups + kJoinThreads - 1) / kJoinThreads)),
+                           dim3(kJoinThreads), 0, st, a, p.slices);
     }
-    hipLaunchKernelGGL((k_a8_tile<OUT_PART, SW, WM, WN, FM, FN, WD, XU, OCC>), grid, threads, 0, st,
-                       a);
-    const long long groups = (long long)a.M * 4 * a.tiles;
-    hipLaunchKernelGGL((k_a8_join<EPI>), dim3((unsigned)((groups + kJoinThreads - 1) / kJoinThreads)),
-                       dim3(kJoinThreads), 0, st, a, p.slices);
 }
 
 template <int EPI, int MT, int NT, int NW, int D>
@@ -664,25 +657,12 @@ template <int EPI>
 void launch(const A8Args& a, const Plan& p, hipStream_t st) {
     constexpr int ALL = 1 << 30;
     if (p.kind == K_T256) {
-        launch_tile<EPI, 2, 4, 8, 4, 4, 3, 2>(a, p, 0, p.cols, st);
+        launch_tile<EPI, true>(a, p, 0, p.cols, st);
         if (p.cols < ceil_div(a.tiles, EPI == EPI_SWIGLU ? 8 : 16))
-            launch_tile<EPI, 2, 2, 4, 4, 4, 3, 2>(a, p, 2 * p.cols, ALL, st);
+            launch_tile<EPI, false>(a, p, 2 * p.cols, ALL, st);
         return;
     }
-    if (p.kind == K_T128) {
-        launch_tile<EPI, 2, 2, 4, 4, 4, 3, 2>(a, p, 0, ALL, st);
-        return;
-    }
-#ifdef A8_TUNE
-    if (getenv("A8M")) {
-        const int mt = atoi(getenv("A8M")), nt = atoi(getenv("A8N")), nw = atoi(getenv("A8W")),
-                  dd = atoi(getenv("A8D"));
-#define TRY(m, n, w, d)                          \
-    if (mt == m && nt == n && nw == w && dd == d) \
-        return launch_stream<EPI, m, n, w, d>(a, st);
-#include "tune_shapes.inc"
-    }
-#endif
+    if (p.kind == K_T128) return launch_tile<EPI, false>(a, p, 0, ALL, st);
     const StreamShape f = stream_shape(a.M, a.tiles, a.K, EPI == EPI_SWIGLU ? 2 : 1);
     if (f.mt == 1 && f.nt == 2) return launch_stream<EPI, 1, 2, 4, 2>(a, st);
     if (f.mt == 1 && f.waves == 8) return launch_stream<EPI, 1, 1, 8, 2>(a, st);
@@ -709,7 +689,7 @@ extern "C" size_t qlm_matmul_a8_workspace_bytes(int M, int N, int K, int epilogu
     // Slices are cut for at most 256 tiles of 128 x 128 sums in all, at most 8
     // of a call: a bound that never falls with M.
     if (M <= kSliceMinRows || K / 64 < 2 * kSliceMinBlocks) return 0;
-    const size_t sums = (size_t)M * (epilogue == EPI_SWIGLU ? 2 : 1) * ((N + 15) / 16 * 16);
+    const size_t sums = (size_t)M * (epilogue == EPI_SWIGLU ? 2 : 1) * (((size_t)N + 15) / 16 * 16);
     const size_t most = (size_t)kSliceTiles * 128 * 128;
     return 4 * (kSliceMost * sums < most ? kSliceMost * sums : most);
 }
@@ -722,6 +702,7 @@ extern "C" int qlm_matmul_a8(const int8_t* x, int ldx, const float* x_scales,
         return QLM_ERR_ARG;
     if (epilogue < EPI_STORE || epilogue > EPI_SWIGLU || ldx < K || ldy < N) return QLM_ERR_ARG;
     if (K % 64 != 0 || K >= 1 << 17 || ldx % 16 != 0 || ldx >= 1 << 23) return QLM_ERR_SHAPE;
+    if (M >= kMaxRows || N >= kMaxOutputs) return QLM_ERR_SHAPE;
     if (((uintptr_t)x | (uintptr_t)q_tiles | (uintptr_t)work) & 15u) return QLM_ERR_SHAPE;
     const Plan p = plan_of(M, N, K, epilogue);
     const size_t need = qlm_matmul_a8_workspace_bytes(M, N, K, epilogue);

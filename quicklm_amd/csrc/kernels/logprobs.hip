@@ -39,7 +39,7 @@ constexpr int kMaxTop = QLM_TOKEN_LOGPROBS_MAX_TOP;
 constexpr int kSlack = 8;             // chunks beyond k that a threshold may name
 constexpr int kCand = 512;            // logits that are ranked by counting
 constexpr int kMaxVocab = 1 << 21;    // chunk maxima of a row fit 32 KB of LDS
-constexpr int kMaxRows = 1 << 23;     // a launch's threads fit 32 bits
+constexpr int kMaxRows = 1 << 22;     // a launch's threads fit 32 bits
 constexpr int kRegMax = 16;           // chunk maxima a lane holds in registers
 constexpr float kFloor = -200.0f;     // exp(kFloor) is 0 in fp32
 
