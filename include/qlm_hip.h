@@ -311,7 +311,8 @@ int qlm_matmul_i8_t_whole_config(const float* x, int ldx, const float* norm_w, f
  * tile-major q_tiles (qlm_mx_swizzle with group K) and s_rows as quantised
  * ([2N] for SwiGLU: gate rows, then up rows). On the int8 matrix cores; the
  * sums are exact in int32 and rounded to fp32 once, so the result differs
- * from the exact one by a few fp32 roundings only, in every form. epilogue
+ * from the exact one by a few fp32 roundings only, in every form, and a row's
+ * result is the same whatever rows are beside it. epilogue
  * 0: y = result; 1: y += result; 2: SwiGLU, y = silu(gate) * up (N outputs).
  * M below 2^20, N below 2^23, K a multiple of 64 below 2^17; x and q_tiles 16-byte
  * aligned, ldx a multiple of 16 below 2^23; y of any stride and alignment,
@@ -353,9 +354,10 @@ int qlm_add_rms_norm(float* res, const float* delta, const float* w, float* y, i
 /* math::add_rms_norm with an output in 8 bits, the input rows of
  * qlm_matmul_a8 (no counterpart in the reference, whose activations stay
  * fp32): r = x + delta (delta NULL: r = x), y = r / sqrt(mean(r^2) + eps) *
- * (1 + w), scales[row] = max|y| / 127 (1 for a row of zeros), q = y / scale
- * rounded to the nearest whole number, ties to even. Statistics and quotient are held in 64
- * bits, so the bytes are those of the exact quotient. sum (may be NULL;
+ * (1 + w), scales[row] = max|y| / 127 (1 for a row of zeros; NaN if eps is
+ * 0 too), q = y / scale rounded to the nearest whole number, ties to even.
+ * Statistics and quotient are held in 64 bits, so the bytes are those of the
+ * exact quotient. sum (may be NULL;
  * needs delta) receives r; it may be x or delta itself with the same row
  * stride, and overlaps neither otherwise. A row with a value that is not
  * finite gets scale NaN and bytes 0: its products come out NaN. x [rows,
@@ -560,7 +562,9 @@ size_t qlm_argmax_workspace_bytes(int B, int n);
  * probability below the fp32 range is -inf. top <= QLM_TOKEN_LOGPROBS_MAX_TOP
  * and top <= n; n at most 2^21, rows at most 2^22. work: device scratch of
  * qlm_token_logprobs_workspace_bytes(rows, n, top) bytes, 16-byte aligned, no
- * initial contents needed; calls sharing it must be ordered on one stream. */
+ * initial contents needed; calls sharing it must be ordered on one stream.
+ * The size may fall as rows grow: one workspace for calls of several sizes is
+ * as large as the largest of them asks for. */
 #define QLM_TOKEN_LOGPROBS_MAX_TOP 64
 size_t qlm_token_logprobs_workspace_bytes(int rows, int n, int top);
 int qlm_token_logprobs(const float* logits, int ldl, int n, int rows, const int* ids, int n_ids,

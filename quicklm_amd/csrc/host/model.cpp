@@ -816,7 +816,7 @@ void DecoderModel::score(const int* toks, int n, int pos, int top, float* logpro
                          float* entropy, int* top_ids, float* top_logprobs) {
     if (n <= 0) return;
     if (!toks) throw std::runtime_error("score: null tokens");
-    if (pos < 0 || pos + n > max_seq_)
+    if (pos < 0 || n > max_seq_ - pos)
         throw std::runtime_error("context length exceeded max_seq_len (" + std::to_string(max_seq_) +
                                  ")");
     const int V = cfg_.vocab_size;

@@ -171,8 +171,8 @@ class DecoderModel : public GreedyModel {
     // rows first..first+count-1 of sequence b's tokens through every layer;
     // with lm_rows, each pass's rows also get the final norm, lm_head and a
     // greedy pick (stored at lm_idx[row - first], device) and, with
-    // logits_host or score, their logits
-    // copied out, or scored (`score`: device arrays of count rows)
+    // logits_host or score, their logits copied out, or scored (`score`:
+    // device arrays of count rows)
     struct ScoreRows {
         int* ids;      // next tokens, -1: none
         float* lp;     // [count]

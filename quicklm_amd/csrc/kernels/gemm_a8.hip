@@ -65,8 +65,9 @@ __device__ __forceinline__ f32x4u load_scales(const float* sw, int n, int N) {
 // 2048 x 9728 SwiGLU took 10 us of a round's 40 with the library's.
 __device__ __forceinline__ float silu_fast(float g) {
     constexpr float kLog2e = 1.44269502e0f, kRest = 1.92596303e-8f, kLn2 = 0.693147182f;
-    const float hi = g * -kLog2e;
-    const float lo = fmaf(g, -kLog2e, -hi) - g * kRest;
+    const float c = fminf(g, 200.0f);  // (an infinite one has no rounding error)
+    const float hi = c * -kLog2e;
+    const float lo = fmaf(c, -kLog2e, -hi) - c * kRest;
     float e = __builtin_amdgcn_exp2f(hi);
     // past the range of fp32 the result is 0; 1 / 3e38 is still not a NaN
     e = fminf(fmaf(e * kLn2, lo, e), 3e38f);

@@ -277,8 +277,8 @@ __device__ __forceinline__ void name_chunks(int nchunk, int top, At at, TopShare
 
 // The first `top` tokens of a row by (logit, then lower id), the chunks that
 // hold them named in `sh` (or all, where there are no more than `top`), `most`
-// the order of its largest logit. CPW: chunks a wave can hold, NW CPW >= top + kSlack. Called by the whole
-// workgroup. emit(rank, id, order of the logit).
+// the order of its largest logit. CPW: chunks a wave can hold, NW CPW >= top +
+// kSlack. Called by the whole workgroup. emit(rank, id, order of the logit).
 template <int CPW, int NW, typename Emit>
 __device__ __forceinline__ void select_top(const float* row, int n, int nchunk, int top, int most,
                                            TopShared& sh, Emit emit) {

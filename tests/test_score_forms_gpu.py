@@ -120,3 +120,21 @@ def test_token_logprobs_offsets_past_32_bits(hip, rng, n):
     assert np.array_equal(ti.to_numpy((rows, top), np.int32), rti)
     assert (np.abs(lp.to_numpy((rows, 1), np.float32) - rlp) <= t1).all()
     assert (np.abs(tl.to_numpy((rows, top), np.float32) - rtl) <= t3).all()
+
+
+@pytest.mark.parametrize("M", [1, 40, 700])
+def test_matmul_a8_results_past_the_range(hip, rng, M):
+    """Scales whose product with a sum leaves fp32: infinities as the formula
+    has them, and silu(+inf) up = +-inf."""
+    N, K = 300, 128
+    x = rng.integers(1, 128, (M, K), dtype=np.int8)
+    q = rng.integers(1, 128, (2 * N, K), dtype=np.int8)
+    q[N + 1::2] *= -1  # up sums of either sign
+    sx, sw = np.full(M, 1e20, np.float32), np.full(2 * N, 1e20, np.float32)
+    sw[N:] = 1e-24
+    say(f"matmul_a8 past the range M={M}")
+    y = np.zeros((M, N), np.float32)
+    got = run_matmul(hip, x, sx, q, sw, y, SWIGLU)
+    assert np.array_equal(got, np.where(np.arange(N) % 2, -np.inf, np.inf) * np.ones((M, 1)))
+    got = run_matmul(hip, x, sx, q[:N], sw[:N], y, STORE)
+    assert np.isposinf(got).all()
