@@ -560,7 +560,7 @@ size_t qlm_argmax_workspace_bytes(int B, int n);
  * still follow the logits, NaN counted as -inf. fp32, sums relative to the
  * running maximum, in an order that depends only on rows and n; a log
  * probability below the fp32 range is -inf. top <= QLM_TOKEN_LOGPROBS_MAX_TOP
- * and top <= n; n at most 2^21, rows at most 2^22. work: device scratch of
+ * and top <= n; n and rows at most 2^21. work: device scratch of
  * qlm_token_logprobs_workspace_bytes(rows, n, top) bytes, 16-byte aligned, no
  * initial contents needed; calls sharing it must be ordered on one stream.
  * The size may fall as rows grow: one workspace for calls of several sizes is

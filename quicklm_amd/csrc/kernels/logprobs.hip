@@ -10,14 +10,20 @@
 // Selection: any token among the first k of a row lies in one of the k chunks
 // with the largest maxima (equal maxima: the earlier chunk), since each of
 // those holds a token that precedes it. So a threshold over the chunk maxima
-// (bisection over the floats' bits, the maxima in registers) names about k
-// chunks of 1 KB, which are read again (1 % of a 152 K row for k = 5); their
-// logits that reach the threshold, little more than k, are ranked by counting.
-// Where too many reach it (few chunks, equal or masked logits) the threshold
-// is bisected over the logits held, and logits equal to it are taken in order.
+// (histograms over the floats' bits, the maxima in one wave's registers) names
+// about k chunks of 1 KB, which are read again (1 % of a 152 K row for
+// k = 5); their logits that reach the threshold, little more than k, are
+// ranked by counting. Where too many reach it (few chunks, equal or masked
+// logits) the threshold is bisected over the logits held, and logits equal to
+// it are taken in order. With few rows all of this is a chain of short steps
+// of one workgroup, where every instruction shows: a bisection step over the
+// chunk maxima takes 0.3 us of one wave, and of 16 waves with a barrier 0.4.
 // One workgroup a row does all of it (k_logprob<.., true>) where the rows fill
 // the GPU; otherwise slices leave (M, z, u) and their maxima to
-// k_logprob_finish. Bound by the one read of the logits.
+// k_logprob_finish. Many rows are bound by the one read of the logits: 2047 x
+// 151936 with 5 alternatives 205 us, 6.06 TB/s. Few are bound by that chain and
+// two launches: 1 x 151936 with 20 alternatives 8.1 us (10.9 with bisections
+// for both thresholds), 37 x 32003 with 64, masked, 11.9 (16.1).
 
 #include <type_traits>
 
@@ -29,7 +35,7 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kThreads = 256;   // of a workgroup that reads a row or a slice
 constexpr int kWaves = kThreads / QLM_WAVE;
-constexpr int kFinishWaves = 8;  // of a workgroup that finishes a sliced row
+constexpr int kFinishWaves = 16;  // of a workgroup that finishes a sliced row
 constexpr int kMostWaves = 16;   // of a workgroup that reads one of few short rows
 constexpr int kChunk = 4 * QLM_WAVE;  // logits of a chunk: a vector of four a lane
 // Chunks a wave keeps in flight: many where one workgroup reads a long row
@@ -39,8 +45,10 @@ constexpr int kMaxTop = QLM_TOKEN_LOGPROBS_MAX_TOP;
 constexpr int kSlack = 8;             // chunks beyond k that a threshold may name
 constexpr int kCand = 512;            // logits that are ranked by counting
 constexpr int kMaxVocab = 1 << 21;    // chunk maxima of a row fit 32 KB of LDS
-constexpr int kMaxRows = 1 << 22;     // a launch's threads fit 32 bits
+constexpr int kMaxRows = 1 << 21;     // a launch's threads fit 32 bits
 constexpr int kRegMax = 16;           // chunk maxima a lane holds in registers
+constexpr int kBuckets = 256;         // of a histogram of the chunk maxima
+constexpr int kSums = 160;            // over the workgroup: at most 2 x 66 steps and 10
 constexpr float kFloor = -200.0f;     // exp(kFloor) is 0 in fp32
 
 struct Part {
@@ -169,12 +177,33 @@ __device__ __forceinline__ Part join_parts(const Part* parts, int count) {
 }
 
 struct TopShared {
-    float m, lz;  // the row's largest logit and log z
-    int red[kMostWaves];
+    float m, lz;   // the row's largest logit and log z
     int nsel, lo;  // chunks named, and their threshold
+    int sums[kSums];  // each sum over the workgroup has its own, zero at the start
+    int wave[kMostWaves];
     int sel[kMaxTop + kSlack];
     int same[kMaxTop + kSlack];
-    long long cand[kCand];  // order of the logit, then what is left of 2^32 - 1 by the id
+    long long cand[kCand];  // order of the logit, then what is left of 2^31 - 1 by the id
+};
+
+// Sums of the waves' counts, for everyone; the next of them each time.
+struct Sums {
+    TopShared& sh;
+    int used = 0;
+    // this wave's place among the counts
+    __device__ __forceinline__ int add(int c) {
+        int place = 0;
+        if ((threadIdx.x & (QLM_WAVE - 1)) == 0) place = atomicAdd(&sh.sums[used], c);
+        return __builtin_amdgcn_readfirstlane(place);
+    }
+    __device__ __forceinline__ int total() {
+        __syncthreads();
+        return __builtin_amdgcn_readfirstlane(sh.sums[used++]);
+    }
+    __device__ __forceinline__ int operator()(int c) {
+        if (c && (threadIdx.x & (QLM_WAVE - 1)) == 0) atomicAdd(&sh.sums[used], c);
+        return total();
+    }
 };
 
 // Sum, minimum and maximum of an int over the wave, for every lane.
@@ -196,261 +225,334 @@ __device__ __forceinline__ int wave_sum_i(int v) {
     return wave_reduce(v, [](int a, int b) { return a + b; });
 }
 
+// Lanes of the mask before this one.
+__device__ __forceinline__ int before_me(unsigned long long mask) {
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
+                                     __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31
+    return v;
+}
+
 // The threshold over a row's chunk maxima and the chunks that reach it, in
-// order, by one wave. at(c): order of chunk c's maximum.
-template <typename At>
-__device__ __forceinline__ void name_chunks(int nchunk, int top, At at, TopShared& sh) {
+// order, by one wave. at(c): order of chunk c's maximum, held in R registers a
+// lane, or (R 0) read each time.
+template <int R, typename At>
+__device__ __forceinline__ void name_chunks_r(int nchunk, int top, At at, TopShared& sh) {
     const int lane = threadIdx.x & (QLM_WAVE - 1);
-    const unsigned long long below = (1ull << lane) - 1;
-    // count(>= lo) >= top, as near to top as the slack, unless maxima tie
-    int lo, hi, above = 0, named = nchunk;  // count(>= hi) = above < top
-    auto bisect = [&](int least, int most, auto count) {
-        lo = wave_reduce(least, [](int a, int b) { return min(a, b); });
-        hi = wave_reduce(most, [](int a, int b) { return max(a, b); }) + 1;
-        // first whether all but a few are equal (a masked row's chunks)
-        for (int m = lo + 1, step = 0; hi - (long long)lo > 1 && named > top + kSlack;
-             m = cut_of(lo, hi, step++)) {
-            const int cnt = count(m);
-            if (cnt >= top) {
-                lo = m;
-                named = cnt;
-            } else {
-                hi = m;
-                above = cnt;
+    int o[R ? R : 1];
+#pragma unroll
+    for (int j = 0; j < R; ++j) o[j] = at(min(j * QLM_WAVE + lane, nchunk - 1));
+    // f(c, order) for every 64 chunks, c this lane's; past the last INT32_MIN
+    auto each = [&](auto f) {
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (j * QLM_WAVE >= nchunk) break;
+                const int c = j * QLM_WAVE + lane;
+                f(c, c < nchunk ? o[j] : INT32_MIN);
             }
+        } else {
+            for (int c = lane; c - lane < nchunk; c += QLM_WAVE)
+                f(c, c < nchunk ? at(c) : INT32_MIN);
         }
     };
-    int listed = 0, left = 0;
-    auto list = [&](int c, int o) {
-        const bool over = c < nchunk && o > lo, same = c < nchunk && o == lo;
-        const unsigned long long bs = __ballot(same);
-        const bool take = over || (same && (int)__popcll(bs & below) < left);
-        const unsigned long long bt = __ballot(take);
-        if (take) sh.sel[listed + (int)__popcll(bt & below)] = c;
-        listed += (int)__popcll(bt);
-        left -= min(left, (int)__popcll(bs));
-    };
-    if (nchunk <= kRegMax * QLM_WAVE) {  // the maxima in registers
-        int o[kRegMax], least = INT32_MAX, most = INT32_MIN;
-#pragma unroll
-        for (int j = 0; j < kRegMax; ++j) {
-            o[j] = INT32_MIN;
-            if (j * QLM_WAVE + lane < nchunk) o[j] = at(j * QLM_WAVE + lane);
-        }
-#pragma unroll
-        for (int j = 0; j < kRegMax; ++j) {
-            most = max(most, o[j]);
-            if (j * QLM_WAVE + lane < nchunk) least = min(least, o[j]);
-        }
-        bisect(least, most, [&](int m) {
-            int cnt = 0;
-#pragma unroll
-            for (int j = 0; j < kRegMax; ++j)
-                if (j * QLM_WAVE < nchunk) cnt += o[j] >= m;
-            return wave_sum_i(cnt);
+    int least = INT32_MAX, most = INT32_MIN;
+    each([&](int c, int v) {
+        most = max(most, v);
+        least = c < nchunk ? min(least, v) : least;
+    });
+    // count(>= lo) = named >= top, as near to top as the slack, unless maxima
+    // tie; count(>= hi) = above < top
+    int lo = wave_reduce(least, [](int x, int y) { return min(x, y); });
+    int hi = wave_reduce(most, [](int x, int y) { return max(x, y); }) + 1;
+    int above = 0, named = nchunk;
+    int* hist = reinterpret_cast<int*>(sh.cand);
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    while (named > top + kSlack && (unsigned)hi - (unsigned)lo > 1) {
+        // lo .. hi - 1 in buckets of 2^shift orders, the highest first
+        const int shift = max(0, 24 - __builtin_clz((unsigned)hi - (unsigned)lo - 1));
+        *reinterpret_cast<i32x4*>(hist + 4 * lane) = i32x4{0, 0, 0, 0};
+        each([&](int, int v) {
+            if (v >= lo && v < hi)
+                atomicAdd(&hist[kBuckets - 1 - (((unsigned)v - (unsigned)lo) >> shift)], 1);
         });
-        left = named > top + kSlack ? top - above : INT32_MAX;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const i32x4 h = *reinterpret_cast<const i32x4*>(hist + 4 * lane);
+        const int s = (h.x + h.y) + (h.z + h.w), upto = wave_scan(s);
+        // the bucket that completes `top`
+        const int l = __ffsll(__ballot(above + upto >= top)) - 1;
+        int b = kBuckets - 1 - 4 * l, got = above + __builtin_amdgcn_readlane(upto - s, l);
 #pragma unroll
-        for (int j = 0; j < kRegMax; ++j)
-            if (j * QLM_WAVE < nchunk) list(j * QLM_WAVE + lane, o[j]);
-    } else {
-        int least = INT32_MAX, most = INT32_MIN;
-        for (int c = lane; c < nchunk; c += QLM_WAVE) {
-            const int o = at(c);
-            least = min(least, o);
-            most = max(most, o);
+        for (int k = 0; k < 4; ++k) {
+            const int next = got + __builtin_amdgcn_readlane(h[k], l);
+            named = next;
+            if (next >= top) break;
+            got = next;
+            --b;
         }
-        bisect(least, most, [&](int m) {
-            int cnt = 0;
-            for (int c = lane; c < nchunk; c += QLM_WAVE) cnt += at(c) >= m;
-            return wave_sum_i(cnt);
-        });
-        left = named > top + kSlack ? top - above : INT32_MAX;
-        for (int c0 = 0; c0 < nchunk; c0 += QLM_WAVE)
-            list(c0 + lane, at(min(c0 + lane, nchunk - 1)));
+        above = got;
+        const unsigned first = (unsigned)lo + ((unsigned)b << shift);
+        if ((unsigned)hi - first > 1u << shift) hi = (int)(first + (1u << shift));
+        lo = (int)first;
     }
+    // None of those equal to lo is left out, or all but the first that complete
+    // `top`. A chunk of the lowest order alone holds nothing else: one is enough
+    // (a shorter one is the row's last).
+    const bool all = named <= top + kSlack;
+    int listed = 0, left = lo == kLowest ? 1 : top - above;
+    each([&](int c, int v) {
+        bool take = v >= lo;
+        if (!all) {
+            const unsigned long long same = __ballot(v == lo);
+            take = v > lo || (v == lo && before_me(same) < left);
+            left -= min(left, (int)__popcll(same));
+        }
+        const unsigned long long m = __ballot(take);
+        if (take) sh.sel[listed + before_me(m)] = c;
+        listed += (int)__popcll(m);
+    });
     if (lane == 0) {
         sh.nsel = listed;
         sh.lo = lo;
     }
 }
+template <typename At>
+__device__ __forceinline__ void name_chunks(int nchunk, int top, At at, TopShared& sh) {
+    if (nchunk <= 2 * QLM_WAVE)
+        name_chunks_r<2>(nchunk, top, at, sh);
+    else if (nchunk <= kRegMax * QLM_WAVE)
+        name_chunks_r<kRegMax>(nchunk, top, at, sh);
+    else
+        name_chunks_r<0>(nchunk, top, at, sh);
+}
 
 // The first `top` tokens of a row by (logit, then lower id), the chunks that
-// hold them named in `sh` (or all, where there are no more than `top`), `most`
-// the order of its largest logit. CPW: chunks a wave can hold, NW CPW >= top +
-// kSlack. Called by the whole workgroup. emit(rank, id, order of the logit).
+// hold them named in `sh` (or all, where there are no more than `top`). CPW:
+// chunks a wave can hold, NW CPW >= top + kSlack. Called by the whole
+// workgroup. emit(rank, id, order of the logit).
 template <int CPW, int NW, typename Emit>
-__device__ __forceinline__ void select_top(const float* row, int n, int nchunk, int top, int most,
-                                           TopShared& sh, Emit emit) {
+__device__ __forceinline__ void select_top(const float* row, int n, int nchunk, int top,
+                                           TopShared& sh, Sums& sum, Emit emit) {
     const int lane = threadIdx.x & (QLM_WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
-    const unsigned long long below = (1ull << lane) - 1;
     const bool listed = nchunk > top;
-    const int nsel = listed ? sh.nsel : nchunk;
-    // The chunks' logits, chunk `wave + j NW` of the list in o[j], all
-    // requested before the first is used; what lies past the row is below all.
-    int o[CPW][4], at[CPW];
-    {
-        f32x4u v[CPW];
+    const int nsel = listed ? __builtin_amdgcn_readfirstlane(sh.nsel) : nchunk;
+    const int lo = listed ? __builtin_amdgcn_readfirstlane(sh.lo) : kLowest;
+    // Chunk `wave + j NW` of the list (number j of the lanes' `mine`) in v[j],
+    // all requested before the first is used. At the row's end a lane's four
+    // overlap those of the lane before: what is not this lane's is masked.
+    const int s = min(wave + min(lane, CPW - 1) * NW, nsel - 1);
+    const int mine = listed ? sh.sel[s] : s;
+    auto chunk = [&](int j) { return __builtin_amdgcn_readlane(mine, j); };
+    auto first_of = [&](int c) { return max(min(c * kChunk + 4 * lane, n - 4), 0); };
+    f32x4u v[CPW];
+#pragma unroll
+    for (int j = 0; j < CPW; ++j) {
+        if (wave + j * NW >= nsel) break;
+        const float* p = row + first_of(chunk(j));
+        if (n >= 4)
+            v[j] = *reinterpret_cast<const f32x4u*>(p);
+        else
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][k] = p[min(k, n - 1)];
+    }
+    auto put = [&](int order, int id, int p) {
+        sh.cand[p] = ((long long)order << 32) | (unsigned)(0x7fffffff - id);
+    };
+    // the waves' places for their candidates, the lanes' from a count of each
+    auto places = [&](int c) {
+        int p = sum.add(wave_sum_i(c));
+#pragma unroll
+        for (int bit = 1; bit <= 4 * CPW; bit *= 2) p += bit * before_me(__ballot(c & bit));
+        return p;
+    };
+    int cnt = kCand + 1;
+    // Ranking many more than `top` costs more than cutting them: 1271 x 5675
+    // with 20 alternatives 35 us where any 512 were ranked.
+    const int enough = max(128, 3 * top);
+    // The threshold says much where chunks were left out; a NaN and what is
+    // masked are below it.
+    if (lo > kLowest && nchunk > top + kSlack) {
+        const float from = value_of(lo);
+        // a lane has one candidate or none, hardly ever more: the last of them
+        // before number `end` of its 4 CPW logits, and how many there are
+        auto last = [&](int end, float& what, int& which) {
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < CPW; ++j) {
+                if (wave + j * NW >= nsel) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = v[j][k] >= from && 4 * j + k < end;
+                    c += in;
+                    what = in ? v[j][k] : what;
+                    which = in ? 4 * j + k : which;
+                }
+            }
+            return c;
+        };
+#pragma unroll
+        for (int j = 0; j < CPW; ++j)
+            if (wave + j * NW < nsel && (chunk(j) + 1) * kChunk > n) {
+                const int skip = chunk(j) * kChunk + 4 * lane - first_of(chunk(j));
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k < skip) v[j][k] = -INFINITY;
+            }
+        float what = 0.0f;
+        int which = 0, c = last(4 * CPW, what, which), p = places(c);
+        while (__ballot(c > 0)) {
+            const int id = first_of(__shfl(mine, which >> 2, QLM_WAVE)) + (which & 3);
+            if (c > 0 && p < kCand) put(order_of(what), id, p);
+            p += 1;
+            c -= 1;
+            if (__ballot(c > 0)) last(which, what, which);
+        }
+        cnt = sum.total();
+    }
+    if (cnt > enough) {
+        int o[CPW][4], first[CPW];  // what is not there is below all
 #pragma unroll
         for (int j = 0; j < CPW; ++j) {
-            const int s = wave + j * NW;
-            if (s < nsel) {
-                const int c = listed ? __builtin_amdgcn_readfirstlane(sh.sel[s]) : s;
-                at[j] = c * kChunk;
-                v[j] = load_chunk(row, n, c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[j][k] = INT32_MIN;
+            if (wave + j * NW < nsel) {
+                first[j] = first_of(chunk(j));
+                const int skip = chunk(j) * kChunk + 4 * lane - first[j];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k >= skip && k < n) o[j][k] = order_of(v[j][k]);
             }
         }
-#pragma unroll
-        for (int j = 0; j < CPW; ++j)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                o[j][k] = INT32_MIN;
-                if (wave + j * NW < nsel && at[j] + 4 * lane + k < n)
-                    o[j][k] = order_of(v[j][k]);
-            }
-    }
-    // a count over the workgroup, its own share left in `mine`
-    auto total = [&](int c) {
-        c = wave_sum_i(c);
-        __syncthreads();
-        if (lane == 0) sh.red[wave] = c;
-        __syncthreads();
-        int t = 0;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) t += sh.red[w];
-        return t;
-    };
-    // how many logits reach `from`
-    auto count_from = [&](int from) {
-        int c = 0;
-#pragma unroll
-        for (int j = 0; j < CPW; ++j)
-            if (wave + j * NW < nsel)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) c += o[j][k] >= from;
-        return total(c);
-    };
-    int from = listed ? sh.lo : kLowest, cnt = count_from(from);
-    bool tied = false;
-    // (ranking many more than `top` costs more than cutting them: 1271 x 5675
-    // with 20 alternatives 35 us where any 512 were ranked)
-    if (cnt > max(128, 3 * top)) {
-        // Logits equal to `from` may be many (masked ones): fewer than `top`
-        // above it leave only those, in order. Otherwise bisect: first over
-        // the threads' largest logits (at least as many logits reach what
-        // `top` of them reach, and hardly more), then, where that was not
-        // enough, over the logits: count(>= from) >= top, <= kCand.
-        int k = count_from(from + 1);
-        if (k >= top) {
-            from += 1;
-            cnt = k;
-            int mine = INT32_MIN;
+        auto count_of = [&](auto in) {
+            int c = 0;
 #pragma unroll
             for (int j = 0; j < CPW; ++j)
+                if (wave + j * NW < nsel)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mine = max(mine, o[j][i]);
-            int hi = most + 1, reach = total(mine >= from);
-            if (reach >= top) {
-                // from what every thread that has logits reaches
-                const int least = wave_reduce(mine >= from ? mine : INT32_MAX,
-                                              [](int a, int b) { return min(a, b); });
-                __syncthreads();
-                if (lane == 0) sh.red[wave] = least;
-                __syncthreads();
-                from = sh.red[0];
+                    for (int k = 0; k < 4; ++k) c += in(o[j][k]);
+            return c;
+        };
+        auto count_from = [&](int from) {
+            return sum(wave_sum_i(count_of([&](int x) { return x >= from; })));
+        };
+        int from = lo;
+        cnt = count_from(from);
+        const int past = order_of(sh.m) + 1;  // the row's largest logit
+        bool tied = false;
+        if (cnt > enough) {
+            // Logits equal to `from` may be many (masked ones): fewer than `top`
+            // above it leave only those, in order. Otherwise bisect: first over
+            // the threads' largest logits (at least as many logits reach what
+            // `top` of them reach, and hardly more), then, where that was not
+            // enough, over the logits: count(>= from) >= top, <= kCand.
+            int k = count_from(from + 1);
+            if (k >= top) {
+                from += 1;
+                cnt = k;
+                int mine = INT32_MIN;
 #pragma unroll
-                for (int w = 1; w < NW; ++w) from = min(from, sh.red[w]);
-                for (int step = 0; hi - (long long)from > 1 && reach > 2 * top; ++step) {
+                for (int j = 0; j < CPW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mine = max(mine, o[j][i]);
+                auto reached = [&](int m) { return sum((int)__popcll(__ballot(mine >= m))); };
+                int hi = past, reach = reached(from);
+                if (reach >= top) {
+                    // from what every thread that has logits reaches
+                    const int least = wave_reduce(mine >= from ? mine : INT32_MAX,
+                                                  [](int x, int y) { return min(x, y); });
+                    if (lane == 0) sh.wave[wave] = least;
+                    __syncthreads();
+                    from = sh.wave[0];
+#pragma unroll
+                    for (int w = 1; w < NW; ++w) from = min(from, sh.wave[w]);
+                    for (int step = 0; hi - (long long)from > 1 && reach > 2 * top; ++step) {
+                        const int m = cut_of(from, hi, step);
+                        k = reached(m);
+                        if (k >= top) {
+                            from = m;
+                            reach = k;
+                        } else {
+                            hi = m;
+                        }
+                    }
+                    cnt = count_from(from);
+                    hi = past;
+                }
+                for (int step = 0; hi - (long long)from > 1 && cnt > kCand; ++step) {
                     const int m = cut_of(from, hi, step);
-                    k = total(mine >= m);
+                    k = count_from(m);
                     if (k >= top) {
                         from = m;
-                        reach = k;
+                        cnt = k;
                     } else {
                         hi = m;
                     }
                 }
-                cnt = count_from(from);
-                hi = most + 1;
             }
-            for (int step = 0; hi - (long long)from > 1 && cnt > kCand; ++step) {
-                const int m = cut_of(from, hi, step);
-                k = count_from(m);
-                if (k >= top) {
-                    from = m;
-                    cnt = k;
-                } else {
-                    hi = m;
-                }
-            }
+            tied = cnt > kCand;
         }
-        tied = cnt > kCand;
-        cnt = count_from(tied ? from + 1 : from);  // the waves' shares again
-    }
-    // candidates, this wave's behind those of the waves before it
-    int place = 0;
-    for (int w = 0; w < wave; ++w) place += sh.red[w];
-    auto take = [&](bool in, int order, int id, int p) {
-        if (in) sh.cand[p] = ((long long)order << 32) | (unsigned)(0x7fffffff - id);
-    };
-    {
         const int least = tied ? from + 1 : from;
+        int p = places(count_of([&](int x) { return x >= least; }));
 #pragma unroll
         for (int j = 0; j < CPW; ++j)
             if (wave + j * NW < nsel)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool in = o[j][k] >= least;
-                    const unsigned long long b = __ballot(in);
-                    if (b == 0) continue;
-                    take(in, o[j][k], at[j] + 4 * lane + k, place + (int)__popcll(b & below));
-                    place += (int)__popcll(b);
-                }
-    }
-    if (tied) {
-        // those equal to `from` follow in the order of their ids: places by
-        // the counts of the chunks before, then of the lanes before
-#pragma unroll
-        for (int j = 0; j < CPW; ++j)
-            if (wave + j * NW < nsel) {
-                int c = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) c += o[j][k] == from;
-                c = wave_sum_i(c);
-                if (lane == 0) sh.same[wave + j * NW] = c;
-            }
-        __syncthreads();
-        int before = cnt, s0 = 0;
-#pragma unroll
-        for (int j = 0; j < CPW; ++j)
-            if (wave + j * NW < nsel) {
-                for (; s0 < wave + j * NW && before < top; ++s0) before += sh.same[s0];
-                if (before >= top) continue;
-                int p = before;
-#pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    p += (int)__popcll(__ballot(o[j][k] == from) & below);
+                    if (o[j][k] >= least) put(o[j][k], first[j] + k, p++);
+        cnt = sum.total();
+        if (tied) {
+            // those equal to `from` follow in the order of their ids: places by
+            // the counts of the chunks before, then of the lanes before
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool in = o[j][k] == from;
-                    take(in && p < top, from, at[j] + 4 * lane + k, p);
-                    p += in;
+            for (int j = 0; j < CPW; ++j)
+                if (wave + j * NW < nsel) {
+                    int c = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) c += (int)__popcll(__ballot(o[j][k] == from));
+                    if (lane == 0) sh.same[wave + j * NW] = c;
                 }
-            }
-        cnt = top;
+            __syncthreads();
+            int before = cnt, s0 = 0;
+#pragma unroll
+            for (int j = 0; j < CPW; ++j)
+                if (wave + j * NW < nsel) {
+                    for (; s0 < wave + j * NW && before < top; ++s0) before += sh.same[s0];
+                    if (before >= top) continue;
+                    int q = before;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) q += before_me(__ballot(o[j][k] == from));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool in = o[j][k] == from;
+                        if (in && q < top) put(from, first[j] + k, q);
+                        q += in;
+                    }
+                }
+            cnt = top;
+            __syncthreads();
+        }
     }
-    __syncthreads();
-    // ranks: four lanes a candidate, each against a quarter of the others
-    for (int i0 = 0; i0 < cnt; i0 += NW * QLM_WAVE / 4) {
-        const int i = i0 + (int)threadIdx.x / 4;
+    // ranks: eight lanes a candidate, each against an eighth of the others
+    constexpr int S = 8;
+    for (int i0 = 0; i0 < cnt; i0 += NW * QLM_WAVE / S) {
+        const int i = i0 + (int)threadIdx.x / S;
         const long long key = sh.cand[min(i, cnt - 1)];
         int rank = 0;
-#pragma unroll 8
-        for (int j = threadIdx.x & 3; j < cnt; j += 4) rank += sh.cand[j] > key;
-        rank += __shfl_xor(rank, 1, QLM_WAVE);
-        rank += __shfl_xor(rank, 2, QLM_WAVE);
-        if ((threadIdx.x & 3) == 0 && i < cnt && rank < top)
+#pragma unroll 4
+        for (int j = threadIdx.x % S; j < cnt; j += S) rank += sh.cand[j] > key;
+#pragma unroll
+        for (int m = 1; m < S; m *= 2) rank += __shfl_xor(rank, m, QLM_WAVE);
+        if (threadIdx.x % S == 0 && i < cnt && rank < top)
             emit(rank, 0x7fffffff - (int)(key & 0x7fffffff), (int)(key >> 32));
     }
 }
@@ -463,6 +565,8 @@ __device__ __forceinline__ void finish_row(const LpArgs& a, int row, const Part*
                                            TopShared& sh, At at) {
     const float* lr = a.logits + (size_t)row * a.ldl;
     const int wave = threadIdx.x / QLM_WAVE, lane = threadIdx.x & (QLM_WAVE - 1);
+    if constexpr (CPW > 0)
+        for (int i = threadIdx.x; i < kSums; i += NW * QLM_WAVE) sh.sums[i] = 0;
     if (wave == NW - 1) {
         const Part p = join_parts(parts, count);
         // no distribution: every logit masked, a NaN, or +inf among them
@@ -484,11 +588,11 @@ __device__ __forceinline__ void finish_row(const LpArgs& a, int row, const Part*
         if (wave == 0 && a.nchunk > a.top) name_chunks(a.nchunk, a.top, at, sh);
         __syncthreads();
         const float m = sh.m, lz = sh.lz;
-        select_top<CPW, NW>(lr, a.n, a.nchunk, a.top, order_of(m), sh,
-                            [&](int rank, int id, int order) {
-                                a.top_ids[(size_t)row * a.top + rank] = id;
-                                a.top_lp[(size_t)row * a.top + rank] = (value_of(order) - m) - lz;
-                            });
+        Sums sum{sh};
+        select_top<CPW, NW>(lr, a.n, a.nchunk, a.top, sh, sum, [&](int rank, int id, int order) {
+            a.top_ids[(size_t)row * a.top + rank] = id;
+            a.top_lp[(size_t)row * a.top + rank] = (value_of(order) - m) - lz;
+        });
     }
 }
 
@@ -536,7 +640,7 @@ void launch_whole(const LpArgs& a, hipStream_t st) {
 
 template <int CPW>
 void launch_sliced(const LpArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_logprob<CPW, kWaves, false>), dim3((unsigned)(a.slices * a.rows)),
+    hipLaunchKernelGGL((k_logprob<(CPW > 0), kWaves, false>), dim3((unsigned)(a.slices * a.rows)),
                        dim3(kThreads), 0, st, a);
     hipLaunchKernelGGL((k_logprob_finish<CPW>), dim3(a.rows), dim3(kFinishWaves * QLM_WAVE), 0, st,
                        a);
@@ -609,19 +713,25 @@ extern "C" int qlm_token_logprobs(const float* logits, int ldl, int n, int rows,
                                       round16((size_t)rows * a.slices * sizeof(Part)));
     hipStream_t st = as_stream(stream);
     // chunks a wave holds: top + kSlack of them over the waves
-    constexpr int kFinish = (kMaxTop + kSlack + kFinishWaves - 1) / kFinishWaves;
-    constexpr int kShort = (kMaxTop + kSlack + kMostWaves - 1) / kMostWaves;
-    const int waves = whole_waves(rows, n);
-    if (!finished(waves, top))
-        top ? launch_sliced<kFinish>(a, st) : launch_sliced<0>(a, st);
-    else if (waves == kMostWaves)
-        top ? launch_whole<kShort, kMostWaves>(a, st) : launch_whole<0, kMostWaves>(a, st);
-    else if (top == 0)
-        launch_whole<0, kWaves>(a, st);
-    else if (top + kSlack <= 4 * kWaves)
-        launch_whole<4, kWaves>(a, st);
-    else
-        launch_whole<8, kWaves>(a, st);
+    const int waves = whole_waves(rows, n), held = top ? top + kSlack : 0;
+    static_assert(kFinishWaves == kMostWaves, "one number of chunks a wave");
+    constexpr int kAll = (kMaxTop + kSlack + kMostWaves - 1) / kMostWaves;
+    const int per = (held + kMostWaves - 1) / kMostWaves;
+    if (!finished(waves, top)) {
+        per == 0   ? launch_sliced<0>(a, st)
+        : per == 1 ? launch_sliced<1>(a, st)
+        : per == 2 ? launch_sliced<2>(a, st)
+                   : launch_sliced<kAll>(a, st);
+    } else if (waves == kMostWaves) {
+        per == 0   ? launch_whole<0, kMostWaves>(a, st)
+        : per == 1 ? launch_whole<1, kMostWaves>(a, st)
+        : per == 2 ? launch_whole<2, kMostWaves>(a, st)
+                   : launch_whole<kAll, kMostWaves>(a, st);
+    } else {
+        held == 0            ? launch_whole<0, kWaves>(a, st)
+        : held <= 4 * kWaves ? launch_whole<4, kWaves>(a, st)
+                             : launch_whole<8, kWaves>(a, st);
+    }
     return qlm_launch_status();
 }
 
