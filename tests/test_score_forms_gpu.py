@@ -138,3 +138,21 @@ def test_matmul_a8_results_past_the_range(hip, rng, M):
     assert np.array_equal(got, np.where(np.arange(N) % 2, -np.inf, np.inf) * np.ones((M, 1)))
     got = run_matmul(hip, x, sx, q[:N], sw[:N], y, STORE)
     assert np.isposinf(got).all()
+
+
+@pytest.mark.parametrize("rows,n,top", [(3, 20001, 20), (2, 300001, 64), (1, 1 << 21, 20),
+                                        (2, 40000, 1), (780, 20001, 24), (20, 9000, 64)])
+@pytest.mark.parametrize("kind", ["whole", "few", "mixed"])
+def test_token_logprobs_ties_over_many_chunks(hip, rng, rows, n, top, kind):
+    """Whole numbers, most chunks' maxima the same; few values over a constant,
+    or over a mask, fewer than asked for in some rows; all three in turn."""
+    say(f"logprobs rows={rows} n={n} top={top} ties {kind}")
+    x = rng.integers(-3, 4, (rows, n)).astype(np.float32)
+    for r in range(rows):
+        if kind == "few" or (kind == "mixed" and r % 2 == 0):
+            x[r] = -np.inf if r % 3 == 0 else 1.0
+            some = rng.integers(0, n, top // 2 + (r % 2) * top)
+            x[r, some] = rng.standard_normal(some.size) + 3
+        if kind == "mixed":
+            x[r, :300] = -np.inf
+    check_logprobs(hip, x, rng.integers(0, n, (rows, 1)), top)
