@@ -11,17 +11,20 @@
 // of x puts them that way. The weights are the first operand: a lane of the
 // result then holds four neighbouring outputs of one row of x.
 //
-// Three forms, taken by what each is reckoned to cost (plan_of):
+// Forms, taken by what each is reckoned to cost (plan_of):
 //   k_a8_stream  few workgroups' worth of tiles: bound by the way of the bytes
 //                to the CUs; every wave streams its share of K by itself.
 //   k_a8_tile    as 128 x 128 tiles, two workgroups a CU, K in slices if they
-//                are few: bound by the bytes' way too.
-//   k_a8_tile    as 256 x 256 tiles: bound by the matrix cores.
+//                are few: bound by the bytes' way too;
+//                as 128 x 256 tiles, one workgroup a CU;
+//                as 256 x 256 tiles: bound by LDS and the matrix cores, both
+//                busy 0.43 us of a block's 0.5 to 0.64, and by the writing of
+//                the outputs at a round's end (a quarter of a round of K 4096).
 // Measured on an MI355X, operands cold in the caches, us (and the larger of
 // the bytes' time at 4.75 TB/s and the products' at 2134 TOP/s): 1 x 9728 x
 // 2560 SwiGLU 11.5 (10.5), 16 x 2560 x 9728 9.1 (5.4), 1000 x 2560 x 2560 18.7
-// (6.1), 2048 x 9728 x 2560 SwiGLU 107 to 116 from card to card (96), 4096 x
-// 12288 x 4096 178 to 190 (193).
+// (6.1), 1000 x 6144 x 2560 27.9 (14.7), 2048 x 9728 x 2560 SwiGLU 105 to 110
+// from card to card (96), 4096 x 12288 x 4096 178 to 190 (193).
 
 #include <algorithm>
 
@@ -558,11 +561,11 @@ StreamShape stream_shape(int M, int tiles, int K, int halves) {
 
 // How a call runs. Times in us, measured on an MI355X with operands cold in
 // the caches; kblk 64-column blocks of K.
-enum { K_STREAM = 0, K_T128 = 1, K_T256 = 2 };
+enum { K_STREAM = 0, K_T128 = 1, K_WIDE = 2, K_T256 = 3 };  // (wide: 128 x 256)
 struct Plan {
-    int kind;            // of the first `cols` column blocks of its tile width;
-    int cols;            // the others run as 128 x 128 tiles (K_T256 only)
-    int slices, bslice;  // of K, and 64-column blocks in each (K_T128 only)
+    int kind;
+    int cols, rest;      // K_T256: of the first columns (256 each), the others' kind
+    int slices, bslice;  // of K, and 64-column blocks in each (K_T128 alone)
 };
 
 constexpr int kMaxRows = 1 << 20, kMaxOutputs = 1 << 23;  // tile numbers fit 32 bits
@@ -580,6 +583,12 @@ double cost128(int n, int kblk) {
     if (rest <= 256) return full * round + (rest ? 6.5 + 0.275 * kblk : 0);
     return full * round + (full ? rest / 512.0 * round : rest <= 384 ? 9 + 0.5 * kblk : round);
 }
+// 128 x 256 tiles, one workgroup a CU: the outputs of two of the above for
+// three quarters of their bytes (512 x 9728 x 2560 26.7 us instead of 30.2).
+double cost_wide(int n, int kblk) {
+    const int full = n / 256, rest = n % 256;
+    return full * (10.5 + 0.42 * kblk) + (rest ? 10.5 + (0.35 + 0.07 * rest / 256.0) * kblk : 0);
+}
 // 256 x 256 tiles, one workgroup a CU: 0.51 a block while the other CUs idle,
 // 0.64 with all of them.
 double cost256(int n, int kblk) {
@@ -589,7 +598,7 @@ double cost256(int n, int kblk) {
 Plan plan_of(int M, int N, int K, int epilogue) {
     const int halves = epilogue == EPI_SWIGLU ? 2 : 1, kblk = K / 64;
     const int tiles = ceil_div(N, 16);
-    Plan best{K_STREAM, 0, 1, kblk};
+    Plan best{K_STREAM, 0, 0, 1, kblk};
     double least = 1e30;
     const int gx1 = ceil_div(tiles, 8 / halves), gy1 = ceil_div(M, 128);
     const int gx2 = ceil_div(tiles, 16 / halves), gy2 = ceil_div(M, 256);
@@ -603,16 +612,19 @@ Plan plan_of(int M, int N, int K, int epilogue) {
             // the slices' sums are written and read back, 3.3 MB a us
             const double join = s == 1 ? 0 : 2.5 + 1.2e-6 * s * M * halves * N;
             const int bs = s == 1 ? kblk : ceil_div(ceil_div(kblk, s), 2) * 2;
-            offer(cost128(gx1 * gy1 * s, bs) + join, Plan{K_T128, gx1, ceil_div(kblk, bs), bs});
+            offer(cost128(gx1 * gy1 * s, bs) + join, Plan{K_T128, 0, 0, ceil_div(kblk, bs), bs});
         }
+        offer(cost_wide(gx2 * gy1, kblk), Plan{K_WIDE, 0, 0, 1, kblk});
     }
     if (M > 128) {
-        offer(cost256(gx2 * gy2, kblk), Plan{K_T256, gx2, 1, kblk});
+        offer(cost256(gx2 * gy2, kblk), Plan{K_T256, gx2, 0, 1, kblk});
         // full rounds of 256 tiles, and the columns left over as smaller ones
         const int full = gx2 * gy2 / 256 * 256 / gy2;
-        if (full > 0 && full < gx2)
-            offer(cost256(full * gy2, kblk) + cost128((gx1 - 2 * full) * gy1, kblk),
-                  Plan{K_T256, full, 1, kblk});
+        if (full > 0 && full < gx2) {
+            const double most = cost256(full * gy2, kblk);
+            offer(most + cost128((gx1 - 2 * full) * gy1, kblk), Plan{K_T256, full, K_T128, 1, kblk});
+            offer(most + cost_wide((gx2 - full) * gy1, kblk), Plan{K_T256, full, K_WIDE, 1, kblk});
+        }
     }
     return best;
 }
@@ -622,20 +634,22 @@ size_t part_bytes(const Plan& p, int M, int N, int epilogue) {
     return (size_t)p.slices * M * (epilogue == EPI_SWIGLU ? 2 : 1) * (ceil_div(N, 16) * 16) * 4;
 }
 
-// Column blocks [first, last) of tiles of 256 x 256 (BIG) or 128 x 128.
-template <int EPI, bool BIG>
+// Columns [first, last), 256 each, as tiles of the kind.
+template <int EPI, int KIND>
 void launch_tile(A8Args a, const Plan& p, int first, int last, hipStream_t st) {
     constexpr bool SW = EPI == EPI_SWIGLU;
-    constexpr int SIDE = BIG ? 256 : 128, OT = SIDE / 16 / (SW ? 2 : 1);
-    a.t_first = first * OT;
-    a.gx = std::min(last, ceil_div(a.tiles, OT)) - first;
-    a.gy = ceil_div(a.M, SIDE);
+    constexpr int WIDTH = KIND == K_T128 ? 128 : 256, OT = WIDTH / 16 / (SW ? 2 : 1);
+    a.t_first = first * (16 / (SW ? 2 : 1));
+    a.gx = ceil_div(std::min(a.tiles, last * (16 / (SW ? 2 : 1))) - a.t_first, OT);
+    a.gy = ceil_div(a.M, KIND == K_T256 ? 256 : 128);
     a.blocks = a.gx * a.gy * p.slices;
     a.per_xcd = ceil_div(a.blocks, 8);
     a.bslice = p.bslice;
-    const dim3 grid(8 * a.per_xcd), threads((BIG ? 8 : 4) * QLM_WAVE);
-    if constexpr (BIG) {
+    const dim3 grid(8 * a.per_xcd), threads((KIND == K_T128 ? 4 : 8) * QLM_WAVE);
+    if constexpr (KIND == K_T256) {
         hipLaunchKernelGGL((k_a8_tile<EPI, SW, 2, 4, 8, 4, 4, 3>), grid, threads, 0, st, a);
+    } else if constexpr (KIND == K_WIDE) {
+        hipLaunchKernelGGL((k_a8_tile<EPI, SW, 2, 4, 4, 4, 4, 4>), grid, threads, 0, st, a);
     } else if (p.slices == 1) {
         hipLaunchKernelGGL((k_a8_tile<EPI, SW, 2, 2, 4, 4, 4, 3>), grid, threads, 0, st, a);
     } else {
@@ -656,14 +670,15 @@ void launch_stream(const A8Args& a, hipStream_t st) {
 
 template <int EPI>
 void launch(const A8Args& a, const Plan& p, hipStream_t st) {
-    constexpr int ALL = 1 << 30;
+    const int all = ceil_div(a.tiles, EPI == EPI_SWIGLU ? 8 : 16);
     if (p.kind == K_T256) {
-        launch_tile<EPI, true>(a, p, 0, p.cols, st);
-        if (p.cols < ceil_div(a.tiles, EPI == EPI_SWIGLU ? 8 : 16))
-            launch_tile<EPI, false>(a, p, 2 * p.cols, ALL, st);
+        launch_tile<EPI, K_T256>(a, p, 0, p.cols, st);
+        if (p.rest == K_T128) launch_tile<EPI, K_T128>(a, p, p.cols, all, st);
+        if (p.rest == K_WIDE) launch_tile<EPI, K_WIDE>(a, p, p.cols, all, st);
         return;
     }
-    if (p.kind == K_T128) return launch_tile<EPI, false>(a, p, 0, ALL, st);
+    if (p.kind == K_WIDE) return launch_tile<EPI, K_WIDE>(a, p, 0, all, st);
+    if (p.kind == K_T128) return launch_tile<EPI, K_T128>(a, p, 0, all, st);
     const StreamShape f = stream_shape(a.M, a.tiles, a.K, EPI == EPI_SWIGLU ? 2 : 1);
     if (f.mt == 1 && f.nt == 2) return launch_stream<EPI, 1, 2, 4, 2>(a, st);
     if (f.mt == 1 && f.waves == 8) return launch_stream<EPI, 1, 1, 8, 2>(a, st);

@@ -22,8 +22,11 @@ pytestmark = pytest.mark.gpu
     # tiles of 128 x 128, whole and with K in 2, 4 and 8 slices, odd blocks of K
     (150, 8200, 192), (513, 4100, 1984), (50, 9000, 9792), (50, 5003, 9792), (100, 2500, 9792),
     (100, 1040, 9792), (100, 5003, 2624),
+    # tiles of 128 x 256
+    (521, 9741, 448), (600, 9100, 1088), (521, 9741, 1024),
     # tiles of 256 x 256, alone and with columns left over
-    (2600, 5003, 192), (1500, 5003, 320), (700, 33000, 192), (4100, 8300, 192)])
+    (2600, 5003, 192), (1500, 5003, 320), (700, 33000, 192), (4100, 8300, 192),
+    (1573, 12985, 448), (1904, 5720, 448)])
 def test_matmul_a8_forms(hip, rng, M, N, K, epilogue):
     say(f"matmul_a8 M={M} N={N} K={K} epilogue={epilogue} forms")
     x, sx, q, sw, y = matmul_inputs(rng, M, N, K, epilogue)
