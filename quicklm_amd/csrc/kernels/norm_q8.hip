@@ -14,7 +14,7 @@
 // exact quotient, and squares of large values do not overflow. gfx950 runs
 // fp64 vector operations at the rate of fp32 ones and the kernel is bound by
 // memory, so this costs nothing that shows: 8192 x 4096 with the sum stored
-// moves 436 MB in 87 us, 5.0 TB/s, the rate of a plain copy.
+// moves 436 MB in 82 to 86 us, 5.1 TB/s and more, a plain copy's rate.
 
 #include "common.hpp"
 
@@ -241,16 +241,19 @@ extern "C" int qlm_add_rms_norm_q8(const float* x, int ldx, const float* delta, 
     if (rows > kMaxRows) return QLM_ERR_SHAPE;
     hipStream_t st = as_stream(stream);
     const int n4 = (n + 3) / 4;
-    // Few rows are bound by latency: more waves share one (1 x 2560 4.9 us with
+    // Few rows are bound by latency: more waves share one (1 x 2560 4.5 us with
     // 4 waves, 3.7 with 8). Many are bound by the loads in flight, of which a
-    // thread then has more (8192 x 2560 65 us with 4 waves, 69 with 8).
-    const bool few = rows <= 2048;
+    // thread then has more while its registers leave room for other rows (8192 x
+    // 2560 54 us with 4 waves of 3 vectors, 59 of 4, 61 with 8 of 2; 8192 x 4096
+    // 85 with 4 of 4, 82 with 8 of 2).
     if (n4 <= 64)
         launch<1, 1>(a, st);
     else if (n4 <= 256)
-        few ? launch<4, 1>(a, st) : launch<1, 4>(a, st);
+        rows <= 2048 ? launch<4, 1>(a, st) : launch<1, 4>(a, st);
+    else if (n4 <= 768)
+        rows < 1024 ? launch<8, 2>(a, st) : launch<4, 3>(a, st);
     else if (n4 <= 1024)
-        few ? launch<8, 2>(a, st) : launch<4, 4>(a, st);
+        launch<8, 2>(a, st);
     else if (n4 <= 4096)
         launch<16, 4>(a, st);
     else
@@ -262,5 +265,5 @@ extern "C" int qlm_add_rms_norm_q8(const float* x, int ldx, const float* delta, 
 // otherwise loads it at the first launch of one of its kernels.
 hipError_t qlm_load_norm_q8() {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(k_norm_q8<4, 4, true>));
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(k_norm_q8<4, 3, true>));
 }

@@ -7,7 +7,7 @@ import pytest
 
 from tests.test_score_ops_gpu import (RESIDUAL, STORE, SWIGLU, buf, check_logprobs, check_norm,
                                       logprobs_ref, matmul_inputs, matmul_ref, norm_ref,
-                                      run_matmul, tiles_of)
+                                      run_matmul, run_norm, tiles_of)
 from tests.util import say
 
 pytestmark = pytest.mark.gpu
@@ -44,6 +44,17 @@ def test_matmul_a8_tiles_of_few_blocks(hip, rng, M, K, epilogue):
     got = run_matmul(hip, x, sx, q, sw, y, epilogue)
     want, tol = matmul_ref(x, sx, q, sw, y, epilogue)
     assert (np.abs(got - want) <= tol * 1.0001 + 1e-37).all()
+
+
+@pytest.mark.parametrize("rows,n", [(1100, 1100), (1024, 2560), (1030, 3001), (1500, 4095),
+                                    (2100, 700), (2100, 200), (1023, 2560)])
+def test_norm_q8_many_rows(hip, rng, rows, n):
+    say(f"norm_q8 rows={rows} n={n}")
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    d = rng.standard_normal((rows, n)).astype(np.float32)
+    w = (rng.standard_normal(n) * 0.1).astype(np.float32)
+    check_norm(run_norm(hip, x, d, w, pad=3), norm_ref(x, d, w, 1e-6))
+    check_norm(run_norm(hip, x, None, w), norm_ref(x, None, w, 1e-6))
 
 
 def put(hip, p, a):
