@@ -115,3 +115,11 @@ def test_score_refusals(engine):
             call()
     lp, ent, ti, tl = e.score([], 0, 3)  # nothing to score
     assert lp.size == ent.size == 0 and ti.shape == tl.shape == (0, 3)
+
+
+def test_score_refuses_a_position_whose_sum_overflows(engine):
+    from quicklm_amd.engine import EngineError
+
+    say("score at the largest position")
+    with pytest.raises(EngineError):
+        engine.score(np.arange(8, dtype=np.int32), 2 ** 31 - 1)

@@ -113,3 +113,12 @@ def test_engine_score_refuses_a_null_handle():
     L = engine.lib()
     assert L.qlm_engine_score(None, None, 0, 0, 0, None, None, None, None) == 1
     assert b"null engine handle" in L.qlm_engine_last_error()
+
+
+@pytest.mark.parametrize("call,kw", [
+    (matmul, dict(M=1 << 20)), (matmul, dict(N=1 << 23, ldy=1 << 23)),
+    (logprobs, dict(rows=(1 << 21) + 1)),
+    (logprobs, dict(rows=2 ** 31 - 1, n=1, ldl=1, top=1)),
+])
+def test_more_than_a_launch_can_number(call, kw):
+    assert call(work_bytes=1 << 60, **kw) == SHAPE
