@@ -92,17 +92,28 @@ __device__ __forceinline__ f32x4u scaled(v4i s0, v4i s1, float sx, f32x4u w0, f3
     return v;
 }
 
+// What is added to, and a result: rounded as product and as sum in every form.
+// Contracted to a fused multiply-add, as the compiler does it in some forms and
+// for some columns, a row's bits would depend on the number of rows.
+__device__ __forceinline__ float added(float old, float v) {
+#pragma clang fp contract(off)
+    return old + v;
+}
+__device__ __forceinline__ f32x4u added(f32x4u old, f32x4u v) {
+    return f32x4u{added(old.x, v.x), added(old.y, v.y), added(old.z, v.z), added(old.w, v.w)};
+}
+
 // Stores (EPI_RESID: adds) the first `left` of four results.
 template <int EPI>
 __device__ __forceinline__ void put(float* dst, f32x4u v, int left) {
     if (left >= 4) {
-        if constexpr (EPI == EPI_RESID) v += *reinterpret_cast<const f32x4u*>(dst);
+        if constexpr (EPI == EPI_RESID) v = added(*reinterpret_cast<const f32x4u*>(dst), v);
         *reinterpret_cast<f32x4u*>(dst) = v;
         return;
     }
 #pragma unroll
     for (int i = 0; i < 3; ++i)
-        if (i < left) dst[i] = EPI == EPI_RESID ? dst[i] + v[i] : v[i];
+        if (i < left) dst[i] = EPI == EPI_RESID ? added(dst[i], v[i]) : v[i];
 }
 
 // Buffer descriptor of a uniform base: a load then takes a lane's 32-bit
@@ -472,7 +483,8 @@ __global__ __launch_bounds__(WM* WN* QLM_WAVE, 2) void k_a8_tile(A8Args a) {
                 const f32x4u v = scaled<EPI>(acc[g + i][j], acc[g + i][SW ? j + OF : j], sx[g + i],
                                              s0[j], SW ? s1[j] : s0[j]);
                 if (inside)
-                    *reinterpret_cast<f32x4u*>(y + 16 * j) = EPI == EPI_RESID ? old[i][j] + v : v;
+                    *reinterpret_cast<f32x4u*>(y + 16 * j) =
+                        EPI == EPI_RESID ? added(old[i][j], v) : v;
                 else if (ml + 16 * (g + i) < a.M)
                     put<EPI>(y + 16 * j, v, a.N - (nl + 16 * j));
             }
