@@ -64,30 +64,57 @@ __device__ __forceinline__ f32x4u load_scales(const float* sw, int n, int N) {
 // g / (1 + exp(-g)) in a third of the instructions of expf and a division:
 // exp2 of the product with log2 e, whose rounding error is put back, and a
 // reciprocal with one Newton step; off by 3 + 1 + 1 + 1 roundings at most (the
-// exponential, the sum, the reciprocal, the product). The epilogue of a
-// 2048 x 9728 SwiGLU took 10 us of a round's 40 with the library's.
+// exponential, the sum, the reciprocal, the product) down to kDeepGate. The
+// epilogue of a 2048 x 9728 SwiGLU took 10 us of a round's 40 with the library's.
+// Every fused multiply-add is written out, so all forms give the same bits.
+constexpr float kDeepGate = -80.0f;
 __device__ __forceinline__ float silu_fast(float g) {
+#pragma clang fp contract(off)
     constexpr float kLog2e = 1.44269502e0f, kRest = 1.92596303e-8f, kLn2 = 0.693147182f;
     const float c = fminf(g, 200.0f);  // (an infinite one has no rounding error)
     const float hi = c * -kLog2e;
-    const float lo = fmaf(c, -kLog2e, -hi) - c * kRest;
+    const float lo = fmaf(-c, kRest, fmaf(c, -kLog2e, -hi));
     float e = __builtin_amdgcn_exp2f(hi);
-    // past the range of fp32 the result is 0; 1 / 3e38 is still not a NaN
-    e = fminf(fmaf(e * kLn2, lo, e), 3e38f);
+    e = fmaf(e * kLn2, lo, e);
     const float d = 1.0f + e;
     float r = __builtin_amdgcn_rcpf(d);
     r = fmaf(fmaf(-d, r, 1.0f), r, r);
     return g * r;
 }
 
+// silu(g) * u for a gate below kDeepGate, where 1 + exp(-g) is exp(-g) to fp32
+// and soon past its range, its reciprocal below the normal range and flushed:
+// g exp(g) u with the exponential as the fourth power of exp(g / 4), multiplied
+// in an order in which nothing but the result can leave the range. Off by 8
+// roundings of the exponentials and 5 of the products, and by half the spacing
+// of subnormal numbers where it is one; 0 for -inf.
+__device__ __forceinline__ float silu_deep_mul(float g, float u) {
+#pragma clang fp contract(off)
+    const float c = fmaxf(g, -300.0f);  // 300 exp(-300) times anything is 0
+    const float h = expf(0.25f * c);
+    return (c * h) * (u * h * h) * h;
+}
+
 // Four results of one row from their sums (SwiGLU: gate and up sums).
 template <int EPI>
 __device__ __forceinline__ f32x4u scaled(v4i s0, v4i s1, float sx, f32x4u w0, f32x4u w1) {
-    f32x4u v;
+#pragma clang fp contract(off)
+    f32x4u v, u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float p = (float)s0[i] * sx * w0[i];
-        v[i] = EPI == EPI_SWIGLU ? silu_fast(p) * ((float)s1[i] * sx * w1[i]) : p;
+        v[i] = (float)s0[i] * sx * w0[i];
+        if constexpr (EPI == EPI_SWIGLU) u[i] = (float)s1[i] * sx * w1[i];
+    }
+    if constexpr (EPI == EPI_SWIGLU) {
+        f32x4u y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = silu_fast(v[i]) * u[i];
+        if (fminf(fminf(v.x, v.y), fminf(v.z, v.w)) < kDeepGate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (v[i] < kDeepGate) y[i] = silu_deep_mul(v[i], u[i]);
+        }
+        return y;
     }
     return v;
 }
