@@ -240,7 +240,7 @@ extern "C" int qlm_add_rms_norm_q8(const float* x, int ldx, const float* delta, 
     const NormArgs a{x, delta, w, sum, q, scales, ldx, ldd, lds, ldq, rows, n, eps};
     if (rows > kMaxRows) return QLM_ERR_SHAPE;
     hipStream_t st = as_stream(stream);
-    const int n4 = (n + 3) / 4;
+    const int n4 = n / 4 + (n % 4 != 0);  // n + 3 may pass 2^31
     // Few rows are bound by latency: more waves share one (1 x 2560 4.5 us with
     // 4 waves, 3.7 with 8). Many are bound by the loads in flight, of which a
     // thread then has more while its registers leave room for other rows (8192 x

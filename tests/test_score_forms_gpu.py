@@ -170,3 +170,28 @@ def test_token_logprobs_ties_over_many_chunks(hip, rng, rows, n, top, kind):
         if kind == "mixed":
             x[r, :300] = -np.inf
     check_logprobs(hip, x, rng.integers(0, n, (rows, 1)), top)
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 4, 2 ** 31 - 5])
+def test_norm_q8_longest_rows(hip, n):
+    """One row of up to 2^31 - 1 values, zero but for a few far apart; the gain
+    is the row itself, so t = r (1 + r). Each value is a whole number, so sums
+    and quotients are those of the definition."""
+    say(f"norm_q8 n={n}")
+    at = np.array([0, 5, 300, 70001, (1 << 30) + 7, n - 6, n - 3, n - 2, n - 1])
+    r = np.float64([3, -2, 5, 1, -6, 4, 2, -4, 6])
+    dx, dq, dsc = hip.DeviceBuffer(4 * n), hip.DeviceBuffer(n + 1), hip.DeviceBuffer(4)
+    dx.zero()
+    hip.call("qlm_fill_u8", dq, 99, n + 1, None)
+    for i, v in zip(at, r.astype(np.float32)):
+        put(hip, dx.ptr + 4 * int(i), np.array([v]))
+    hip.call("qlm_add_rms_norm_q8", dx, n, None, 0, dx, 1e-6, None, 0, dq, n, dsc, 1, n, None)
+    q = dq.to_numpy(n + 1, np.int8)
+    t = r * (1 + r)
+    top = np.abs(t).max()
+    scale = top / 127 / np.sqrt((r * r).sum() / n + np.float64(np.float32(1e-6)))
+    assert q[n] == 99
+    assert np.array_equal(q[at], np.rint(127 * t / top).astype(np.int8))
+    q[at] = 0
+    assert not q[:n].any()
+    assert abs(dsc.to_numpy(1, np.float32)[0] - scale) <= 2.0 ** -24 * scale * (1 + 1e-6)
