@@ -773,7 +773,7 @@ int DecoderModel::forward_greedy(int token, int pos) {
 void DecoderModel::forward_batch(const int* toks, int n, int pos, int* argmax, float* logits) {
     if (n <= 0) return;
     if (!toks) throw std::runtime_error("forward_batch: null tokens");
-    if (pos < 0 || pos + n > max_seq_)
+    if (pos < 0 || n > max_seq_ - pos)
         throw std::runtime_error("context length exceeded max_seq_len (" + std::to_string(max_seq_) +
                                  ")");
     for (int i = 0; i < n; ++i)
@@ -869,7 +869,7 @@ double DecoderModel::steps(int k, bool use_graph) {
     if (run_B_ == 0) throw std::runtime_error("steps: call start() first");
     // positions 0 .. run_steps_+k-1 are forwarded; the last token is written
     // at position run_steps_+k, which the token array must hold
-    if (run_steps_ + k > max_seq_)
+    if (k > max_seq_ - run_steps_)
         throw std::runtime_error("context length exceeded max_seq_len (" + std::to_string(max_seq_) +
                                  ")");
     // whole groups of kStepsPerGraph steps replay one graph each (the
@@ -899,7 +899,7 @@ double DecoderModel::steps(int k, bool use_graph) {
 }
 
 void DecoderModel::tokens(int b, int first, int count, int* out) const {
-    if (b < 0 || b >= run_B_ || first < 0 || first + count > ld_tokens_)
+    if (b < 0 || b >= run_B_ || first < 0 || count > ld_tokens_ - first)
         throw std::runtime_error("tokens: range outside the token stream");
     check(qlm_memcpy_d2h(out, tokens_.get<int>() + (size_t)b * ld_tokens_ + first,
                          (size_t)count * sizeof(int), stream_),
@@ -910,7 +910,8 @@ void DecoderModel::tokens(int b, int first, int count, int* out) const {
 void DecoderModel::generate(const int* prompts, int B, int n, int n_new, int* out, GenStats* st,
                             bool use_graph, int prefill_mode) {
     if (n_new < 0) throw std::runtime_error("generate: negative token count");
-    if (n + n_new - 1 > max_seq_)
+    if (n <= 0) throw std::runtime_error("generate: empty prompt");
+    if (n > max_seq_ || n_new > max_seq_ - n + 1)
         throw std::runtime_error("context length exceeded max_seq_len (" + std::to_string(max_seq_) +
                                  ")");
     const double t0 = now_s();
