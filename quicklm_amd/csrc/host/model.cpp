@@ -537,6 +537,7 @@ void DecoderModel::forward(int token, int pos, float* logits_host) {
 }
 
 void DecoderModel::last_logits(int b, float* host) const {
+    if (b < 0 || b >= max_batch_) throw std::runtime_error("last_logits: no such sequence");
     check(qlm_memcpy_d2h(host, logits_.get<float>() + (size_t)b * cfg_.vocab_size,
                          (size_t)cfg_.vocab_size * sizeof(float), stream_),
           "download");
@@ -867,6 +868,7 @@ void DecoderModel::score(const int* toks, int n, int pos, int top, float* logpro
 
 double DecoderModel::steps(int k, bool use_graph) {
     if (run_B_ == 0) throw std::runtime_error("steps: call start() first");
+    if (k < 0) throw std::runtime_error("steps: negative count");
     // positions 0 .. run_steps_+k-1 are forwarded; the last token is written
     // at position run_steps_+k, which the token array must hold
     if (k > max_seq_ - run_steps_)
@@ -899,7 +901,7 @@ double DecoderModel::steps(int k, bool use_graph) {
 }
 
 void DecoderModel::tokens(int b, int first, int count, int* out) const {
-    if (b < 0 || b >= run_B_ || first < 0 || count > ld_tokens_ - first)
+    if (b < 0 || b >= run_B_ || first < 0 || count < 0 || count > ld_tokens_ - first)
         throw std::runtime_error("tokens: range outside the token stream");
     check(qlm_memcpy_d2h(out, tokens_.get<int>() + (size_t)b * ld_tokens_ + first,
                          (size_t)count * sizeof(int), stream_),

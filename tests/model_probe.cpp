@@ -21,7 +21,8 @@
 #undef private
 
 // call 0 forward_batch(a tokens at b), 1 steps(a after b), 2 tokens(a from b),
-// 3 generate(prompt of a, b new), 4 score(a tokens at b). The error's text.
+// 3 generate(prompt of a, b new), 4 score(a tokens at b), 5 last_logits(of a).
+// The error's text.
 extern "C" void model_ranges(int call, int max_seq, int a, int b, char* err, int n) {
     qlm::DecoderModel m;
     m.max_seq_ = max_seq;
@@ -37,6 +38,7 @@ extern "C" void model_ranges(int call, int max_seq, int a, int b, char* err, int
         if (call == 2) m.tokens(0, b, a, out.data());
         if (call == 3) m.generate(some.data(), 1, a, b, out.data(), nullptr);
         if (call == 4) m.score(some.data(), a, b, 0, nullptr, nullptr, nullptr, nullptr);
+        if (call == 5) m.last_logits(a, reinterpret_cast<float*>(out.data()));
     } catch (const std::exception& e) {
         text = e.what();
     }

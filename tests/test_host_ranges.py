@@ -15,7 +15,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "quicklm_amd")
 BIG = 2 ** 31 - 1
 MAX_SEQ = 512
-BATCH, STEPS, TOKENS, GENERATE, SCORE = range(5)
+BATCH, STEPS, TOKENS, GENERATE, SCORE, LOGITS = range(6)
 
 
 @pytest.fixture(scope="module")
@@ -61,3 +61,14 @@ def test_a_range_past_the_context_is_refused(call, which, a, b, text):
     (TOKENS, 8, MAX_SEQ - 7), (GENERATE, 8, MAX_SEQ - 7)])
 def test_a_range_that_fits_reaches_the_device(call, which, a, b):
     assert call(which, a, b) not in (EXCEEDED, OUTSIDE, "no error")
+
+
+@pytest.mark.parametrize("which,a,b,text", [
+    # a negative number of steps would move the count of positions back
+    (STEPS, -1, 5, "steps: negative count"), (STEPS, -BIG - 1, 0, "steps: negative count"),
+    (TOKENS, -1, 5, OUTSIDE), (TOKENS, -BIG - 1, 0, OUTSIDE),
+    (LOGITS, -1, 0, "last_logits: no such sequence"),
+    (LOGITS, 1, 0, "last_logits: no such sequence"),
+    (LOGITS, BIG, 0, "last_logits: no such sequence")])
+def test_a_negative_count_or_another_sequence_is_refused(call, which, a, b, text):
+    assert call(which, a, b) == text
