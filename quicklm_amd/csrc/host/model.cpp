@@ -823,8 +823,9 @@ void DecoderModel::score(const int* toks, int n, int pos, int top, float* logpro
     const int V = cfg_.vocab_size;
     for (int i = 0; i < n; ++i)
         if (toks[i] < 0 || toks[i] >= V) throw std::runtime_error("score: token id out of range");
-    const size_t work = qlm_token_logprobs_workspace_bytes(1, V, top);
-    if (top < 0 || top > std::min(V, QLM_TOKEN_LOGPROBS_MAX_TOP) || work == 0)
+    if (qlm_token_logprobs_workspace_bytes(1, V, 0) == 0)
+        throw std::runtime_error("score: vocabulary too large");
+    if (top < 0 || top > std::min(V, QLM_TOKEN_LOGPROBS_MAX_TOP))
         throw std::runtime_error("score: top out of range");
     if (top > 0 && (!top_ids || !top_logprobs)) throw std::runtime_error("score: null output");
     // one buffer: next tokens, log probabilities, entropies, alternatives

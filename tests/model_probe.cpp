@@ -21,8 +21,8 @@
 #undef private
 
 // call 0 forward_batch(a tokens at b), 1 steps(a after b), 2 tokens(a from b),
-// 3 generate(prompt of a, b new), 4 score(a tokens at b), 5 last_logits(of a).
-// The error's text.
+// 3 generate(prompt of a, b new), 4 score(a tokens at b), 5 last_logits(of a),
+// 6 score(2 tokens at 0 over a vocabulary of a, b alternatives). The error's text.
 extern "C" void model_ranges(int call, int max_seq, int a, int b, char* err, int n) {
     qlm::DecoderModel m;
     m.max_seq_ = max_seq;
@@ -39,6 +39,11 @@ extern "C" void model_ranges(int call, int max_seq, int a, int b, char* err, int
         if (call == 3) m.generate(some.data(), 1, a, b, out.data(), nullptr);
         if (call == 4) m.score(some.data(), a, b, 0, nullptr, nullptr, nullptr, nullptr);
         if (call == 5) m.last_logits(a, reinterpret_cast<float*>(out.data()));
+        if (call == 6) {
+            m.cfg_.vocab_size = a;
+            m.score(some.data(), 2, 0, b, nullptr, nullptr, out.data(),
+                    reinterpret_cast<float*>(out.data()));
+        }
     } catch (const std::exception& e) {
         text = e.what();
     }

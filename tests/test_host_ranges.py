@@ -15,7 +15,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "quicklm_amd")
 BIG = 2 ** 31 - 1
 MAX_SEQ = 512
-BATCH, STEPS, TOKENS, GENERATE, SCORE, LOGITS = range(6)
+BATCH, STEPS, TOKENS, GENERATE, SCORE, LOGITS, WIDE = range(7)
 
 
 @pytest.fixture(scope="module")
@@ -72,3 +72,11 @@ def test_a_range_that_fits_reaches_the_device(call, which, a, b):
     (LOGITS, BIG, 0, "last_logits: no such sequence")])
 def test_a_negative_count_or_another_sequence_is_refused(call, which, a, b, text):
     assert call(which, a, b) == text
+
+
+@pytest.mark.parametrize("vocab,top,text", [
+    ((1 << 21) + 1, 0, "score: vocabulary too large"), (BIG, 5, "score: vocabulary too large"),
+    (1 << 21, 65, "score: top out of range"), (4, 5, "score: top out of range"),
+    (4, -1, "score: top out of range")])
+def test_score_names_what_it_refuses(call, vocab, top, text):
+    assert call(WIDE, vocab, top) == text
