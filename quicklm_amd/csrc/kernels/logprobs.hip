@@ -99,7 +99,6 @@ __device__ __forceinline__ f32x4u load_chunk(const float* row, int n, int c) {
 
 // Floats as integers in their order, -0 as +0, NaN as -inf.
 constexpr int kLowest = (int)0xff800000 ^ 0x7fffffff;  // order of -inf
-constexpr int kPast = 0x7f800001;                      // above the order of +inf
 __device__ __forceinline__ int order_of(float v) {
     const int b = __float_as_int(v + 0.0f);
     return v != v ? kLowest : b < 0 ? b ^ 0x7fffffff : b;
