@@ -310,10 +310,13 @@ int qlm_matmul_i8_t_whole_config(const float* x, int ldx, const float* norm_w, f
  * qlm_quantize_q8_f32 with group K), int8 weights with one scale a row:
  * tile-major q_tiles (qlm_mx_swizzle with group K) and s_rows as quantised
  * ([2N] for SwiGLU: gate rows, then up rows). On the int8 matrix cores; the
- * sums are exact in int32 and rounded to fp32 once, so the result differs
- * from the exact one by a few fp32 roundings only, in every form, and a row's
- * result is the same whatever rows are beside it. epilogue
- * 0: y = result; 1: y += result; 2: SwiGLU, y = silu(gate) * up (N outputs).
+ * sums are exact in int32, rounded to fp32 once, multiplied by the row's scale
+ * and then by the channel's (a sum times its row's scale has to lie within
+ * fp32). Each step is rounded by itself, so the result differs from the exact
+ * one by a few fp32 roundings only, and a row's result is the same bits
+ * whatever rows are beside it. epilogue
+ * 0: y = result; 1: y += result; 2: SwiGLU, y = silu(gate) * up (N outputs;
+ * a gate of -inf leaves 0).
  * M below 2^20, N below 2^23, K a multiple of 64 below 2^17; x and q_tiles 16-byte
  * aligned, ldx a multiple of 16 below 2^23; y of any stride and alignment,
  * its columns past N left as they are. work: device scratch of
@@ -356,13 +359,14 @@ int qlm_add_rms_norm(float* res, const float* delta, const float* w, float* y, i
  * fp32): r = x + delta (delta NULL: r = x), y = r / sqrt(mean(r^2) + eps) *
  * (1 + w), scales[row] = max|y| / 127 (1 for a row of zeros; NaN if eps is
  * 0 too), q = y / scale rounded to the nearest whole number, ties to even.
- * Statistics and quotient are held in 64 bits, so the bytes are those of the
- * exact quotient. sum (may be NULL;
- * needs delta) receives r; it may be x or delta itself with the same row
+ * 1 + w, statistics and quotient are held in 64 bits, so the bytes are those
+ * of the exact quotient but where it lies within 1e-13 of a border. sum (may be
+ * NULL; needs delta) receives r; it may be x or delta itself with the same row
  * stride, and overlaps neither otherwise. A row with a value that is not
- * finite gets scale NaN and bytes 0: its products come out NaN. x [rows,
- * ldx], delta [rows, ldd], sum [rows, lds] fp32, q [rows, ldq]; any n and
- * alignment; rows at most 2^21; columns past n are left as they are. */
+ * finite (a sum past fp32 among them), or whose scale is past fp32, gets scale
+ * NaN and bytes 0: its products come out NaN. x [rows, ldx], delta [rows, ldd],
+ * sum [rows, lds] fp32, q [rows, ldq]; any n and alignment; rows at most 2^21;
+ * columns past n are left as they are. */
 int qlm_add_rms_norm_q8(const float* x, int ldx, const float* delta, int ldd, const float* w,
                         float eps, float* sum, int lds, int8_t* q, int ldq, float* scales,
                         int rows, int n, void* stream);
