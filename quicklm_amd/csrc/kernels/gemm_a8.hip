@@ -21,10 +21,12 @@
 //                busy 0.43 us of a block's 0.5 to 0.64, and by the writing of
 //                the outputs at a round's end (a quarter of a round of K 4096).
 // Measured on an MI355X, operands cold in the caches, us (and the larger of
-// the bytes' time at 4.75 TB/s and the products' at 2134 TOP/s): 1 x 9728 x
-// 2560 SwiGLU 11.5 (10.5), 16 x 2560 x 9728 9.1 (5.4), 1000 x 2560 x 2560 18.7
-// (6.1), 1000 x 6144 x 2560 27.9 (14.7), 2048 x 9728 x 2560 SwiGLU 105 to 110
-// from card to card (96), 4096 x 12288 x 4096 178 to 190 (193).
+// the bytes' time at a 4 GiB copy's 4.75 TB/s and the products' at the 2134
+// TOP/s of an 8192-wide int8 library product): 1 x 9728 x 2560 SwiGLU 11.6
+// (10.5), 16 x 2560 x 9728 10.7 (5.4), 64 x 2560 x 9728 16.0 (5.7), 512 x 2560 x
+// 2560 18.5 (3.9), 1000 x 2560 x 2560 19 (6.1), 1000 x 6144 x 2560 28 (14.7),
+// 2048 x 9728 x 2560 SwiGLU 104 to 110 from card to card (96), 4096 x 12288 x
+// 4096 178 to 190 (193), 8192 x 8192 x 8192 424 (515; 2.6 POP/s).
 
 #include <algorithm>
 

@@ -12,10 +12,10 @@
 // rounding error (2^-24 of up to 127 steps) moves about one byte in 10^5 to
 // the other side of a rounding border; in 64 bits the byte is that of the exact
 // quotient, unless that lies within 127 2^-50 of a border, and squares of large
-// values do not overflow. gfx950 runs
-// fp64 vector operations at the rate of fp32 ones and the kernel is bound by
-// memory, so this costs nothing that shows: 8192 x 4096 with the sum stored
-// moves 436 MB in 82 to 86 us, 5.1 TB/s and more, a plain copy's rate.
+// values do not overflow. gfx950 runs fp64 vector operations at the rate of
+// unpacked fp32 ones and the kernel is bound by memory, so this costs nothing
+// that shows: 8192 x 4096 with the sum stored moves 436 MB in 82 to 87 us, 5.0
+// to 5.3 TB/s, where a 4 GiB copy reaches 4.75.
 
 #include "common.hpp"
 
@@ -246,7 +246,12 @@ extern "C" int qlm_add_rms_norm_q8(const float* x, int ldx, const float* delta, 
     // 4 waves, 3.7 with 8). Many are bound by the loads in flight, of which a
     // thread then has more while its registers leave room for other rows (8192 x
     // 2560 54 us with 4 waves of 3 vectors, 59 of 4, 61 with 8 of 2; 8192 x 4096
-    // 85 with 4 of 4, 82 with 8 of 2).
+    // 85 with 4 of 4, 82 with 8 of 2). Up to 1024 values a wave takes a row alone
+    // once rows are many (n 1024, four waves a row and one: 2048 rows 9.9 and 11.4
+    // us, 4096 rows 16.5 and 15.8, 16384 rows 49.2 and 47.6). From 4097 values on 16
+    // waves hold the row up to 16384 of them, which beats reading it twice also
+    // where most of their places are empty (2048 x 5120 35.8 us and 40.3, 8192 x
+    // 8192 167 and 183, 2048 x 16384 87 and 99).
     if (n4 <= 64)
         launch<1, 1>(a, st);
     else if (n4 <= 256)
