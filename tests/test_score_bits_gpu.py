@@ -1,11 +1,13 @@
 """The 8-bit matrix product's bits: the number of rows picks the form (streamed,
 tiles of three sizes, K in slices), and a row's result is the same in each, with
-every rounding of the epilogue where the definition has it."""
+every rounding of the epilogue where the definition has it. The token log
+probabilities' bits, whose form the number of alternatives picks."""
 
 import numpy as np
 import pytest
 
-from tests.test_score_ops_gpu import RESIDUAL, STORE, SWIGLU, matmul_inputs, run_matmul, tiles_of
+from tests.test_score_ops_gpu import (RESIDUAL, STORE, SWIGLU, matmul_inputs, run_logprobs,
+                                      run_matmul, tiles_of)
 from tests.util import say
 
 pytestmark = pytest.mark.gpu
@@ -92,3 +94,21 @@ def test_matmul_a8_swiglu_gate_past_the_range(hip, M):
     assert np.isposinf(got[:, 0::3]).all()
     assert (got[:, 1::3] == 0).all()
     assert np.isnan(got[:, 2::3]).all()
+
+
+@pytest.mark.parametrize("rows,n", [(1, 300), (3, 151936), (20, 9000), (256, 16384), (300, 70001),
+                                    (800, 5003), (800, 40000), (3000, 700)])
+def test_token_logprobs_bits_whatever_is_asked_for(hip, rng, rows, n):
+    """The sums' order goes by rows and n alone: any number of alternatives
+    leaves the same log probabilities and entropies, and fewer alternatives are
+    the first of more."""
+    x = (rng.standard_normal((rows, n)) * rng.uniform(0.5, 6, (rows, 1))).astype(np.float32)
+    x[::5, rng.integers(0, n, n // 3)] = -np.inf
+    ids = rng.integers(0, n, (rows, 2))
+    say(f"logprobs bits rows={rows} n={n} top=64")
+    lp, H, ti, tl = run_logprobs(hip, x, ids, 64)
+    for top in (0, 1, 5, 8, 9, 24, 25, 40):
+        say(f"logprobs bits rows={rows} n={n} top={top}")
+        got = run_logprobs(hip, x, ids, top)
+        for a, b in zip(got, (lp, H, ti[:, :top], tl[:, :top])):
+            assert np.array_equal(a, b, equal_nan=a.dtype == np.float32), top

@@ -64,3 +64,36 @@ def test_score_over_several_passes(model_dir):
         assert np.array_equal(e.generate(prompt, 12)[0], before)
     finally:
         e.close()
+
+
+def test_score_without_some_outputs(model_dir):
+    """Outputs that are not wanted may be null; alternatives need both arrays."""
+    from quicklm_amd.engine import Engine, lib
+
+    e = Engine(model_dir, max_seq_len=128, max_batch=1, precision="int8")
+    try:
+        toks = np.random.default_rng(5).integers(0, e.vocab, 70).astype(np.int32)
+        say("score without some outputs")
+        e.reset()
+        lp, ent, ti, tl = e.score(toks, 0, 3)
+        want = e.forward_greedy(1, 70)
+
+        def call(top, *outs):
+            e.reset()
+            return lib().qlm_engine_score(e.h, toks.ctypes.data, toks.size, 0, top,
+                                          *(None if a is None else a.ctypes.data for a in outs))
+
+        a, b = np.empty_like(lp), np.empty_like(ent)
+        ids, lps = np.empty_like(ti), np.empty_like(tl)
+        for top, outs, wants in ((0, (None,) * 4, ()), (0, (a, None, None, None), ((a, lp),)),
+                                 (0, (None, b, None, None), ((b, ent),)),
+                                 (3, (None, None, ids, lps), ((ids, ti), (lps, tl)))):
+            for o in (a, b, ids, lps):
+                o.fill(-7)
+            assert call(top, *outs) == 0
+            for got, w in wants:
+                assert np.array_equal(got, w, equal_nan=got.dtype == np.float32)
+            assert e.forward_greedy(1, 70) == want
+        assert call(3, a, b, None, lps) != 0 and call(3, a, b, ids, None) != 0
+    finally:
+        e.close()
