@@ -544,6 +544,139 @@ int qlm_attention_decode_noalloc(const float* q, const void* k_cache, const void
                                  int kv_dtype, int max_seq, int ctx, float* out, int B, int n_q,
                                  int n_kv, int hd, void* stream);
 
+/* ---- ragged rows, trees of drafted tokens and a paged KV cache ---------------
+ * (no counterpart in the reference, whose cache is contiguous and whose drafts
+ * are a chain; its design notes leave paging unbuilt)
+ *
+ * The rows of a call: sequence b owns rows row_start[b] .. row_start[b + 1] - 1
+ * (none, one or many), which follow the ctx_len[b] positions whose keys and
+ * values its cache already holds: its row i goes to slot ctx_len[b] + i.
+ * parent NULL: row i follows row i - 1. Otherwise the rows are a tree:
+ * parent[r] is the row of the same sequence, counted from its first, that row r
+ * follows (an earlier one), or -1 for one that follows the context directly. A
+ * row's LINE is itself, the row it follows and so on up. A row with any other
+ * parent, a row below one, and every row past a sequence's first QLM_TREE_MAX
+ * are outside the tree: they see nothing, nothing sees them and their outputs
+ * are 0. Rows of no sequence (before row_start[0], from row_start[B] on) are
+ * left as they were. The arrays are device memory and read by the kernels
+ * alone, so one captured graph serves any contents. row_start never falls; a
+ * value outside 0..rows counts as the nearer end, as does a ctx_len outside
+ * 0..2^30. */
+#define QLM_TREE_MAX 64
+typedef struct qlm_row_batch {
+    int B;                /* sequences, at most 65535 */
+    int rows;             /* rows that the call's arrays hold, at most 2^21 */
+    const int* row_start; /* [B + 1] */
+    const int* ctx_len;   /* [B] */
+    const int* parent;    /* [rows], or NULL */
+} qlm_row_batch;
+
+/* Keys and values in pages of page_size slots (a power of two, 16 to 256):
+ * [n_pages, n_kv, page_size, hd], so that a head's slots of a page are one
+ * piece of memory. Slot s of sequence b is slot s % page_size of page
+ * table[b * ld_table + s / page_size]. Slots from ld_table * page_size on, and
+ * those of a page number outside 0..n_pages-1, are not there: not written, and
+ * seen by no row. What lies in slots that no row sees is never used, NaN
+ * included. dtype 0 = fp32, 1 = bf16 (rounded to nearest even when written);
+ * hd 128 or 256; k, v 16-byte aligned. */
+typedef struct qlm_kv_pages {
+    void* k;
+    void* v;
+    int dtype;
+    int n_pages;
+    int page_size;
+    int n_kv;
+    int hd;
+    const int* table; /* [B, ld_table] */
+    int ld_table;     /* at most 2^30 / page_size */
+} qlm_kv_pages;
+
+/* New rows into the pages: of each row of qkv [rows, ldqkv], laid out as
+ * qlm_gqa_prefill's, the query and key heads normalised (zero-centred gain,
+ * eps 1e-6; q_norm, k_norm [hd] or NULL: not), their first rot_dim elements
+ * rotated (pairs j, j + rot_dim / 2), the queries written to q_out
+ * [rows, ldq] (n_q heads of hd; qkv is not changed and must not overlap it), the
+ * keys and the values to their slots. The gate part of qkv is not read.
+ * Pair j of row r turns by row positions[pair_axis[j] * ld_pos + r] of the
+ * tables [n_pos, rot_dim / 2]: positions [n_axes, ld_pos] int32, pair_axis
+ * [rot_dim / 2] int32 of 0..n_axes-1, NULL: axis 0 for all. positions NULL: a
+ * row's position is ctx_len plus the number of rows above it on its line. A
+ * position outside 0..n_pos-1, or an axis that is not there, leaves NaN in its
+ * pair. Rows outside the tree: queries 0, no slot written. Two rows never share
+ * a slot unless two sequences share a page there, which must then not be
+ * written by both. */
+int qlm_paged_append(const float* qkv, int ldqkv, const float* q_norm, const float* k_norm,
+                     const float* cos_tab, const float* sin_tab, int n_pos, int rot_dim,
+                     const int* positions, int ld_pos, const int* pair_axis, int n_axes,
+                     const qlm_row_batch* batch, const qlm_kv_pages* pages, float* q_out, int ldq,
+                     int n_q, int gated, void* stream);
+
+/* Attention of the rows over the pages, after qlm_paged_append has written
+ * theirs: head h of row r of sequence b
+ *   out[r, h] = softmax(q . K^T / sqrt(hd)) . V * sigmoid(gate)
+ * over slots 0..ctx_len[b]-1 and those of the rows of r's line (parent NULL:
+ * of the rows up to r). q [rows, ldq], out [rows, ldo]: n_q heads of hd, not
+ * overlapping; n_q / n_kv 1, 2, 4 or 8. gate NULL: none; else head h's gate of
+ * row r is at gate + r * ldg + h * gate_stride (qkv + hd, ldqkv and 2 * hd after
+ * a gated qlm_paged_append). A row that sees nothing gives 0. Products run on
+ * the bf16 matrix cores: queries, probabilities and fp32 keys and values each
+ * split into two bf16 terms (to 2^-17), sums, maxima and exponentials in fp32;
+ * results that do not come out finite are computed again in fp32. Single
+ * tokens, trees, prompts and mixtures take the same call; a long context is
+ * split over the GPU and joined, by lengths that are read on the device, so
+ * the sums' order depends on the batch's lengths. work: device scratch of
+ * qlm_paged_attention_workspace_bytes(rows, B, n_q, n_kv, hd, slots) bytes, slots
+ * = ld_table * page_size, 16-byte aligned, no initial contents needed; calls
+ * sharing it must be ordered on one stream. The size may fall as rows grow:
+ * one workspace for calls of several sizes is as large as the largest of them
+ * asks for. 0 for sizes that are refused. */
+size_t qlm_paged_attention_workspace_bytes(int rows, int B, int n_q, int n_kv, int hd,
+                                           long long slots);
+int qlm_paged_attention(const float* q, int ldq, const qlm_row_batch* batch,
+                        const qlm_kv_pages* pages, const float* gate, int ldg, int gate_stride,
+                        float* out, int ldo, int n_q, void* work, size_t work_bytes, void* stream);
+
+/* The end of a greedy verification: tokens [rows] are the tree's tokens, picks
+ * [rows] the target's greedy token after each row (qlm_argmax). A sequence's
+ * row 0 (parent -1) is the token that the last step chose and is always
+ * accepted; then, as long as there is one, the first row that follows the last
+ * accepted row and holds its pick. path [B, ld_path] int32, ld_path >=
+ * QLM_TREE_MAX: the accepted rows in order, then -1; accepted [B]: their number;
+ * next_token [B]: the pick of the last one, the sequence's next row 0 (-1 for a
+ * sequence without rows); new_len [B]: ctx_len + accepted (not ctx_len itself,
+ * or NULL). The accepted rows' keys and values move to slots ctx_len + 0, 1, ..,
+ * in `layers` layers, layer i's pools at pages->k, pages->v + i * layer_stride
+ * elements; the other slots are left as they were. batch->parent is needed. A
+ * second call on the same batch would move what the first has moved. */
+int qlm_tree_commit(const int* tokens, const int* picks, const qlm_row_batch* batch,
+                    const qlm_kv_pages* pages, int layers, long long layer_stride, int* path,
+                    int ld_path, int* accepted, int* next_token, int* new_len, void* stream);
+
+/* The Gated DeltaNet mixer of qlm_deltanet_decode over a tree: every row's
+ * convolution, recurrence and output as if its line's rows alone had followed
+ * the sequence's state [B, H, d, d] and conv ring [B, 3, 3*H*d] (oldest tap row =
+ * ctx_len[b] % 3), neither of which is changed. Rows past a sequence's first
+ * QLM_TREE_MAX are outside, without a parent array too. proj, out as
+ * qlm_deltanet_prefill's, within 1e-4 of it (reassociated fp32). d = 128. work:
+ * device scratch of qlm_deltanet_tree_workspace_bytes(rows, H, d) bytes (0 for
+ * sizes that are refused), 16-byte aligned, no initial contents needed; calls
+ * sharing it must be ordered on one stream. */
+size_t qlm_deltanet_tree_workspace_bytes(int rows, int H, int d);
+int qlm_deltanet_tree(const float* proj, int ldp, const qlm_row_batch* batch,
+                      const float* conv_state, const float* conv_w_t, const float* A_log,
+                      const float* dt_bias, const float* norm_w, const float* state, float* out,
+                      int ldo, int H, int d, void* work, size_t work_bytes, void* stream);
+
+/* The states' and rings' advance along the accepted rows, given as
+ * qlm_tree_commit leaves them: sequence b's first accepted[b] entries of path
+ * (at most QLM_TREE_MAX; it ends at an entry that is no row of the sequence). proj is
+ * the verification's; batch->parent is not read. state and conv_state are left
+ * as a decode step at position ctx_len + accepted expects them. */
+int qlm_deltanet_tree_commit(const float* proj, int ldp, const qlm_row_batch* batch,
+                             const int* path, int ld_path, const int* accepted,
+                             float* conv_state, const float* conv_w_t, const float* A_log,
+                             const float* dt_bias, float* state, int H, int d, void* stream);
+
 /* ---- A14: greedy sampling ---------------------------------------------------
  * DecoderModel::sample with temperature <= 0 (model.cpp:263-274): index of
  * the first maximum (strict >, lowest index wins ties) of each of the B rows

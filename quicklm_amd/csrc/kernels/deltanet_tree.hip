@@ -1,0 +1,606 @@
+// The Gated DeltaNet mixer over a tree of drafted tokens (qlm_deltanet_tree) and
+// the states' advance along the accepted path (qlm_deltanet_tree_commit).
+//
+// A node t follows its parent p: S_t = a_t S_p + k_t w_t^T with w_t = b_t (v_t -
+// a_t S_p^T k_t), o_t = S_t^T q_t / sqrt(d). No node's state is formed: with g_t
+// the product of the a over t's line (itself and all above it),
+//   S_t = g_t S + sum over s on t's line of (g_t / g_s) k_s w_s^T,
+// S the sequence's state, so that
+//   (I + A) W = R,  A_ts = b_t (g_t / g_s) k_t . k_s  for s strictly above t,
+//                   R_t  = b_t (v_t - g_t S^T k_t)
+//   o_t = (g_t S^T q_t + sum over s on t's line of (g_t / g_s) (q_t . k_s) w_s) / sqrt(d).
+// Parents come before their children, so A is strictly lower triangular and W
+// follows by substitution; a chain is a tree like any other. The state is read
+// once and, in a verification, not written.
+//
+// A workgroup takes one head of one sequence and 16 NC of its 128 value
+// columns. Products run on the fp32 matrix cores. Logarithms of the decays are
+// summed in 64 bits along each line: a ratio of two products far below the fp32
+// range is as good as any other.
+
+#include "paged.hpp"
+
+namespace {
+
+constexpr int kD = 128;
+constexpr int kThreads = 256, kNW = kThreads / QLM_WAVE;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct TreeArgs {
+    const float* proj;
+    const float* conv;  // [B, 3, 3 H d]
+    const float* wt;    // [4, 3 H d]
+    const float* A_log;
+    const float* dt_bias;
+    const float* norm_w;
+    float* state;  // read, or advanced (commit)
+    float* raw;    // outputs before their head norm [rows, H d]
+    float* out;
+    const int *path, *accepted;  // commit: the rows to advance along
+    long long ldp, ldo;
+    int H, ld_path;
+    qlm_row_batch bt;
+};
+
+template <int TM, int NC>
+struct TreeShared {
+    static constexpr int QS = kD + 4, TS = TM + 4, WS = 16 * NC + 4;  // row strides
+    float q[TM][QS];   // conv inputs, then outputs after SiLU (not normalised)
+    float k[TM][QS];
+    float w[TM][WS];   // v, then R, then W
+    float at[TM][TS];  // A transposed: at[s][t]
+    float m[TM][TS];   // (g_t / g_s) (q_t . k_s) / sqrt(d), s on t's line
+    double c[TM];      // log g
+    unsigned long long line[TM];
+    int tap[TM][4];    // where a node's conv inputs lie, oldest first: a node, or -1 - ring row
+    float beta[TM], sq[TM], sk[TM];  // b; 1 / |q| and 1 / |k|
+    int row[TM];       // proj rows
+    int bad;           // a node whose outputs did not come out finite
+};
+
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// 32 floats of a row: an operand's elements 32 qd .. + 31 (step s: element 32 qd + s)
+__device__ __forceinline__ void load32(float (&d)[32], const float* p) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p + 4 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[4 * j + i] = x[i];
+    }
+}
+
+__device__ __forceinline__ f32x4 dot32(const float (&a)[32], const float (&b)[32]) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+#pragma unroll
+    for (int s = 0; s < 32; s += 2) {
+        x = mfma4(a[s], b[s], x);
+        y = mfma4(a[s + 1], b[s + 1], y);
+    }
+    return x + y;
+}
+
+// lane n of this lane's 16-lane row
+template <int n>
+__device__ __forceinline__ float row_lane(float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + n, 0xf, 0xf, false));
+}
+
+// Forward substitution: lane (r, j) = (l % 16, l / 16) holds rows RP r .. of
+// columns NC of its own; step t takes w_t from lane t / RP and leaves
+// A_{t', t} w_t out of every later row's rest.
+template <int TM, int NC, int T0>
+__device__ __forceinline__ void solve_from(const float (&at)[TM][TM + 4],
+                                           float (&x)[NC][TM / 16], int nodes) {
+    constexpr int RP = TM / 16;
+    if constexpr (T0 < 16) {
+        if (T0 * RP >= nodes) return;
+        const int r = threadIdx.x & 15;
+#pragma unroll
+        for (int i = 0; i < RP; ++i) {
+            float a[RP];
+#pragma unroll
+            for (int e = 0; e < RP; ++e) a[e] = at[T0 * RP + i][RP * r + e];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float w = row_lane<T0>(x[c][i]);
+#pragma unroll
+                for (int e = 0; e < RP; ++e) x[c][e] = fmaf(-a[e], w, x[c][e]);
+            }
+        }
+        solve_from<TM, NC, T0 + 1>(at, x, nodes);
+    }
+}
+
+// Decay's logarithm and b of a row.
+__device__ __forceinline__ void gates(const TreeArgs& a, int row, int h, double& alpha,
+                                      float& beta) {
+    const float* g = a.proj + (size_t)row * a.ldp + 4 * (size_t)a.H * kD;
+    const float dt = g[a.H + h] + a.dt_bias[h];
+    const float sp = dt > 20.0f ? dt : log1pf(expf(dt));
+    const float x = -expf(a.A_log[h]) * sp;
+    alpha = x < -1e4f ? -1e4 : (double)x;  // (0 in fp32 long before)
+    beta = sigmoid_f(g[h]);
+}
+
+template <int TM, int NC, bool COMMIT>
+__global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
+    using SH = TreeShared<TM, NC>;
+    constexpr int CW = 16 * NC, SPLIT = kD / CW, RT = TM / 16, P = kNW / RT;
+    constexpr float kScale = 0.08838834764831845f;  // 1 / sqrt(d)
+    __shared__ __align__(16) SH sh;
+    const int h = blockIdx.x / SPLIT, c0 = blockIdx.x % SPLIT * CW, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, qd = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / QLM_WAVE);
+    const int HD = a.H * kD, C = 3 * HD;
+    const SeqRows sq = seq_rows(a.bt, b);
+
+    // ---- the nodes: rows, lines, decays (a lane a node, every wave alike) ----
+    int T, row = sq.first, parent;
+    if constexpr (COMMIT) {
+        const int want = min(max(a.accepted[b], 0), min(a.ld_path, QLM_TREE_MAX));
+        const int p = lane < want ? a.path[(size_t)b * a.ld_path + lane] : -1;
+        const unsigned long long ends = __ballot(p < 0 || p >= sq.n);
+        T = ends ? __ffsll((long long)ends) - 1 : QLM_WAVE;
+        row += lane < T ? p : 0;
+        parent = lane < T ? lane - 1 : -2;
+    } else {
+        T = min(sq.n, QLM_TREE_MAX);
+        row += lane < T ? lane : 0;
+        parent = tree_parent(a.bt, sq, lane);
+    }
+    T = min(T, TM);
+    if (T == 0) return;
+    if (tid == 0) sh.bad = -1;
+    if (wave == 0) {
+        const unsigned long long line = tree_line(parent);
+        double alpha = 0.0;
+        float beta = 0.0f;
+        if (line && lane < T) gates(a, row, h, alpha, beta);
+        double c = alpha;
+        int up = line ? parent : -1;
+        // conv inputs: itself and three above; behind the root the ring
+        int tap[4] = {-1, -1, -1, lane}, at = lane, old = 3;
+        for (int j = 2; j >= 0; --j) {
+            const int from = at >= 0 ? at : lane;
+            const int p = __shfl(up, from);
+            at = at >= 0 ? p : -1;
+            if (at < 0) --old;
+            tap[j] = at >= 0 ? at : -1 - (sq.ctx % 3 + old) % 3;
+        }
+        while (__ballot(up >= 0)) {
+            const int from = up >= 0 ? up : lane;
+            const double x = __shfl(c, from);
+            const int next = __shfl(up, from);
+            if (up >= 0) {
+                c += x;
+                up = next;
+            }
+        }
+        if (lane < TM) {
+            sh.line[lane] = lane < T ? line : 0;
+            sh.c[lane] = c;
+            sh.beta[lane] = beta;
+            sh.row[lane] = row;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sh.tap[lane][j] = tap[j];
+        }
+    }
+    // ---- conv inputs of q and k: a channel a thread, all nodes ----
+    const int ch = (tid >> 7) * HD + h * kD + (tid & 127);
+    const float* cs = a.conv + (size_t)b * 3 * C;
+    float ring[3], w4[4];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) ring[j] = cs[(size_t)j * C + ch];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w4[j] = a.wt[(size_t)j * C + ch];
+    float* const col = tid < kD ? &sh.q[0][tid] : &sh.k[0][tid - kD];
+#pragma unroll 1
+    for (int i0 = 0; i0 < TM; i0 += 16) {
+        if (i0 >= T) break;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[i] = a.proj[(size_t)__shfl(row, i0 + i) * a.ldp + ch];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) col[(i0 + i) * SH::QS] = x[i];
+    }
+    __syncthreads();
+    // v: nodes tid / CW, ... of column tid % CW
+    {
+        const int vc = tid % CW, vch = 2 * HD + h * kD + c0 + vc;
+        float vr[3], vw[4];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) vr[j] = cs[(size_t)j * C + vch];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vw[j] = a.wt[(size_t)j * C + vch];
+#pragma unroll 4
+        for (int i = tid / CW; i < TM; i += kThreads / CW) {
+            float acc = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = sh.tap[i][j];
+                const float x = t >= 0 ? a.proj[(size_t)sh.row[t] * a.ldp + vch]
+                                       : t == -1 ? vr[0] : t == -2 ? vr[1] : vr[2];
+                acc = nc_add_mul(acc, x, vw[j]);
+            }
+            sh.w[i][vc] = i < T ? silu_f(acc) : 0.0f;
+        }
+    }
+    // q and k in place, last nodes first: what a node reads is its own or
+    // an earlier node's, and a batch reads before it writes
+    {
+        constexpr int NB = 8;
+#pragma unroll 1
+        for (int i0 = (T - 1) / NB * NB; i0 >= 0; i0 -= NB) {
+            float y[NB];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                float acc = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int t = sh.tap[i0 + i][j];
+                    const float x = t >= 0 ? col[t * SH::QS]
+                                           : t == -1 ? ring[0] : t == -2 ? ring[1] : ring[2];
+                    acc = nc_add_mul(acc, x, w4[j]);
+                }
+                y[i] = silu_f(acc);
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i) col[(i0 + i) * SH::QS] = i0 + i < T ? y[i] : 0.0f;
+        }
+        for (int i = (T - 1) / NB * NB + NB; i < TM; ++i) col[i * SH::QS] = 0.0f;
+    }
+    __syncthreads();
+    // ---- norms: four threads a node ----
+    for (int i = tid / 4; i < TM; i += kThreads / 4) {
+        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int at = 4 * (4 * e + (tid & 3));
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&sh.q[i][at]);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(&sh.k[i][at]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s0 = fmaf(x[j], x[j], s0);
+                s1 = fmaf(y[j], y[j], s1);
+            }
+        }
+        s0 = group_sum<4>(s0);
+        s1 = group_sum<4>(s1);
+        if ((tid & 3) == 0) {
+            sh.sq[i] = 1.0f / sqrtf(s0 + 1e-6f);
+            sh.sk[i] = 1.0f / sqrtf(s1 + 1e-6f);
+        }
+    }
+    __syncthreads();
+    // ---- products of keys and queries with keys: pairs of 16-node tiles in turn ----
+    const int tiles = (T + 15) / 16;
+    for (int p = wave; p < RT * RT; p += kNW) {
+        const int ti = p / RT, si = p % RT;
+        f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
+        if (si <= ti && ti < tiles) {
+            float ka[32], kb[32];
+            load32(kb, &sh.k[16 * si + n][32 * qd]);
+            load32(ka, &sh.k[16 * ti + n][32 * qd]);
+            kk = dot32(ka, kb);
+            if constexpr (!COMMIT) {
+                load32(ka, &sh.q[16 * ti + n][32 * qd]);
+                qk = dot32(ka, kb);
+            }
+        }
+        const int s = 16 * si + n;
+        const double cs_ = sh.c[s];
+        const float ks = sh.sk[s];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 16 * ti + 4 * qd + i;
+            const bool on = sh.line[t] >> s & 1ull;
+            const float d = on ? expf((float)(sh.c[t] - cs_)) * ks : 0.0f;
+            sh.at[s][t] = on && s != t ? sh.beta[t] * sh.sk[t] * d * kk[i] : 0.0f;
+            if constexpr (!COMMIT) sh.m[t][s] = on ? sh.sq[t] * kScale * d * qk[i] : 0.0f;
+        }
+    }
+    // ---- products with the state: wave (role, tile); R in place of v ----
+    const int ti = wave % RT, role = wave / RT;  // roles: P of them share a tile
+    const float* S = a.state + ((size_t)b * a.H + h) * kD * kD + c0;
+    f32x4 o[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const bool do_k = ti < tiles && (P == 1 || role == 0);
+    const bool do_q = !COMMIT && ti < tiles && (P == 1 || role == 1);
+    if (do_k || do_q) {
+        float ka[32], qa[32];
+        if (do_k) load32(ka, &sh.k[16 * ti + n][32 * qd]);
+        if (do_q) load32(qa, &sh.q[16 * ti + n][32 * qd]);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float sb[32];
+#pragma unroll
+            for (int s = 0; s < 32; ++s) sb[s] = S[(size_t)(32 * qd + s) * kD + 16 * c + n];
+            if (do_k) {
+                const f32x4 ks = dot32(ka, sb);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = 16 * ti + 4 * qd + i;
+                    float* r = &sh.w[t][16 * c + n];
+                    const float g = expf((float)sh.c[t]) * sh.sk[t];
+                    *r = sh.line[t] ? sh.beta[t] * (*r - g * ks[i]) : 0.0f;
+                }
+            }
+            if (do_q) {
+                o[c] = dot32(qa, sb);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = 16 * ti + 4 * qd + i;
+                    o[c][i] *= expf((float)sh.c[t]) * sh.sq[t] * kScale;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    // ---- W by substitution: a wave a quarter of the columns ----
+    {
+        constexpr int RP = TM / 16;
+        float x[NC][RP];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < RP; ++e) x[c][e] = sh.w[RP * n + e][4 * (NC * wave + c) + qd];
+        solve_from<TM, NC, 0>(sh.at, x, T);
+        const double end = sh.c[T - 1];
+#pragma unroll
+        for (int e = 0; e < RP; ++e) {
+            float f = 1.0f;  // commit: what is left of a node at the path's end
+            const int t = RP * n + e;
+            if constexpr (COMMIT) f = t < T ? expf((float)(end - sh.c[t])) * sh.sk[t] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) sh.w[t][4 * (NC * wave + c) + qd] = f * x[c][e];
+        }
+    }
+    __syncthreads();
+    if constexpr (COMMIT) {
+        // S' = g S + sum of k_s w_s^T: 16-row tiles of the state, two a wave
+        const float g = expf((float)sh.c[T - 1]);
+        float* Sw = a.state + ((size_t)b * a.H + h) * kD * kD + c0;
+#pragma unroll 1
+        for (int ri = wave; ri < kD / 16; ri += kNW) {
+            float kc[TM / 4];
+#pragma unroll
+            for (int s = 0; s < TM / 4; ++s) kc[s] = sh.k[4 * s + qd][16 * ri + n];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                f32x4 x;
+                float* at = Sw + (size_t)(16 * ri + 4 * qd) * kD + 16 * c + n;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = g * at[(size_t)i * kD];
+#pragma unroll
+                for (int s = 0; s < TM / 4; ++s)
+                    x = mfma4(kc[s], sh.w[4 * s + qd][16 * c + n], x);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) at[(size_t)i * kD] = x[i];
+            }
+        }
+        return;
+    }
+    // ---- outputs: the state's part, and what the nodes above have added ----
+    if (do_q) {
+        bool fine = true;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int s = 0; s < TM / 4; ++s)
+                o[c] = mfma4(sh.m[16 * ti + n][4 * s + qd], sh.w[4 * s + qd][16 * c + n], o[c]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 16 * ti + 4 * qd + i;
+                const bool live = sh.line[t] != 0;
+                if (live) fine &= fabsf(o[c][i]) < INFINITY;
+                if (t < T)
+                    a.raw[(size_t)sh.row[t] * HD + h * kD + c0 + 16 * c + n] =
+                        live ? o[c][i] : 0.0f;
+            }
+        }
+        if (!fine) sh.bad = 0;
+    }
+    __syncthreads();
+    if (sh.bad < 0) return;
+    // ---- some output is not finite: every node again, along its own line ----
+    // (a node's NaN has reached others through products with 0). Thread (i, j)
+    // keeps rows 8 i .. + 7 of columns j, j + 16, ..; the sums over rows meet in
+    // sh.m, which nothing reads any more.
+    float* red = &sh.m[0][0];  // [16][16]
+    const int j = tid & 15, i8 = tid >> 4;
+#pragma unroll 1
+    for (int t = 0; t < T; ++t) {
+        const unsigned long long line = sh.line[t];
+        if (!line) continue;
+#pragma unroll 1
+        for (int c = 0; c < NC; ++c) {
+            float s[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = S[(size_t)(8 * i8 + e) * kD + 16 * c + j];
+            double was = 0.0;
+            for (unsigned long long left = line; left; left &= left - 1) {
+                const int u = __ffsll((long long)left) - 1;
+                const float dec = expf((float)(sh.c[u] - was));
+                was = sh.c[u];
+                float kv = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    s[e] *= dec;
+                    kv = fmaf(sh.k[u][8 * i8 + e] * sh.sk[u], s[e], kv);
+                }
+                __syncthreads();
+                red[i8 * 16 + j] = kv;
+                __syncthreads();
+                float sum = 0.0f;
+                for (int e = 0; e < 16; ++e) sum += red[e * 16 + j];
+                // v again: its place holds W
+                const int vch = 2 * HD + h * kD + c0 + 16 * c + j;
+                float acc = 0.0f;
+                for (int e = 0; e < 4; ++e) {
+                    const int tp = sh.tap[u][e];
+                    const float x = tp >= 0 ? a.proj[(size_t)sh.row[tp] * a.ldp + vch]
+                                            : cs[(size_t)(-1 - tp) * C + vch];
+                    acc = nc_add_mul(acc, x, a.wt[(size_t)e * C + vch]);
+                }
+                const float w = sh.beta[u] * (silu_f(acc) - sum);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] = fmaf(sh.k[u][8 * i8 + e] * sh.sk[u], w, s[e]);
+            }
+            float y = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y = fmaf(sh.q[t][8 * i8 + e], s[e], y);
+            __syncthreads();
+            red[i8 * 16 + j] = y;
+            __syncthreads();
+            float sum = 0.0f;
+            for (int e = 0; e < 16; ++e) sum += red[e * 16 + j];
+            if (i8 == 0)
+                a.raw[(size_t)sh.row[t] * HD + h * kD + c0 + 16 * c + j] = sum * sh.sq[t] * kScale;
+        }
+    }
+}
+
+// Head norm and SiLU(z) gate, a head a wave; rows outside the tree are 0.
+__global__ __launch_bounds__(kThreads) void k_dn_tree_norm(TreeArgs a) {
+    const int row = blockIdx.x, lane = threadIdx.x & 63, b = seq_of_row(a.bt, row);
+    if (b < 0) return;
+    const SeqRows sq = seq_rows(a.bt, b);
+    const int i = row - sq.first, HD = a.H * kD;
+    if (i < 0 || i >= sq.n) return;
+    const unsigned long long mine = tree_line(tree_parent(a.bt, sq, lane));
+    const bool live = __ballot(mine != 0) >> min(i, QLM_TREE_MAX - 1) & 1ull && i < QLM_TREE_MAX;
+    for (int h = blockIdx.y * kNW + threadIdx.x / QLM_WAVE; h < a.H; h += gridDim.y * kNW) {
+        float* to = a.out + (size_t)row * a.ldo + h * kD + lane;
+        if (!live) {
+            to[0] = 0.0f;
+            to[64] = 0.0f;
+            continue;
+        }
+        const float* o = a.raw + (size_t)row * HD + h * kD + lane;
+        const float* z = a.proj + (size_t)row * a.ldp + 3 * (size_t)HD + h * kD + lane;
+        const float o0 = o[0], o1 = o[64], z0 = z[0], z1 = z[64];
+        const float sn = 1.0f / sqrtf(wave_sum(fmaf(o0, o0, o1 * o1)) / (float)kD + 1e-6f);
+        to[0] = (o0 * sn) * a.norm_w[lane] * silu_f(z0);
+        to[64] = (o1 * sn) * a.norm_w[lane + 64] * silu_f(z1);
+    }
+}
+
+// The rings' advance: the last three of (the ring's three, the path's inputs),
+// put where position ctx_len + accepted expects them. After k_dn_tree, whose
+// workgroups all read the old ring.
+__global__ __launch_bounds__(kThreads) void k_dn_tree_ring(TreeArgs a, float* conv) {
+    const int b = blockIdx.y, lane = threadIdx.x & 63, C = 3 * a.H * kD;
+    const SeqRows sq = seq_rows(a.bt, b);
+    const int want = min(max(a.accepted[b], 0), min(a.ld_path, QLM_TREE_MAX));
+    const int p = lane < want ? a.path[(size_t)b * a.ld_path + lane] : -1;
+    const unsigned long long ends = __ballot(p < 0 || p >= sq.n);
+    const int T = ends ? __ffsll((long long)ends) - 1 : QLM_WAVE;
+    if (T == 0) return;
+    int row[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) row[j] = T + j >= 3 ? sq.first + __shfl(p, max(T + j - 3, 0)) : -1;
+    const int ch = blockIdx.x * kThreads + threadIdx.x, ctx = sq.ctx % 3;
+    if (ch >= C) return;
+    float* cs = conv + (size_t)b * 3 * C + ch;
+    float x[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j)  // place T + j of that line
+        x[j] = row[j] >= 0 ? a.proj[(size_t)row[j] * a.ldp + ch]
+                           : cs[(size_t)((ctx + T + j) % 3) * C];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) cs[(size_t)((ctx + T + j) % 3) * C] = x[j];
+}
+
+template <int TM, int NC, bool COMMIT>
+int launch_tree(const TreeArgs& a, hipStream_t st) {
+    static_assert(sizeof(TreeShared<TM, NC>) <= 160 * 1024, "fits a CU");
+    hipLaunchKernelGGL((k_dn_tree<TM, NC, COMMIT>), dim3(a.H * (kD / (16 * NC)), a.bt.B),
+                       dim3(kThreads), 0, st, a);
+    return qlm_launch_status();
+}
+
+template <int TM, bool COMMIT>
+int launch_columns(const TreeArgs& a, hipStream_t st) {
+    const long long heads = (long long)a.H * a.bt.B;
+    if (heads >= 128) return launch_tree<TM, 8, COMMIT>(a, st);
+    if (heads >= 64) return launch_tree<TM, 4, COMMIT>(a, st);
+    if (heads >= 32) return launch_tree<TM, 2, COMMIT>(a, st);
+    return launch_tree<TM, 1, COMMIT>(a, st);
+}
+
+template <bool COMMIT>
+int launch_nodes(const TreeArgs& a, hipStream_t st) {
+    // no sequence has more nodes than the call has rows
+    if (a.bt.rows <= 16) return launch_columns<16, COMMIT>(a, st);
+    if (a.bt.rows <= 32) return launch_columns<32, COMMIT>(a, st);
+    return launch_columns<64, COMMIT>(a, st);
+}
+
+int check_tree(const float* proj, int ldp, const qlm_row_batch* batch, int H, int d) {
+    const int rc = check_row_batch(batch);
+    if (rc != QLM_OK) return rc;
+    if (!proj || H <= 0) return QLM_ERR_ARG;
+    if (d != kD || H > 4096) return QLM_ERR_SHAPE;
+    return ldp < 4 * H * d + 2 * H ? QLM_ERR_SHAPE : QLM_OK;
+}
+
+}  // namespace
+
+extern "C" size_t qlm_deltanet_tree_workspace_bytes(int rows, int H, int d) {
+    if (rows <= 0 || rows > kMaxBatchRows || H <= 0 || H > 4096 || d != kD) return 0;
+    return (size_t)rows * H * d * sizeof(float);
+}
+
+extern "C" int qlm_deltanet_tree(const float* proj, int ldp, const qlm_row_batch* batch,
+                                 const float* conv_state, const float* conv_w_t,
+                                 const float* A_log, const float* dt_bias, const float* norm_w,
+                                 const float* state, float* out, int ldo, int H, int d, void* work,
+                                 size_t work_bytes, void* stream) {
+    const int rc = check_tree(proj, ldp, batch, H, d);
+    if (rc != QLM_OK) return rc;
+    if (!conv_state || !conv_w_t || !A_log || !dt_bias || !norm_w || !state || !out || !work)
+        return QLM_ERR_ARG;
+    if (work_bytes < qlm_deltanet_tree_workspace_bytes(batch->rows, H, d)) return QLM_ERR_ARG;
+    if (ldo < H * d || ((uintptr_t)work & 15u)) return QLM_ERR_SHAPE;
+    const TreeArgs a{proj,   conv_state, conv_w_t, A_log, dt_bias, norm_w, const_cast<float*>(state),
+                     reinterpret_cast<float*>(work), out, nullptr, nullptr, ldp, ldo, H, 0, *batch};
+    hipStream_t st = as_stream(stream);
+    const int r = launch_nodes<false>(a, st);
+    if (r != QLM_OK) return r;
+    hipLaunchKernelGGL(k_dn_tree_norm, dim3(batch->rows, (H + kNW - 1) / kNW), dim3(kThreads), 0, st,
+                       a);
+    return qlm_launch_status();
+}
+
+extern "C" int qlm_deltanet_tree_commit(const float* proj, int ldp, const qlm_row_batch* batch,
+                                        const int* path, int ld_path, const int* accepted,
+                                        float* conv_state, const float* conv_w_t,
+                                        const float* A_log, const float* dt_bias, float* state,
+                                        int H, int d, void* stream) {
+    const int rc = check_tree(proj, ldp, batch, H, d);
+    if (rc != QLM_OK) return rc;
+    if (!path || !accepted || !conv_state || !conv_w_t || !A_log || !dt_bias || !state ||
+        ld_path <= 0)
+        return QLM_ERR_ARG;
+    const TreeArgs a{proj,  conv_state, conv_w_t, A_log,    dt_bias, nullptr, state, nullptr,
+                     nullptr, path,     accepted, ldp, 0, H, ld_path, *batch};
+    hipStream_t st = as_stream(stream);
+    const int r = launch_nodes<true>(a, st);
+    if (r != QLM_OK) return r;
+    hipLaunchKernelGGL(k_dn_tree_ring, dim3((3 * H * d + kThreads - 1) / kThreads, batch->B),
+                       dim3(kThreads), 0, st, a, conv_state);
+    return qlm_launch_status();
+}
+
+// Loads this file's code object on the current device now; the runtime
+// otherwise loads it at the first launch of one of its kernels.
+hipError_t qlm_load_deltanet_tree() {
+    hipFuncAttributes a;
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(k_dn_tree_norm));
+}

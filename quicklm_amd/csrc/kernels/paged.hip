@@ -1,0 +1,276 @@
+// New rows into a paged KV cache (qlm_paged_append) and the end of a greedy
+// verification of drafted trees (qlm_tree_commit).
+//
+// Append, a head of a row:  r = x / sqrt(mean(x^2) + eps) * (1 + gain), then
+// for each pair (j, j + rot / 2) of its first rot elements
+//   (r_j, r_j+h) -> (r_j cos - r_j+h sin, r_j+h cos + r_j sin)
+// with the angle of the row's position on the pair's axis. Queries go to their
+// own array, keys and values (as they are) to the row's slot. Every value is
+// read once and written once.
+
+#include "paged.hpp"
+
+namespace {
+
+// vectors of four aligned to one element only: rows of any stride
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kAppendThreads = 256;
+
+struct AppendArgs {
+    const float* qkv;
+    const float *qn, *kn;  // gains, NULL: that head is not normalised
+    const float *cos_tab, *sin_tab;
+    const int *positions, *pair_axis;
+    float* q_out;
+    long long ldqkv, ldq, ld_pos;
+    int n_pos, rot, n_axes, n_q, q_stride;
+    qlm_row_batch bt;
+    qlm_kv_pages pg;
+};
+
+// A group of HD / 4 lanes takes a head of the row blockIdx.x, four elements a
+// lane: query heads first, then keys, then values.
+template <int HD, typename KV>
+__global__ __launch_bounds__(kAppendThreads) void k_paged_append(AppendArgs a) {
+    constexpr int LPH = HD / 4, HPB = kAppendThreads / LPH;  // lanes a head, heads a workgroup
+    __shared__ __align__(16) float sh[HPB][HD];
+    const int grp = threadIdx.x / LPH, l = threadIdx.x % LPH, e0 = 4 * l;
+    const int row = blockIdx.x, n_kv = a.pg.n_kv;
+    const int head = blockIdx.y * HPB + grp, heads = a.n_q + 2 * n_kv;
+    const int hc = min(head, heads - 1);  // groups past the last head do its work, unstored
+    const bool is_q = hc < a.n_q, is_v = hc >= a.n_q + n_kv;
+    const int g = is_q ? 0 : is_v ? hc - a.n_q - n_kv : hc - a.n_q;
+    // the row's operands are requested before its sequence is looked up
+    const float* x = a.qkv + (size_t)row * a.ldqkv +
+                     (is_q ? (size_t)hc * a.q_stride
+                           : (size_t)a.n_q * a.q_stride + (size_t)(hc - a.n_q) * HD);
+    f32x4u v = *reinterpret_cast<const f32x4u*>(x + e0);
+    const float* gain = is_q ? a.qn : is_v ? nullptr : a.kn;
+    f32x4u gn = f32x4u{0.0f, 0.0f, 0.0f, 0.0f};
+    if (gain) gn = *reinterpret_cast<const f32x4u*>(gain + e0);
+
+    const int b = seq_of_row(a.bt, row);
+    if (b < 0) return;  // the whole workgroup
+    const SeqRows sq = seq_rows(a.bt, b);
+    const int i = row - sq.first;
+    if (i < 0 || i >= sq.n) return;
+    bool live = true;
+    int depth = i;
+    if (a.bt.parent) {
+        const unsigned long long line = tree_line(tree_parent(a.bt, sq, threadIdx.x & 63));
+        const int at = min(i, QLM_TREE_MAX - 1);
+        const unsigned long long mine = (unsigned long long)__shfl((unsigned)(line >> 32), at) << 32 |
+                                        __shfl((unsigned)line, at);
+        live = i < QLM_TREE_MAX && mine != 0;
+        depth = __popcll(mine) - 1;
+    }
+
+    float ss = fmaf(v.x, v.x, fmaf(v.y, v.y, fmaf(v.z, v.z, v.w * v.w)));
+    ss = group_sum<LPH>(ss);
+    if (gain) {
+        const float s = 1.0f / sqrtf(ss / (float)HD + 1e-6f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (v[j] * s) * (1.0f + gn[j]);
+    }
+    const int half = a.rot / 2;
+    if (half > 0) {
+        // a pair's other element is some lane's of the same group, so of the
+        // same wave
+        *reinterpret_cast<f32x4u*>(&sh[grp][e0]) = v;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (!is_v && e0 < a.rot) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = e0 + j;
+                if (e >= a.rot) break;
+                const bool low = e < half;
+                const int pair = low ? e : e - half;
+                int pos = sq.ctx + depth, axis = 0;
+                if (a.positions) {
+                    if (a.pair_axis) axis = a.pair_axis[pair];
+                    const bool there = axis >= 0 && axis < a.n_axes;
+                    pos = a.positions[(size_t)(there ? axis : 0) * a.ld_pos + row];
+                    if (!there) pos = -1;
+                }
+                float c = NAN, s = NAN;  // no angle
+                if (pos >= 0 && pos < a.n_pos) {
+                    c = a.cos_tab[(size_t)pos * half + pair];
+                    s = a.sin_tab[(size_t)pos * half + pair];
+                }
+                const float y = sh[grp][low ? e + half : pair];
+                v[j] = low ? nc_mul_sub(v[j], c, y, s) : nc_mul_add2(v[j], c, y, s);
+            }
+        }
+    }
+    if (head >= heads) return;
+    if (is_q) {
+        if (!live) v = f32x4u{0.0f, 0.0f, 0.0f, 0.0f};
+        *reinterpret_cast<f32x4u*>(a.q_out + (size_t)row * a.ldq + (size_t)head * HD + e0) = v;
+        return;
+    }
+    const int page = live ? page_of(a.pg, b, sq.ctx + i) : -1;
+    if (page < 0) return;
+    KV* to = reinterpret_cast<KV*>(is_v ? a.pg.v : a.pg.k) + slot_at(a.pg, page, g, sq.ctx + i) + e0;
+    if constexpr (sizeof(KV) == 4) {
+        *reinterpret_cast<float4*>(to) = make_float4(v.x, v.y, v.z, v.w);
+    } else {
+        unsigned w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = (unsigned)__builtin_bit_cast(unsigned short, (__bf16)v[j]);
+        *reinterpret_cast<uint2*>(to) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    }
+}
+
+// ---- commit ------------------------------------------------------------------
+// The walk: from row 0 to the first row that follows the last accepted one and
+// holds its pick, a row a lane, one ballot a step. Every workgroup of a sequence
+// walks for itself (a handful of steps) and so needs no other launch.
+// The move: row path[i] -> slot ctx + i. Rows of a path are in rising order and
+// path[i] >= i, so that a place is only written once the row it held has been
+// read, if one thread moves its 16 bytes of every row of the path in order.
+constexpr int kCommitThreads = 256;
+constexpr int kMoveBatch = 8;  // rows in flight a thread
+
+struct CommitArgs {
+    const int *tokens, *picks;
+    int *path, *accepted, *next, *new_len;
+    int ld_path, layers, pieces;  // pieces: 16 bytes each, of a slot of a head
+    long long layer_bytes;
+    qlm_row_batch bt;
+    qlm_kv_pages pg;
+};
+
+__global__ __launch_bounds__(kCommitThreads) void k_tree_commit(CommitArgs a) {
+    __shared__ long long from[QLM_TREE_MAX], to[QLM_TREE_MAX];  // bytes, -1: not there
+    __shared__ int moves;
+    const int b = blockIdx.y, lane = threadIdx.x & (QLM_WAVE - 1);
+    if (threadIdx.x < QLM_WAVE) {
+        const SeqRows sq = seq_rows(a.bt, b);
+        const bool there = lane < sq.n;
+        const int parent = tree_parent(a.bt, sq, lane);
+        const int token = there ? a.tokens[sq.first + lane] : 0;
+        const int pick = there ? a.picks[sq.first + lane] : 0;
+        int mine = -1, count = 0, next = -1;
+        int cur = __ballot(parent == -1) & 1ull ? 0 : -1;
+        while (cur >= 0) {
+            if (lane == count) mine = cur;
+            ++count;
+            next = __shfl(pick, cur);
+            const unsigned long long c = __ballot(parent == cur && lane > cur && token == next);
+            cur = c ? __ffsll((long long)c) - 1 : -1;
+        }
+        if (blockIdx.x == 0) {
+            int* path = a.path + (size_t)b * a.ld_path;
+            for (int i = lane; i < a.ld_path; i += QLM_WAVE) path[i] = i < QLM_WAVE ? mine : -1;
+            if (lane == 0) {
+                a.accepted[b] = count;
+                a.next[b] = next;
+                if (a.new_len) a.new_len[b] = sq.ctx + count;
+            }
+        }
+        // the rows that move, of those whose slots are there
+        const bool move = lane < count && mine != lane;
+        const int fp = move ? page_of(a.pg, b, sq.ctx + mine) : -1;
+        const int tp = move ? page_of(a.pg, b, sq.ctx + lane) : -1;
+        const bool both = fp >= 0 && tp >= 0;
+        const unsigned long long who = __ballot(both);
+        if (both) {
+            const int at = __popcll(who & ((1ull << lane) - 1ull));
+            const long long size = a.pg.dtype == 0 ? 4 : 2;
+            from[at] = (long long)slot_at(a.pg, fp, 0, sq.ctx + mine) * size;
+            to[at] = (long long)slot_at(a.pg, tp, 0, sq.ctx + lane) * size;
+        }
+        if (lane == 0) moves = __popcll(who);
+    }
+    __syncthreads();
+    const int n = moves;
+    // this thread's piece: of a layer, a pool and a head
+    long long p = (long long)blockIdx.x * kCommitThreads + threadIdx.x;
+    const int piece = (int)(p % a.pieces);
+    p /= a.pieces;
+    const int g = (int)(p % a.pg.n_kv);
+    p /= a.pg.n_kv;
+    if (n == 0 || p >= 2LL * a.layers) return;
+    char* pool = reinterpret_cast<char*>(p & 1 ? a.pg.v : a.pg.k) + (p >> 1) * a.layer_bytes +
+                 (size_t)g * a.pg.page_size * a.pieces * 16 + piece * 16;
+    for (int i0 = 0; i0 < n; i0 += kMoveBatch) {
+        uint4 v[kMoveBatch];
+#pragma unroll
+        for (int i = 0; i < kMoveBatch; ++i)
+            v[i] = *reinterpret_cast<const uint4*>(pool + from[min(i0 + i, n - 1)]);
+#pragma unroll
+        for (int i = 0; i < kMoveBatch; ++i)
+            if (i0 + i < n) *reinterpret_cast<uint4*>(pool + to[i0 + i]) = v[i];
+    }
+}
+
+template <int HD, typename KV>
+void launch_append(const AppendArgs& a, hipStream_t st) {
+    const int per = kAppendThreads / (HD / 4), heads = a.n_q + 2 * a.pg.n_kv;
+    hipLaunchKernelGGL((k_paged_append<HD, KV>), dim3(a.bt.rows, (heads + per - 1) / per),
+                       dim3(kAppendThreads), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" int qlm_paged_append(const float* qkv, int ldqkv, const float* q_norm,
+                                const float* k_norm, const float* cos_tab, const float* sin_tab,
+                                int n_pos, int rot_dim, const int* positions, int ld_pos,
+                                const int* pair_axis, int n_axes, const qlm_row_batch* batch,
+                                const qlm_kv_pages* pages, float* q_out, int ldq, int n_q,
+                                int gated, void* stream) {
+    int rc = check_row_batch(batch);
+    if (rc == QLM_OK) rc = check_kv_pages(pages);
+    if (rc != QLM_OK) return rc;
+    if (!qkv || !q_out || qkv == q_out || n_q <= 0) return QLM_ERR_ARG;
+    if (rot_dim > 0 && (!cos_tab || !sin_tab || n_pos <= 0)) return QLM_ERR_ARG;
+    if (positions && (ld_pos < batch->rows || n_axes <= 0)) return QLM_ERR_ARG;
+    const int hd = pages->hd;
+    if (rot_dim < 0 || rot_dim > hd || rot_dim % 2 != 0) return QLM_ERR_SHAPE;
+    if (n_q > 8192) return QLM_ERR_SHAPE;
+    const int q_stride = gated ? 2 * hd : hd;
+    if (ldqkv < n_q * q_stride + 2 * pages->n_kv * hd || ldq < n_q * hd) return QLM_ERR_SHAPE;
+    const AppendArgs a{qkv, q_norm, k_norm, cos_tab, sin_tab, positions, pair_axis, q_out, ldqkv,
+                       ldq, ld_pos, n_pos, rot_dim, n_axes, n_q, q_stride, *batch, *pages};
+    hipStream_t st = as_stream(stream);
+    if (hd == 128)
+        pages->dtype == 0 ? launch_append<128, float>(a, st) : launch_append<128, uint16_t>(a, st);
+    else
+        pages->dtype == 0 ? launch_append<256, float>(a, st) : launch_append<256, uint16_t>(a, st);
+    return qlm_launch_status();
+}
+
+extern "C" int qlm_tree_commit(const int* tokens, const int* picks, const qlm_row_batch* batch,
+                               const qlm_kv_pages* pages, int layers, long long layer_stride,
+                               int* path, int ld_path, int* accepted, int* next_token,
+                               int* new_len, void* stream) {
+    int rc = check_row_batch(batch);
+    if (rc == QLM_OK) rc = check_kv_pages(pages);
+    if (rc != QLM_OK) return rc;
+    if (!tokens || !picks || !path || !accepted || !next_token || !batch->parent || layers <= 0)
+        return QLM_ERR_ARG;
+    if (new_len == batch->ctx_len || ld_path < QLM_TREE_MAX) return QLM_ERR_ARG;
+    const long long pool = (long long)pages->n_pages * pages->n_kv * pages->page_size * pages->hd;
+    if (layer_stride < 0 || (layers > 1 && layer_stride < pool)) return QLM_ERR_ARG;
+    const long long size = pages->dtype == 0 ? 4 : 2;
+    if (layers > 1 && layer_stride * size % 16 != 0) return QLM_ERR_SHAPE;
+    if (layers > 4096) return QLM_ERR_SHAPE;
+    const int pieces = (int)(pages->hd * size / 16);
+    const CommitArgs a{tokens, picks, path, accepted, next_token, new_len, ld_path, layers, pieces,
+                       layer_stride * size, *batch, *pages};
+    const long long threads = 2LL * layers * pages->n_kv * pieces;
+    hipLaunchKernelGGL(k_tree_commit,
+                       dim3((unsigned)((threads + kCommitThreads - 1) / kCommitThreads), batch->B),
+                       dim3(kCommitThreads), 0, as_stream(stream), a);
+    return qlm_launch_status();
+}
+
+// Loads this file's code object on the current device now; the runtime
+// otherwise loads it at the first launch of one of its kernels.
+hipError_t qlm_load_paged() {
+    hipFuncAttributes a;
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(k_tree_commit));
+}

@@ -29,6 +29,24 @@ class L2Plan(C.Structure):
                 ("tiles", C.c_int * 8), ("nseg", C.c_int)]
 
 
+class RowBatch(C.Structure):
+    """qlm_row_batch: the rows of ragged sequences, as chains or trees (device
+    arrays row_start [B + 1], ctx_len [B], parent [rows] or None)."""
+    _fields_ = [("B", C.c_int), ("rows", C.c_int), ("row_start", C.c_void_p),
+                ("ctx_len", C.c_void_p), ("parent", C.c_void_p)]
+
+
+class KvPages(C.Structure):
+    """qlm_kv_pages: pools [n_pages, n_kv, page_size, hd] of keys and values and
+    the sequences' page table [B, ld_table] (device memory; dtype 0 = fp32,
+    1 = bf16)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int),
+                ("table", C.c_void_p), ("ld_table", C.c_int)]
+
+
+_ll, _pb, _pp = C.c_longlong, C.POINTER(RowBatch), C.POINTER(KvPages)
+
 # name -> (restype, argtypes)
 _SIGS = {
     "qlm_error_string": (C.c_char_p, [_i]),
@@ -123,6 +141,16 @@ _SIGS = {
     "qlm_attention_decode": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp]),
     "qlm_attention_decode_noalloc_bytes": (_sz, [_i, _i, _i, _i]),
     "qlm_attention_decode_noalloc": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp]),
+    "qlm_paged_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _pb, _pp, _vp,
+                              _i, _i, _i, _vp]),
+    "qlm_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _ll]),
+    "qlm_paged_attention": (_i, [_vp, _i, _pb, _pp, _vp, _i, _i, _vp, _i, _i, _vp, _sz, _vp]),
+    "qlm_tree_commit": (_i, [_vp, _vp, _pb, _pp, _i, _ll, _vp, _i, _vp, _vp, _vp, _vp]),
+    "qlm_deltanet_tree_workspace_bytes": (_sz, [_i, _i, _i]),
+    "qlm_deltanet_tree": (_i, [_vp, _i, _pb, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp,
+                               _sz, _vp]),
+    "qlm_deltanet_tree_commit": (_i, [_vp, _i, _pb, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i,
+                                      _vp]),
     "qlm_argmax": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
     "qlm_argmax_workspace_bytes": (_sz, [_i, _i]),
     "qlm_token_logprobs": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
