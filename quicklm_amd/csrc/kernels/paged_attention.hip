@@ -54,11 +54,16 @@ struct PaArgs {
     int2* desc;  // [rows, n_kv]: a row's first record (of the kv head's first query head), chunks
     long long ldq, ldg, ldo;
     int gate_stride, n_q, lg;  // G = 1 << lg
-    int target, items, rec_rows, slots;
+    int target, least, alone;  // items to cut a kv head's keys into; keys of an item, at
+                               // least; of a batch's longest sequence that is not cut
+    int items, rec_rows, slots;
     float qscale;  // log2(e) / sqrt(hd)
     qlm_row_batch bt;
     qlm_kv_pages pg;
 };
+
+// a value that is the same in all lanes, in a scalar register
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // ---- which work a workgroup does ----
 
@@ -67,7 +72,6 @@ struct Item {
     int b, tile, chunk;  // chunk: which
     int len;             // keys of a chunk
     int rec;             // the unit's first record block
-    bool split;          // the sequence's units may have several chunks
 };
 
 __device__ __forceinline__ int tiles_of(int n, int lg, int mt) {
@@ -79,24 +83,39 @@ __device__ __forceinline__ int seen_rows(const PaArgs& a, const SeqRows& s) {
     return a.bt.parent ? min(s.n, QLM_TREE_MAX) : s.n;
 }
 
+// Sums over the lanes up to each (DPP: shifts within rows of 16, then the rows'
+// last lanes to the rows behind).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return v;
+}
+
 // Item `want` of a kv head, counted over the sequences: the longest prompts'
-// last tiles, which see the most keys, first. Every lane gets it.
-constexpr int kMinChunk = 128;  // keys of a chunk at least
+// last tiles, which see the most keys, first. Every lane gets it. Sums that
+// only say how long a chunk is are in fp32, the same in every wave.
 template <int MT>
 __device__ __forceinline__ bool find_item(const PaArgs& a, int want, Item& it) {
     const int lane = threadIdx.x & (QLM_WAVE - 1), B = a.bt.B;
-    double cost = 0.0;
+    float cost = 0.0f, longest = 0.0f;
     SeqRows s{};
     for (int i = 0; i < B; i += QLM_WAVE) {
         s = seq_rows(a.bt, min(i + lane, B - 1));
         if (i + lane >= B) s.n = 0;
-        if (s.n > 0)
-            cost += (double)tiles_of(s.n, a.lg, MT) * min(s.ctx + seen_rows(a, s), a.slots);
+        if (s.n > 0) {
+            const float keys = (float)min(s.ctx + seen_rows(a, s), a.slots);
+            cost += (float)tiles_of(s.n, a.lg, MT) * keys;
+            longest = fmaxf(longest, keys);
+        }
     }
-#pragma unroll
-    for (int d = 1; d < QLM_WAVE; d <<= 1) cost += __shfl_xor(cost, d);
-    const double share = ceil(cost / (double)a.target / 32.0) * 32.0;
-    it.len = (int)fmin(fmax(share, (double)kMinChunk), (double)(1 << 30));
+    const float share = wave_sum(cost) / (float)a.target;
+    it.len = uni(min((int)fminf(share, (float)(1 << 29)) / 32 * 32 + 32, 1 << 29));
+    it.len = max(it.len, wave_max(longest) <= (float)a.alone ? a.alone : a.least);
+    it.len = uni(it.len);
     int before = 0, rec = 0;
     for (int i = 0; i < B; i += QLM_WAVE) {
         if (B > QLM_WAVE) {
@@ -110,27 +129,17 @@ __device__ __forceinline__ bool find_item(const PaArgs& a, int want, Item& it) {
             items = tiles_of(s.n, a.lg, MT) * nch;
             recs = nch > 1 ? items : 0;
         }
-        int ic = items, rc = recs;  // inclusive sums
-#pragma unroll
-        for (int d = 1; d < QLM_WAVE; d <<= 1) {
-            const int x = __shfl_up(ic, d), y = __shfl_up(rc, d);
-            if (lane >= d) {
-                ic += x;
-                rc += y;
-            }
-        }
+        const int ic = wave_scan(items), rc = wave_scan(recs);
         const unsigned long long at = __ballot(before + ic > want);
         if (at) {
             const int w = __ffsll((long long)at) - 1;
             auto of = [&](int x) { return __builtin_amdgcn_readlane(x, w); };
             it.b = i + w;
             it.sq = SeqRows{of(s.first), of(s.n), of(s.ctx)};
-            it.len = __builtin_amdgcn_readfirstlane(it.len);
             const int mine = want - before - of(ic - items);
             const int tiles = tiles_of(it.sq.n, a.lg, MT), nch = of(items) / tiles;
             it.chunk = mine % nch;
             it.tile = tiles - 1 - mine / nch;
-            it.split = nch > 1;
             it.rec = rec + of(rc - recs) + mine - it.chunk;
             return true;
         }
@@ -184,8 +193,8 @@ __device__ __forceinline__ Group group_at(const PaArgs& a, int b, int slot, int 
         reinterpret_cast<uintptr_t>(a.pg.table));
     const int p = table[(size_t)b * a.pg.ld_table + (in ? i : 0)];
     Group g;
-    g.valid = in && (unsigned)p < (unsigned)a.pg.n_pages ? min(end - slot, 16) : 0;
-    g.page = g.valid > 0 ? p : 0;
+    g.valid = uni(in && (unsigned)p < (unsigned)a.pg.n_pages ? min(end - slot, 16) : 0);
+    g.page = uni(g.valid > 0 ? p : 0);
     return g;
 }
 
@@ -220,31 +229,46 @@ __device__ __forceinline__ void fetch_group(const PaArgs& a, const void* pool, c
     for (int j = 0; j < L::LOADS; ++j) load_to_lds(r, to + j * 1024, L::src(j), 0);
 }
 
+// LDS by its own 32-bit addresses
+__device__ __forceinline__ uint32_t lds_at(const char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+template <typename T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+    return *(__attribute__((address_space(3))) const T*)(uintptr_t)at;
+}
+
 __device__ __forceinline__ unsigned pk_bf16(float x, float y) {
     const f32x2 v = {x, y};
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
 }
 
-// eight floats as two bf16 terms each
+// Eight floats as two bf16 terms each. What the first term leaves is x - h,
+// exact: one product with -1 and its sum with x (v_dot2_f32_bf16) instead of
+// widening h and subtracting it.
 __device__ __forceinline__ void split8(const float (&x)[8], u32x4& h, u32x4& l) {
+    // (-1, 0) and (0, -1); in registers, since the compiler writes the second as the
+    // inline constant -1.0, which the instruction does not read as that pair
+    unsigned c0 = 0x0000bf80u, c1 = 0xbf800000u;
+    asm("" : "+v"(c0), "+v"(c1));
+    const bf16x2 first = __builtin_bit_cast(bf16x2, c0), second = __builtin_bit_cast(bf16x2, c1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const unsigned w = pk_bf16(x[2 * i], x[2 * i + 1]);
-        h[i] = w;
-        l[i] = pk_bf16(x[2 * i] - __uint_as_float(w << 16),
-                       x[2 * i + 1] - __uint_as_float(w & 0xffff0000u));
+        const f32x2 v = {x[2 * i], x[2 * i + 1]};
+        const bf16x2 w = __builtin_convertvector(v, bf16x2);
+        h[i] = __builtin_bit_cast(unsigned, w);
+        l[i] = pk_bf16(__builtin_amdgcn_fdot2_f32_bf16(w, first, v.x, false),
+                       __builtin_amdgcn_fdot2_f32_bf16(w, second, v.y, false));
     }
 }
 
-// A raw fp32 group (or part p of `parts` of it) into its two planes.
+// A raw fp32 group into its two planes.
 template <int HD>
-__device__ __forceinline__ void split_group(const char* raw, char* hi, char* lo, int part,
-                                            int parts) {
+__device__ __forceinline__ void split_group(const char* raw, char* hi, char* lo) {
     constexpr int ROW = HD * 2, PPR = ROW / 16, N = 16 * PPR / QLM_WAVE;
     const int lane = threadIdx.x & (QLM_WAVE - 1);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        if (parts > 1 && j % parts != part) continue;
         const int at = j * QLM_WAVE + lane, row = at / PPR, piece = at % PPR;
         const f32x4 x0 = *reinterpret_cast<const f32x4*>(raw + at * 32);
         const f32x4 x1 = *reinterpret_cast<const f32x4*>(raw + at * 32 + 16);
@@ -272,33 +296,67 @@ __device__ __forceinline__ float cols_sum(float v) { return xor32_add(xor16_add(
 __device__ __forceinline__ float fold8(float v) { return v + dpp_mov<0x128>(v); }  // row_ror:8
 
 // RT tiles of 16 rows; PACK: one tile of 8 rows, h and l terms side by side.
+// A row's scores come out of the products relative to a reference `m` (the
+// accumulators begin at -m): the largest score of the row's first block, and of
+// a later one where a score passes it by more than kRise. So exponentials go
+// up to 2^kRise, sums over 2^30 keys stay in range, and what is lost below 2^-126
+// is less than that part of the row's largest; no block needs a maximum over
+// the lanes, and the sums are hardly ever scaled. A block that moves a reference
+// is begun again (the loops below): with the scaling inside of the loop's body
+// its registers were copied every time, a third of its vector instructions.
+constexpr float kRise = 60.0f;
+constexpr int kAnyScore = (int)0x80000000;
 template <int HD, int RT, bool PACK>
 struct Rows {
     static constexpr int KS = HD / 32, CB = HD / 16, QT = PACK ? 1 : 2;
     u32x4 q[RT][QT][KS];
     f32x4 acc[RT][CB];
-    float m[RT], l[RT];
+    f32x4 from[RT];       // four times -m
+    float m[RT], l[RT];   // m -inf: no score yet
+    int high[RT];         // bits of the relative score that moves it: kRise, at first any
     int lim[RT];  // slots below this one are seen; -1: a row outside the tree
     unsigned long long line[RT];  // new rows seen beside those
 };
 
-// Query rows r0 + 16 t + n of the unit (r: its token and head) and what they see.
+// Query rows r0 + 16 t + n of the unit (r: its token and head): requested here.
 template <int HD, int RT, bool PACK>
-__device__ __forceinline__ void load_rows(const PaArgs& a, const Item& it, int g, int r0,
-                                          Rows<HD, RT, PACK>& R) {
-    using T = Rows<HD, RT, PACK>;
+struct Queries {
+    f32x4u x[RT][HD / 32][2];
+};
+template <int HD, int RT, bool PACK>
+__device__ __forceinline__ void request_rows(const PaArgs& a, const Item& it, int g, int r0,
+                                             Queries<HD, RT, PACK>& Q) {
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
+    const int total = it.sq.n << a.lg;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int rc = min(r0 + 16 * t + (PACK ? n & 7 : n), total - 1);
+        const float* qr = a.q + (size_t)(it.sq.first + (rc >> a.lg)) * a.ldq +
+                          ((size_t)(g << a.lg) + (rc & ((1 << a.lg) - 1))) * HD + 8 * qd;
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s) {
+            Q.x[t][s][0] = *reinterpret_cast<const f32x4u*>(qr + 32 * s);
+            Q.x[t][s][1] = *reinterpret_cast<const f32x4u*>(qr + 32 * s + 4);
+        }
+    }
+}
+
+// What the rows see, and their queries' terms.
+template <int HD, int RT, bool PACK>
+__device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r0,
+                                          const Queries<HD, RT, PACK>& Q, Rows<HD, RT, PACK>& R) {
+    using T = Rows<HD, RT, PACK>;
+    const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15;
     const int total = it.sq.n << a.lg;
     unsigned long long mine = 0;
     if (a.bt.parent) mine = tree_line(tree_parent(a.bt, it.sq, lane));
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const int r = r0 + 16 * t + (PACK ? n & 7 : n);
-        const int rc = min(r, total - 1), tok = rc >> a.lg, h = rc & ((1 << a.lg) - 1);
-        const float* qr = a.q + (size_t)(it.sq.first + tok) * a.ldq +
-                          ((size_t)(g << a.lg) + h) * HD;
+        const int tok = min(r0 + 16 * t + (PACK ? n & 7 : n), total - 1) >> a.lg;
         R.m[t] = -INFINITY;
         R.l[t] = 0.0f;
+        R.from[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        R.high[t] = kAnyScore;
         R.lim[t] = it.sq.ctx + tok + 1;
         R.line[t] = 0;
         if (a.bt.parent) {
@@ -308,17 +366,11 @@ __device__ __forceinline__ void load_rows(const PaArgs& a, const Item& it, int g
             R.line[t] = tok < QLM_TREE_MAX ? ln : 0;
             R.lim[t] = R.line[t] ? it.sq.ctx : -1;
         }
-        f32x4u x[T::KS][2];
-#pragma unroll
-        for (int s = 0; s < T::KS; ++s) {
-            x[s][0] = *reinterpret_cast<const f32x4u*>(qr + 32 * s + 8 * qd);
-            x[s][1] = *reinterpret_cast<const f32x4u*>(qr + 32 * s + 8 * qd + 4);
-        }
 #pragma unroll
         for (int s = 0; s < T::KS; ++s) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = x[s][i / 4][i % 4] * a.qscale;
+            for (int i = 0; i < 8; ++i) v[i] = Q.x[t][s][i / 4][i % 4] * a.qscale;
             u32x4 hi, lo;
             split8(v, hi, lo);
             if constexpr (PACK) {
@@ -333,12 +385,14 @@ __device__ __forceinline__ void load_rows(const PaArgs& a, const Item& it, int g
     }
 }
 
-// A block of 32 keys from slot k0 on; kp, vp: its K and V planes (of an fp32
-// cache the h planes, the l planes `lo` bytes behind). `all`: every row sees
-// every key of it.
+// Scores of a block of 32 keys from slot k0 on, relative to the references, of
+// keys that a row does not see -inf: x[t][4 h + i] of key 16 h + 4 qd + i. kp:
+// the block's K plane (of an fp32 cache the h plane, the l plane `lo` bytes
+// behind). `all`: every row sees every key of it.
 template <int HD, int RT, bool PACK, bool F32>
-__device__ __forceinline__ void block32(Rows<HD, RT, PACK>& R, const char* kp, const char* vp,
-                                        int lo, int k0, int ctx, int valid0, int valid1, bool all) {
+__device__ __forceinline__ void scores(const Rows<HD, RT, PACK>& R, const char* kp, int lo, int k0,
+                                       int ctx, int valid0, int valid1, bool all,
+                                       float (&x)[RT][8]) {
     using T = Rows<HD, RT, PACK>;
     constexpr int ROW = HD * 2, GRP = 16 * ROW;
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
@@ -346,83 +400,164 @@ __device__ __forceinline__ void block32(Rows<HD, RT, PACK>& R, const char* kp, c
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) s[h][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < RT; ++t) s[h][t] = R.from[t];
+    constexpr int KC = T::KS < 4 ? T::KS : 4;  // k-steps read at once
+    // piece (4 k + qd) ^ n of row n: the bits of k come in by an exclusive or
+    const uint32_t ka = lds_at(kp) + n * ROW + ((qd ^ n) * 16);
 #pragma unroll
-    for (int k = 0; k < T::KS; ++k) {
+    for (int k0s = 0; k0s < T::KS; k0s += KC) {
+        u32x4 kh[KC][2], kl[F32 ? KC : 1][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = h * GRP + n * ROW + (((4 * k + qd) ^ n) * 16);
-            const u32x4 kh = *reinterpret_cast<const u32x4*>(kp + at);
-            u32x4 kl;
-            if constexpr (F32) kl = *reinterpret_cast<const u32x4*>(kp + lo + at);
+        for (int k = 0; k < KC; ++k)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                if constexpr (F32) s[h][t] = mfma(kl, R.q[t][0][k], s[h][t]);
-                if constexpr (!PACK) s[h][t] = mfma(kh, R.q[t][1][k], s[h][t]);
-                s[h][t] = mfma(kh, R.q[t][0][k], s[h][t]);
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t at = (ka ^ (64u * (k0s + k))) + h * GRP;
+                kh[k][h] = lds_read<u32x4>(at);
+                if constexpr (F32) kl[k][h] = lds_read<u32x4>(at + lo);
             }
+        __builtin_amdgcn_sched_barrier(0);
+        // (a sum's terms apart from each other: each waits for the one before)
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            const int ks = k0s + k;
+            if constexpr (F32) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+                        s[h][t] = mfma(kl[k][h], R.q[t][0][ks], s[h][t]);
+            }
+            if constexpr (!PACK) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+                        s[h][t] = mfma(kh[k][h], R.q[t][1][ks], s[h][t]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < RT; ++t) s[h][t] = mfma(kh[k][h], R.q[t][0][ks], s[h][t]);
         }
     }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[t][j] = s[j / 4][t][j % 4];
+            if constexpr (PACK) x[t][j] = fold8(x[t][j]);
+        }
+    if (all) return;
+    asm volatile("");  // (a branch, not selections that every block would compute)
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int in = 4 * qd + j % 4, slot = k0 + 16 * (j / 4) + in, row = slot - ctx;
+            bool sees = slot < R.lim[t];
+            if (row >= 0 && row < QLM_TREE_MAX) sees |= (R.line[t] >> row) & 1ull;
+            sees &= in < (j < 4 ? valid0 : valid1);
+            x[t][j] = sees ? x[t][j] : -INFINITY;
+        }
+}
+
+// Whether some score is too far above its row's reference.
+template <int HD, int RT, bool PACK>
+__device__ __forceinline__ bool too_high(const Rows<HD, RT, PACK>& R, const float (&x)[RT][8]) {
+    bool high = false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        // as integers, in whose order positive floats are: no canonical forms
+        int top = __float_as_int(x[t][0]);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = max(top, __float_as_int(x[t][j]));
+        high |= top > R.high[t];
+    }
+    return __ballot(high) != 0;
+}
+
+// Moves the references to the block's largest scores where those are higher.
+template <int HD, int RT, bool PACK>
+__device__ __forceinline__ void raise(Rows<HD, RT, PACK>& R, const float (&x)[RT][8]) {
+    using T = Rows<HD, RT, PACK>;
+    const int n = threadIdx.x & 15;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float top = x[t][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[t][j]);
+        top = cols_max(top);
+        const bool first = R.m[t] == -INFINITY;
+        const bool moves = top > (first ? -INFINITY : 0.0f);
+        const float by = moves ? top : 0.0f;
+        const float f = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+        R.m[t] = moves ? (first ? 0.0f : R.m[t]) + by : R.m[t];
+        R.l[t] *= f;
+#pragma unroll
+        for (int c = 0; c < T::CB; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) R.acc[t][c][i] *= f;
+        // (a packed tile's two halves are added: one of them begins at 0)
+        const float from = moves && !(PACK && n >= 8) ? -R.m[t] : R.from[t][0];
+        R.from[t] = f32x4{from, from, from, from};
+        // a row that has seen nothing in the block waits for its first score
+        R.high[t] = R.m[t] == -INFINITY ? kAnyScore : __float_as_int(kRise);
+    }
+}
+
+// The block's probabilities into the rows' sums; vp: its V plane.
+template <int HD, int RT, bool PACK, bool F32>
+__device__ __forceinline__ void accumulate(Rows<HD, RT, PACK>& R, float (&x)[RT][8], const char* vp,
+                                           int lo) {
+    using T = Rows<HD, RT, PACK>;
+    constexpr int ROW = HD * 2, GRP = 16 * ROW;
+    const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
+    // V^T: lane l of a group reads 4 columns of key 4 qd + (l % 16) / 4
+    const int key = 4 * qd + (n >> 2);
+    const uint32_t va = lds_at(vp) + key * ROW + ((((n >> 1) & 1) ^ key) * 16) + (n & 1) * 8;
+    auto tr = [&](uint32_t at) {
+        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                             (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
+    };
+    auto read_v = [&](int c, int plane) {  // piece (2 c + ..) ^ key of row `key`
+        const uint32_t at = (va ^ (32u * c)) + plane;
+        const u32x2 v0 = tr(at), v1 = tr(at + GRP);
+        return u32x4{v0.x, v0.y, v1.x, v1.y};
+    };
+    constexpr int VC = 4;  // column blocks read at once, the first before the exponentials
+    u32x4 vh[VC], vl[F32 ? VC : 1];
+    auto read_some = [&](int c0) {
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+            vh[c] = read_v(c0 + c, 0);
+            if constexpr (F32) vl[c] = read_v(c0 + c, lo);
+        }
+    };
+    read_some(0);
+    __builtin_amdgcn_sched_barrier(0);
     u32x4 ph[RT], pl[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[j] = s[j / 4][t][j % 4];
-            if constexpr (PACK) x[j] = fold8(x[j]);
-        }
-        if (!all) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int in = 4 * qd + j % 4, slot = k0 + 16 * (j / 4) + in, row = slot - ctx;
-                bool sees = slot < R.lim[t];
-                if (row >= 0 && row < QLM_TREE_MAX) sees |= (R.line[t] >> row) & 1ull;
-                sees &= in < (j < 4 ? valid0 : valid1);
-                x[j] = sees ? x[j] : -INFINITY;
-            }
-        }
-        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                          fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        top = fmaxf(cols_max(top), R.m[t]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        if (__ballot(top > R.m[t])) {  // a row's maximum has risen
-            const float f = __builtin_amdgcn_exp2f(R.m[t] - ref);  // 0 the first time
-            R.l[t] *= f;
-#pragma unroll
-            for (int c = 0; c < T::CB; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) R.acc[t][c][i] *= f;
-            R.m[t] = top;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
-        R.l[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        split8(x, ph[t], pl[t]);
+        for (int j = 0; j < 8; ++j) x[t][j] = __builtin_amdgcn_exp2f(x[t][j]);
+        R.l[t] += ((x[t][0] + x[t][1]) + (x[t][2] + x[t][3])) +
+                  ((x[t][4] + x[t][5]) + (x[t][6] + x[t][7]));
+        split8(x[t], ph[t], pl[t]);
         if constexpr (PACK) ph[t] = n < 8 ? ph[t] : pl[t];
     }
-    // V^T: lane l of a group reads 4 columns of key 4 qd + (l % 16) / 4
-    const int key = 4 * qd + (n >> 2);
 #pragma unroll
-    for (int c = 0; c < T::CB; ++c) {
-        const int at = key * ROW + (((2 * c + ((n >> 1) & 1)) ^ key) * 16) + (n & 1) * 8;
-        auto tr = [&](const char* p) {
-            return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                 (__attribute__((address_space(3))) s16x4*)p));
+    for (int c0 = 0; c0 < T::CB; c0 += VC) {
+        if (c0) read_some(c0);
+        auto add = [&](const u32x4* v, const u32x4* p) {
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    R.acc[t][c0 + c] = mfma(v[c], p[t], R.acc[t][c0 + c]);
         };
-        const u32x2 v0 = tr(vp + at), v1 = tr(vp + GRP + at);
-        const u32x4 vh = {v0.x, v0.y, v1.x, v1.y};
-        u32x4 vl;
-        if constexpr (F32) {
-            const u32x2 w0 = tr(vp + lo + at), w1 = tr(vp + lo + GRP + at);
-            vl = u32x4{w0.x, w0.y, w1.x, w1.y};
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            if constexpr (F32) R.acc[t][c] = mfma(vl, ph[t], R.acc[t][c]);
-            if constexpr (!PACK) R.acc[t][c] = mfma(vh, pl[t], R.acc[t][c]);
-            R.acc[t][c] = mfma(vh, ph[t], R.acc[t][c]);
-        }
+        if constexpr (F32) add(vl, ph);
+        if constexpr (!PACK) add(vh, pl);
+        add(vh, ph);
     }
 }
 
@@ -485,25 +620,39 @@ __device__ void row_in_fp32(const PaArgs& a, int b, const SeqRows& sq, int i, in
     for (int j = 0; j < E; ++j) o[j] = any ? o[j] / l : 0.0f;
 }
 
+// The gate of a row and head, requested ahead of its use (element lane + 64 j).
+template <int HD>
+__device__ __forceinline__ void load_gate(const PaArgs& a, const SeqRows& sq, int i, int h,
+                                          float (&g)[HD / QLM_WAVE]) {
+    if (!a.gate) return;
+    const float* p = a.gate + (size_t)(sq.first + i) * a.ldg + (size_t)h * a.gate_stride +
+                     (threadIdx.x & (QLM_WAVE - 1));
+#pragma unroll
+    for (int j = 0; j < HD / QLM_WAVE; ++j) g[j] = p[64 * j];
+}
+
 // A row's outputs, E of them a lane (element lane + 64 j): checked, gated, stored.
+// l < 0: a row outside the tree.
 template <int HD, typename KV>
 __device__ __forceinline__ void put_row(const PaArgs& a, int b, const SeqRows& sq, int i, int h,
-                                        float (&o)[HD / QLM_WAVE], float l) {
+                                        float (&o)[HD / QLM_WAVE], float l,
+                                        const float (&g)[HD / QLM_WAVE]) {
     constexpr int E = HD / QLM_WAVE;
     const int lane = threadIdx.x & (QLM_WAVE - 1);
+    const bool dead = l < 0.0f;
     bool fine = l > 0.0f && l < INFINITY;
+    const float inv = 1.0f / l;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-        o[j] /= l;
+        o[j] *= inv;
         fine &= fabsf(o[j]) < INFINITY;
     }
-    if (__ballot(!fine)) row_in_fp32<HD, KV>(a, b, sq, i, h, o);
-    const size_t r = (size_t)(sq.first + i);
+    if (__ballot(!fine && !dead)) row_in_fp32<HD, KV>(a, b, sq, i, h, o);
+    float* to = a.out + (size_t)(sq.first + i) * a.ldo + (size_t)h * HD + lane;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-        const int e = lane + 64 * j;
-        if (a.gate) o[j] *= sigmoid_f(a.gate[r * a.ldg + (size_t)h * a.gate_stride + e]);
-        a.out[r * a.ldo + (size_t)h * HD + e] = o[j];
+        if (a.gate) o[j] *= sigmoid_f(g[j]);
+        to[64 * j] = dead ? 0.0f : o[j];
     }
 }
 
@@ -511,6 +660,84 @@ __device__ __forceinline__ void put_row(const PaArgs& a, int b, const SeqRows& s
 __device__ __forceinline__ int keys_end(const PaArgs& a, const SeqRows& sq, int last) {
     const int n = a.bt.parent ? seen_rows(a, sq) : last + 1;
     return min(sq.ctx + n, a.slots);
+}
+
+// A row's record of a chunk.
+template <int HD>
+__device__ __forceinline__ void put_record(const PaArgs& a, int at, float m, float l,
+                                           const float (&o)[HD / QLM_WAVE]) {
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    if (at >= a.rec_rows) return;
+    float* rec = a.rec + (size_t)at * (HD + 4);
+    if (lane == 0) {
+        rec[0] = m;
+        rec[1] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < HD / QLM_WAVE; ++e) rec[4 + lane + 64 * e] = o[e];
+}
+
+// A tile's rows as they lie in the accumulators: lane (qd, n) has row n's elements
+// 16 c + 4 qd .. + 3. `r`: the lane's row of the unit; l < 0: outside the tree.
+template <int HD>
+__device__ __forceinline__ void put_records(const PaArgs& a, int at, bool real, float m, float l,
+                                            const f32x4 (&acc)[HD / 16]) {
+    const int qd = (threadIdx.x & (QLM_WAVE - 1)) >> 4;
+    if (!real || at >= a.rec_rows) return;
+    float* rec = a.rec + (size_t)at * (HD + 4);
+    if (qd == 0) {
+        rec[0] = m;
+        rec[1] = l;
+    }
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) *reinterpret_cast<f32x4*>(rec + 4 + 16 * c + 4 * qd) = acc[c];
+}
+template <int HD, typename KV>
+__device__ __forceinline__ void put_tile(const PaArgs& a, int b, const SeqRows& sq, int g, int r,
+                                         int total, float l, f32x4 (&acc)[HD / 16]) {
+    constexpr int CB = HD / 16;
+    const int lane = threadIdx.x & (QLM_WAVE - 1), qd = lane >> 4;
+    const bool real = r < total, dead = l < 0.0f;
+    const int rc = min(r, total - 1), tok = rc >> a.lg, h = (g << a.lg) + (rc & ((1 << a.lg) - 1));
+    const size_t row = (size_t)(sq.first + tok);
+    f32x4u gate[CB];
+    if (a.gate) {
+        const float* p = a.gate + row * a.ldg + (size_t)h * a.gate_stride + 4 * qd;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) gate[c] = *reinterpret_cast<const f32x4u*>(p + 16 * c);
+    }
+    const float inv = 1.0f / l;
+    bool fine = l > 0.0f && l < INFINITY;
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            acc[c][i] *= inv;
+            fine &= fabsf(acc[c][i]) < INFINITY;
+        }
+    unsigned long long bad = __ballot(real && !dead && !fine);
+    bad |= bad >> 32;
+    bad = (bad | bad >> 16) & 0xffffull;
+    float* to = a.out + row * a.ldo + (size_t)h * HD + 4 * qd;
+    if (real && !(bad >> (lane & 15) & 1ull)) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+            f32x4u o = acc[c];
+            if (a.gate) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] *= sigmoid_f(gate[c][i]);
+            }
+            if (dead) o = f32x4u{0.0f, 0.0f, 0.0f, 0.0f};
+            *reinterpret_cast<f32x4u*>(to + 16 * c) = o;
+        }
+    }
+    for (; bad; bad &= bad - 1) {  // a row at a time, the whole wave
+        const int from = __ffsll((long long)bad) - 1;
+        const int i = __builtin_amdgcn_readlane(tok, from), hh = __builtin_amdgcn_readlane(h, from);
+        float o[HD / QLM_WAVE] = {}, gr[HD / QLM_WAVE] = {};
+        load_gate<HD>(a, sq, i, hh, gr);
+        put_row<HD, KV>(a, b, sq, i, hh, o, 0.0f, gr);
+    }
 }
 
 // Where the unit's rows leave their results: descriptors for k_pa_join.
@@ -530,7 +757,7 @@ __device__ __forceinline__ void put_desc(const PaArgs& a, const Item& it, int g,
 template <int HD, bool F32>
 struct FewShape {
     static constexpr int BLK = 2 * 2 * Lay<HD, F32>::RAW;  // a block's bytes: K, V, two groups
-    static constexpr int NW = 65536 * 2 / (2 * BLK);       // 128 KB of LDS: two blocks a wave
+    static constexpr int NW = 128 * 1024 / (2 * BLK);      // 128 KB of LDS: two blocks a wave
 };
 
 template <int HD, bool F32, bool PACK>
@@ -549,13 +776,14 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     head_and_item(blockIdx.x, a.pg.n_kv, g, want);
     Item it;
     if (want >= a.items || !find_item<MT>(a, want, it)) return;
-    const int total = it.sq.n << a.lg, r0 = it.tile * MT;
-    const int end = keys_end(a, it.sq, (min(r0 + MT, total) - 1) >> a.lg);
-    const int nch = (end - 1) / it.len + 1;
+    it.sq = SeqRows{uni(it.sq.first), uni(it.sq.n), uni(it.sq.ctx)};
+    const int total = uni(it.sq.n << a.lg), r0 = uni(it.tile * MT);
+    const int end = uni(keys_end(a, it.sq, (min(r0 + MT, total) - 1) >> a.lg));
+    const int nch = uni((end - 1) / it.len + 1);
     if (it.chunk >= nch) return;
-    const int b = it.b, k0 = it.chunk * it.len, k1 = min(k0 + it.len, end);
-    const int lgp = 31 - __clz(a.pg.page_size);
-    const int blocks = (k1 - k0 + 31) / 32, mine = (blocks - wave + NW - 1) / NW;
+    const int b = uni(it.b), k0 = uni(it.chunk * it.len), k1 = uni(min(k0 + it.len, end));
+    const int lgp = uni(31 - __clz(a.pg.page_size));
+    const int blocks = uni((k1 - k0 + 31) / 32), mine = uni((blocks - wave + NW - 1) / NW);
     char* ring = smem + wave * 2 * S::BLK;
     auto slot_of = [&](int j) { return k0 + 32 * (wave + j * NW); };
     auto groups = [&](int j, Group (&gr)[2]) {
@@ -575,49 +803,61 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     Group gr[3][2];                 // of blocks j, j + 1 and j + 2
 #pragma unroll
     for (int j = 0; j < 3; ++j) groups(j, gr[j]);
-    Rows<HD, 1, PACK> R;
-    load_rows<HD, 1, PACK>(a, it, g, r0, R);
-    // (the queries' loads are waited for before any of the ring's goes out)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // queries first: what is waited for first
+    Queries<HD, 1, PACK> Q;
+    request_rows<HD, 1, PACK>(a, it, g, r0, Q);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < D; ++j)
         if (j < mine) fetch(j, gr[j]);
+    __builtin_amdgcn_sched_barrier(0);
+    Rows<HD, 1, PACK> R;
+    take_rows<HD, 1, PACK>(a, it, r0, Q, R);
+    int staged = -1, raised = -1;  // the block that is there, and the last one begun again
+    float x[1][8];
+    for (int j = 0;;) {
+        bool move = false;
 #pragma unroll 1
-    for (int j = 0; j < mine; ++j) {
-        if (!F32 && j + 1 < mine)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const int s0 = slot_of(j);
-        const bool all = s0 + 32 <= it.sq.ctx && gr[0][0].valid == 16 && gr[0][1].valid == 16;
-        char* at = ring + (F32 ? 0 : j & 1) * S::BLK;
-        if constexpr (F32) {
+        for (; j < mine; ++j) {
+            const int s0 = slot_of(j);
+            char* at = ring + (F32 ? 0 : j & 1) * S::BLK;
             // planes: K h, K l, V h, V l
-            char* pl = ring + S::BLK;
+            char* const pl = F32 ? ring + S::BLK : at;
+            if (staged != j) {
+                staged = j;
+                if (!F32 && j + 1 < mine)
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                if constexpr (F32) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                split_group<HD>(at + h * RAW, pl + h * GRP, pl + (2 + h) * GRP, 0, 1);
-                split_group<HD>(at + (2 + h) * RAW, pl + (4 + h) * GRP, pl + (6 + h) * GRP, 0, 1);
+                    for (int h = 0; h < 2; ++h) {
+                        split_group<HD>(at + h * RAW, pl + h * GRP, pl + (2 + h) * GRP);
+                        split_group<HD>(at + (2 + h) * RAW, pl + (4 + h) * GRP, pl + (6 + h) * GRP);
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (j + 1 < mine) fetch(j + 1, gr[1]);
+                }
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (j + 1 < mine) fetch(j + 1, gr[1]);
-            block32<HD, 1, PACK, F32>(R, pl, pl + 4 * GRP, 2 * GRP, s0, it.sq.ctx, gr[0][0].valid,
-                                      gr[0][1].valid, all);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        } else {
-            block32<HD, 1, PACK, F32>(R, at, at + 2 * RAW, 0, s0, it.sq.ctx, gr[0][0].valid,
-                                      gr[0][1].valid, all);
+            const bool all = s0 + 32 <= it.sq.ctx && gr[0][0].valid == 16 && gr[0][1].valid == 16;
+            scores<HD, 1, PACK, F32>(R, pl, 2 * GRP, s0, it.sq.ctx, gr[0][0].valid, gr[0][1].valid,
+                                     all, x);
+            move = raised != j && too_high(R, x);
+            if (move) break;
+            accumulate<HD, 1, PACK, F32>(R, x, pl + (F32 ? 4 * GRP : 2 * RAW), 2 * GRP);
             // the block is read: its place takes the next but one
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (j + 2 < mine) fetch(j + 2, gr[2]);
-        }
+            if (!F32 && j + 2 < mine) fetch(j + 2, gr[2]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            gr[0][h] = gr[1][h];
-            gr[1][h] = gr[2][h];
+            for (int h = 0; h < 2; ++h) {
+                gr[0][h] = gr[1][h];
+                gr[1][h] = gr[2][h];
+            }
+            groups(j + 3, gr[2]);
         }
-        groups(j + 3, gr[2]);
+        if (!move) break;
+        raise(R, x);
+        raised = j;  // once a block: a score that is not finite stays too high
     }
     // ---- the waves' sums meet ----
     __syncthreads();
@@ -642,7 +882,9 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     if (it.chunk == 0 && a.desc) put_desc<MT>(a, it, g, nch);
     const int rows = min(MT, total - r0);
     for (int r = wave; r < rows; r += NW) {
-        float m = -INFINITY, l = 0.0f, o[HD / 64] = {};
+        const int tok = (r0 + r) >> a.lg, h = (g << a.lg) + ((r0 + r) & ((1 << a.lg) - 1));
+        float m = -INFINITY, l = 0.0f, o[HD / 64] = {}, gate[HD / 64] = {};
+        if (nch == 1) load_gate<HD>(a, it.sq, tok, h, gate);
 #pragma unroll
         for (int w = 0; w < NW; ++w) m = fmaxf(m, pm[w * 16 + r]);
         const float ref = m == -INFINITY ? 0.0f : m;
@@ -655,223 +897,276 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
                 o[e] = fmaf(po[(w * 16 + r) * OST + lane + 64 * e], f, o[e]);
         }
         // (blocks that every row sees go unmasked: a row outside the tree too)
-        if (__shfl(R.lim[0], r) < 0) l = 0.0f;
-        const int tok = (r0 + r) >> a.lg, h = (g << a.lg) + ((r0 + r) & ((1 << a.lg) - 1));
-        if (nch == 1) {
-            put_row<HD, KV>(a, b, it.sq, tok, h, o, l);
-        } else {
-            const int at = ((it.rec + it.chunk) * a.pg.n_kv + g) * MT + r;
-            if (at < a.rec_rows) {
-                float* rec = a.rec + (size_t)at * (HD + 4);
-                if (lane == 0) {
-                    rec[0] = m;
-                    rec[1] = l;
-                }
-#pragma unroll
-                for (int e = 0; e < HD / 64; ++e) rec[4 + lane + 64 * e] = o[e];
-            }
-        }
+        if (__shfl(R.lim[0], r) < 0) l = -1.0f;
+        if (nch == 1)
+            put_row<HD, KV>(a, b, it.sq, tok, h, o, l, gate);
+        else
+            put_record<HD>(a, ((it.rec + it.chunk) * a.pg.n_kv + g) * MT + r, m, l, o);
     }
 }
 
 // ---- more rows: four waves share each block of keys ----
+// WK such fours take the blocks in turn, each through LDS of its own, so that
+// every SIMD has two waves whose products and exponentials take turns; they
+// meet at the end. (An fp32 cache of 256-wide heads fills LDS with one.)
 template <int HD, bool F32>
 struct TileShape {
+    static constexpr int WK = HD == 256 && F32 ? 1 : 2;
     static constexpr int KB = HD == 128 && !F32 ? 64 : 32;  // keys of a block
     static constexpr int BLK = KB / 16 * 2 * Lay<HD, F32>::RAW;
-    static constexpr int OST = HD + 4;  // floats of an output row on its way out
-    static constexpr int LDS = std::max(F32 ? BLK + KB / 16 * 4 * Lay<HD, F32>::GRP : 2 * BLK,
-                                        4 * 16 * OST * 4);
+    // of a four: two blocks, or a raw block and its planes
+    static constexpr int LDS = F32 ? BLK + KB / 16 * 4 * Lay<HD, F32>::GRP : 2 * BLK;
+    static constexpr int ALL = WK * LDS;
 };
 
 template <int HD, bool F32, int RT>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void k_pa_tile(PaArgs a) {
+__global__ __launch_bounds__(256 * (HD == 256 && F32 ? 1 : 2), HD == 256 && F32 ? 1 : 2)
+void k_pa_tile(PaArgs a) {
     using L = Lay<HD, F32>;
     using S = TileShape<HD, F32>;
     using KV = typename std::conditional<F32, float, uint16_t>::type;
-    constexpr int NW = 4, MT = 16 * RT * NW, KB = S::KB, NG = KB / 16, GRP = L::GRP, RAW = L::RAW;
-    constexpr int OST = S::OST;
-    __shared__ __attribute__((aligned(1024))) char smem[S::LDS];
-    const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
+    constexpr int NW = 4, WK = S::WK, MT = 16 * RT * NW, KB = S::KB, NG = KB / 16;
+    constexpr int GRP = L::GRP, RAW = L::RAW;
+    constexpr int PART = RT * (HD / 16) * 1024 + RT * 512;  // a wave's sums on their way to join
+    static_assert(WK == 1 || NW * PART <= S::ALL, "the sums fit");
+    __shared__ __attribute__((aligned(1024))) char smem[S::ALL];
+    __shared__ int there[WK][2][NG];  // slots of a block's groups that are there
+    const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE % NW);
+    const int four = __builtin_amdgcn_readfirstlane(threadIdx.x / (QLM_WAVE * NW));
     int g, want;
     head_and_item(blockIdx.x, a.pg.n_kv, g, want);
     Item it;
     if (want >= a.items || !find_item<MT>(a, want, it)) return;
-    const int total = it.sq.n << a.lg, r0 = it.tile * MT;
-    const int end = keys_end(a, it.sq, (min(r0 + MT, total) - 1) >> a.lg);
-    const int nch = (end - 1) / it.len + 1;
+    it.sq = SeqRows{uni(it.sq.first), uni(it.sq.n), uni(it.sq.ctx)};
+    const int total = uni(it.sq.n << a.lg), r0 = uni(it.tile * MT);
+    const int end = uni(keys_end(a, it.sq, (min(r0 + MT, total) - 1) >> a.lg));
+    const int nch = uni((end - 1) / it.len + 1);
     if (it.chunk >= nch) return;
-    const int b = it.b, k0 = it.chunk * it.len, k1 = min(k0 + it.len, end);
-    const int lgp = 31 - __clz(a.pg.page_size);
-    const int blocks = (k1 - k0 + KB - 1) / KB;
-    // units (a group's K or V) u = wave, wave + 4, ... are this wave's to fetch
-    auto groups = [&](int j, Group (&gr)[NG]) {
+    const int b = uni(it.b), k0 = uni(it.chunk * it.len), k1 = uni(min(k0 + it.len, end));
+    const int lgp = uni(31 - __clz(a.pg.page_size));
+    // this four's blocks four, four + WK, ..: as many steps as the first four has
+    const int blocks = uni(((k1 - k0 + KB - 1) / KB + WK - 1) / WK);
+    auto slot_of = [&](int j) { return k0 + (j * WK + four) * KB; };
+    char* const lds = smem + four * S::LDS;
+    // units (a group's K or V) u = wave, wave + 4, ... are this wave's to fetch:
+    // all of one group
+    static_assert(NW % NG == 0, "a wave's units are one group's");
+    const int own = wave % NG;
+    auto group = [&](int j) { return group_at(a, b, slot_of(j) + 16 * own, k1, lgp); };
+    auto fetch = [&](int j, const Group& gr) {
+        char* to = lds + (F32 ? 0 : j & 1) * S::BLK;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) gr[i] = group_at(a, b, k0 + j * KB + 16 * i, k1, lgp);
+        for (int u = 0; u < 2 * NG; u += NW)
+            fetch_group<HD, F32>(a, u + wave < NG ? a.pg.k : a.pg.v, gr, g, slot_of(j) + 16 * own,
+                                 to + (u + wave) * RAW);
+        if (lane == 0) there[four][j & 1][own] = gr.valid;
     };
-    auto fetch = [&](int j, const Group (&gr)[NG]) {
-        char* to = smem + (F32 ? 0 : j & 1) * S::BLK;
-#pragma unroll
-        for (int u = 0; u < 2 * NG; ++u) {
-            if (u % NW != wave) continue;
-            fetch_group<HD, F32>(a, u < NG ? a.pg.k : a.pg.v, gr[u % NG], g,
-                                 k0 + j * KB + 16 * (u % NG), to + u * RAW);
-        }
-    };
-    Group gr[2][NG];
-    groups(0, gr[0]);
-    groups(1, gr[1]);
-    Rows<HD, RT, false> R;
-    const int w0 = r0 + 16 * RT * wave;  // this wave's first row
-    load_rows<HD, RT, false>(a, it, g, w0, R);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    Group gr[2] = {group(0), group(1)};
+    const int w0 = uni(r0 + 16 * RT * wave);  // this wave's first row
+    Queries<HD, RT, false> Q;
+    request_rows<HD, RT, false>(a, it, g, w0, Q);
     __builtin_amdgcn_sched_barrier(0);
     fetch(0, gr[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    Rows<HD, RT, false> R;
+    take_rows<HD, RT, false>(a, it, w0, Q, R);
     // what all of this wave's rows see without a mask, and all they can see
-    const int wave_end = min(w0 < total ? keys_end(a, it.sq, (min(w0 + 16 * RT, total) - 1) >> a.lg) : 0, k1);
-    const int free_end = a.bt.parent ? it.sq.ctx : it.sq.ctx + (w0 >> a.lg) + 1;
+    const int wave_end = uni(
+        w0 < total ? min(keys_end(a, it.sq, (min(w0 + 16 * RT, total) - 1) >> a.lg), k1) : 0);
+    const int free_end = uni(a.bt.parent ? it.sq.ctx : it.sq.ctx + (w0 >> a.lg) + 1);
+    constexpr int SUB = KB / 32;  // 32-key parts of a block
+    int staged = -1, raised = -1, valid[NG];
+    float x[RT][8];
+    for (int i = 0;;) {
+        bool move = false;
 #pragma unroll 1
-    for (int j = 0; j < blocks; ++j) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // the block is there, and every wave is done with the last one
-        char* at = smem + (F32 ? 0 : j & 1) * S::BLK;
-        if constexpr (F32) {
-            char* pl = smem + S::BLK;  // planes: K h, K l, V h, V l
+        for (; i < blocks * SUB; ++i) {
+            const int j = i / SUB, h = i % SUB, s0 = slot_of(j) + 32 * h;
+            char* at = lds + (F32 ? 0 : j & 1) * S::BLK;
+            char* const pl = lds + S::BLK;  // fp32: planes K h, K l, V h, V l
+            if (staged != j) {
+                staged = j;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();  // the block is there, and every wave is done with the last one
+                if constexpr (F32) {
 #pragma unroll
-            for (int u = 0; u < 2 * NG; ++u) {
-                if (u % NW != wave) continue;
-                char* to = pl + (u < NG ? u : u + NG) * GRP;
-                split_group<HD>(at + u * RAW, to, to + NG * GRP, 0, 1);
+                    for (int u = 0; u < 2 * NG; u += NW) {
+                        const int v = u + wave;
+                        char* to = pl + (v < NG ? v : v + NG) * GRP;
+                        split_group<HD>(at + v * RAW, to, to + NG * GRP);
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int k = 0; k < NG; ++k) valid[k] = uni(there[four][j & 1][k]);
+                if (j + 1 < blocks) fetch(j + 1, gr[1]);
+                gr[1] = group(j + 2);
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __syncthreads();
-        }
-        if (j + 1 < blocks) fetch(j + 1, gr[1]);
-#pragma unroll
-        for (int h = 0; h < NG / 2; ++h) {
-            const int s0 = k0 + j * KB + 32 * h;
-            if (s0 >= wave_end) break;
-            const int va = gr[0][2 * h].valid, vb = gr[0][2 * h + 1].valid;
+            if (s0 >= wave_end) continue;
+            int va = valid[0], vb = valid[1];
+            if (SUB > 1 && h) {
+                va = valid[NG - 2];
+                vb = valid[NG - 1];
+            }
             const bool all = s0 + 32 <= free_end && va == 16 && vb == 16;
-            const char* kp = F32 ? smem + S::BLK + 2 * h * GRP : at + 2 * h * RAW;
-            const char* vp = F32 ? kp + 2 * NG * GRP : kp + NG * RAW;
-            block32<HD, RT, false, F32>(R, kp, vp, NG * GRP, s0, it.sq.ctx, va, vb, all);
+            const char* kp = F32 ? pl : at + 2 * h * RAW;
+            scores<HD, RT, false, F32>(R, kp, NG * GRP, s0, it.sq.ctx, va, vb, all, x);
+            move = raised != i && too_high(R, x);
+            if (move) break;
+            accumulate<HD, RT, false, F32>(R, x, kp + (F32 ? 2 * NG * GRP : NG * RAW), NG * GRP);
         }
-#pragma unroll
-        for (int i = 0; i < NG; ++i) gr[0][i] = gr[1][i];
-        groups(j + 2, gr[1]);
+        if (!move) break;
+        raise(R, x);
+        raised = i;  // once a part: a score that is not finite stays too high
     }
     if (it.chunk == 0 && a.desc) put_desc<MT>(a, it, g, nch);
-    // a tile at a time through LDS, a row a time out of it
     __syncthreads();
-    float* po = reinterpret_cast<float*>(smem) + wave * 16 * OST;
+    if constexpr (WK == 2) {
+        // the second four's sums to the wave of the first that has the same rows
+        char* const to = smem + wave * PART;
+        float* const st = reinterpret_cast<float*>(to + RT * (HD / 16) * 1024);
+        if (four) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const float lsum = cols_sum(R.l[t]);
+            for (int t = 0; t < RT; ++t) {
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c)
-            *reinterpret_cast<f32x4*>(po + n * OST + 16 * c + 4 * qd) = R.acc[t][c];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const int rows = min(16, total - w0 - 16 * t);
-        for (int i = 0; i < rows; ++i) {
-            const int r = w0 + 16 * t + i;
-            const float m = __shfl(R.m[t], i);
-            const float l = __shfl(R.lim[t], i) < 0 ? 0.0f : __shfl(lsum, i);
-            float o[HD / 64];
-#pragma unroll
-            for (int e = 0; e < HD / 64; ++e) o[e] = po[i * OST + lane + 64 * e];
-            if (nch == 1) {
-                put_row<HD, KV>(a, b, it.sq, r >> a.lg, (g << a.lg) + (r & ((1 << a.lg) - 1)), o,
-                                l);
-            } else {
-                const int to = ((it.rec + it.chunk) * a.pg.n_kv + g) * MT + r - r0;
-                if (to < a.rec_rows) {
-                    float* rec = a.rec + (size_t)to * (HD + 4);
-                    if (lane == 0) {
-                        rec[0] = m;
-                        rec[1] = l;
-                    }
-#pragma unroll
-                    for (int e = 0; e < HD / 64; ++e) rec[4 + lane + 64 * e] = o[e];
-                }
+                for (int c = 0; c < HD / 16; ++c)
+                    *reinterpret_cast<f32x4*>(to + (t * (HD / 16) + c) * 1024 + lane * 16) =
+                        R.acc[t][c];
+                st[t * 128 + lane] = R.m[t];
+                st[t * 128 + 64 + lane] = R.l[t];
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        __syncthreads();
+        if (four) return;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const float m1 = st[t * 128 + lane], l1 = st[t * 128 + 64 + lane];
+            const float m = fmaxf(R.m[t], m1), ref = m == -INFINITY ? 0.0f : m;
+            const float f0 = __builtin_amdgcn_exp2f(R.m[t] - ref);
+            const float f1 = __builtin_amdgcn_exp2f(m1 - ref);
+            R.m[t] = m;
+            R.l[t] = R.l[t] * f0 + l1 * f1;
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                const f32x4 o = *reinterpret_cast<const f32x4*>(to + (t * (HD / 16) + c) * 1024 +
+                                                               lane * 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) R.acc[t][c][i] = R.acc[t][c][i] * f0 + o[i] * f1;
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float l = R.lim[t] < 0 ? -1.0f : cols_sum(R.l[t]);
+        const int r = w0 + 16 * t + n;
+        if (nch == 1)
+            put_tile<HD, KV>(a, b, it.sq, g, r, total, l, R.acc[t]);
+        else
+            put_records<HD>(a, ((it.rec + it.chunk) * a.pg.n_kv + g) * MT + r - r0, r < total, R.m[t],
+                            l, R.acc[t]);
     }
 }
 
-// ---- the chunks' records of a row and head, merged: a workgroup a row and head ----
-template <int HD, typename KV>
-__global__ __launch_bounds__(256) void k_pa_join(PaArgs a, int mt) {
-    constexpr int E = HD / QLM_WAVE, NW = 4;
+// ---- the chunks' records, merged: a row and head a task ----
+// WPT waves take a task's records in turn, kJoinFlight of them in flight each,
+// and meet in LDS. Few tasks (tokens) have many records: four waves a task.
+// Many (trees, prompts) have few or one: a wave a task, which looks `per` tasks'
+// descriptors up at once, since most rows of a prompt have nothing to merge.
+constexpr int kJoinThreads = 256, kJoinFlight = 8;
+
+template <int HD, typename KV, int WPT>
+__global__ __launch_bounds__(kJoinThreads) void k_pa_join(PaArgs a, int mt, int per) {
+    constexpr int E = HD / QLM_WAVE, NW = kJoinThreads / QLM_WAVE;
     __shared__ float pm[NW], pl[NW], po[NW][HD];
-    const int row = blockIdx.x, h = blockIdx.y, g = h >> a.lg, lane = threadIdx.x & 63;
-    const int wave = threadIdx.x / QLM_WAVE;
-    const int2 d = a.desc[(size_t)row * a.pg.n_kv + g];
-    const int b = seq_of_row(a.bt, row);
-    if (b < 0) return;
-    const SeqRows sq = seq_rows(a.bt, b);
-    const int i = row - sq.first, nch = d.y;
-    if (i < 0 || i >= sq.n || nch <= 1) return;
+    const int lane = threadIdx.x & 63, G = 1 << a.lg, tasks = a.bt.rows * a.n_q;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE);
+    const int first = (blockIdx.x * (NW / WPT) + wave / WPT) * per;
+    int2 d = make_int2(0, 0);
+    if (lane < per && first + lane < tasks) {
+        const int row = (first + lane) / a.n_q, h = first + lane - row * a.n_q;
+        d = a.desc[(size_t)row * a.pg.n_kv + (h >> a.lg)];
+        d.x += h & (G - 1);
+    }
     const long long stride = (long long)a.pg.n_kv * mt;
-    const long long base = (long long)d.x + (h & ((1 << a.lg) - 1));
-    if (d.x < 0 || base + (nch - 1) * stride >= a.rec_rows) return;
-    float m = -INFINITY, l = 0.0f, o[E] = {};
-    // four records a wave in flight
-    for (int c0 = wave; c0 < nch; c0 += 4 * NW) {
-        float rm[4], rl[4], ro[4][E];
+    // (a row of no sequence has no descriptor: whatever lies there)
+    unsigned long long todo =
+        __ballot(d.y > 1 && d.x >= 0 && d.x + (d.y - 1) * stride < a.rec_rows);
+    for (; todo; todo &= todo - 1) {  // WPT > 1: one task, the same in all its waves
+        const int k = __ffsll((long long)todo) - 1;
+        const int nch = __builtin_amdgcn_readlane(d.y, k);
+        const int task = first + k, row = task / a.n_q, h = task - row * a.n_q;
+        const int b = seq_of_row(a.bt, row);
+        if (b < 0) continue;
+        const SeqRows sq = seq_rows(a.bt, b);
+        const int i = row - sq.first;
+        if (i < 0 || i >= sq.n) continue;
+        float gate[E] = {};
+        load_gate<HD>(a, sq, i, h, gate);
+        const float* rec = a.rec + (size_t)__builtin_amdgcn_readlane(d.x, k) * (HD + 4);
+        const size_t step = (size_t)stride * (HD + 4);
+        float m = -INFINITY, l = 0.0f, o[E] = {};
+        for (int c0 = wave % WPT; c0 < nch; c0 += kJoinFlight * WPT) {
+            float rm[kJoinFlight], rl[kJoinFlight], ro[kJoinFlight][E];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int c = min(c0 + u * NW, nch - 1);
-            const float* rec = a.rec + (size_t)(base + c * stride) * (HD + 4);
-            rm[u] = rec[0];
-            rl[u] = rec[1];
+            for (int u = 0; u < kJoinFlight; ++u) {
+                const float* r = rec + (size_t)min(c0 + u * WPT, nch - 1) * step;
+                rm[u] = r[0];
+                rl[u] = r[1];
 #pragma unroll
-            for (int e = 0; e < E; ++e) ro[u][e] = rec[4 + lane + 64 * e];
+                for (int e = 0; e < E; ++e) ro[u][e] = r[4 + lane + 64 * e];
+            }
+            if (rl[0] < 0.0f) {  // a row outside the tree, in every chunk
+                m = -INFINITY;
+                l = -1.0f;
+                break;
+            }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < kJoinFlight; ++u) top = fmaxf(top, rm[u]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            const float f = __builtin_amdgcn_exp2f(m - ref);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= f;
+#pragma unroll
+            for (int u = 0; u < kJoinFlight; ++u) {
+                if (c0 + u * WPT >= nch) break;
+                const float w = __builtin_amdgcn_exp2f(rm[u] - ref);
+                l = fmaf(rl[u], w, l);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = fmaf(ro[u][e], w, o[e]);
+            }
+            m = top;
         }
-        float top = m;
+        if constexpr (WPT > 1) {
+            if (lane == 0) {
+                pm[wave] = m;
+                pl[wave] = l;
+            }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) top = fmaxf(top, rm[u]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        const float f = __builtin_amdgcn_exp2f(m - ref);
-        l *= f;
+            for (int e = 0; e < E; ++e) po[wave][lane + 64 * e] = o[e];
+            __syncthreads();
+            if (wave) return;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= f;
+            for (int w = 0; w < WPT; ++w) m = fmaxf(m, pm[w]);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            const bool dead = l < 0.0f;
+            l = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (c0 + u * NW >= nch) break;
-            const float w = __builtin_amdgcn_exp2f(rm[u] - ref);
-            l = fmaf(rl[u], w, l);
+            for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(ro[u][e], w, o[e]);
+            for (int w = 0; w < WPT; ++w) {
+                const float f = __builtin_amdgcn_exp2f(pm[w] - ref);
+                l = fmaf(pl[w], f, l);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = fmaf(po[w][lane + 64 * e], f, o[e]);
+            }
+            if (dead) l = -1.0f;
         }
-        m = top;
+        put_row<HD, KV>(a, b, sq, i, h, o, l, gate);
     }
-    if (lane == 0) {
-        pm[wave] = m;
-        pl[wave] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) po[wave][lane + 64 * e] = o[e];
-    __syncthreads();
-    if (wave) return;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, pm[w]);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const float f = __builtin_amdgcn_exp2f(pm[w] - ref);
-        l = fmaf(pl[w], f, l);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(po[w][lane + 64 * e], f, o[e]);
-    }
-    put_row<HD, KV>(a, b, sq, i, h, o, l);
 }
 
 // ---- the host's part ----
@@ -879,6 +1174,7 @@ __global__ __launch_bounds__(256) void k_pa_join(PaArgs a, int mt) {
 struct PaPlan {
     int mt;              // rows of a unit: 8, 16 (k_pa_few), 64 or 128 (k_pa_tile)
     int target;          // items a kv head to cut the keys into
+    int least, alone;    // keys of an item, at least; of a sequence that is not cut
     int items;           // at most
     int rec_rows;        // records
     bool join;           // some unit may have several chunks
@@ -889,13 +1185,15 @@ PaPlan plan_of(int rows, int B, int G, int n_kv, int hd, long long slots) {
     PaPlan p{};
     // about the rows of a sequence
     const long long per = ((long long)rows * G + B - 1) / B;
-    p.mt = per <= 8 ? 8 : per <= 16 ? 16 : per <= 64 ? 64 : 128;
-    const int wanted = p.mt <= 16 ? 512 : 512;
+    p.mt = per <= 8 ? 8 : per <= 16 ? 16 : per <= 64 || hd == 256 ? 64 : 128;
+        const int wanted = p.mt <= 16 ? 512 : 256;  // a CU holds one workgroup of either
     p.target = std::max(1, wanted / n_kv);
     const long long units = ((long long)rows * G) / p.mt + B;
-    p.items = (int)(units + p.target);
-    p.join = slots > kMinChunk;
-    if (p.join) p.rec_rows = 2 * p.target * n_kv * p.mt;
+    p.items = (int)(units + p.target + 8);  // (8: what fp32 sums may be off by)
+    p.alone = p.mt <= 16 ? 1024 : 128;
+    p.least = p.mt <= 16 ? 256 : 128;
+    p.join = slots > p.alone;
+    if (p.join) p.rec_rows = (2 * p.target + 16) * n_kv * p.mt;
     const size_t rec = (size_t)p.rec_rows * (hd + 4) * sizeof(float);
     p.desc_at = rec;
     p.bytes = p.join ? rec + (size_t)rows * n_kv * sizeof(int2) : 0;
@@ -922,19 +1220,26 @@ template <int HD, bool F32>
 int launch_attention(const PaArgs& a, const PaPlan& p, hipStream_t st) {
     using KV = typename std::conditional<F32, float, uint16_t>::type;
     const dim3 grid((unsigned)groups_of(p.items, a.pg.n_kv));
+    const dim3 few(FewShape<HD, F32>::NW * QLM_WAVE), tile(256 * TileShape<HD, F32>::WK);
     if (p.mt == 8)
-        hipLaunchKernelGGL((k_pa_few<HD, F32, true>), grid, dim3(FewShape<HD, F32>::NW * QLM_WAVE),
-                           0, st, a);
+        hipLaunchKernelGGL((k_pa_few<HD, F32, true>), grid, few, 0, st, a);
     else if (p.mt == 16)
-        hipLaunchKernelGGL((k_pa_few<HD, F32, false>), grid, dim3(FewShape<HD, F32>::NW * QLM_WAVE),
-                           0, st, a);
+        hipLaunchKernelGGL((k_pa_few<HD, F32, false>), grid, few, 0, st, a);
     else if (p.mt == 64)
-        hipLaunchKernelGGL((k_pa_tile<HD, F32, 1>), grid, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_pa_tile<HD, F32, 2>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_pa_tile<HD, F32, 1>), grid, tile, 0, st, a);
+    else if constexpr (HD == 128)
+        hipLaunchKernelGGL((k_pa_tile<HD, F32, 2>), grid, tile, 0, st, a);
     const int rc = qlm_launch_status();
     if (rc != QLM_OK || !p.join) return rc;
-    hipLaunchKernelGGL((k_pa_join<HD, KV>), dim3(a.bt.rows, a.n_q), dim3(256), 0, st, a, p.mt);
+    const int tasks = a.bt.rows * a.n_q;
+    if (tasks <= 2048) {
+        hipLaunchKernelGGL((k_pa_join<HD, KV, 4>), dim3(tasks), dim3(kJoinThreads), 0, st, a, p.mt,
+                           1);
+    } else {
+        const int per = std::min((tasks + 8191) / 8192, QLM_WAVE);
+        hipLaunchKernelGGL((k_pa_join<HD, KV, 1>), dim3((tasks + 4 * per - 1) / (4 * per)),
+                           dim3(kJoinThreads), 0, st, a, p.mt, per);
+    }
     return qlm_launch_status();
 }
 
@@ -961,7 +1266,7 @@ extern "C" int qlm_paged_attention(const float* q, int ldq, const qlm_row_batch*
     if (gate && (gate_stride < hd || ldg < (n_q - 1) * gate_stride + hd)) return QLM_ERR_SHAPE;
     const int G = n_q / n_kv;
     const PaPlan p = plan_of(batch->rows, batch->B, G, n_kv, hd, slots);
-    if (groups_of(p.items, n_kv) >= 1LL << 24) return QLM_ERR_SHAPE;  // a launch's threads fit 32 bits
+    if (groups_of(p.items, n_kv) >= 1LL << 23) return QLM_ERR_SHAPE;  // a launch's threads fit 32 bits
     if (p.bytes > 0 && (!work || work_bytes < p.bytes)) return QLM_ERR_ARG;
     if ((uintptr_t)work & 15u) return QLM_ERR_SHAPE;
     PaArgs a{};
@@ -977,6 +1282,8 @@ extern "C" int qlm_paged_attention(const float* q, int ldq, const qlm_row_batch*
     a.n_q = n_q;
     while ((1 << a.lg) < G) ++a.lg;
     a.target = p.target;
+    a.least = p.least;
+    a.alone = p.alone;
     a.items = p.items;
     a.rec_rows = p.rec_rows;
     a.slots = (int)slots;
@@ -995,5 +1302,5 @@ extern "C" int qlm_paged_attention(const float* q, int ldq, const qlm_row_batch*
 // otherwise loads it at the first launch of one of its kernels.
 hipError_t qlm_load_paged_attention() {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>((k_pa_join<128, float>)));
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>((k_pa_join<128, float, 1>)));
 }
