@@ -629,7 +629,7 @@ int qlm_paged_append(const float* qkv, int ldqkv, const float* q_norm, const flo
  * = ld_table * page_size, 16-byte aligned, no initial contents needed; calls
  * sharing it must be ordered on one stream. The size may fall as rows grow:
  * one workspace for calls of several sizes is as large as the largest of them
- * asks for. 0 for sizes that are refused. */
+ * asks for. 0: none is needed (work may be NULL), or sizes that are refused. */
 size_t qlm_paged_attention_workspace_bytes(int rows, int B, int n_q, int n_kv, int hd,
                                            long long slots);
 int qlm_paged_attention(const float* q, int ldq, const qlm_row_batch* batch,

@@ -1186,7 +1186,7 @@ PaPlan plan_of(int rows, int B, int G, int n_kv, int hd, long long slots) {
     // about the rows of a sequence
     const long long per = ((long long)rows * G + B - 1) / B;
     p.mt = per <= 8 ? 8 : per <= 16 ? 16 : per <= 64 || hd == 256 ? 64 : 128;
-        const int wanted = p.mt <= 16 ? 512 : 256;  // a CU holds one workgroup of either
+    const int wanted = p.mt <= 16 ? 512 : 256;  // a CU holds one workgroup of either
     p.target = std::max(1, wanted / n_kv);
     const long long units = ((long long)rows * G) / p.mt + B;
     p.items = (int)(units + p.target + 8);  // (8: what fp32 sums may be off by)

@@ -152,7 +152,7 @@ def test_deltanet_tree_commit_refusals(kw, rc):
 
 
 @pytest.mark.parametrize("rows,B,n_q,n_kv,hd,slots", [
-    (1, 1, 16, 4, 128, 1024), (512, 8, 16, 4, 128, 4096), (2048, 1, 16, 2, 256, 32768),
+    (1, 1, 16, 4, 128, 1040), (512, 8, 16, 4, 128, 4096), (2048, 1, 16, 2, 256, 32768),
     (64, 64, 8, 8, 128, 8192)])
 def test_attention_workspace(rows, B, n_q, n_kv, hd, slots):
     L = hip.lib()
@@ -166,6 +166,11 @@ def test_attention_workspace(rows, B, n_q, n_kv, hd, slots):
                 (rows, B, n_q + 1, n_kv, hd, slots), (rows, B, n_q, n_kv, 64, slots),
                 (rows, B, n_q, n_kv, hd, 0), (rows, B, 16 * n_kv, n_kv, hd, slots)]:
         assert L.qlm_paged_attention_workspace_bytes(*bad) == 0
+
+
+def test_attention_without_a_workspace():
+    """Few rows and few slots: nothing is cut, nothing joined."""
+    assert hip.lib().qlm_paged_attention_workspace_bytes(4, 4, 16, 4, 128, 1024) == 0
 
 
 def test_deltanet_tree_workspace():
