@@ -669,8 +669,8 @@ int qlm_deltanet_tree(const float* proj, int ldp, const qlm_row_batch* batch,
 
 /* The states' and rings' advance along the accepted rows, given as
  * qlm_tree_commit leaves them: sequence b's first accepted[b] entries of path
- * (at most QLM_TREE_MAX; it ends at an entry that is no row of the sequence). proj is
- * the verification's; batch->parent is not read. state and conv_state are left
+ * (at most QLM_TREE_MAX; it ends at an entry that is no row of the sequence behind
+ * the one before). proj is the verification's; batch->parent is not read. state and conv_state are left
  * as a decode step at position ctx_len + accepted expects them. */
 int qlm_deltanet_tree_commit(const float* proj, int ldp, const qlm_row_batch* batch,
                              const int* path, int ld_path, const int* accepted,

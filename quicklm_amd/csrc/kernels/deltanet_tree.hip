@@ -45,18 +45,36 @@ struct TreeArgs {
 template <int TM, int NC>
 struct TreeShared {
     static constexpr int QS = kD + 4, TS = TM + 4, WS = 16 * NC + 4;  // row strides
-    float q[TM][QS];   // conv inputs, then outputs after SiLU (not normalised)
-    float k[TM][QS];
-    float w[TM][WS];   // v, then R, then W
-    float at[TM][TS];  // A transposed: at[s][t]
-    float m[TM][TS];   // (g_t / g_s) (q_t . k_s) / sqrt(d), s on t's line
-    double c[TM];      // log g
+    // conv inputs, behind the nodes' the ring's three; then outputs after SiLU
+    // (not normalised)
+    float q[TM + 3][QS];
+    float k[TM + 3][QS];
+    float w[TM + 3][WS];  // the same of v, then R, then W
+    float at[TM][TS];     // A transposed: at[s][t]
+    float m[TM][TS];      // (g_t / g_s) (q_t . k_s) / sqrt(d), s on t's line (tiles up to t's)
+    double c[TM];         // log g
     unsigned long long line[TM];
-    int tap[TM][4];    // where a node's conv inputs lie, oldest first: a node, or -1 - ring row
+    int tap[TM][4];       // rows of q, k, w that a node's conv reads, oldest first
     float beta[TM], sq[TM], sk[TM];  // b; 1 / |q| and 1 / |k|
-    int row[TM];       // proj rows
-    int bad;           // a node whose outputs did not come out finite
+    int row[TM];          // proj rows
+    int bad;              // >= 0: outputs that did not come out finite
 };
+
+// x / (1 + exp(-x)) to four roundings: v_exp_f32 of the product with log2 e, whose
+// own rounding error is put back, v_rcp_f32 and a Newton step, instead of expf
+// and a division (half the conv's instructions). Below -80 the exponential
+// stays at exp(80): what is left is less than 1e-32.
+__device__ __forceinline__ float silu_fast(float x) {
+    constexpr float kLog2e = 1.44269502e0f, kLn2 = 0.693147182f;
+    const float c = fmaxf(x, -80.0f), hi = c * -kLog2e;
+    const float lo = fmaf(c, -1.92596303e-8f, fmaf(c, -kLog2e, -hi));
+    float e = __builtin_amdgcn_exp2f(hi);
+    e = fmaf(e * kLn2, lo, e);
+    const float d = 1.0f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    return x * r;
+}
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -115,6 +133,17 @@ __device__ __forceinline__ void solve_from(const float (&at)[TM][TM + 4],
     }
 }
 
+// A sequence's accepted path: its length, and in lane i its row i. It ends
+// where it does not rise to another row of the sequence.
+__device__ __forceinline__ int path_of(const TreeArgs& a, int b, const SeqRows& sq, int& p) {
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    const int want = min(max(a.accepted[b], 0), min(a.ld_path, QLM_TREE_MAX));
+    p = lane < want ? a.path[(size_t)b * a.ld_path + lane] : -1;
+    const int last = __shfl_up(p, 1);
+    const unsigned long long ends = __ballot(p < 0 || p >= sq.n || (lane > 0 && p <= last));
+    return ends ? __ffsll((long long)ends) - 1 : QLM_WAVE;
+}
+
 // Decay's logarithm and b of a row.
 __device__ __forceinline__ void gates(const TreeArgs& a, int row, int h, double& alpha,
                                       float& beta) {
@@ -129,7 +158,7 @@ __device__ __forceinline__ void gates(const TreeArgs& a, int row, int h, double&
 template <int TM, int NC, bool COMMIT>
 __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
     using SH = TreeShared<TM, NC>;
-    constexpr int CW = 16 * NC, SPLIT = kD / CW, RT = TM / 16, P = kNW / RT;
+    constexpr int CW = 16 * NC, SPLIT = kD / CW, RT = TM / 16;
     constexpr float kScale = 0.08838834764831845f;  // 1 / sqrt(d)
     __shared__ __align__(16) SH sh;
     const int h = blockIdx.x / SPLIT, c0 = blockIdx.x % SPLIT * CW, b = blockIdx.y;
@@ -141,10 +170,8 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
     // ---- the nodes: rows, lines, decays (a lane a node, every wave alike) ----
     int T, row = sq.first, parent;
     if constexpr (COMMIT) {
-        const int want = min(max(a.accepted[b], 0), min(a.ld_path, QLM_TREE_MAX));
-        const int p = lane < want ? a.path[(size_t)b * a.ld_path + lane] : -1;
-        const unsigned long long ends = __ballot(p < 0 || p >= sq.n);
-        T = ends ? __ffsll((long long)ends) - 1 : QLM_WAVE;
+        int p;
+        T = path_of(a, b, sq, p);
         row += lane < T ? p : 0;
         parent = lane < T ? lane - 1 : -2;
     } else {
@@ -152,25 +179,62 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         row += lane < T ? lane : 0;
         parent = tree_parent(a.bt, sq, lane);
     }
-    T = min(T, TM);
+    T = __builtin_amdgcn_readfirstlane(min(T, TM));
     if (T == 0) return;
+    // ---- conv inputs: a channel of q or k a thread, all nodes ----
+    const int ch = (tid >> 7) * HD + h * kD + (tid & 127);
+    const float* cs = a.conv + (size_t)b * 3 * C;
+    float* const col = tid < kD ? &sh.q[0][tid] : &sh.k[0][tid - kD];
+    float w4[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w4[j] = a.wt[(size_t)j * C + ch];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) col[(TM + j) * SH::QS] = cs[(size_t)j * C + ch];
+    // v: a column a thread, nodes VG apart
+    constexpr int VG = kThreads / CW, VN = TM / VG;
+    const int vc = tid % CW, vg = tid / CW, vch = 2 * HD + h * kD + c0 + vc;
+    float vw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vw[j] = a.wt[(size_t)j * C + vch];
+    if (vg < 3) sh.w[TM + vg][vc] = cs[(size_t)vg * C + vch];
+    if (VG < 3 && vg == 0) sh.w[TM + 2][vc] = cs[(size_t)2 * C + vch];
+#pragma unroll 1
+    for (int i0 = 0; i0 < T; i0 += 16) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[i] = a.proj[(size_t)__builtin_amdgcn_readlane(row, i0 + i) * a.ldp + ch];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) col[(i0 + i) * SH::QS] = x[i];
+    }
+#pragma unroll
+    for (int j = 0; j < VN; ++j) {
+        const int i = vg + j * VG;
+        const int r = __shfl(row, i);  // (every lane active; past the last node the first row)
+        const float x = a.proj[(size_t)r * a.ldp + vch];
+        sh.w[i][vc] = i < T ? x : 0.0f;
+    }
+    for (int i = tid; i < TM * SH::TS; i += kThreads) (&sh.at[0][0])[i] = 0.0f;
     if (tid == 0) sh.bad = -1;
+    // a node's inputs: itself and three above; behind the root the ring
+    const unsigned long long line = tree_line(parent);
+    int up = line ? parent : -1;
+    int tap[4] = {0, 0, 0, lane};
+    {
+        int at = lane, old = 3;
+#pragma unroll
+        for (int j = 2; j >= 0; --j) {
+            const int p = __shfl(up, max(at, 0));
+            at = at >= 0 ? p : -1;
+            if (at < 0) --old;
+            tap[j] = at >= 0 ? at : TM + (sq.ctx % 3 + old) % 3;
+        }
+    }
     if (wave == 0) {
-        const unsigned long long line = tree_line(parent);
         double alpha = 0.0;
         float beta = 0.0f;
         if (line && lane < T) gates(a, row, h, alpha, beta);
         double c = alpha;
-        int up = line ? parent : -1;
-        // conv inputs: itself and three above; behind the root the ring
-        int tap[4] = {-1, -1, -1, lane}, at = lane, old = 3;
-        for (int j = 2; j >= 0; --j) {
-            const int from = at >= 0 ? at : lane;
-            const int p = __shfl(up, from);
-            at = at >= 0 ? p : -1;
-            if (at < 0) --old;
-            tap[j] = at >= 0 ? at : -1 - (sq.ctx % 3 + old) % 3;
-        }
         while (__ballot(up >= 0)) {
             const int from = up >= 0 ? up : lane;
             const double x = __shfl(c, from);
@@ -189,72 +253,47 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             for (int j = 0; j < 4; ++j) sh.tap[lane][j] = tap[j];
         }
     }
-    // ---- conv inputs of q and k: a channel a thread, all nodes ----
-    const int ch = (tid >> 7) * HD + h * kD + (tid & 127);
-    const float* cs = a.conv + (size_t)b * 3 * C;
-    float ring[3], w4[4];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) ring[j] = cs[(size_t)j * C + ch];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w4[j] = a.wt[(size_t)j * C + ch];
-    float* const col = tid < kD ? &sh.q[0][tid] : &sh.k[0][tid - kD];
-#pragma unroll 1
-    for (int i0 = 0; i0 < TM; i0 += 16) {
-        if (i0 >= T) break;
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            x[i] = a.proj[(size_t)__shfl(row, i0 + i) * a.ldp + ch];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) col[(i0 + i) * SH::QS] = x[i];
-    }
-    __syncthreads();
-    // v: nodes tid / CW, ... of column tid % CW
-    {
-        const int vc = tid % CW, vch = 2 * HD + h * kD + c0 + vc;
-        float vr[3], vw[4];
-#pragma unroll
-        for (int j = 0; j < 3; ++j) vr[j] = cs[(size_t)j * C + vch];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vw[j] = a.wt[(size_t)j * C + vch];
-#pragma unroll 4
-        for (int i = tid / CW; i < TM; i += kThreads / CW) {
-            float acc = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int t = sh.tap[i][j];
-                const float x = t >= 0 ? a.proj[(size_t)sh.row[t] * a.ldp + vch]
-                                       : t == -1 ? vr[0] : t == -2 ? vr[1] : vr[2];
-                acc = nc_add_mul(acc, x, vw[j]);
-            }
-            sh.w[i][vc] = i < T ? silu_f(acc) : 0.0f;
-        }
-    }
     // q and k in place, last nodes first: what a node reads is its own or
     // an earlier node's, and a batch reads before it writes
     {
         constexpr int NB = 8;
 #pragma unroll 1
         for (int i0 = (T - 1) / NB * NB; i0 >= 0; i0 -= NB) {
-            float y[NB];
+            float x[NB][4];
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x[i][j] = col[__builtin_amdgcn_readlane(tap[j], i0 + i) * SH::QS];
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 float acc = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int t = sh.tap[i0 + i][j];
-                    const float x = t >= 0 ? col[t * SH::QS]
-                                           : t == -1 ? ring[0] : t == -2 ? ring[1] : ring[2];
-                    acc = nc_add_mul(acc, x, w4[j]);
-                }
-                y[i] = silu_f(acc);
+                for (int j = 0; j < 4; ++j) acc = nc_add_mul(acc, x[i][j], w4[j]);
+                col[(i0 + i) * SH::QS] = i0 + i < T ? silu_fast(acc) : 0.0f;
             }
-#pragma unroll
-            for (int i = 0; i < NB; ++i) col[(i0 + i) * SH::QS] = i0 + i < T ? y[i] : 0.0f;
         }
-        for (int i = (T - 1) / NB * NB + NB; i < TM; ++i) col[i * SH::QS] = 0.0f;
+#pragma unroll 1
+        for (int i = (T + NB - 1) / NB * NB; i < TM; ++i) col[i * SH::QS] = 0.0f;
     }
     __syncthreads();
+    // v in place: every read before the first write
+    {
+        float y[VN];
+#pragma unroll
+        for (int j = 0; j < VN; ++j) {
+            const int i = vg + j * VG;
+            const int4 tp = *reinterpret_cast<const int4*>(sh.tap[i]);
+            float acc = nc_add_mul(0.0f, sh.w[tp.x][vc], vw[0]);
+            acc = nc_add_mul(acc, sh.w[tp.y][vc], vw[1]);
+            acc = nc_add_mul(acc, sh.w[tp.z][vc], vw[2]);
+            acc = nc_add_mul(acc, sh.w[tp.w][vc], vw[3]);
+            y[j] = i < T ? silu_fast(acc) : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < VN; ++j) sh.w[vg + j * VG][vc] = y[j];
+    }
     // ---- norms: four threads a node ----
     for (int i = tid / 4; i < TM; i += kThreads / 4) {
         float s0 = 0.0f, s1 = 0.0f;
@@ -276,13 +315,29 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             sh.sk[i] = 1.0f / sqrtf(s1 + 1e-6f);
         }
     }
+    // ---- who multiplies what with the state: WC waves over the column tiles, the
+    // others over the row tiles, or over keys and queries ----
+    constexpr int WC = NC < kNW ? NC : kNW, CPW = NC / WC, WR = kNW / WC;
+    constexpr int WT = WR < RT ? WR : RT, TPW = RT / WT;  // waves over row tiles, tiles of one
+    const int cw = wave % WC, tw = wave / WC % WT, role = wave / (WC * WT);
+    const bool do_k = WR <= RT || role == 0, do_q = !COMMIT && (WR <= RT || role == 1);
+    const float* S = a.state + ((size_t)b * a.H + h) * kD * kD + c0;
+    float sb[CPW][32];
+    if (do_k || do_q) {
+#pragma unroll
+        for (int c = 0; c < CPW; ++c)
+#pragma unroll
+            for (int s = 0; s < 32; ++s)
+                sb[c][s] = S[(size_t)(32 * qd + s) * kD + 16 * (cw + c * WC) + n];
+    }
     __syncthreads();
     // ---- products of keys and queries with keys: pairs of 16-node tiles in turn ----
     const int tiles = (T + 15) / 16;
-    for (int p = wave; p < RT * RT; p += kNW) {
-        const int ti = p / RT, si = p % RT;
-        f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
-        if (si <= ti && ti < tiles) {
+#pragma unroll 1
+    for (int p = wave; p < tiles * (tiles + 1) / 2; p += kNW) {
+        const int ti = p >= 6 ? 3 : p >= 3 ? 2 : p >= 1 ? 1 : 0, si = p - ti * (ti + 1) / 2;
+        f32x4 kk, qk = {0.0f, 0.0f, 0.0f, 0.0f};
+        {
             float ka[32], kb[32];
             load32(kb, &sh.k[16 * si + n][32 * qd]);
             load32(ka, &sh.k[16 * ti + n][32 * qd]);
@@ -304,39 +359,38 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             if constexpr (!COMMIT) sh.m[t][s] = on ? sh.sq[t] * kScale * d * qk[i] : 0.0f;
         }
     }
-    // ---- products with the state: wave (role, tile); R in place of v ----
-    const int ti = wave % RT, role = wave / RT;  // roles: P of them share a tile
-    const float* S = a.state + ((size_t)b * a.H + h) * kD * kD + c0;
-    f32x4 o[NC];
+    // ---- products with the state; R in place of v ----
+    f32x4 o[TPW][CPW];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const bool do_k = ti < tiles && (P == 1 || role == 0);
-    const bool do_q = !COMMIT && ti < tiles && (P == 1 || role == 1);
-    if (do_k || do_q) {
-        float ka[32], qa[32];
-        if (do_k) load32(ka, &sh.k[16 * ti + n][32 * qd]);
-        if (do_q) load32(qa, &sh.q[16 * ti + n][32 * qd]);
+    for (int k = 0; k < TPW; ++k) {
+        const int ti = tw + k * WT;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            float sb[32];
+        for (int c = 0; c < CPW; ++c) o[k][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (ti >= tiles) break;
+        float ka[32];
+        if (do_k) {
+            load32(ka, &sh.k[16 * ti + n][32 * qd]);
 #pragma unroll
-            for (int s = 0; s < 32; ++s) sb[s] = S[(size_t)(32 * qd + s) * kD + 16 * c + n];
-            if (do_k) {
-                const f32x4 ks = dot32(ka, sb);
+            for (int c = 0; c < CPW; ++c) {
+                const f32x4 ks = dot32(ka, sb[c]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int t = 16 * ti + 4 * qd + i;
-                    float* r = &sh.w[t][16 * c + n];
+                    float* r = &sh.w[t][16 * (cw + c * WC) + n];
                     const float g = expf((float)sh.c[t]) * sh.sk[t];
                     *r = sh.line[t] ? sh.beta[t] * (*r - g * ks[i]) : 0.0f;
                 }
             }
-            if (do_q) {
-                o[c] = dot32(qa, sb);
+        }
+        if (do_q) {
+            load32(ka, &sh.q[16 * ti + n][32 * qd]);
+#pragma unroll
+            for (int c = 0; c < CPW; ++c) {
+                o[k][c] = dot32(ka, sb[c]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int t = 16 * ti + 4 * qd + i;
-                    o[c][i] *= expf((float)sh.c[t]) * sh.sq[t] * kScale;
+                    o[k][c][i] *= expf((float)sh.c[t]) * sh.sq[t] * kScale;
                 }
             }
         }
@@ -390,18 +444,30 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
     if (do_q) {
         bool fine = true;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
+        for (int k = 0; k < TPW; ++k) {
+            const int ti = tw + k * WT;
+            if (ti >= tiles) break;
+#pragma unroll 1
+            for (int si = 0; si <= ti; ++si)
 #pragma unroll
-            for (int s = 0; s < TM / 4; ++s)
-                o[c] = mfma4(sh.m[16 * ti + n][4 * s + qd], sh.w[4 * s + qd][16 * c + n], o[c]);
+                for (int s = 0; s < 4; ++s) {
+                    const int at = 16 * si + 4 * s + qd;
+                    const float m = sh.m[16 * ti + n][at];
+#pragma unroll
+                    for (int c = 0; c < CPW; ++c)
+                        o[k][c] = mfma4(m, sh.w[at][16 * (cw + c * WC) + n], o[k][c]);
+                }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = 16 * ti + 4 * qd + i;
                 const bool live = sh.line[t] != 0;
-                if (live) fine &= fabsf(o[c][i]) < INFINITY;
-                if (t < T)
-                    a.raw[(size_t)sh.row[t] * HD + h * kD + c0 + 16 * c + n] =
-                        live ? o[c][i] : 0.0f;
+#pragma unroll
+                for (int c = 0; c < CPW; ++c) {
+                    if (live) fine &= fabsf(o[k][c][i]) < INFINITY;
+                    if (t < T)
+                        a.raw[(size_t)sh.row[t] * HD + h * kD + c0 + 16 * (cw + c * WC) + n] =
+                            live ? o[k][c][i] : 0.0f;
+                }
             }
         }
         if (!fine) sh.bad = 0;
@@ -444,11 +510,11 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                 float acc = 0.0f;
                 for (int e = 0; e < 4; ++e) {
                     const int tp = sh.tap[u][e];
-                    const float x = tp >= 0 ? a.proj[(size_t)sh.row[tp] * a.ldp + vch]
-                                            : cs[(size_t)(-1 - tp) * C + vch];
+                    const float x = tp < TM ? a.proj[(size_t)sh.row[tp] * a.ldp + vch]
+                                            : cs[(size_t)(tp - TM) * C + vch];
                     acc = nc_add_mul(acc, x, a.wt[(size_t)e * C + vch]);
                 }
-                const float w = sh.beta[u] * (silu_f(acc) - sum);
+                const float w = sh.beta[u] * (silu_fast(acc) - sum);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[e] = fmaf(sh.k[u][8 * i8 + e] * sh.sk[u], w, s[e]);
             }
@@ -495,12 +561,10 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree_norm(TreeArgs a) {
 // put where position ctx_len + accepted expects them. After k_dn_tree, whose
 // workgroups all read the old ring.
 __global__ __launch_bounds__(kThreads) void k_dn_tree_ring(TreeArgs a, float* conv) {
-    const int b = blockIdx.y, lane = threadIdx.x & 63, C = 3 * a.H * kD;
+    const int b = blockIdx.y, C = 3 * a.H * kD;
     const SeqRows sq = seq_rows(a.bt, b);
-    const int want = min(max(a.accepted[b], 0), min(a.ld_path, QLM_TREE_MAX));
-    const int p = lane < want ? a.path[(size_t)b * a.ld_path + lane] : -1;
-    const unsigned long long ends = __ballot(p < 0 || p >= sq.n);
-    const int T = ends ? __ffsll((long long)ends) - 1 : QLM_WAVE;
+    int p;
+    const int T = path_of(a, b, sq, p);
     if (T == 0) return;
     int row[3];
 #pragma unroll

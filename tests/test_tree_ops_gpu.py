@@ -515,10 +515,15 @@ def run_tree(hip, rows, inp, H, ldo=None):
     return out.to_numpy((rows.rows, ldo), np.float32)
 
 
-# What fp32 arithmetic may leave of the largest output, normwise: the framework's
-# bound for reassociated DeltaNet forms. A line of 64 nodes is at most 64 steps
-# of ~10 roundings whose effect the decays and the unit keys keep from growing:
-# 64 * 10 * 2^-24 = 4e-5.
+# What fp32 arithmetic may leave of a head's largest output, normwise: the
+# framework's bound for reassociated DeltaNet forms. A line of 64 nodes is at
+# most 64 steps of ~10 roundings whose effect the decays and the unit keys keep
+# from growing: 64 * 10 * 2^-24 = 4e-5. But o = sum q_i S_ij is no better than
+# its terms: q has the conv's (8), SiLU's (4) and the norm's (12) roundings, S
+# as many of its own, the sum 16 more, so it is off by up to 64 2^-24 of sum |q_i|
+# |S_ij|, whatever is left of that sum. A strong decay leaves S about k w^T, so
+# that o is about (q . k) w, where q . k of a node may be 10^-3 of its terms' sum:
+# numpy's own fp32 then has 2e-5, with q . k = -3e-4.
 DN_TOL = 4e-5
 
 
@@ -536,11 +541,12 @@ def check_tree(rows, inp, H, out, skip=()):
                 continue
             if first + i in skip:
                 continue
-            o = done[i][1]
+            o, cond = done[i][1], done[i][3]
             z = inp["proj"][first + i, 3 * H * 128:4 * H * 128].reshape(H, 128).astype(np.float64)
             want = o / np.sqrt((o * o).mean(1, keepdims=True) + 1e-6) * inp["norm"]
-            want = (want * z / (1 + np.exp(-z))).ravel()
-            assert np.abs(x - want).max() <= DN_TOL * np.abs(want).max(), (b, i)
+            want = want * z / (1 + np.exp(-z))
+            tol = np.maximum(DN_TOL, 64 * U * cond) * np.abs(want).max(1)
+            assert (np.abs(x.reshape(H, 128) - want).max(1) <= tol).all(), (b, i)
     assert (out[~seen] == FILL).all() and (out[:, H * 128:] == FILL).all()
 
 
@@ -632,7 +638,7 @@ def test_deltanet_commit(hip, rng, H, B, n):
         done = deltanet_ref(rows, b, lines(parents[b], n), inp["proj"], inp["conv"][b],
                             inp["conv_w"], inp["A_log"], inp["dt"], inp["state"][b], H,
                             rows.start[b], ctx[b])
-        S, _, line = done[paths[b][-1]]
+        S, _, line, _ = done[paths[b][-1]]
         assert np.abs(state[b] - S).max() <= DN_TOL * np.abs(S).max()
         for j in range(3):
             assert np.array_equal(conv[b, (ctx[b] + len(paths[b]) + j) % 3], line[j])

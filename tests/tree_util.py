@@ -171,7 +171,8 @@ def rope_ref(x, pos, half, cos, sin):
 
 def deltanet_ref(rows, b, ls, proj, conv, conv_w, A_log, dt, state, H, first, ctx, d=128):
     """Every node of `ls` (lines) along its own line, one step at a time in 64
-    bits: yields (row, o before the head norm [H, d], state, line's inputs)."""
+    bits: {row: (state, o before the head norm [H, d], the last three inputs, the
+    heads' conditions: how much the terms of o's sums cancel)}."""
     C = 3 * H * d
     ring = [conv[(ctx + j) % 3].astype(np.float64) for j in range(3)]
     done = {}
@@ -193,5 +194,7 @@ def deltanet_ref(rows, b, ls, proj, conv, conv_w, A_log, dt, state, H, first, ct
         w = beta[:, None] * (v - np.einsum("hij,hi->hj", S, k))
         S = S + k[:, :, None] * w[:, None, :]
         o = np.einsum("hij,hi->hj", S, q) / np.sqrt(d)
-        done[i] = (S, o, xs[-3:])
+        # how much larger than a head's largest output the terms of one are
+        size = np.einsum("hij,hi->hj", np.abs(S), np.abs(q)).max(1) / np.sqrt(d)
+        done[i] = (S, o, xs[-3:], size / np.abs(o).max(1))
     return done
