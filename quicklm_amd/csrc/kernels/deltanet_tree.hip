@@ -23,7 +23,7 @@
 namespace {
 
 constexpr int kD = 128;
-constexpr int kThreads = 256, kNW = kThreads / QLM_WAVE;
+constexpr int kThreads = 512, kNW = kThreads / QLM_WAVE;  // two waves a SIMD: LDS holds one workgroup
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct TreeArgs {
@@ -155,6 +155,19 @@ __device__ __forceinline__ void gates(const TreeArgs& a, int row, int h, double&
     beta = sigmoid_f(g[h]);
 }
 
+// Head norm and SiLU(z) gate of a row's head, a wave: o0, o1 its elements lane
+// and lane + 64 (not normalised). A row outside the tree: 0.
+__device__ __forceinline__ void put_head(const TreeArgs& a, int row, int h, bool live, float o0,
+                                         float o1) {
+    const int lane = threadIdx.x & (QLM_WAVE - 1);
+    float* to = a.out + (size_t)row * a.ldo + h * kD + lane;
+    const float* z = a.proj + (size_t)row * a.ldp + 3 * (size_t)a.H * kD + h * kD + lane;
+    const float z0 = z[0], z1 = z[64];
+    const float sn = 1.0f / sqrtf(wave_sum(fmaf(o0, o0, o1 * o1)) / (float)kD + 1e-6f);
+    to[0] = live ? (o0 * sn) * a.norm_w[lane] * silu_f(z0) : 0.0f;
+    to[64] = live ? (o1 * sn) * a.norm_w[lane + 64] * silu_f(z1) : 0.0f;
+}
+
 template <int TM, int NC, bool COMMIT>
 __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
     using SH = TreeShared<TM, NC>;
@@ -181,38 +194,39 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
     }
     T = __builtin_amdgcn_readfirstlane(min(T, TM));
     if (T == 0) return;
-    // ---- conv inputs: a channel of q or k a thread, all nodes ----
-    const int ch = (tid >> 7) * HD + h * kD + (tid & 127);
+    // ---- conv inputs: a channel of q or k a thread, every other node ----
+    const int qk = tid & 255, hf = wave >> 2;
+    const int ch = (qk >> 7) * HD + h * kD + (qk & 127);
     const float* cs = a.conv + (size_t)b * 3 * C;
-    float* const col = tid < kD ? &sh.q[0][tid] : &sh.k[0][tid - kD];
+    float* const col = qk < kD ? &sh.q[0][qk] : &sh.k[0][qk - kD];
     float w4[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) w4[j] = a.wt[(size_t)j * C + ch];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) col[(TM + j) * SH::QS] = cs[(size_t)j * C + ch];
+    col[(TM + hf) * SH::QS] = cs[(size_t)hf * C + ch];
+    if (hf == 0) col[(TM + 2) * SH::QS] = cs[(size_t)2 * C + ch];
     // v: a column a thread, nodes VG apart
-    constexpr int VG = kThreads / CW, VN = TM / VG;
+    constexpr int VG = kThreads / CW, VN = TM > VG ? TM / VG : 1;
     const int vc = tid % CW, vg = tid / CW, vch = 2 * HD + h * kD + c0 + vc;
+    const bool v_on = TM >= VG || vg < TM;
     float vw[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) vw[j] = a.wt[(size_t)j * C + vch];
     if (vg < 3) sh.w[TM + vg][vc] = cs[(size_t)vg * C + vch];
-    if (VG < 3 && vg == 0) sh.w[TM + 2][vc] = cs[(size_t)2 * C + vch];
 #pragma unroll 1
     for (int i0 = 0; i0 < T; i0 += 16) {
-        float x[16];
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            x[i] = a.proj[(size_t)__builtin_amdgcn_readlane(row, i0 + i) * a.ldp + ch];
+        for (int i = 0; i < 8; ++i)
+            x[i] = a.proj[(size_t)__builtin_amdgcn_readlane(row, i0 + 2 * i + hf) * a.ldp + ch];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) col[(i0 + i) * SH::QS] = x[i];
+        for (int i = 0; i < 8; ++i) col[(i0 + 2 * i + hf) * SH::QS] = x[i];
     }
 #pragma unroll
     for (int j = 0; j < VN; ++j) {
         const int i = vg + j * VG;
-        const int r = __shfl(row, i);  // (every lane active; past the last node the first row)
+        const int r = __shfl(row, i & 63);  // (every lane active; past the last node the first row)
         const float x = a.proj[(size_t)r * a.ldp + vch];
-        sh.w[i][vc] = i < T ? x : 0.0f;
+        if (v_on) sh.w[i][vc] = i < T ? x : 0.0f;
     }
     for (int i = tid; i < TM * SH::TS; i += kThreads) (&sh.at[0][0])[i] = 0.0f;
     if (tid == 0) sh.bad = -1;
@@ -253,49 +267,53 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             for (int j = 0; j < 4; ++j) sh.tap[lane][j] = tap[j];
         }
     }
-    // q and k in place, last nodes first: what a node reads is its own or
-    // an earlier node's, and a batch reads before it writes
+    __syncthreads();
+    // q, k and v in place: every read before the first write
     {
-        constexpr int NB = 8;
-#pragma unroll 1
-        for (int i0 = (T - 1) / NB * NB; i0 >= 0; i0 -= NB) {
-            float x[NB][4];
+        float y[TM / 2], yv[VN];
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+        for (int i0 = 0; i0 < TM / 2; i0 += 8) {
+            if (2 * i0 < T) {
+                float x[8][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    x[i][j] = col[__builtin_amdgcn_readlane(tap[j], i0 + i) * SH::QS];
+                for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                float acc = 0.0f;
+                    for (int j = 0; j < 4; ++j)
+                        x[i][j] =
+                            col[__builtin_amdgcn_readlane(tap[j], 2 * (i0 + i) + hf) * SH::QS];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc = nc_add_mul(acc, x[i][j], w4[j]);
-                col[(i0 + i) * SH::QS] = i0 + i < T ? silu_fast(acc) : 0.0f;
+                for (int i = 0; i < 8; ++i) {
+                    float acc = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc = nc_add_mul(acc, x[i][j], w4[j]);
+                    y[i0 + i] = 2 * (i0 + i) + hf < T ? silu_fast(acc) : 0.0f;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i0 + i] = 0.0f;
             }
         }
-#pragma unroll 1
-        for (int i = (T + NB - 1) / NB * NB; i < TM; ++i) col[i * SH::QS] = 0.0f;
-    }
-    __syncthreads();
-    // v in place: every read before the first write
-    {
-        float y[VN];
 #pragma unroll
         for (int j = 0; j < VN; ++j) {
-            const int i = vg + j * VG;
+            const int i = min(vg + j * VG, TM - 1);
             const int4 tp = *reinterpret_cast<const int4*>(sh.tap[i]);
             float acc = nc_add_mul(0.0f, sh.w[tp.x][vc], vw[0]);
             acc = nc_add_mul(acc, sh.w[tp.y][vc], vw[1]);
             acc = nc_add_mul(acc, sh.w[tp.z][vc], vw[2]);
             acc = nc_add_mul(acc, sh.w[tp.w][vc], vw[3]);
-            y[j] = i < T ? silu_fast(acc) : 0.0f;
+            yv[j] = i < T ? silu_fast(acc) : 0.0f;
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < VN; ++j) sh.w[vg + j * VG][vc] = y[j];
+        for (int i = 0; i < TM / 2; ++i) col[(2 * i + hf) * SH::QS] = y[i];
+#pragma unroll
+        for (int j = 0; j < VN; ++j)
+            if (v_on) sh.w[vg + j * VG][vc] = yv[j];
     }
+    __syncthreads();
     // ---- norms: four threads a node ----
-    for (int i = tid / 4; i < TM; i += kThreads / 4) {
+    static_assert(kThreads / 4 >= QLM_TREE_MAX, "every node");
+    if (const int i = tid / 4; i < TM) {
         float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -396,23 +414,25 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         }
     }
     __syncthreads();
-    // ---- W by substitution: a wave a quarter of the columns ----
+    // ---- W by substitution: four columns a wave, or NC / 2 times four ----
     {
-        constexpr int RP = TM / 16;
-        float x[NC][RP];
+        constexpr int RP = TM / 16, NCW = NC * 4 > kNW ? NC * 4 / kNW : 1;
+        if (NC * 4 >= kNW || wave < NC * 4) {
+            float x[NCW][RP];
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NCW; ++c)
 #pragma unroll
-            for (int e = 0; e < RP; ++e) x[c][e] = sh.w[RP * n + e][4 * (NC * wave + c) + qd];
-        solve_from<TM, NC, 0>(sh.at, x, T);
-        const double end = sh.c[T - 1];
+                for (int e = 0; e < RP; ++e) x[c][e] = sh.w[RP * n + e][4 * (NCW * wave + c) + qd];
+            solve_from<TM, NCW, 0>(sh.at, x, T);
+            const double end = sh.c[T - 1];
 #pragma unroll
-        for (int e = 0; e < RP; ++e) {
-            float f = 1.0f;  // commit: what is left of a node at the path's end
-            const int t = RP * n + e;
-            if constexpr (COMMIT) f = t < T ? expf((float)(end - sh.c[t])) * sh.sk[t] : 0.0f;
+            for (int e = 0; e < RP; ++e) {
+                float f = 1.0f;  // commit: what is left of a node at the path's end
+                const int t = RP * n + e;
+                if constexpr (COMMIT) f = t < T ? expf((float)(end - sh.c[t])) * sh.sk[t] : 0.0f;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) sh.w[t][4 * (NC * wave + c) + qd] = f * x[c][e];
+                for (int c = 0; c < NCW; ++c) sh.w[t][4 * (NCW * wave + c) + qd] = f * x[c][e];
+            }
         }
     }
     __syncthreads();
@@ -464,7 +484,7 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
 #pragma unroll
                 for (int c = 0; c < CPW; ++c) {
                     if (live) fine &= fabsf(o[k][c][i]) < INFINITY;
-                    if (t < T)
+                    if (NC < 8 && t < T)
                         a.raw[(size_t)sh.row[t] * HD + h * kD + c0 + 16 * (cw + c * WC) + n] =
                             live ? o[k][c][i] : 0.0f;
                 }
@@ -473,13 +493,33 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         if (!fine) sh.bad = 0;
     }
     __syncthreads();
+    if constexpr (NC == 8) {
+        // the whole head is here: its norm and gate, a row a wave
+        if (sh.bad < 0) {
+#pragma unroll
+            for (int k = 0; k < TPW; ++k) {
+                if (tw + k * WT >= tiles) break;
+#pragma unroll
+                for (int c = 0; c < CPW; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sh.w[16 * (tw + k * WT) + 4 * qd + i][16 * (cw + c * WC) + n] = o[k][c][i];
+            }
+            __syncthreads();
+            for (int t = wave; t < T; t += kNW)
+                put_head(a, sh.row[t], h, sh.line[t] != 0, sh.w[t][lane], sh.w[t][lane + 64]);
+            for (int t = QLM_TREE_MAX + wave; t < sq.n; t += kNW)
+                put_head(a, sq.first + t, h, false, 0.0f, 0.0f);
+            return;
+        }
+    }
     if (sh.bad < 0) return;
     // ---- some output is not finite: every node again, along its own line ----
     // (a node's NaN has reached others through products with 0). Thread (i, j)
     // keeps rows 8 i .. + 7 of columns j, j + 16, ..; the sums over rows meet in
     // sh.m, which nothing reads any more.
     float* red = &sh.m[0][0];  // [16][16]
-    const int j = tid & 15, i8 = tid >> 4;
+    const int j = tid & 15, i8 = (tid >> 4) & 15;  // (the second 256 threads do the same again)
 #pragma unroll 1
     for (int t = 0; t < T; ++t) {
         const unsigned long long line = sh.line[t];
@@ -530,10 +570,21 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                 a.raw[(size_t)sh.row[t] * HD + h * kD + c0 + 16 * c + j] = sum * sh.sq[t] * kScale;
         }
     }
+    if constexpr (NC == 8) {
+        __threadfence_block();
+        __syncthreads();
+        for (int t = wave; t < T; t += kNW) {
+            const float* r = a.raw + (size_t)sh.row[t] * HD + h * kD + lane;
+            put_head(a, sh.row[t], h, sh.line[t] != 0, r[0], r[64]);
+        }
+        for (int t = QLM_TREE_MAX + wave; t < sq.n; t += kNW)
+            put_head(a, sq.first + t, h, false, 0.0f, 0.0f);
+    }
 }
 
-// Head norm and SiLU(z) gate, a head a wave; rows outside the tree are 0.
-__global__ __launch_bounds__(kThreads) void k_dn_tree_norm(TreeArgs a) {
+// Head norm and gate where a head's columns are several workgroups'.
+constexpr int kNormThreads = 256, kNormWaves = kNormThreads / QLM_WAVE;
+__global__ __launch_bounds__(kNormThreads) void k_dn_tree_norm(TreeArgs a) {
     const int row = blockIdx.x, lane = threadIdx.x & 63, b = seq_of_row(a.bt, row);
     if (b < 0) return;
     const SeqRows sq = seq_rows(a.bt, b);
@@ -541,19 +592,10 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree_norm(TreeArgs a) {
     if (i < 0 || i >= sq.n) return;
     const unsigned long long mine = tree_line(tree_parent(a.bt, sq, lane));
     const bool live = __ballot(mine != 0) >> min(i, QLM_TREE_MAX - 1) & 1ull && i < QLM_TREE_MAX;
-    for (int h = blockIdx.y * kNW + threadIdx.x / QLM_WAVE; h < a.H; h += gridDim.y * kNW) {
-        float* to = a.out + (size_t)row * a.ldo + h * kD + lane;
-        if (!live) {
-            to[0] = 0.0f;
-            to[64] = 0.0f;
-            continue;
-        }
+    for (int h = blockIdx.y * kNormWaves + threadIdx.x / QLM_WAVE; h < a.H;
+         h += gridDim.y * kNormWaves) {
         const float* o = a.raw + (size_t)row * HD + h * kD + lane;
-        const float* z = a.proj + (size_t)row * a.ldp + 3 * (size_t)HD + h * kD + lane;
-        const float o0 = o[0], o1 = o[64], z0 = z[0], z1 = z[64];
-        const float sn = 1.0f / sqrtf(wave_sum(fmaf(o0, o0, o1 * o1)) / (float)kD + 1e-6f);
-        to[0] = (o0 * sn) * a.norm_w[lane] * silu_f(z0);
-        to[64] = (o1 * sn) * a.norm_w[lane + 64] * silu_f(z1);
+        put_head(a, row, h, live, live ? o[0] : 0.0f, live ? o[64] : 0.0f);
     }
 }
 
@@ -589,13 +631,19 @@ int launch_tree(const TreeArgs& a, hipStream_t st) {
     return qlm_launch_status();
 }
 
+// Column tiles of a workgroup: as many as leave every CU one.
+int columns_of(long long heads) {
+    return heads >= 128 ? 8 : heads >= 64 ? 4 : heads >= 32 ? 2 : 1;
+}
+
 template <int TM, bool COMMIT>
 int launch_columns(const TreeArgs& a, hipStream_t st) {
-    const long long heads = (long long)a.H * a.bt.B;
-    if (heads >= 128) return launch_tree<TM, 8, COMMIT>(a, st);
-    if (heads >= 64) return launch_tree<TM, 4, COMMIT>(a, st);
-    if (heads >= 32) return launch_tree<TM, 2, COMMIT>(a, st);
-    return launch_tree<TM, 1, COMMIT>(a, st);
+    switch (columns_of((long long)a.H * a.bt.B)) {
+        case 8: return launch_tree<TM, 8, COMMIT>(a, st);
+        case 4: return launch_tree<TM, 4, COMMIT>(a, st);
+        case 2: return launch_tree<TM, 2, COMMIT>(a, st);
+        default: return launch_tree<TM, 1, COMMIT>(a, st);
+    }
 }
 
 template <bool COMMIT>
@@ -636,9 +684,9 @@ extern "C" int qlm_deltanet_tree(const float* proj, int ldp, const qlm_row_batch
                      reinterpret_cast<float*>(work), out, nullptr, nullptr, ldp, ldo, H, 0, *batch};
     hipStream_t st = as_stream(stream);
     const int r = launch_nodes<false>(a, st);
-    if (r != QLM_OK) return r;
-    hipLaunchKernelGGL(k_dn_tree_norm, dim3(batch->rows, (H + kNW - 1) / kNW), dim3(kThreads), 0, st,
-                       a);
+    if (r != QLM_OK || columns_of((long long)H * batch->B) == 8) return r;
+    hipLaunchKernelGGL(k_dn_tree_norm, dim3(batch->rows, (H + kNormWaves - 1) / kNormWaves),
+                       dim3(kNormThreads), 0, st, a);
     return qlm_launch_status();
 }
 
