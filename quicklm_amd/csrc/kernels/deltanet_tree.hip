@@ -39,6 +39,7 @@ struct TreeArgs {
     const int *path, *accepted;  // commit: the rows to advance along
     long long ldp, ldo;
     int H, ld_path;
+    int above;  // a launch takes the sequences of more nodes than this
     qlm_row_batch bt;
 };
 
@@ -192,8 +193,8 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         row += lane < T ? lane : 0;
         parent = tree_parent(a.bt, sq, lane);
     }
-    T = __builtin_amdgcn_readfirstlane(min(T, TM));
-    if (T == 0) return;
+    T = __builtin_amdgcn_readfirstlane(T);
+    if (T <= a.above || T > TM) return;  // nothing to do, or another launch's
     // ---- conv inputs: a channel of q or k a thread, every other node ----
     const int qk = tid & 255, hf = wave >> 2;
     const int ch = (qk >> 7) * HD + h * kD + (qk & 127);
@@ -631,9 +632,12 @@ int launch_tree(const TreeArgs& a, hipStream_t st) {
     return qlm_launch_status();
 }
 
-// Column tiles of a workgroup: as many as leave every CU one.
+// Column tiles of a workgroup: the fewest that need no more workgroups than CUs,
+// since all of a head repeat its convolutions and its nodes' products (16 heads,
+// trees of 64, us with 1, 2, 4 and 8: 2 sequences 28, 29, 34, 45; 4 49, 31, 36, 46;
+// 8 93, 56, 39, 47; 16 181, 106, 72, 50).
 int columns_of(long long heads) {
-    return heads >= 128 ? 8 : heads >= 64 ? 4 : heads >= 32 ? 2 : 1;
+    return heads > 128 ? 8 : heads > 64 ? 4 : heads > 32 ? 2 : 1;
 }
 
 template <int TM, bool COMMIT>
@@ -646,10 +650,18 @@ int launch_columns(const TreeArgs& a, hipStream_t st) {
     }
 }
 
+// LDS for 64 nodes leaves a CU one workgroup, for 16 it has room for four. No
+// sequence has more nodes than the call has rows; where that does not bound
+// them and 16 are likely to do (the accepted path of a tree; short trees on
+// average), sequences of up to 16 have a launch of their own.
 template <bool COMMIT>
-int launch_nodes(const TreeArgs& a, hipStream_t st) {
-    // no sequence has more nodes than the call has rows
+int launch_nodes(TreeArgs a, hipStream_t st) {
     if (a.bt.rows <= 16) return launch_columns<16, COMMIT>(a, st);
+    if (COMMIT || a.bt.rows <= 20LL * a.bt.B) {
+        const int rc = launch_columns<16, COMMIT>(a, st);
+        if (rc != QLM_OK) return rc;
+        a.above = 16;
+    }
     if (a.bt.rows <= 32) return launch_columns<32, COMMIT>(a, st);
     return launch_columns<64, COMMIT>(a, st);
 }
@@ -681,7 +693,7 @@ extern "C" int qlm_deltanet_tree(const float* proj, int ldp, const qlm_row_batch
     if (work_bytes < qlm_deltanet_tree_workspace_bytes(batch->rows, H, d)) return QLM_ERR_ARG;
     if (ldo < H * d || ((uintptr_t)work & 15u)) return QLM_ERR_SHAPE;
     const TreeArgs a{proj,   conv_state, conv_w_t, A_log, dt_bias, norm_w, const_cast<float*>(state),
-                     reinterpret_cast<float*>(work), out, nullptr, nullptr, ldp, ldo, H, 0, *batch};
+                     reinterpret_cast<float*>(work), out, nullptr, nullptr, ldp, ldo, H, 0, 0, *batch};
     hipStream_t st = as_stream(stream);
     const int r = launch_nodes<false>(a, st);
     if (r != QLM_OK || columns_of((long long)H * batch->B) == 8) return r;
@@ -701,7 +713,7 @@ extern "C" int qlm_deltanet_tree_commit(const float* proj, int ldp, const qlm_ro
         ld_path <= 0)
         return QLM_ERR_ARG;
     const TreeArgs a{proj,  conv_state, conv_w_t, A_log,    dt_bias, nullptr, state, nullptr,
-                     nullptr, path,     accepted, ldp, 0, H, ld_path, *batch};
+                     nullptr, path,     accepted, ldp, 0, H, ld_path, 0, *batch};
     hipStream_t st = as_stream(stream);
     const int r = launch_nodes<true>(a, st);
     if (r != QLM_OK) return r;
