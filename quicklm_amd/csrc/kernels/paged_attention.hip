@@ -12,11 +12,14 @@
 //     probabilities are the B operand in the registers that computed them, and
 //     V^T comes out of row-major LDS through the transposing LDS read (4 keys
 //     of 16 columns a lane group).
-// fp32 operands are split into two bf16 terms, x = h + l to 2^-17 of x: queries
-// and probabilities take two products each, with an fp32 cache three (h h, h l,
-// l h; what is left out is below 2^-16). Up to 8 rows need one product
-// where others need two: rows 0..7 of the tile hold the h terms, rows 8..15 the
-// l terms, and the two halves are added.
+// With a bf16 cache queries and probabilities, fp32, are split into three bf16
+// terms, x = h + m + l (24 bits: exact), a product each, so that nothing is lost
+// but in the fp32 sums; two terms, two thirds of the products, left 5e-6 of the
+// result, five times what fp32 arithmetic does. Up to 8 rows take two products:
+// rows 0..7 of the tile hold the h terms and rows 8..15 the m terms, then the l
+// terms and zeros, and the halves are added. An fp32 cache takes the fp32 matrix
+// cores (16x16x4), a sixteenth of the rate but no split of every key and value:
+// single tokens and trees are bound by the cache's bytes all the same.
 //
 // Keys and values go straight from the pages to LDS. A 16-key group lies in one
 // page and is read through a buffer descriptor that ends where the group's
@@ -198,27 +201,25 @@ __device__ __forceinline__ Group group_at(const PaArgs& a, int b, int slot, int 
     return g;
 }
 
-// The layouts of a 16-key group in LDS. bf16: rows of HD, pieces swizzled.
-// fp32: rows as they are, split into two such planes afterwards.
+// A 16-key group in LDS: rows as they are in the page, 16-byte pieces swizzled.
 template <int HD, bool F32>
 struct Lay {
-    static constexpr int ROW = HD * 2;        // bytes of a plane's row
-    static constexpr int GRP = 16 * ROW;      // of a plane's group
-    static constexpr int RAW = F32 ? 2 * GRP : GRP;  // of a group as it is loaded
-    static constexpr int LOADS = RAW / 1024;  // a wave's loads of a group
+    static constexpr int ROW = HD * (F32 ? 4 : 2);  // bytes of a row
+    static constexpr int GRP = 16 * ROW;
+    static constexpr int LOADS = GRP / 1024;  // a wave's loads of a group
     // the lane's source offset of load j
     __device__ static __forceinline__ int src(int j) {
         const int lane = threadIdx.x & (QLM_WAVE - 1);
-        if constexpr (F32) return j * 1024 + lane * 16;
         constexpr int PPR = ROW / 16;  // pieces of a row
-        const int row = (j * QLM_WAVE + lane) / PPR, piece = lane % PPR;
+        const int row = (j * QLM_WAVE + lane) / PPR, piece = (j * QLM_WAVE + lane) % PPR;
         return row * ROW + ((piece ^ row) * 16);
     }
 };
 
-template <int HD, bool F32>
+// Loads J0 .. J0 + N - 1 of a group.
+template <int HD, bool F32, int N = Lay<HD, F32>::LOADS>
 __device__ __forceinline__ void fetch_group(const PaArgs& a, const void* pool, const Group& gr,
-                                            int g, int slot, char* to) {
+                                            int g, int slot, char* to, int j0 = 0) {
     using L = Lay<HD, F32>;
     constexpr int SIZE = F32 ? 4 : 2;
     const size_t at = (((size_t)gr.page * a.pg.n_kv + g) * a.pg.page_size +
@@ -226,7 +227,7 @@ __device__ __forceinline__ void fetch_group(const PaArgs& a, const void* pool, c
     const __amdgpu_buffer_rsrc_t r =
         make_rsrc(reinterpret_cast<const char*>(pool) + at, (unsigned)gr.valid * (HD * SIZE));
 #pragma unroll
-    for (int j = 0; j < L::LOADS; ++j) load_to_lds(r, to + j * 1024, L::src(j), 0);
+    for (int j = 0; j < N; ++j) load_to_lds(r, to + (j0 + j) * 1024, L::src(j0 + j), 0);
 }
 
 // LDS by its own 32-bit addresses
@@ -238,15 +239,10 @@ __device__ __forceinline__ T lds_read(uint32_t at) {
     return *(__attribute__((address_space(3))) const T*)(uintptr_t)at;
 }
 
-__device__ __forceinline__ unsigned pk_bf16(float x, float y) {
-    const f32x2 v = {x, y};
-    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
-}
-
-// Eight floats as two bf16 terms each. What the first term leaves is x - h,
-// exact: one product with -1 and its sum with x (v_dot2_f32_bf16) instead of
-// widening h and subtracting it.
-__device__ __forceinline__ void split8(const float (&x)[8], u32x4& h, u32x4& l) {
+// Eight floats as three bf16 terms each (24 bits: exact). What a term leaves is
+// x - h, exact: one product with -1 and its sum with x (v_dot2_f32_bf16) instead
+// of widening h and subtracting it.
+__device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&term)[3]) {
     // (-1, 0) and (0, -1); in registers, since the compiler writes the second as the
     // inline constant -1.0, which the instruction does not read as that pair
     unsigned c0 = 0x0000bf80u, c1 = 0xbf800000u;
@@ -254,30 +250,14 @@ __device__ __forceinline__ void split8(const float (&x)[8], u32x4& h, u32x4& l) 
     const bf16x2 first = __builtin_bit_cast(bf16x2, c0), second = __builtin_bit_cast(bf16x2, c1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const f32x2 v = {x[2 * i], x[2 * i + 1]};
-        const bf16x2 w = __builtin_convertvector(v, bf16x2);
-        h[i] = __builtin_bit_cast(unsigned, w);
-        l[i] = pk_bf16(__builtin_amdgcn_fdot2_f32_bf16(w, first, v.x, false),
-                       __builtin_amdgcn_fdot2_f32_bf16(w, second, v.y, false));
-    }
-}
-
-// A raw fp32 group into its two planes.
-template <int HD>
-__device__ __forceinline__ void split_group(const char* raw, char* hi, char* lo) {
-    constexpr int ROW = HD * 2, PPR = ROW / 16, N = 16 * PPR / QLM_WAVE;
-    const int lane = threadIdx.x & (QLM_WAVE - 1);
+        f32x2 v = {x[2 * i], x[2 * i + 1]};
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const int at = j * QLM_WAVE + lane, row = at / PPR, piece = at % PPR;
-        const f32x4 x0 = *reinterpret_cast<const f32x4*>(raw + at * 32);
-        const f32x4 x1 = *reinterpret_cast<const f32x4*>(raw + at * 32 + 16);
-        const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-        u32x4 h, l;
-        split8(x, h, l);
-        const int to = row * ROW + ((piece ^ row) * 16);
-        *reinterpret_cast<u32x4*>(hi + to) = h;
-        *reinterpret_cast<u32x4*>(lo + to) = l;
+        for (int k = 0; k < 3; ++k) {
+            const bf16x2 w = __builtin_convertvector(v, bf16x2);
+            term[k][i] = __builtin_bit_cast(unsigned, w);
+            v.x = __builtin_amdgcn_fdot2_f32_bf16(w, first, v.x, false);
+            v.y = __builtin_amdgcn_fdot2_f32_bf16(w, second, v.y, false);
+        }
     }
 }
 
@@ -288,6 +268,10 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
 // over the four lane groups of a column
 __device__ __forceinline__ float cols_max(float v) { return xor32_max(xor16_max(v)); }
 __device__ __forceinline__ float cols_sum(float v) { return xor32_add(xor16_add(v)); }
@@ -295,21 +279,29 @@ __device__ __forceinline__ float cols_sum(float v) { return xor32_add(xor16_add(
 // v(l) + v(l ^ 8) of each 16 lanes
 __device__ __forceinline__ float fold8(float v) { return v + dpp_mov<0x128>(v); }  // row_ror:8
 
-// RT tiles of 16 rows; PACK: one tile of 8 rows, h and l terms side by side.
+// Keys go through in parts of NH 16-key halves; a lane has XN scores of a row.
+template <bool F32>
+struct Part {
+    static constexpr int NH = F32 ? 1 : 2, XN = 4 * NH, KEYS = 16 * NH;
+};
+
+// RT tiles of 16 rows; PACK: one tile of 8 rows (bf16: h and m terms side by side,
+// then l terms and zeros).
 // A row's scores come out of the products relative to a reference `m` (the
-// accumulators begin at -m): the largest score of the row's first block, and of
+// accumulators begin at -m): the largest score of the row's first part, and of
 // a later one where a score passes it by more than kRise. So exponentials go
 // up to 2^kRise, sums over 2^30 keys stay in range, and what is lost below 2^-126
-// is less than that part of the row's largest; no block needs a maximum over
-// the lanes, and the sums are hardly ever scaled. A block that moves a reference
+// is less than that part of the row's largest; no part needs a maximum over
+// the lanes, and the sums are hardly ever scaled. A part that moves a reference
 // is begun again (the loops below): with the scaling inside of the loop's body
 // its registers were copied every time, a third of its vector instructions.
 constexpr float kRise = 60.0f;
 constexpr int kAnyScore = (int)0x80000000;
-template <int HD, int RT, bool PACK>
+template <int HD, int RT, bool PACK, bool F32>
 struct Rows {
-    static constexpr int KS = HD / 32, CB = HD / 16, QT = PACK ? 1 : 2;
-    u32x4 q[RT][QT][KS];
+    static constexpr int KS = HD / 32, CB = HD / 16, QT = PACK ? 2 : 3;
+    u32x4 q[F32 ? 1 : RT][F32 ? 1 : QT][F32 ? 1 : KS];
+    f32x4 qf[F32 ? RT : 1][F32 ? HD / 16 : 1];  // lane (qd, n): elements 16 s + 4 qd .. + 3
     f32x4 acc[RT][CB];
     f32x4 from[RT];       // four times -m
     float m[RT], l[RT];   // m -inf: no score yet
@@ -319,33 +311,34 @@ struct Rows {
 };
 
 // Query rows r0 + 16 t + n of the unit (r: its token and head): requested here.
-template <int HD, int RT, bool PACK>
+// (bf16: elements 32 s + 8 qd .. + 7; fp32: 16 s + 4 qd .. + 3.)
+template <int HD, int RT>
 struct Queries {
-    f32x4u x[RT][HD / 32][2];
+    f32x4u x[RT][HD / 16];
 };
-template <int HD, int RT, bool PACK>
+template <int HD, int RT, bool PACK, bool F32>
 __device__ __forceinline__ void request_rows(const PaArgs& a, const Item& it, int g, int r0,
-                                             Queries<HD, RT, PACK>& Q) {
+                                             Queries<HD, RT>& Q) {
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
     const int total = it.sq.n << a.lg;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int rc = min(r0 + 16 * t + (PACK ? n & 7 : n), total - 1);
         const float* qr = a.q + (size_t)(it.sq.first + (rc >> a.lg)) * a.ldq +
-                          ((size_t)(g << a.lg) + (rc & ((1 << a.lg) - 1))) * HD + 8 * qd;
+                          ((size_t)(g << a.lg) + (rc & ((1 << a.lg) - 1))) * HD;
 #pragma unroll
-        for (int s = 0; s < HD / 32; ++s) {
-            Q.x[t][s][0] = *reinterpret_cast<const f32x4u*>(qr + 32 * s);
-            Q.x[t][s][1] = *reinterpret_cast<const f32x4u*>(qr + 32 * s + 4);
+        for (int s = 0; s < HD / 16; ++s) {
+            const int e = F32 ? 16 * s + 4 * qd : 32 * (s / 2) + 8 * qd + 4 * (s % 2);
+            Q.x[t][s] = *reinterpret_cast<const f32x4u*>(qr + e);
         }
     }
 }
 
 // What the rows see, and their queries' terms.
-template <int HD, int RT, bool PACK>
+template <int HD, int RT, bool PACK, bool F32>
 __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r0,
-                                          const Queries<HD, RT, PACK>& Q, Rows<HD, RT, PACK>& R) {
-    using T = Rows<HD, RT, PACK>;
+                                          const Queries<HD, RT>& Q, Rows<HD, RT, PACK, F32>& R) {
+    using T = Rows<HD, RT, PACK, F32>;
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15;
     const int total = it.sq.n << a.lg;
     unsigned long long mine = 0;
@@ -366,18 +359,26 @@ __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r
             R.line[t] = tok < QLM_TREE_MAX ? ln : 0;
             R.lim[t] = R.line[t] ? it.sq.ctx : -1;
         }
+        if constexpr (F32) {
 #pragma unroll
-        for (int s = 0; s < T::KS; ++s) {
-            float v[8];
+            for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = Q.x[t][s][i / 4][i % 4] * a.qscale;
-            u32x4 hi, lo;
-            split8(v, hi, lo);
-            if constexpr (PACK) {
-                R.q[t][0][s] = n < 8 ? hi : lo;
-            } else {
-                R.q[t][0][s] = hi;
-                R.q[t][1][s] = lo;
+                for (int i = 0; i < 4; ++i) R.qf[t][s][i] = Q.x[t][s][i] * a.qscale;
+        } else {
+#pragma unroll
+            for (int s = 0; s < T::KS; ++s) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = Q.x[t][2 * s + i / 4][i % 4] * a.qscale;
+                u32x4 term[3];
+                split8(v, term);
+                if constexpr (PACK) {
+                    R.q[t][0][s] = n < 8 ? term[0] : term[1];
+                    R.q[t][1][s] = n < 8 ? term[2] : u32x4{0u, 0u, 0u, 0u};
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) R.q[t][k][s] = term[k];
+                }
             }
         }
 #pragma unroll
@@ -385,74 +386,68 @@ __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r
     }
 }
 
-// Scores of a block of 32 keys from slot k0 on, relative to the references, of
+// Scores of a part of the keys, from slot k0 on, relative to the references, of
 // keys that a row does not see -inf: x[t][4 h + i] of key 16 h + 4 qd + i. kp:
-// the block's K plane (of an fp32 cache the h plane, the l plane `lo` bytes
-// behind). `all`: every row sees every key of it.
+// its K groups in LDS. `all`: every row sees every key of it.
 template <int HD, int RT, bool PACK, bool F32>
-__device__ __forceinline__ void scores(const Rows<HD, RT, PACK>& R, const char* kp, int lo, int k0,
+__device__ __forceinline__ void scores(const Rows<HD, RT, PACK, F32>& R, const char* kp, int k0,
                                        int ctx, int valid0, int valid1, bool all,
-                                       float (&x)[RT][8]) {
-    using T = Rows<HD, RT, PACK>;
-    constexpr int ROW = HD * 2, GRP = 16 * ROW;
+                                       float (&x)[RT][Part<F32>::XN]) {
+    using T = Rows<HD, RT, PACK, F32>;
+    using L = Lay<HD, F32>;
+    constexpr int NH = Part<F32>::NH, XN = Part<F32>::XN;
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
-    f32x4 s[2][RT];
+    f32x4 s[NH][RT];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int t = 0; t < RT; ++t) s[h][t] = R.from[t];
-    constexpr int KC = T::KS < 4 ? T::KS : 4;  // k-steps read at once
     // piece (4 k + qd) ^ n of row n: the bits of k come in by an exclusive or
-    const uint32_t ka = lds_at(kp) + n * ROW + ((qd ^ n) * 16);
+    const uint32_t ka = lds_at(kp) + n * L::ROW + ((qd ^ n) * 16);
+    constexpr int KN = L::ROW / 64;         // pieces of a row a lane
+    constexpr int KC = KN < 4 ? KN : 4;     // read at once
 #pragma unroll
-    for (int k0s = 0; k0s < T::KS; k0s += KC) {
-        u32x4 kh[KC][2], kl[F32 ? KC : 1][2];
+    for (int k0s = 0; k0s < KN; k0s += KC) {
+        u32x4 kf[KC][NH];
 #pragma unroll
         for (int k = 0; k < KC; ++k)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t at = (ka ^ (64u * (k0s + k))) + h * GRP;
-                kh[k][h] = lds_read<u32x4>(at);
-                if constexpr (F32) kl[k][h] = lds_read<u32x4>(at + lo);
-            }
+            for (int h = 0; h < NH; ++h)
+                kf[k][h] = lds_read<u32x4>((ka ^ (64u * (k0s + k))) + h * L::GRP);
         __builtin_amdgcn_sched_barrier(0);
         // (a sum's terms apart from each other: each waits for the one before)
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
-            const int ks = k0s + k;
             if constexpr (F32) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int t = 0; t < RT; ++t)
-                        s[h][t] = mfma(kl[k][h], R.q[t][0][ks], s[h][t]);
+                        s[0][t] = mfma(__uint_as_float(kf[k][0][i]), R.qf[t][k0s + k][i], s[0][t]);
+            } else {
+#pragma unroll
+                for (int p = T::QT - 1; p >= 0; --p)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t)
+                            s[h][t] = mfma(kf[k][h], R.q[t][p][k0s + k], s[h][t]);
             }
-            if constexpr (!PACK) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int t = 0; t < RT; ++t)
-                        s[h][t] = mfma(kh[k][h], R.q[t][1][ks], s[h][t]);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int t = 0; t < RT; ++t) s[h][t] = mfma(kh[k][h], R.q[t][0][ks], s[h][t]);
         }
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < XN; ++j) {
             x[t][j] = s[j / 4][t][j % 4];
-            if constexpr (PACK) x[t][j] = fold8(x[t][j]);
+            if constexpr (PACK && !F32) x[t][j] = fold8(x[t][j]);
         }
     if (all) return;
-    asm volatile("");  // (a branch, not selections that every block would compute)
+    asm volatile("");  // (a branch, not selections that every part would compute)
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < XN; ++j) {
             const int in = 4 * qd + j % 4, slot = k0 + 16 * (j / 4) + in, row = slot - ctx;
             bool sees = slot < R.lim[t];
             if (row >= 0 && row < QLM_TREE_MAX) sees |= (R.line[t] >> row) & 1ull;
@@ -462,30 +457,32 @@ __device__ __forceinline__ void scores(const Rows<HD, RT, PACK>& R, const char* 
 }
 
 // Whether some score is too far above its row's reference.
-template <int HD, int RT, bool PACK>
-__device__ __forceinline__ bool too_high(const Rows<HD, RT, PACK>& R, const float (&x)[RT][8]) {
+template <int HD, int RT, bool PACK, bool F32>
+__device__ __forceinline__ bool too_high(const Rows<HD, RT, PACK, F32>& R,
+                                         const float (&x)[RT][Part<F32>::XN]) {
     bool high = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         // as integers, in whose order positive floats are: no canonical forms
         int top = __float_as_int(x[t][0]);
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = max(top, __float_as_int(x[t][j]));
+        for (int j = 1; j < Part<F32>::XN; ++j) top = max(top, __float_as_int(x[t][j]));
         high |= top > R.high[t];
     }
     return __ballot(high) != 0;
 }
 
-// Moves the references to the block's largest scores where those are higher.
-template <int HD, int RT, bool PACK>
-__device__ __forceinline__ void raise(Rows<HD, RT, PACK>& R, const float (&x)[RT][8]) {
-    using T = Rows<HD, RT, PACK>;
+// Moves the references to the part's largest scores where those are higher.
+template <int HD, int RT, bool PACK, bool F32>
+__device__ __forceinline__ void raise(Rows<HD, RT, PACK, F32>& R,
+                                      const float (&x)[RT][Part<F32>::XN]) {
+    using T = Rows<HD, RT, PACK, F32>;
     const int n = threadIdx.x & 15;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         float top = x[t][0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[t][j]);
+        for (int j = 1; j < Part<F32>::XN; ++j) top = fmaxf(top, x[t][j]);
         top = cols_max(top);
         const bool first = R.m[t] == -INFINITY;
         const bool moves = top > (first ? -INFINITY : 0.0f);
@@ -498,66 +495,102 @@ __device__ __forceinline__ void raise(Rows<HD, RT, PACK>& R, const float (&x)[RT
 #pragma unroll
             for (int i = 0; i < 4; ++i) R.acc[t][c][i] *= f;
         // (a packed tile's two halves are added: one of them begins at 0)
-        const float from = moves && !(PACK && n >= 8) ? -R.m[t] : R.from[t][0];
+        const float from = moves && !(PACK && !F32 && n >= 8) ? -R.m[t] : R.from[t][0];
         R.from[t] = f32x4{from, from, from, from};
-        // a row that has seen nothing in the block waits for its first score
+        // a row that has seen nothing in the part waits for its first score
         R.high[t] = R.m[t] == -INFINITY ? kAnyScore : __float_as_int(kRise);
     }
 }
 
-// The block's probabilities into the rows' sums; vp: its V plane.
+// The part's probabilities into the rows' sums; vp: its V groups in LDS.
 template <int HD, int RT, bool PACK, bool F32>
-__device__ __forceinline__ void accumulate(Rows<HD, RT, PACK>& R, float (&x)[RT][8], const char* vp,
-                                           int lo) {
-    using T = Rows<HD, RT, PACK>;
-    constexpr int ROW = HD * 2, GRP = 16 * ROW;
+__device__ __forceinline__ void accumulate(Rows<HD, RT, PACK, F32>& R,
+                                           float (&x)[RT][Part<F32>::XN], const char* vp) {
+    using T = Rows<HD, RT, PACK, F32>;
+    using L = Lay<HD, F32>;
+    constexpr int XN = Part<F32>::XN;
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
-    // V^T: lane l of a group reads 4 columns of key 4 qd + (l % 16) / 4
-    const int key = 4 * qd + (n >> 2);
-    const uint32_t va = lds_at(vp) + key * ROW + ((((n >> 1) & 1) ^ key) * 16) + (n & 1) * 8;
-    auto tr = [&](uint32_t at) {
-        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                             (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
+    auto exponentials = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < XN; ++j) x[t][j] = __builtin_amdgcn_exp2f(x[t][j]);
+        float sum = (x[t][0] + x[t][1]) + (x[t][2] + x[t][3]);
+        if constexpr (XN == 8) sum += (x[t][4] + x[t][5]) + (x[t][6] + x[t][7]);
+        R.l[t] += sum;
     };
-    auto read_v = [&](int c, int plane) {  // piece (2 c + ..) ^ key of row `key`
-        const uint32_t at = (va ^ (32u * c)) + plane;
-        const u32x2 v0 = tr(at), v1 = tr(at + GRP);
-        return u32x4{v0.x, v0.y, v1.x, v1.y};
-    };
-    constexpr int VC = 4;  // column blocks read at once, the first before the exponentials
-    u32x4 vh[VC], vl[F32 ? VC : 1];
-    auto read_some = [&](int c0) {
+    if constexpr (F32) {
+        // step i: keys 4 qd + i; lane (qd, n) reads element 16 c + n of its key, in
+        // piece (4 c + n / 4) ^ key: 64 banks once
+        uint32_t va[4];
 #pragma unroll
-        for (int c = 0; c < VC; ++c) {
-            vh[c] = read_v(c0 + c, 0);
-            if constexpr (F32) vl[c] = read_v(c0 + c, lo);
-        }
-    };
-    read_some(0);
-    __builtin_amdgcn_sched_barrier(0);
-    u32x4 ph[RT], pl[RT];
+        for (int i = 0; i < 4; ++i)
+            va[i] = lds_at(vp) + (4 * qd + i) * L::ROW + (((n >> 2) ^ (4 * qd + i)) * 16) +
+                    (n & 3) * 4;
+        constexpr int VC = 8;
+        float v[4][VC];
+        auto read_some = [&](int c0) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[t][j] = __builtin_amdgcn_exp2f(x[t][j]);
-        R.l[t] += ((x[t][0] + x[t][1]) + (x[t][2] + x[t][3])) +
-                  ((x[t][4] + x[t][5]) + (x[t][6] + x[t][7]));
-        split8(x[t], ph[t], pl[t]);
-        if constexpr (PACK) ph[t] = n < 8 ? ph[t] : pl[t];
-    }
-#pragma unroll
-    for (int c0 = 0; c0 < T::CB; c0 += VC) {
-        if (c0) read_some(c0);
-        auto add = [&](const u32x4* v, const u32x4* p) {
-#pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    R.acc[t][c0 + c] = mfma(v[c], p[t], R.acc[t][c0 + c]);
+                for (int c = 0; c < VC; ++c) v[i][c] = lds_read<float>(va[i] ^ (64u * (c0 + c)));
         };
-        if constexpr (F32) add(vl, ph);
-        if constexpr (!PACK) add(vh, pl);
-        add(vh, ph);
+        read_some(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) exponentials(t);
+#pragma unroll
+        for (int c0 = 0; c0 < T::CB; c0 += VC) {
+            if (c0) read_some(c0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+                        R.acc[t][c0 + c] = mfma(v[i][c], x[t][i], R.acc[t][c0 + c]);
+        }
+    } else {
+        // V^T: lane l of a group reads 4 columns of key 4 qd + (l % 16) / 4
+        const int key = 4 * qd + (n >> 2);
+        const uint32_t va =
+            lds_at(vp) + key * L::ROW + ((((n >> 1) & 1) ^ key) * 16) + (n & 1) * 8;
+        auto tr = [&](uint32_t at) {
+            return __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
+        };
+        constexpr int VC = 4;  // column blocks read at once, the first before the exponentials
+        u32x4 v[VC];
+        auto read_some = [&](int c0) {  // piece (2 c + ..) ^ key of row `key`
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                const uint32_t at = va ^ (32u * (c0 + c));
+                const u32x2 v0 = tr(at), v1 = tr(at + L::GRP);
+                v[c] = u32x4{v0.x, v0.y, v1.x, v1.y};
+            }
+        };
+        read_some(0);
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 p[RT][3];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            exponentials(t);
+            split8(x[t], p[t]);
+            if constexpr (PACK) {
+                p[t][0] = n < 8 ? p[t][0] : p[t][1];
+                p[t][1] = n < 8 ? p[t][2] : u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+#pragma unroll
+        for (int c0 = 0; c0 < T::CB; c0 += VC) {
+            if (c0) read_some(c0);
+#pragma unroll
+            for (int k = T::QT - 1; k >= 0; --k)
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+                        R.acc[t][c0 + c] = mfma(v[c], p[t][k], R.acc[t][c0 + c]);
+        }
     }
 }
 
@@ -756,8 +789,8 @@ __device__ __forceinline__ void put_desc(const PaArgs& a, const Item& it, int g,
 // its own, and meet at the end: nothing waits for another wave's loads.
 template <int HD, bool F32>
 struct FewShape {
-    static constexpr int BLK = 2 * 2 * Lay<HD, F32>::RAW;  // a block's bytes: K, V, two groups
-    static constexpr int NW = 128 * 1024 / (2 * BLK);      // 128 KB of LDS: two blocks a wave
+    static constexpr int BLK = 2 * Part<F32>::NH * Lay<HD, F32>::GRP;  // a part's K and V
+    static constexpr int NW = 128 * 1024 / (2 * BLK);  // 128 KB of LDS: two parts a wave
 };
 
 template <int HD, bool F32, bool PACK>
@@ -765,8 +798,9 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     using L = Lay<HD, F32>;
     using S = FewShape<HD, F32>;
     using KV = typename std::conditional<F32, float, uint16_t>::type;
-    constexpr int MT = PACK ? 8 : 16, NW = S::NW, GRP = L::GRP, RAW = L::RAW;
-    constexpr int LOADS = 4 * L::LOADS;  // a block's
+    using P = Part<F32>;
+    constexpr int MT = PACK ? 8 : 16, NW = S::NW, NH = P::NH, GRP = L::GRP;
+    constexpr int LOADS = 2 * NH * L::LOADS;  // a block's
     constexpr int OST = HD + 4;
     static_assert(NW * 16 * OST * 4 + NW * 16 * 8 <= NW * 2 * S::BLK, "the join fits the rings");
     __shared__ __attribute__((aligned(1024))) char smem[NW * 2 * S::BLK];
@@ -783,73 +817,61 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     if (it.chunk >= nch) return;
     const int b = uni(it.b), k0 = uni(it.chunk * it.len), k1 = uni(min(k0 + it.len, end));
     const int lgp = uni(31 - __clz(a.pg.page_size));
-    const int blocks = uni((k1 - k0 + 31) / 32), mine = uni((blocks - wave + NW - 1) / NW);
+    const int blocks = uni((k1 - k0 + P::KEYS - 1) / P::KEYS);
+    const int mine = uni((blocks - wave + NW - 1) / NW);
     char* ring = smem + wave * 2 * S::BLK;
-    auto slot_of = [&](int j) { return k0 + 32 * (wave + j * NW); };
-    auto groups = [&](int j, Group (&gr)[2]) {
-        gr[0] = group_at(a, b, slot_of(j), k1, lgp);
-        gr[1] = group_at(a, b, slot_of(j) + 16, k1, lgp);
+    auto slot_of = [&](int j) { return k0 + P::KEYS * (wave + j * NW); };
+    auto groups = [&](int j, Group (&gr)[NH]) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) gr[h] = group_at(a, b, slot_of(j) + 16 * h, k1, lgp);
     };
     // a block in LDS: K groups, V groups
-    auto fetch = [&](int j, const Group (&gr)[2]) {
-        char* to = ring + (F32 ? 0 : j & 1) * S::BLK;
+    auto fetch = [&](int j, const Group (&gr)[NH]) {
+        char* to = ring + (j & 1) * S::BLK;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            fetch_group<HD, F32>(a, a.pg.k, gr[h], g, slot_of(j) + 16 * h, to + h * RAW);
-            fetch_group<HD, F32>(a, a.pg.v, gr[h], g, slot_of(j) + 16 * h, to + (2 + h) * RAW);
+        for (int h = 0; h < NH; ++h) {
+            fetch_group<HD, F32>(a, a.pg.k, gr[h], g, slot_of(j) + 16 * h, to + h * GRP);
+            fetch_group<HD, F32>(a, a.pg.v, gr[h], g, slot_of(j) + 16 * h, to + (NH + h) * GRP);
         }
     };
-    constexpr int D = F32 ? 1 : 2;  // blocks in flight
-    Group gr[3][2];                 // of blocks j, j + 1 and j + 2
+    Group gr[3][NH];  // of blocks j, j + 1 and j + 2
 #pragma unroll
     for (int j = 0; j < 3; ++j) groups(j, gr[j]);
     // queries first: what is waited for first
-    Queries<HD, 1, PACK> Q;
-    request_rows<HD, 1, PACK>(a, it, g, r0, Q);
+    Queries<HD, 1> Q;
+    request_rows<HD, 1, PACK, F32>(a, it, g, r0, Q);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < D; ++j)
-        if (j < mine) fetch(j, gr[j]);
+    if (mine > 0) fetch(0, gr[0]);
+    if (mine > 1) fetch(1, gr[1]);
     __builtin_amdgcn_sched_barrier(0);
-    Rows<HD, 1, PACK> R;
-    take_rows<HD, 1, PACK>(a, it, r0, Q, R);
+    Rows<HD, 1, PACK, F32> R;
+    take_rows<HD, 1, PACK, F32>(a, it, r0, Q, R);
     int staged = -1, raised = -1;  // the block that is there, and the last one begun again
-    float x[1][8];
+    float x[1][P::XN];
     for (int j = 0;;) {
         bool move = false;
 #pragma unroll 1
         for (; j < mine; ++j) {
             const int s0 = slot_of(j);
-            char* at = ring + (F32 ? 0 : j & 1) * S::BLK;
-            // planes: K h, K l, V h, V l
-            char* const pl = F32 ? ring + S::BLK : at;
+            const char* at = ring + (j & 1) * S::BLK;
             if (staged != j) {
                 staged = j;
-                if (!F32 && j + 1 < mine)
+                if (j + 1 < mine)
                     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
                 else
                     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                if constexpr (F32) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        split_group<HD>(at + h * RAW, pl + h * GRP, pl + (2 + h) * GRP);
-                        split_group<HD>(at + (2 + h) * RAW, pl + (4 + h) * GRP, pl + (6 + h) * GRP);
-                    }
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    if (j + 1 < mine) fetch(j + 1, gr[1]);
-                }
             }
-            const bool all = s0 + 32 <= it.sq.ctx && gr[0][0].valid == 16 && gr[0][1].valid == 16;
-            scores<HD, 1, PACK, F32>(R, pl, 2 * GRP, s0, it.sq.ctx, gr[0][0].valid, gr[0][1].valid,
-                                     all, x);
+            const int va = gr[0][0].valid, vb = gr[0][NH - 1].valid;
+            const bool all = s0 + P::KEYS <= it.sq.ctx && va == 16 && vb == 16;
+            scores<HD, 1, PACK, F32>(R, at, s0, it.sq.ctx, va, vb, all, x);
             move = raised != j && too_high(R, x);
             if (move) break;
-            accumulate<HD, 1, PACK, F32>(R, x, pl + (F32 ? 4 * GRP : 2 * RAW), 2 * GRP);
+            accumulate<HD, 1, PACK, F32>(R, x, at + NH * GRP);
             // the block is read: its place takes the next but one
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (!F32 && j + 2 < mine) fetch(j + 2, gr[2]);
+            if (j + 2 < mine) fetch(j + 2, gr[2]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < NH; ++h) {
                 gr[0][h] = gr[1][h];
                 gr[1][h] = gr[2][h];
             }
@@ -872,7 +894,7 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
 #pragma unroll
     for (int c = 0; c < HD / 16; ++c) {
         f32x4 o = R.acc[0][c];
-        if constexpr (PACK) {
+        if constexpr (PACK && !F32) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = fold8(o[i]);
         }
@@ -908,28 +930,28 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
 // ---- more rows: four waves share each block of keys ----
 // WK such fours take the blocks in turn, each through LDS of its own, so that
 // every SIMD has two waves whose products and exponentials take turns; they
-// meet at the end. (An fp32 cache of 256-wide heads fills LDS with one.)
+// meet at the end.
 template <int HD, bool F32>
 struct TileShape {
-    static constexpr int WK = HD == 256 && F32 ? 1 : 2;
-    static constexpr int KB = HD == 128 && !F32 ? 64 : 32;  // keys of a block
-    static constexpr int BLK = KB / 16 * 2 * Lay<HD, F32>::RAW;
-    // of a four: two blocks, or a raw block and its planes
-    static constexpr int LDS = F32 ? BLK + KB / 16 * 4 * Lay<HD, F32>::GRP : 2 * BLK;
-    static constexpr int ALL = WK * LDS;
+    static constexpr int WK = 2;
+    static constexpr int KB = 64 * 128 / HD / (F32 ? 2 : 1);  // keys of a block: 16 KB of each pool
+    static constexpr int BLK = KB / 16 * 2 * Lay<HD, F32>::GRP;
+    static constexpr int LDS = 2 * BLK;  // of a four: two blocks
 };
 
-template <int HD, bool F32, int RT>
-__global__ __launch_bounds__(256 * (HD == 256 && F32 ? 1 : 2), HD == 256 && F32 ? 1 : 2)
-void k_pa_tile(PaArgs a) {
+template <int HD, bool F32>
+__global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
     using L = Lay<HD, F32>;
     using S = TileShape<HD, F32>;
+    using P = Part<F32>;
     using KV = typename std::conditional<F32, float, uint16_t>::type;
-    constexpr int NW = 4, WK = S::WK, MT = 16 * RT * NW, KB = S::KB, NG = KB / 16;
-    constexpr int GRP = L::GRP, RAW = L::RAW;
+    // (two tiles a wave, 128 rows a workgroup: half the LDS reads, but out of
+    // registers and fewer workgroups: 2048 rows after 2048 166 us, one tile 150)
+    constexpr int RT = 1, NW = 4, WK = S::WK, MT = 16 * RT * NW, KB = S::KB, NG = KB / 16;
+    constexpr int GRP = L::GRP, NH = P::NH;
     constexpr int PART = RT * (HD / 16) * 1024 + RT * 512;  // a wave's sums on their way to join
-    static_assert(WK == 1 || NW * PART <= S::ALL, "the sums fit");
-    __shared__ __attribute__((aligned(1024))) char smem[S::ALL];
+    static_assert(NW * PART <= WK * S::LDS, "the sums fit");
+    __shared__ __attribute__((aligned(1024))) char smem[WK * S::LDS];
     __shared__ int there[WK][2][NG];  // slots of a block's groups that are there
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / QLM_WAVE % NW);
@@ -949,73 +971,62 @@ void k_pa_tile(PaArgs a) {
     const int blocks = uni(((k1 - k0 + KB - 1) / KB + WK - 1) / WK);
     auto slot_of = [&](int j) { return k0 + (j * WK + four) * KB; };
     char* const lds = smem + four * S::LDS;
-    // units (a group's K or V) u = wave, wave + 4, ... are this wave's to fetch:
-    // all of one group
-    static_assert(NW % NG == 0, "a wave's units are one group's");
-    const int own = wave % NG;
+    // a wave fetches a quarter of a block: loads of K and of V of one group
+    constexpr int SHARE = NW / NG;          // waves of a group
+    constexpr int LPW = L::LOADS / SHARE;  // a wave's loads of either
+    static_assert(NW % NG == 0 && L::LOADS % SHARE == 0, "whole loads a wave");
+    const int own = wave % NG, j0 = wave / NG * LPW;
     auto group = [&](int j) { return group_at(a, b, slot_of(j) + 16 * own, k1, lgp); };
     auto fetch = [&](int j, const Group& gr) {
-        char* to = lds + (F32 ? 0 : j & 1) * S::BLK;
-#pragma unroll
-        for (int u = 0; u < 2 * NG; u += NW)
-            fetch_group<HD, F32>(a, u + wave < NG ? a.pg.k : a.pg.v, gr, g, slot_of(j) + 16 * own,
-                                 to + (u + wave) * RAW);
+        char* to = lds + (j & 1) * S::BLK + own * GRP;
+        fetch_group<HD, F32, LPW>(a, a.pg.k, gr, g, slot_of(j) + 16 * own, to, j0);
+        fetch_group<HD, F32, LPW>(a, a.pg.v, gr, g, slot_of(j) + 16 * own, to + NG * GRP, j0);
         if (lane == 0) there[four][j & 1][own] = gr.valid;
     };
     Group gr[2] = {group(0), group(1)};
     const int w0 = uni(r0 + 16 * RT * wave);  // this wave's first row
-    Queries<HD, RT, false> Q;
-    request_rows<HD, RT, false>(a, it, g, w0, Q);
+    Queries<HD, RT> Q;
+    request_rows<HD, RT, false, F32>(a, it, g, w0, Q);
     __builtin_amdgcn_sched_barrier(0);
     fetch(0, gr[0]);
     __builtin_amdgcn_sched_barrier(0);
-    Rows<HD, RT, false> R;
-    take_rows<HD, RT, false>(a, it, w0, Q, R);
+    Rows<HD, RT, false, F32> R;
+    take_rows<HD, RT, false, F32>(a, it, w0, Q, R);
     // what all of this wave's rows see without a mask, and all they can see
     const int wave_end = uni(
         w0 < total ? min(keys_end(a, it.sq, (min(w0 + 16 * RT, total) - 1) >> a.lg), k1) : 0);
     const int free_end = uni(a.bt.parent ? it.sq.ctx : it.sq.ctx + (w0 >> a.lg) + 1);
-    constexpr int SUB = KB / 32;  // 32-key parts of a block
+    constexpr int SUB = KB / P::KEYS;  // parts of a block
     int staged = -1, raised = -1, valid[NG];
-    float x[RT][8];
+    float x[RT][P::XN];
     for (int i = 0;;) {
         bool move = false;
 #pragma unroll 1
         for (; i < blocks * SUB; ++i) {
-            const int j = i / SUB, h = i % SUB, s0 = slot_of(j) + 32 * h;
-            char* at = lds + (F32 ? 0 : j & 1) * S::BLK;
-            char* const pl = lds + S::BLK;  // fp32: planes K h, K l, V h, V l
+            const int j = i / SUB, h = i % SUB, s0 = slot_of(j) + P::KEYS * h;
             if (staged != j) {
                 staged = j;
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();  // the block is there, and every wave is done with the last one
-                if constexpr (F32) {
-#pragma unroll
-                    for (int u = 0; u < 2 * NG; u += NW) {
-                        const int v = u + wave;
-                        char* to = pl + (v < NG ? v : v + NG) * GRP;
-                        split_group<HD>(at + v * RAW, to, to + NG * GRP);
-                    }
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    __syncthreads();
-                }
 #pragma unroll
                 for (int k = 0; k < NG; ++k) valid[k] = uni(there[four][j & 1][k]);
                 if (j + 1 < blocks) fetch(j + 1, gr[1]);
                 gr[1] = group(j + 2);
             }
             if (s0 >= wave_end) continue;
-            int va = valid[0], vb = valid[1];
-            if (SUB > 1 && h) {
-                va = valid[NG - 2];
-                vb = valid[NG - 1];
-            }
-            const bool all = s0 + 32 <= free_end && va == 16 && vb == 16;
-            const char* kp = F32 ? pl : at + 2 * h * RAW;
-            scores<HD, RT, false, F32>(R, kp, NG * GRP, s0, it.sq.ctx, va, vb, all, x);
+            int va = valid[0], vb = valid[NH - 1];
+#pragma unroll
+            for (int k = 1; k < SUB; ++k)
+                if (h == k) {
+                    va = valid[k * NH];
+                    vb = valid[k * NH + NH - 1];
+                }
+            const bool all = s0 + P::KEYS <= free_end && va == 16 && vb == 16;
+            const char* kp = lds + (j & 1) * S::BLK + h * NH * GRP;
+            scores<HD, RT, false, F32>(R, kp, s0, it.sq.ctx, va, vb, all, x);
             move = raised != i && too_high(R, x);
             if (move) break;
-            accumulate<HD, RT, false, F32>(R, x, kp + (F32 ? 2 * NG * GRP : NG * RAW), NG * GRP);
+            accumulate<HD, RT, false, F32>(R, x, kp + NG * GRP);
         }
         if (!move) break;
         raise(R, x);
@@ -1023,7 +1034,7 @@ void k_pa_tile(PaArgs a) {
     }
     if (it.chunk == 0 && a.desc) put_desc<MT>(a, it, g, nch);
     __syncthreads();
-    if constexpr (WK == 2) {
+    {
         // the second four's sums to the wave of the first that has the same rows
         char* const to = smem + wave * PART;
         float* const st = reinterpret_cast<float*>(to + RT * (HD / 16) * 1024);
@@ -1172,7 +1183,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_pa_join(PaArgs a, int mt, int 
 // ---- the host's part ----
 
 struct PaPlan {
-    int mt;              // rows of a unit: 8, 16 (k_pa_few), 64 or 128 (k_pa_tile)
+    int mt;              // rows of a unit: 8, 16 (k_pa_few) or 64 (k_pa_tile)
     int target;          // items a kv head to cut the keys into
     int least, alone;    // keys of an item, at least; of a sequence that is not cut
     int items;           // at most
@@ -1185,7 +1196,7 @@ PaPlan plan_of(int rows, int B, int G, int n_kv, int hd, long long slots) {
     PaPlan p{};
     // about the rows of a sequence
     const long long per = ((long long)rows * G + B - 1) / B;
-    p.mt = per <= 8 ? 8 : per <= 16 ? 16 : per <= 64 || hd == 256 ? 64 : 128;
+    p.mt = per <= 8 ? 8 : per <= 16 ? 16 : 64;
     const int wanted = p.mt <= 16 ? 512 : 256;  // a CU holds one workgroup of either
     p.target = std::max(1, wanted / n_kv);
     const long long units = ((long long)rows * G) / p.mt + B;
@@ -1220,15 +1231,13 @@ template <int HD, bool F32>
 int launch_attention(const PaArgs& a, const PaPlan& p, hipStream_t st) {
     using KV = typename std::conditional<F32, float, uint16_t>::type;
     const dim3 grid((unsigned)groups_of(p.items, a.pg.n_kv));
-    const dim3 few(FewShape<HD, F32>::NW * QLM_WAVE), tile(256 * TileShape<HD, F32>::WK);
+    const dim3 few(FewShape<HD, F32>::NW * QLM_WAVE), tile(512);
     if (p.mt == 8)
         hipLaunchKernelGGL((k_pa_few<HD, F32, true>), grid, few, 0, st, a);
     else if (p.mt == 16)
         hipLaunchKernelGGL((k_pa_few<HD, F32, false>), grid, few, 0, st, a);
-    else if (p.mt == 64)
-        hipLaunchKernelGGL((k_pa_tile<HD, F32, 1>), grid, tile, 0, st, a);
-    else if constexpr (HD == 128)
-        hipLaunchKernelGGL((k_pa_tile<HD, F32, 2>), grid, tile, 0, st, a);
+    else
+        hipLaunchKernelGGL((k_pa_tile<HD, F32>), grid, tile, 0, st, a);
     const int rc = qlm_launch_status();
     if (rc != QLM_OK || !p.join) return rc;
     const int tasks = a.bt.rows * a.n_q;

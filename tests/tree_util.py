@@ -146,16 +146,20 @@ def attention_ref(rows, pages, q, n_q, gate=None, k=None, v=None):
 
 
 def attention_tol(pv, qk, keys, fp32_cache):
-    """The largest difference that qlm_paged_attention's roundings allow. A split
-    into two bf16 terms leaves 2^-17 of a value. Scores: queries 2^-17, fp32
-    keys another, the product of two l terms that is left out 2^-16, and hd / 32
-    + 8 fp32 additions and the scale's product; a score off by e moves each
-    probability by e relatively, and their sum too. Then the probabilities' and
-    fp32 values' own splits with the l terms' product, the exponential (2 ulp),
-    and the fp32 sums over keys (a block's 32 at a time, and the chunks')."""
-    u, t = 2.0 ** -24, 2.0 ** -17
-    score = qk * ((4 * t if fp32_cache else t) + 20 * u)
-    rel = 2 * score + (4 * t if fp32_cache else t) + (16 + keys / 16) * u
+    """The largest difference that qlm_paged_attention's fp32 arithmetic allows.
+    Products of bf16 terms are exact, and so is a split into three (2^-25 of a
+    value). A score: the scale's product and its rounding (2), one accumulation
+    for every 32 products of each of the three terms and up to 5 inside of them
+    (bf16: 3 * 8 + 5), or one for every product (fp32, 256), beginning at a
+    reference no larger than the largest sum |q k|: twice. A score that is off by e
+    moves its probability by e relatively, and their sum too. Then the
+    exponential and its split (3), and the sums over keys: bf16 one accumulation
+    for every 32 keys and term, fp32 one for every key, the probabilities' own
+    sum the same, and of chunks and waves that meet at most 40 more."""
+    u = 2.0 ** -24
+    score = 2 * qk * (260 if fp32_cache else 31) * u
+    sums = keys if fp32_cache else 3 * keys / 32 + 5
+    rel = 2 * score + (3 + 2 * sums + 40) * u
     return rel[:, None] * pv + 1e-30
 
 
