@@ -145,25 +145,22 @@ __device__ __forceinline__ int path_of(const TreeArgs& a, int b, const SeqRows& 
     return ends ? __ffsll((long long)ends) - 1 : QLM_WAVE;
 }
 
-// Decay's logarithm and b of a row.
-__device__ __forceinline__ void gates(const TreeArgs& a, int row, int h, double& alpha,
+// Decay's logarithm and b from a row's two gate inputs.
+__device__ __forceinline__ void gates(float ga, float gb, float dt_bias, float A_log, double& alpha,
                                       float& beta) {
-    const float* g = a.proj + (size_t)row * a.ldp + 4 * (size_t)a.H * kD;
-    const float dt = g[a.H + h] + a.dt_bias[h];
+    const float dt = ga + dt_bias;
     const float sp = dt > 20.0f ? dt : log1pf(expf(dt));
-    const float x = -expf(a.A_log[h]) * sp;
+    const float x = -expf(A_log) * sp;
     alpha = x < -1e4f ? -1e4 : (double)x;  // (0 in fp32 long before)
-    beta = sigmoid_f(g[h]);
+    beta = sigmoid_f(gb);
 }
 
 // Head norm and SiLU(z) gate of a row's head, a wave: o0, o1 its elements lane
 // and lane + 64 (not normalised). A row outside the tree: 0.
 __device__ __forceinline__ void put_head(const TreeArgs& a, int row, int h, bool live, float o0,
-                                         float o1) {
+                                         float o1, float z0, float z1) {
     const int lane = threadIdx.x & (QLM_WAVE - 1);
     float* to = a.out + (size_t)row * a.ldo + h * kD + lane;
-    const float* z = a.proj + (size_t)row * a.ldp + 3 * (size_t)a.H * kD + h * kD + lane;
-    const float z0 = z[0], z1 = z[64];
     const float sn = 1.0f / sqrtf(wave_sum(fmaf(o0, o0, o1 * o1)) / (float)kD + 1e-6f);
     to[0] = live ? (o0 * sn) * a.norm_w[lane] * silu_f(z0) : 0.0f;
     to[64] = live ? (o1 * sn) * a.norm_w[lane + 64] * silu_f(z1) : 0.0f;
@@ -195,6 +192,9 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
     }
     T = __builtin_amdgcn_readfirstlane(T);
     if (T <= a.above || T > TM) return;  // nothing to do, or another launch's
+    // gate inputs, used when the lines are known (a lane a node)
+    const float* gp = a.proj + (size_t)row * a.ldp + 4 * (size_t)HD + h;
+    const float gb = gp[0], ga = gp[a.H], gdt = a.dt_bias[h], galog = a.A_log[h];
     // ---- conv inputs: a channel of q or k a thread, every other node ----
     const int qk = tid & 255, hf = wave >> 2;
     const int ch = (qk >> 7) * HD + h * kD + (qk & 127);
@@ -229,6 +229,34 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         const float x = a.proj[(size_t)r * a.ldp + vch];
         if (v_on) sh.w[i][vc] = i < T ? x : 0.0f;
     }
+    // ---- who multiplies what with the state: WC waves over the column tiles, the
+    // others over the row tiles, or over keys and queries ----
+    constexpr int WC = NC < kNW ? NC : kNW, CPW = NC / WC, WR = kNW / WC;
+    constexpr int WT = WR < RT ? WR : RT, TPW = RT / WT;  // waves over row tiles, tiles of one
+    const int cw = wave % WC, tw = wave / WC % WT, role = wave / (WC * WT);
+    const bool do_k = WR <= RT || role == 0, do_q = !COMMIT && (WR <= RT || role == 1);
+    const float* S = a.state + ((size_t)b * a.H + h) * kD * kD + c0;
+    float sb[CPW][32];
+    if (do_k || do_q) {
+#pragma unroll
+        for (int c = 0; c < CPW; ++c)
+#pragma unroll
+            for (int s = 0; s < 32; ++s)
+                sb[c][s] = S[(size_t)(32 * qd + s) * kD + 16 * (cw + c * WC) + n];
+    }
+    // the output gates of the rows that this wave will finish
+    constexpr int ZN = NC == 8 && !COMMIT ? TM / kNW : 1;
+    float z0[ZN], z1[ZN];
+    if constexpr (NC == 8 && !COMMIT) {
+#pragma unroll
+        for (int k = 0; k < ZN; ++k) {
+            const float* z = a.proj +
+                             (size_t)__builtin_amdgcn_readlane(row, wave + k * kNW) * a.ldp +
+                             3 * (size_t)HD + h * kD + lane;
+            z0[k] = z[0];
+            z1[k] = z[64];
+        }
+    }
     for (int i = tid; i < TM * SH::TS; i += kThreads) (&sh.at[0][0])[i] = 0.0f;
     if (tid == 0) sh.bad = -1;
     // a node's inputs: itself and three above; behind the root the ring
@@ -248,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
     if (wave == 0) {
         double alpha = 0.0;
         float beta = 0.0f;
-        if (line && lane < T) gates(a, row, h, alpha, beta);
+        if (line && lane < T) gates(ga, gb, gdt, galog, alpha, beta);
         double c = alpha;
         while (__ballot(up >= 0)) {
             const int from = up >= 0 ? up : lane;
@@ -286,7 +314,7 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                 for (int i = 0; i < 8; ++i) {
                     float acc = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc = nc_add_mul(acc, x[i][j], w4[j]);
+                    for (int j = 0; j < 4; ++j) acc = fmaf(x[i][j], w4[j], acc);
                     y[i0 + i] = 2 * (i0 + i) + hf < T ? silu_fast(acc) : 0.0f;
                 }
             } else {
@@ -298,10 +326,10 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         for (int j = 0; j < VN; ++j) {
             const int i = min(vg + j * VG, TM - 1);
             const int4 tp = *reinterpret_cast<const int4*>(sh.tap[i]);
-            float acc = nc_add_mul(0.0f, sh.w[tp.x][vc], vw[0]);
-            acc = nc_add_mul(acc, sh.w[tp.y][vc], vw[1]);
-            acc = nc_add_mul(acc, sh.w[tp.z][vc], vw[2]);
-            acc = nc_add_mul(acc, sh.w[tp.w][vc], vw[3]);
+            float acc = sh.w[tp.x][vc] * vw[0];
+            acc = fmaf(sh.w[tp.y][vc], vw[1], acc);
+            acc = fmaf(sh.w[tp.z][vc], vw[2], acc);
+            acc = fmaf(sh.w[tp.w][vc], vw[3], acc);
             yv[j] = i < T ? silu_fast(acc) : 0.0f;
         }
         __syncthreads();
@@ -334,38 +362,18 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             sh.sk[i] = 1.0f / sqrtf(s1 + 1e-6f);
         }
     }
-    // ---- who multiplies what with the state: WC waves over the column tiles, the
-    // others over the row tiles, or over keys and queries ----
-    constexpr int WC = NC < kNW ? NC : kNW, CPW = NC / WC, WR = kNW / WC;
-    constexpr int WT = WR < RT ? WR : RT, TPW = RT / WT;  // waves over row tiles, tiles of one
-    const int cw = wave % WC, tw = wave / WC % WT, role = wave / (WC * WT);
-    const bool do_k = WR <= RT || role == 0, do_q = !COMMIT && (WR <= RT || role == 1);
-    const float* S = a.state + ((size_t)b * a.H + h) * kD * kD + c0;
-    float sb[CPW][32];
-    if (do_k || do_q) {
-#pragma unroll
-        for (int c = 0; c < CPW; ++c)
-#pragma unroll
-            for (int s = 0; s < 32; ++s)
-                sb[c][s] = S[(size_t)(32 * qd + s) * kD + 16 * (cw + c * WC) + n];
-    }
     __syncthreads();
     // ---- products of keys and queries with keys: pairs of 16-node tiles in turn ----
     const int tiles = (T + 15) / 16;
+    constexpr int KINDS = COMMIT ? 1 : 2;  // keys, queries
 #pragma unroll 1
-    for (int p = wave; p < tiles * (tiles + 1) / 2; p += kNW) {
+    for (int job = wave; job < tiles * (tiles + 1) / 2 * KINDS; job += kNW) {
+        const int p = job / KINDS, kind = job % KINDS;
         const int ti = p >= 6 ? 3 : p >= 3 ? 2 : p >= 1 ? 1 : 0, si = p - ti * (ti + 1) / 2;
-        f32x4 kk, qk = {0.0f, 0.0f, 0.0f, 0.0f};
-        {
-            float ka[32], kb[32];
-            load32(kb, &sh.k[16 * si + n][32 * qd]);
-            load32(ka, &sh.k[16 * ti + n][32 * qd]);
-            kk = dot32(ka, kb);
-            if constexpr (!COMMIT) {
-                load32(ka, &sh.q[16 * ti + n][32 * qd]);
-                qk = dot32(ka, kb);
-            }
-        }
+        float ra[32], kb[32];
+        load32(kb, &sh.k[16 * si + n][32 * qd]);
+        load32(ra, kind ? &sh.q[16 * ti + n][32 * qd] : &sh.k[16 * ti + n][32 * qd]);
+        const f32x4 prod = dot32(ra, kb);
         const int s = 16 * si + n;
         const double cs_ = sh.c[s];
         const float ks = sh.sk[s];
@@ -374,8 +382,10 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             const int t = 16 * ti + 4 * qd + i;
             const bool on = sh.line[t] >> s & 1ull;
             const float d = on ? expf((float)(sh.c[t] - cs_)) * ks : 0.0f;
-            sh.at[s][t] = on && s != t ? sh.beta[t] * sh.sk[t] * d * kk[i] : 0.0f;
-            if constexpr (!COMMIT) sh.m[t][s] = on ? sh.sq[t] * kScale * d * qk[i] : 0.0f;
+            if (kind)
+                sh.m[t][s] = on ? sh.sq[t] * kScale * d * prod[i] : 0.0f;
+            else
+                sh.at[s][t] = on && s != t ? sh.beta[t] * sh.sk[t] * d * prod[i] : 0.0f;
         }
     }
     // ---- products with the state; R in place of v ----
@@ -494,8 +504,21 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         if (!fine) sh.bad = 0;
     }
     __syncthreads();
+    // where the whole head is here: its norm and gate, a row a wave, and rows past
+    // the tree's last
+    auto finish = [&](auto of) {
+#pragma unroll
+        for (int k = 0; k < ZN; ++k) {
+            const int t = wave + k * kNW;
+            if (t >= T) break;
+            float o0, o1;
+            of(t, o0, o1);
+            put_head(a, sh.row[t], h, sh.line[t] != 0, o0, o1, z0[k], z1[k]);
+        }
+        for (int t = QLM_TREE_MAX + wave; t < sq.n; t += kNW)
+            put_head(a, sq.first + t, h, false, 0.0f, 0.0f, 0.0f, 0.0f);
+    };
     if constexpr (NC == 8) {
-        // the whole head is here: its norm and gate, a row a wave
         if (sh.bad < 0) {
 #pragma unroll
             for (int k = 0; k < TPW; ++k) {
@@ -507,10 +530,10 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                         sh.w[16 * (tw + k * WT) + 4 * qd + i][16 * (cw + c * WC) + n] = o[k][c][i];
             }
             __syncthreads();
-            for (int t = wave; t < T; t += kNW)
-                put_head(a, sh.row[t], h, sh.line[t] != 0, sh.w[t][lane], sh.w[t][lane + 64]);
-            for (int t = QLM_TREE_MAX + wave; t < sq.n; t += kNW)
-                put_head(a, sq.first + t, h, false, 0.0f, 0.0f);
+            finish([&](int t, float& o0, float& o1) {
+                o0 = sh.w[t][lane];
+                o1 = sh.w[t][lane + 64];
+            });
             return;
         }
     }
@@ -553,7 +576,7 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                     const int tp = sh.tap[u][e];
                     const float x = tp < TM ? a.proj[(size_t)sh.row[tp] * a.ldp + vch]
                                             : cs[(size_t)(tp - TM) * C + vch];
-                    acc = nc_add_mul(acc, x, a.wt[(size_t)e * C + vch]);
+                    acc = fmaf(x, a.wt[(size_t)e * C + vch], acc);
                 }
                 const float w = sh.beta[u] * (silu_fast(acc) - sum);
 #pragma unroll
@@ -572,14 +595,12 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         }
     }
     if constexpr (NC == 8) {
-        __threadfence_block();
         __syncthreads();
-        for (int t = wave; t < T; t += kNW) {
+        finish([&](int t, float& o0, float& o1) {
             const float* r = a.raw + (size_t)sh.row[t] * HD + h * kD + lane;
-            put_head(a, sh.row[t], h, sh.line[t] != 0, r[0], r[64]);
-        }
-        for (int t = QLM_TREE_MAX + wave; t < sq.n; t += kNW)
-            put_head(a, sq.first + t, h, false, 0.0f, 0.0f);
+            o0 = r[0];
+            o1 = r[64];
+        });
     }
 }
 
@@ -596,7 +617,8 @@ __global__ __launch_bounds__(kNormThreads) void k_dn_tree_norm(TreeArgs a) {
     for (int h = blockIdx.y * kNormWaves + threadIdx.x / QLM_WAVE; h < a.H;
          h += gridDim.y * kNormWaves) {
         const float* o = a.raw + (size_t)row * HD + h * kD + lane;
-        put_head(a, row, h, live, live ? o[0] : 0.0f, live ? o[64] : 0.0f);
+        const float* z = a.proj + (size_t)row * a.ldp + 3 * (size_t)HD + h * kD + lane;
+        put_head(a, row, h, live, live ? o[0] : 0.0f, live ? o[64] : 0.0f, z[0], z[64]);
     }
 }
 
