@@ -1272,7 +1272,8 @@ extern "C" int qlm_paged_attention(const float* q, int ldq, const qlm_row_batch*
     const long long slots = (long long)pages->ld_table * pages->page_size;
     if (!pa_shape(batch->rows, batch->B, n_q, n_kv, hd, slots)) return QLM_ERR_SHAPE;
     if (ldq < n_q * hd || ldo < n_q * hd) return QLM_ERR_SHAPE;
-    if (gate && (gate_stride < hd || ldg < (n_q - 1) * gate_stride + hd)) return QLM_ERR_SHAPE;
+    if (gate && (gate_stride < hd || ldg < (long long)(n_q - 1) * gate_stride + hd))
+        return QLM_ERR_SHAPE;
     const int G = n_q / n_kv;
     const PaPlan p = plan_of(batch->rows, batch->B, G, n_kv, hd, slots);
     if (groups_of(p.items, n_kv) >= 1LL << 23) return QLM_ERR_SHAPE;  // a launch's threads fit 32 bits

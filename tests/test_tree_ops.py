@@ -111,6 +111,7 @@ def test_append_refusals(kw, rc):
     (dict(n_q=3), SHAPE), (dict(n_q=6), SHAPE), (dict(n_q=32, ldq=4096, ldo=4096), SHAPE),
     (dict(ldq=511), SHAPE), (dict(ldo=511), SHAPE), (dict(gate=P, ldg=511, gs=128), SHAPE),
     (dict(gate=P, ldg=2048, gs=127), SHAPE), (dict(work=P + 8), SHAPE),
+    (dict(n_q=16, ldq=2048, ldo=2048, gate=P, ldg=2048, gs=1 << 29), SHAPE),  # 15 2^29 > 2^32
 ])
 def test_attention_refusals(kw, rc):
     assert attention(**kw) == rc
