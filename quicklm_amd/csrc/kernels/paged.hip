@@ -286,8 +286,8 @@ extern "C" int qlm_tree_commit(const int* tokens, const int* picks, const qlm_ro
     const long long pool = (long long)pages->n_pages * pages->n_kv * pages->page_size * pages->hd;
     if (layer_stride < 0 || (layers > 1 && layer_stride < pool)) return QLM_ERR_ARG;
     const long long size = pages->dtype == 0 ? 4 : 2;
+    if (layers > 4096 || layer_stride > 1LL << 48) return QLM_ERR_SHAPE;
     if (layers > 1 && layer_stride * size % 16 != 0) return QLM_ERR_SHAPE;
-    if (layers > 4096) return QLM_ERR_SHAPE;
     const int pieces = (int)(pages->hd * size / 16);
     const CommitArgs a{tokens, picks, path, accepted, next_token, new_len, ld_path, layers, pieces,
                        layer_stride * size, *batch, *pages};

@@ -123,6 +123,7 @@ def test_attention_refusals(kw, rc):
     (dict(ld_path=63), ARG), (dict(new_len=2 * P), ARG),  # ctx_len itself
     (dict(stride=8 * 2 * 16 * 128 - 1), ARG),  # layers that overlap
     (dict(stride=-1), ARG), (dict(stride=(1 << 20) + 4), SHAPE), (dict(layers=4097), SHAPE),
+    (dict(stride=(1 << 48) + 16), SHAPE), (dict(stride=1 << 62), SHAPE),  # bytes past 64 bits
 ])
 def test_commit_refusals(kw, rc):
     assert commit(**kw) == rc
