@@ -658,7 +658,8 @@ int qlm_tree_commit(const int* tokens, const int* picks, const qlm_row_batch* ba
  * the sequence's state [B, H, d, d] and conv ring [B, 3, 3*H*d] (oldest tap row =
  * ctx_len[b] % 3), neither of which is changed. Rows past a sequence's first
  * QLM_TREE_MAX are outside, without a parent array too. proj, out as
- * qlm_deltanet_prefill's, within 1e-4 of it (reassociated fp32). d = 128. work:
+ * qlm_deltanet_prefill's (out must not overlap proj), within 1e-4 of it
+ * (reassociated fp32). d = 128. work:
  * device scratch of qlm_deltanet_tree_workspace_bytes(rows, H, d) bytes (0 for
  * sizes that are refused), 16-byte aligned, no initial contents needed; calls
  * sharing it must be ordered on one stream. */

@@ -714,6 +714,7 @@ extern "C" int qlm_deltanet_tree(const float* proj, int ldp, const qlm_row_batch
         return QLM_ERR_ARG;
     if (work_bytes < qlm_deltanet_tree_workspace_bytes(batch->rows, H, d)) return QLM_ERR_ARG;
     if (ldo < H * d || ((uintptr_t)work & 15u)) return QLM_ERR_SHAPE;
+    if (proj == out) return QLM_ERR_ARG;  // heads read what others would have written
     const TreeArgs a{proj,   conv_state, conv_w_t, A_log, dt_bias, norm_w, const_cast<float*>(state),
                      reinterpret_cast<float*>(work), out, nullptr, nullptr, ldp, ldo, H, 0, 0, *batch};
     hipStream_t st = as_stream(stream);

@@ -138,7 +138,7 @@ def test_commit_needs_a_tree():
     (dict(dt=None), ARG), (dict(norm=None), ARG), (dict(state=None), ARG), (dict(out=None), ARG),
     (dict(work=None), ARG), (dict(H=0), ARG), (dict(work_bytes=4 * 256 * 4 - 1), ARG),
     (dict(d=64), SHAPE), (dict(ldp=1027), SHAPE), (dict(ldo=255), SHAPE), (dict(work=P + 4), SHAPE),
-    (dict(H=4097, ldp=1 << 22, ldo=1 << 20), SHAPE),
+    (dict(H=4097, ldp=1 << 22, ldo=1 << 20), SHAPE), (dict(proj=2 * P, out=2 * P), ARG),
 ])
 def test_deltanet_tree_refusals(kw, rc):
     assert tree(**kw) == rc

@@ -413,6 +413,52 @@ def test_attention_of_one_batch_is_repeatable(hip, rng):
     assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("bf16", [True, False])
+def test_attention_many_rows_and_heads(hip, rng, bf16):
+    """More tasks than the joining launch has waves, of three kv heads. The
+    oracle takes a copy that has all but a few rows' queries left out."""
+    say(f"attention many rows bf16={bf16}")
+    n, ctx, n_q = [300, 1, 500], [40, 200, 0], 12
+    rows = Rows(hip, n, ctx)
+    pages = Pages(hip, rng, [a + c for a, c in zip(n, ctx)], 3, 128, 32, bf16)
+    got, q, _ = run_attention(hip, rng, rows, pages, n_q)
+    for r, i in [(0, 0), (150, 150), (299, 299), (301, 0), (540, 239), (800, 499)]:
+        b = 0 if r < 300 else 2
+        one = Rows(hip, [1], [ctx[b] + i])
+        own = Pages.__new__(Pages)
+        own.__dict__.update(pages.__dict__, table=pages.table[b:b + 1])
+        o, pv, qk, keys = attention_ref(one, own, q[r:r + 1], n_q)[0]
+        err, tol = np.abs(got[r].reshape(n_q, 128) - o), attention_tol(pv, qk, keys, not bf16)
+        assert (err <= tol).all(), (r, float((err / tol).max()))
+
+
+def test_attention_two_calls_at_once(hip, rng):
+    """Two streams, a workspace each, one cache; and one workspace for two calls
+    of different sizes on one stream."""
+    say("attention on two streams")
+    L, st = hip.lib(), [hip.Stream(), hip.Stream()]
+    batches = [Rows(hip, [1, 1], [2000, 900]), Rows(hip, [70, 9], [1500, 20])]
+    pages = Pages(hip, rng, [2001, 900], 2, 128, 64, True)
+    q = [rng.standard_normal((r.rows, 1024)).astype(np.float32) for r in batches]
+    want = [run_attention(hip, rng, r, pages, 8, q=x)[0] for r, x in zip(batches, q)]
+    size = [L.qlm_paged_attention_workspace_bytes(r.rows, 2, 8, 2, 128, pages.ld * 64)
+            for r in batches]
+    dq = [buf(hip, x) for x in q]
+    for shared in (False, True):
+        work = [buf(hip, np.full(max(size), 0xff, np.uint8)) for _ in batches]
+        out = [buf(hip, np.full_like(x, FILL)) for x in q]
+        for _ in range(3):
+            for i, r in enumerate(batches):
+                w = work[0 if shared else i]
+                hip.call("qlm_paged_attention", dq[i], 1024, r.c, pages.c, None, 0, 0, out[i],
+                         1024, 8, w, max(size), st[0 if shared else i].ptr)
+        for s in st:
+            s.sync()
+        # (slot 900 of the second sequence holds NaN, and the row that sees it gives it)
+        for x, o in zip(want, out):
+            assert np.array_equal(x, o.to_numpy(x.shape, np.float32), equal_nan=True)
+
+
 # ---- commit ----------------------------------------------------------------------
 
 
@@ -570,6 +616,24 @@ def test_deltanet_tree_batches(hip, rng, B, H):
     rows = Rows(hip, n, [b % 5 for b in range(B)], [random_tree(rng, k) for k in n])
     inp = dn_inputs(rng, rows, H, B)
     check_tree(rows, inp, H, run_tree(hip, rows, inp, H))
+
+
+@pytest.mark.parametrize("B,H", [(1, 33), (5, 16), (9, 16)])
+def test_deltanet_tree_odd_values_and_many_rows(hip, rng, B, H):
+    """Where a head's columns are four workgroups', two's and one's: rows past
+    the 64th, and a node that is not finite."""
+    say(f"deltanet odd values B={B} H={H}")
+    n = [70] + [3] * (B - 1)
+    parents = [[-1] + [max(0, i - 2) for i in range(1, k)] for k in n]
+    rows = Rows(hip, n, [b % 3 for b in range(B)], parents, behind=1)
+    inp = dn_inputs(rng, rows, H, B)
+    check_tree(rows, inp, H, run_tree(hip, rows, inp, H))
+    clean = {k: v.copy() for k, v in inp.items()}
+    inp["proj"][40, H * 128 + 9] = np.nan  # a key channel of head 0
+    out = run_tree(hip, rows, inp, H)
+    below = {i for i, l in enumerate(lines(parents[0], n[0])) if l and 40 in l}
+    check_tree(rows, clean, H, out, skip=below)
+    assert np.isnan(out[40, :128]).any() and np.isfinite(out[40, 128:]).all()
 
 
 def test_deltanet_chain_equals_prefill(hip, rng):
