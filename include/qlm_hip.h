@@ -619,10 +619,10 @@ int qlm_paged_append(const float* qkv, int ldqkv, const float* q_norm, const flo
  * overlapping; n_q / n_kv 1, 2, 4 or 8. gate NULL: none; else head h's gate of
  * row r is at gate + r * ldg + h * gate_stride (qkv + hd, ldqkv and 2 * hd after
  * a gated qlm_paged_append). A row that sees nothing gives 0. fp32
- * arithmetic throughout: a bf16 cache's products run on the bf16 matrix cores,
- * queries and probabilities split exactly into three bf16 terms, an fp32
- * cache's on the fp32 ones; results that do not come out finite are computed
- * again without the keys that a row does not see. Single
+ * arithmetic throughout: products run on the bf16 matrix cores, queries,
+ * probabilities and fp32 keys and values split exactly into three bf16 terms, or
+ * on the fp32 ones; results that do not come out finite are computed again
+ * without the keys that a row does not see. Single
  * tokens, trees, prompts and mixtures take the same call; a long context is
  * split over the GPU and joined, by lengths that are read on the device, so
  * the sums' order depends on the batch's lengths. work: device scratch of

@@ -17,9 +17,13 @@
 // but in the fp32 sums; two terms, two thirds of the products, left 5e-6 of the
 // result, five times what fp32 arithmetic does. Up to 8 rows take two products:
 // rows 0..7 of the tile hold the h terms and rows 8..15 the m terms, then the l
-// terms and zeros, and the halves are added. An fp32 cache takes the fp32 matrix
-// cores (16x16x4), a sixteenth of the rate but no split of every key and value:
-// single tokens and trees are bound by the cache's bytes all the same.
+// terms and zeros, and the halves are added. An fp32 cache's keys and values are
+// split likewise: six products of terms (the three others are below 2^-25 of the
+// whole), which the rows of a tile of 64 share the splitting for; the fp32 matrix
+// cores (16x16x4), a sixteenth of the rate, took 503 us where this takes 326 (2048
+// rows after 2048, 16 / 4 heads of 128) and 977 where this takes 626 (16 / 2 of
+// 256), and with the splitting in every wave 482 and 908. Up to 16 rows a unit
+// stay on them, bound by the cache's bytes all the same.
 //
 // Keys and values go straight from the pages to LDS. A 16-key group lies in one
 // page and is read through a buffer descriptor that ends where the group's
@@ -216,16 +220,22 @@ struct Lay {
     }
 };
 
+// A head's group in a pool, ending where its slots do.
+template <int HD, bool F32>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t group_rsrc(const PaArgs& a, const void* pool,
+                                                             const Group& gr, int g, int slot) {
+    constexpr int SIZE = F32 ? 4 : 2;
+    const size_t at = (((size_t)gr.page * a.pg.n_kv + g) * a.pg.page_size +
+                       (slot & (a.pg.page_size - 1))) * (HD * SIZE);
+    return make_rsrc(reinterpret_cast<const char*>(pool) + at, (unsigned)gr.valid * (HD * SIZE));
+}
+
 // Loads J0 .. J0 + N - 1 of a group.
 template <int HD, bool F32, int N = Lay<HD, F32>::LOADS>
 __device__ __forceinline__ void fetch_group(const PaArgs& a, const void* pool, const Group& gr,
                                             int g, int slot, char* to, int j0 = 0) {
     using L = Lay<HD, F32>;
-    constexpr int SIZE = F32 ? 4 : 2;
-    const size_t at = (((size_t)gr.page * a.pg.n_kv + g) * a.pg.page_size +
-                       (slot & (a.pg.page_size - 1))) * (HD * SIZE);
-    const __amdgpu_buffer_rsrc_t r =
-        make_rsrc(reinterpret_cast<const char*>(pool) + at, (unsigned)gr.valid * (HD * SIZE));
+    const __amdgpu_buffer_rsrc_t r = group_rsrc<HD, F32>(a, pool, gr, g, slot);
 #pragma unroll
     for (int j = 0; j < N; ++j) load_to_lds(r, to + (j0 + j) * 1024, L::src(j0 + j), 0);
 }
@@ -239,17 +249,18 @@ __device__ __forceinline__ T lds_read(uint32_t at) {
     return *(__attribute__((address_space(3))) const T*)(uintptr_t)at;
 }
 
-// Eight floats as three bf16 terms each (24 bits: exact). What a term leaves is
-// x - h, exact: one product with -1 and its sum with x (v_dot2_f32_bf16) instead
-// of widening h and subtracting it.
-__device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&term)[3]) {
+// N floats (four, eight) as three bf16 terms each (24 bits: exact). What a term
+// leaves is x - h, exact: one product with -1 and its sum with x (v_dot2_f32_bf16)
+// instead of widening h and subtracting it.
+template <int N, typename V>
+__device__ __forceinline__ void split_terms(const float (&x)[N], V (&term)[3]) {
     // (-1, 0) and (0, -1); in registers, since the compiler writes the second as the
     // inline constant -1.0, which the instruction does not read as that pair
     unsigned c0 = 0x0000bf80u, c1 = 0xbf800000u;
     asm("" : "+v"(c0), "+v"(c1));
     const bf16x2 first = __builtin_bit_cast(bf16x2, c0), second = __builtin_bit_cast(bf16x2, c1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N / 2; ++i) {
         f32x2 v = {x[2 * i], x[2 * i + 1]};
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
@@ -279,6 +290,13 @@ __device__ __forceinline__ float cols_sum(float v) { return xor32_add(xor16_add(
 // v(l) + v(l ^ 8) of each 16 lanes
 __device__ __forceinline__ float fold8(float v) { return v + dpp_mov<0x128>(v); }  // row_ror:8
 
+// How products are formed: of a bf16 cache; of an fp32 cache on the fp32 matrix
+// cores; of an fp32 cache whose keys and values lie in LDS as three bf16 terms.
+enum Math { kBf16, kF32, kSplit };
+
+// Split keys (or values) of a block, 4096 elements: planes of their h, m and l terms.
+constexpr int kPlane = 4096 * 2;
+
 // Keys go through in parts of NH 16-key halves; a lane has XN scores of a row.
 template <bool F32>
 struct Part {
@@ -297,11 +315,12 @@ struct Part {
 // its registers were copied every time, a third of its vector instructions.
 constexpr float kRise = 60.0f;
 constexpr int kAnyScore = (int)0x80000000;
-template <int HD, int RT, bool PACK, bool F32>
+template <int HD, int RT, bool PACK, Math M>
 struct Rows {
     static constexpr int KS = HD / 32, CB = HD / 16, QT = PACK ? 2 : 3;
-    u32x4 q[F32 ? 1 : RT][F32 ? 1 : QT][F32 ? 1 : KS];
-    f32x4 qf[F32 ? RT : 1][F32 ? HD / 16 : 1];  // lane (qd, n): elements 16 s + 4 qd .. + 3
+    u32x4 q[M == kF32 ? 1 : RT][M == kF32 ? 1 : QT][M == kF32 ? 1 : KS];
+    // lane (qd, n): elements 16 s + 4 qd .. + 3
+    f32x4 qf[M == kF32 ? RT : 1][M == kF32 ? HD / 16 : 1];
     f32x4 acc[RT][CB];
     f32x4 from[RT];       // four times -m
     float m[RT], l[RT];   // m -inf: no score yet
@@ -311,12 +330,12 @@ struct Rows {
 };
 
 // Query rows r0 + 16 t + n of the unit (r: its token and head): requested here.
-// (bf16: elements 32 s + 8 qd .. + 7; fp32: 16 s + 4 qd .. + 3.)
+// (bf16 cores: elements 32 s + 8 qd .. + 7; fp32: 16 s + 4 qd .. + 3.)
 template <int HD, int RT>
 struct Queries {
     f32x4u x[RT][HD / 16];
 };
-template <int HD, int RT, bool PACK, bool F32>
+template <int HD, int RT, bool PACK, Math M>
 __device__ __forceinline__ void request_rows(const PaArgs& a, const Item& it, int g, int r0,
                                              Queries<HD, RT>& Q) {
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
@@ -328,17 +347,17 @@ __device__ __forceinline__ void request_rows(const PaArgs& a, const Item& it, in
                           ((size_t)(g << a.lg) + (rc & ((1 << a.lg) - 1))) * HD;
 #pragma unroll
         for (int s = 0; s < HD / 16; ++s) {
-            const int e = F32 ? 16 * s + 4 * qd : 32 * (s / 2) + 8 * qd + 4 * (s % 2);
+            const int e = M == kF32 ? 16 * s + 4 * qd : 32 * (s / 2) + 8 * qd + 4 * (s % 2);
             Q.x[t][s] = *reinterpret_cast<const f32x4u*>(qr + e);
         }
     }
 }
 
 // What the rows see, and their queries' terms.
-template <int HD, int RT, bool PACK, bool F32>
+template <int HD, int RT, bool PACK, Math M>
 __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r0,
-                                          const Queries<HD, RT>& Q, Rows<HD, RT, PACK, F32>& R) {
-    using T = Rows<HD, RT, PACK, F32>;
+                                          const Queries<HD, RT>& Q, Rows<HD, RT, PACK, M>& R) {
+    using T = Rows<HD, RT, PACK, M>;
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15;
     const int total = it.sq.n << a.lg;
     unsigned long long mine = 0;
@@ -359,7 +378,7 @@ __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r
             R.line[t] = tok < QLM_TREE_MAX ? ln : 0;
             R.lim[t] = R.line[t] ? it.sq.ctx : -1;
         }
-        if constexpr (F32) {
+        if constexpr (M == kF32) {
 #pragma unroll
             for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
@@ -371,7 +390,7 @@ __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = Q.x[t][2 * s + i / 4][i % 4] * a.qscale;
                 u32x4 term[3];
-                split8(v, term);
+                split_terms(v, term);
                 if constexpr (PACK) {
                     R.q[t][0][s] = n < 8 ? term[0] : term[1];
                     R.q[t][1][s] = n < 8 ? term[2] : u32x4{0u, 0u, 0u, 0u};
@@ -386,16 +405,23 @@ __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r
     }
 }
 
+// Keeps the compiler from holding what it derives from x over the loop: with heads
+// of 256 the addresses of every piece, 24 registers, drove queries into scratch.
+template <int HD>
+__device__ __forceinline__ void fresh(uint32_t& x) {
+    if constexpr (HD > 128) asm volatile("" : "+v"(x));
+}
+
 // Scores of a part of the keys, from slot k0 on, relative to the references, of
 // keys that a row does not see -inf: x[t][4 h + i] of key 16 h + 4 qd + i. kp:
 // its K groups in LDS. `all`: every row sees every key of it.
-template <int HD, int RT, bool PACK, bool F32>
-__device__ __forceinline__ void scores(const Rows<HD, RT, PACK, F32>& R, const char* kp, int k0,
+template <int HD, int RT, bool PACK, Math M>
+__device__ __forceinline__ void scores(const Rows<HD, RT, PACK, M>& R, const char* kp, int k0,
                                        int ctx, int valid0, int valid1, bool all,
-                                       float (&x)[RT][Part<F32>::XN]) {
-    using T = Rows<HD, RT, PACK, F32>;
-    using L = Lay<HD, F32>;
-    constexpr int NH = Part<F32>::NH, XN = Part<F32>::XN;
+                                       float (&x)[RT][Part<M != kBf16>::XN]) {
+    using T = Rows<HD, RT, PACK, M>;
+    using L = Lay<HD, M == kF32>;
+    constexpr int NH = Part<M != kBf16>::NH, XN = Part<M != kBf16>::XN;
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
     f32x4 s[NH][RT];
 #pragma unroll
@@ -403,35 +429,65 @@ __device__ __forceinline__ void scores(const Rows<HD, RT, PACK, F32>& R, const c
 #pragma unroll
         for (int t = 0; t < RT; ++t) s[h][t] = R.from[t];
     // piece (4 k + qd) ^ n of row n: the bits of k come in by an exclusive or
-    const uint32_t ka = lds_at(kp) + n * L::ROW + ((qd ^ n) * 16);
-    constexpr int KN = L::ROW / 64;         // pieces of a row a lane
-    constexpr int KC = KN < 4 ? KN : 4;     // read at once
+    uint32_t ka = lds_at(kp) + n * L::ROW + ((qd ^ n) * 16);
+    if constexpr (M == kSplit) {
+        fresh<HD>(ka);
+        // of the nine products of terms the last three are below 2^-25; two sums,
+        // whose products take turns
+        f32x4 other[RT];
 #pragma unroll
-    for (int k0s = 0; k0s < KN; k0s += KC) {
-        u32x4 kf[KC][NH];
+        for (int t = 0; t < RT; ++t) other[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < KC; ++k)
+        for (int k = 0; k < T::KS; k += 2) {
+            u32x4 kt[2][3];
 #pragma unroll
-            for (int h = 0; h < NH; ++h)
-                kf[k][h] = lds_read<u32x4>((ka ^ (64u * (k0s + k))) + h * L::GRP);
-        __builtin_amdgcn_sched_barrier(0);
-        // (a sum's terms apart from each other: each waits for the one before)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int k = 0; k < KC; ++k) {
-            if constexpr (F32) {
+                for (int p = 0; p < 3; ++p)
+                    kt[e][p] = lds_read<u32x4>((ka ^ (64u * (k + e))) + p * kPlane);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+            for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
-                    for (int t = 0; t < RT; ++t)
-                        s[0][t] = mfma(__uint_as_float(kf[k][0][i]), R.qf[t][k0s + k][i], s[0][t]);
-            } else {
+                for (int p = 0; p <= sum; ++p)
 #pragma unroll
-                for (int p = T::QT - 1; p >= 0; --p)
+                    for (int t = 0; t < RT; ++t) {
+                        s[0][t] = mfma(kt[0][sum - p], R.q[t][p][k], s[0][t]);
+                        other[t] = mfma(kt[1][sum - p], R.q[t][p][k + 1], other[t]);
+                    }
+        }
 #pragma unroll
-                    for (int h = 0; h < NH; ++h)
+        for (int t = 0; t < RT; ++t) s[0][t] += other[t];
+    } else {
+        constexpr int KN = L::ROW / 64;         // pieces of a row a lane
+        constexpr int KC = KN < 4 ? KN : 4;     // read at once
+#pragma unroll
+        for (int k0s = 0; k0s < KN; k0s += KC) {
+            u32x4 kf[KC][NH];
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+                    kf[k][h] = lds_read<u32x4>((ka ^ (64u * (k0s + k))) + h * L::GRP);
+            __builtin_amdgcn_sched_barrier(0);
+            // (a sum's terms apart from each other: each waits for the one before)
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                if constexpr (M == kF32) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int t = 0; t < RT; ++t)
-                            s[h][t] = mfma(kf[k][h], R.q[t][p][k0s + k], s[h][t]);
+                            s[0][t] = mfma(__uint_as_float(kf[k][0][i]), R.qf[t][k0s + k][i],
+                                           s[0][t]);
+                } else {
+#pragma unroll
+                    for (int p = T::QT - 1; p >= 0; --p)
+#pragma unroll
+                        for (int h = 0; h < NH; ++h)
+#pragma unroll
+                            for (int t = 0; t < RT; ++t)
+                                s[h][t] = mfma(kf[k][h], R.q[t][p][k0s + k], s[h][t]);
+                }
             }
         }
     }
@@ -440,7 +496,7 @@ __device__ __forceinline__ void scores(const Rows<HD, RT, PACK, F32>& R, const c
 #pragma unroll
         for (int j = 0; j < XN; ++j) {
             x[t][j] = s[j / 4][t][j % 4];
-            if constexpr (PACK && !F32) x[t][j] = fold8(x[t][j]);
+            if constexpr (PACK && M == kBf16) x[t][j] = fold8(x[t][j]);
         }
     if (all) return;
     asm volatile("");  // (a branch, not selections that every part would compute)
@@ -457,32 +513,32 @@ __device__ __forceinline__ void scores(const Rows<HD, RT, PACK, F32>& R, const c
 }
 
 // Whether some score is too far above its row's reference.
-template <int HD, int RT, bool PACK, bool F32>
-__device__ __forceinline__ bool too_high(const Rows<HD, RT, PACK, F32>& R,
-                                         const float (&x)[RT][Part<F32>::XN]) {
+template <int HD, int RT, bool PACK, Math M>
+__device__ __forceinline__ bool too_high(const Rows<HD, RT, PACK, M>& R,
+                                         const float (&x)[RT][Part<M != kBf16>::XN]) {
     bool high = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         // as integers, in whose order positive floats are: no canonical forms
         int top = __float_as_int(x[t][0]);
 #pragma unroll
-        for (int j = 1; j < Part<F32>::XN; ++j) top = max(top, __float_as_int(x[t][j]));
+        for (int j = 1; j < Part<M != kBf16>::XN; ++j) top = max(top, __float_as_int(x[t][j]));
         high |= top > R.high[t];
     }
     return __ballot(high) != 0;
 }
 
 // Moves the references to the part's largest scores where those are higher.
-template <int HD, int RT, bool PACK, bool F32>
-__device__ __forceinline__ void raise(Rows<HD, RT, PACK, F32>& R,
-                                      const float (&x)[RT][Part<F32>::XN]) {
-    using T = Rows<HD, RT, PACK, F32>;
+template <int HD, int RT, bool PACK, Math M>
+__device__ __forceinline__ void raise(Rows<HD, RT, PACK, M>& R,
+                                      const float (&x)[RT][Part<M != kBf16>::XN]) {
+    using T = Rows<HD, RT, PACK, M>;
     const int n = threadIdx.x & 15;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         float top = x[t][0];
 #pragma unroll
-        for (int j = 1; j < Part<F32>::XN; ++j) top = fmaxf(top, x[t][j]);
+        for (int j = 1; j < Part<M != kBf16>::XN; ++j) top = fmaxf(top, x[t][j]);
         top = cols_max(top);
         const bool first = R.m[t] == -INFINITY;
         const bool moves = top > (first ? -INFINITY : 0.0f);
@@ -495,7 +551,7 @@ __device__ __forceinline__ void raise(Rows<HD, RT, PACK, F32>& R,
 #pragma unroll
             for (int i = 0; i < 4; ++i) R.acc[t][c][i] *= f;
         // (a packed tile's two halves are added: one of them begins at 0)
-        const float from = moves && !(PACK && !F32 && n >= 8) ? -R.m[t] : R.from[t][0];
+        const float from = moves && !(PACK && M == kBf16 && n >= 8) ? -R.m[t] : R.from[t][0];
         R.from[t] = f32x4{from, from, from, from};
         // a row that has seen nothing in the part waits for its first score
         R.high[t] = R.m[t] == -INFINITY ? kAnyScore : __float_as_int(kRise);
@@ -503,12 +559,12 @@ __device__ __forceinline__ void raise(Rows<HD, RT, PACK, F32>& R,
 }
 
 // The part's probabilities into the rows' sums; vp: its V groups in LDS.
-template <int HD, int RT, bool PACK, bool F32>
-__device__ __forceinline__ void accumulate(Rows<HD, RT, PACK, F32>& R,
-                                           float (&x)[RT][Part<F32>::XN], const char* vp) {
-    using T = Rows<HD, RT, PACK, F32>;
-    using L = Lay<HD, F32>;
-    constexpr int XN = Part<F32>::XN;
+template <int HD, int RT, bool PACK, Math M>
+__device__ __forceinline__ void accumulate(Rows<HD, RT, PACK, M>& R,
+                                           float (&x)[RT][Part<M != kBf16>::XN], const char* vp) {
+    using T = Rows<HD, RT, PACK, M>;
+    using L = Lay<HD, M == kF32>;
+    constexpr int XN = Part<M != kBf16>::XN;
     const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15, qd = lane >> 4;
     auto exponentials = [&](int t) {
 #pragma unroll
@@ -517,7 +573,7 @@ __device__ __forceinline__ void accumulate(Rows<HD, RT, PACK, F32>& R,
         if constexpr (XN == 8) sum += (x[t][4] + x[t][5]) + (x[t][6] + x[t][7]);
         R.l[t] += sum;
     };
-    if constexpr (F32) {
+    if constexpr (M == kF32) {
         // step i: keys 4 qd + i; lane (qd, n) reads element 16 c + n of its key, in
         // piece (4 c + n / 4) ^ key: 64 banks once
         uint32_t va[4];
@@ -551,13 +607,55 @@ __device__ __forceinline__ void accumulate(Rows<HD, RT, PACK, F32>& R,
     } else {
         // V^T: lane l of a group reads 4 columns of key 4 qd + (l % 16) / 4
         const int key = 4 * qd + (n >> 2);
-        const uint32_t va =
+        uint32_t va =
             lds_at(vp) + key * L::ROW + ((((n >> 1) & 1) ^ key) * 16) + (n & 1) * 8;
         auto tr = [&](uint32_t at) {
             return __builtin_bit_cast(
                 u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                            (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
         };
+        if constexpr (M == kSplit) {
+            // the eight k-slots of a lane group are its four keys twice, so that a
+            // product of 32 slots takes two pairs of terms: (h, m) with the
+            // probabilities' (h, h) and (m, m), (l, h) with (h, l)
+            constexpr int VC = 4;
+            fresh<HD>(va);
+            u32x2 v[3][VC];
+            auto read_some = [&](int c0) {
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+                        v[p][c] = tr((va ^ (32u * (c0 + c))) + p * kPlane);
+            };
+            read_some(0);
+            __builtin_amdgcn_sched_barrier(0);
+            u32x4 p[RT][3];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                exponentials(t);
+                u32x2 w[3];
+                split_terms(x[t], w);
+                p[t][0] = u32x4{w[0].x, w[0].y, w[0].x, w[0].y};
+                p[t][1] = u32x4{w[1].x, w[1].y, w[1].x, w[1].y};
+                p[t][2] = u32x4{w[0].x, w[0].y, w[2].x, w[2].y};
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < T::CB; c0 += VC) {
+                if (c0) read_some(c0);
+#pragma unroll
+                for (int k = 2; k >= 0; --k)
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        const u32x2 a = v[k == 2 ? 2 : 0][c], b = v[k == 2 ? 0 : 1][c];
+#pragma unroll
+                        for (int t = 0; t < RT; ++t)
+                            R.acc[t][c0 + c] =
+                                mfma(u32x4{a.x, a.y, b.x, b.y}, p[t][k], R.acc[t][c0 + c]);
+                    }
+            }
+            return;
+        }
         constexpr int VC = 4;  // column blocks read at once, the first before the exponentials
         u32x4 v[VC];
         auto read_some = [&](int c0) {  // piece (2 c + ..) ^ key of row `key`
@@ -574,7 +672,7 @@ __device__ __forceinline__ void accumulate(Rows<HD, RT, PACK, F32>& R,
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             exponentials(t);
-            split8(x[t], p[t]);
+            split_terms(x[t], p[t]);
             if constexpr (PACK) {
                 p[t][0] = n < 8 ? p[t][0] : p[t][1];
                 p[t][1] = n < 8 ? p[t][2] : u32x4{0u, 0u, 0u, 0u};
@@ -799,6 +897,7 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     using S = FewShape<HD, F32>;
     using KV = typename std::conditional<F32, float, uint16_t>::type;
     using P = Part<F32>;
+    constexpr Math M = F32 ? kF32 : kBf16;
     constexpr int MT = PACK ? 8 : 16, NW = S::NW, NH = P::NH, GRP = L::GRP;
     constexpr int LOADS = 2 * NH * L::LOADS;  // a block's
     constexpr int OST = HD + 4;
@@ -839,13 +938,13 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     for (int j = 0; j < 3; ++j) groups(j, gr[j]);
     // queries first: what is waited for first
     Queries<HD, 1> Q;
-    request_rows<HD, 1, PACK, F32>(a, it, g, r0, Q);
+    request_rows<HD, 1, PACK, M>(a, it, g, r0, Q);
     __builtin_amdgcn_sched_barrier(0);
     if (mine > 0) fetch(0, gr[0]);
     if (mine > 1) fetch(1, gr[1]);
     __builtin_amdgcn_sched_barrier(0);
-    Rows<HD, 1, PACK, F32> R;
-    take_rows<HD, 1, PACK, F32>(a, it, r0, Q, R);
+    Rows<HD, 1, PACK, M> R;
+    take_rows<HD, 1, PACK, M>(a, it, r0, Q, R);
     int staged = -1, raised = -1;  // the block that is there, and the last one begun again
     float x[1][P::XN];
     for (int j = 0;;) {
@@ -863,10 +962,10 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
             }
             const int va = gr[0][0].valid, vb = gr[0][NH - 1].valid;
             const bool all = s0 + P::KEYS <= it.sq.ctx && va == 16 && vb == 16;
-            scores<HD, 1, PACK, F32>(R, at, s0, it.sq.ctx, va, vb, all, x);
+            scores<HD, 1, PACK, M>(R, at, s0, it.sq.ctx, va, vb, all, x);
             move = raised != j && too_high(R, x);
             if (move) break;
-            accumulate<HD, 1, PACK, F32>(R, x, at + NH * GRP);
+            accumulate<HD, 1, PACK, M>(R, x, at + NH * GRP);
             // the block is read: its place takes the next but one
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (j + 2 < mine) fetch(j + 2, gr[2]);
@@ -935,8 +1034,11 @@ template <int HD, bool F32>
 struct TileShape {
     static constexpr int WK = 2;
     static constexpr int KB = 64 * 128 / HD / (F32 ? 2 : 1);  // keys of a block: 16 KB of each pool
-    static constexpr int BLK = KB / 16 * 2 * Lay<HD, F32>::GRP;
-    static constexpr int LDS = 2 * BLK;  // of a four: two blocks
+    static constexpr int GRP = Lay<HD, false>::GRP;  // a group in LDS, or of a plane
+    static constexpr int POOL = F32 ? 3 * kPlane : KB / 16 * GRP;
+    static_assert(!F32 || KB / 16 * GRP == kPlane, "a block's planes");
+    // of a four: two blocks, or one in three terms
+    static constexpr int LDS = F32 ? 2 * POOL : 4 * POOL;
 };
 
 template <int HD, bool F32>
@@ -944,11 +1046,12 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
     using L = Lay<HD, F32>;
     using S = TileShape<HD, F32>;
     using P = Part<F32>;
+    constexpr Math M = F32 ? kSplit : kBf16;
     using KV = typename std::conditional<F32, float, uint16_t>::type;
     // (two tiles a wave, 128 rows a workgroup: half the LDS reads, but out of
     // registers and fewer workgroups: 2048 rows after 2048 166 us, one tile 150)
     constexpr int RT = 1, NW = 4, WK = S::WK, MT = 16 * RT * NW, KB = S::KB, NG = KB / 16;
-    constexpr int GRP = L::GRP, NH = P::NH;
+    constexpr int GRP = S::GRP, NH = P::NH;
     constexpr int PART = RT * (HD / 16) * 1024 + RT * 512;  // a wave's sums on their way to join
     static_assert(NW * PART <= WK * S::LDS, "the sums fit");
     __shared__ __attribute__((aligned(1024))) char smem[WK * S::LDS];
@@ -977,21 +1080,55 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
     static_assert(NW % NG == 0 && L::LOADS % SHARE == 0, "whole loads a wave");
     const int own = wave % NG, j0 = wave / NG * LPW;
     auto group = [&](int j) { return group_at(a, b, slot_of(j) + 16 * own, k1, lgp); };
+    // bf16: to LDS, two blocks in turn. fp32: to registers; when the block before is
+    // done with, each wave splits what it has loaded, for all four.
+    u32x4 staged_x[F32 ? 2 : 1][F32 ? LPW : 1];
     auto fetch = [&](int j, const Group& gr) {
-        char* to = lds + (j & 1) * S::BLK + own * GRP;
-        fetch_group<HD, F32, LPW>(a, a.pg.k, gr, g, slot_of(j) + 16 * own, to, j0);
-        fetch_group<HD, F32, LPW>(a, a.pg.v, gr, g, slot_of(j) + 16 * own, to + NG * GRP, j0);
+        if constexpr (F32) {
+#pragma unroll
+            for (int pool = 0; pool < 2; ++pool) {
+                const __amdgpu_buffer_rsrc_t r = group_rsrc<HD, F32>(
+                    a, pool ? a.pg.v : a.pg.k, gr, g, slot_of(j) + 16 * own);
+#pragma unroll
+                for (int i = 0; i < LPW; ++i)
+                    staged_x[pool][i] = __builtin_bit_cast(
+                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                   r, ((j0 + i) * QLM_WAVE + lane) * 16, 0, 0));
+            }
+        } else {
+            char* to = lds + (j & 1) * 2 * S::POOL + own * GRP;
+            fetch_group<HD, F32, LPW>(a, a.pg.k, gr, g, slot_of(j) + 16 * own, to, j0);
+            fetch_group<HD, F32, LPW>(a, a.pg.v, gr, g, slot_of(j) + 16 * own, to + S::POOL, j0);
+        }
         if (lane == 0) there[four][j & 1][own] = gr.valid;
+    };
+    auto split_staged = [&]() {
+#pragma unroll
+        for (int pool = 0; pool < 2; ++pool)
+#pragma unroll
+            for (int i = 0; i < LPW; ++i) {
+                const int at = (j0 + i) * QLM_WAVE + lane, row = at / (HD / 4), e4 = at % (HD / 4);
+                float x4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x4[e] = __uint_as_float(staged_x[pool][i][e]);
+                u32x2 w[3];
+                split_terms(x4, w);
+                char* to = lds + pool * S::POOL + own * GRP + row * (HD * 2) +
+                           (((e4 >> 1) ^ row) * 16) + (e4 & 1) * 8;
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<u32x2*>(to + p * kPlane) = w[p];
+            }
     };
     Group gr[2] = {group(0), group(1)};
     const int w0 = uni(r0 + 16 * RT * wave);  // this wave's first row
     Queries<HD, RT> Q;
-    request_rows<HD, RT, false, F32>(a, it, g, w0, Q);
+    request_rows<HD, RT, false, M>(a, it, g, w0, Q);
     __builtin_amdgcn_sched_barrier(0);
     fetch(0, gr[0]);
     __builtin_amdgcn_sched_barrier(0);
-    Rows<HD, RT, false, F32> R;
-    take_rows<HD, RT, false, F32>(a, it, w0, Q, R);
+    Rows<HD, RT, false, M> R;
+    take_rows<HD, RT, false, M>(a, it, w0, Q, R);
     // what all of this wave's rows see without a mask, and all they can see
     const int wave_end = uni(
         w0 < total ? min(keys_end(a, it.sq, (min(w0 + 16 * RT, total) - 1) >> a.lg), k1) : 0);
@@ -1006,8 +1143,14 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
             const int j = i / SUB, h = i % SUB, s0 = slot_of(j) + P::KEYS * h;
             if (staged != j) {
                 staged = j;
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();  // the block is there, and every wave is done with the last one
+                if constexpr (F32) {
+                    __syncthreads();  // every wave is done with the last block
+                    split_staged();
+                    __syncthreads();
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    __syncthreads();  // the block is there, and every wave is done with the last
+                }
 #pragma unroll
                 for (int k = 0; k < NG; ++k) valid[k] = uni(there[four][j & 1][k]);
                 if (j + 1 < blocks) fetch(j + 1, gr[1]);
@@ -1022,11 +1165,11 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
                     vb = valid[k * NH + NH - 1];
                 }
             const bool all = s0 + P::KEYS <= free_end && va == 16 && vb == 16;
-            const char* kp = lds + (j & 1) * S::BLK + h * NH * GRP;
-            scores<HD, RT, false, F32>(R, kp, s0, it.sq.ctx, va, vb, all, x);
+            const char* kp = lds + (F32 ? 0 : (j & 1) * 2 * S::POOL) + h * NH * GRP;
+            scores<HD, RT, false, M>(R, kp, s0, it.sq.ctx, va, vb, all, x);
             move = raised != i && too_high(R, x);
             if (move) break;
-            accumulate<HD, RT, false, F32>(R, x, kp + NG * GRP);
+            accumulate<HD, RT, false, M>(R, x, kp + S::POOL);
         }
         if (!move) break;
         raise(R, x);
