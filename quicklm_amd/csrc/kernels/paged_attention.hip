@@ -32,9 +32,9 @@
 // a row sits at piece c ^ (key % 16), which spreads the 16 rows that an LDS
 // access touches over all banks.
 //
-// Lengths are known on the device alone. A launch has room for `target` + units
-// work items a kv head; each workgroup reads the lengths, forms the chunk that
-// cuts all sequences' keys into about `target` items and finds its own. A unit of
+// Lengths are known on the device alone. Each workgroup reads them, forms the
+// chunk length that cuts all sequences' keys into about `target` items a kv head,
+// and finds its own; a launch has room for as many as there can be. A unit of
 // more than one chunk leaves records [m, l, O] that k_pa_join merges; the others
 // write their outputs.
 
@@ -102,37 +102,48 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
+// Sequences that are all about as long are cut so that every CU has one item: 64
+// single tokens after 4096 slots 99 us (16 / 4 heads of 128, bf16), in twice as
+// many 104; one after 32768 26 and 36. Where the longest is well above the mean
+// one item a CU leaves most of them waiting for it: half as many items again, 64
+// after 256 to 8192 slots 108 us, 126 without, 120 with twice as many.
+constexpr float kUneven = 2.0f / 3.0f;
+
 // Item `want` of a kv head, counted over the sequences: the longest prompts'
 // last tiles, which see the most keys, first. Every lane gets it. Sums that
 // only say how long a chunk is are in fp32, the same in every wave.
 template <int MT>
 __device__ __forceinline__ bool find_item(const PaArgs& a, int want, Item& it) {
     const int lane = threadIdx.x & (QLM_WAVE - 1), B = a.bt.B;
-    float cost = 0.0f, longest = 0.0f;
+    float cost = 0.0f, longest = 0.0f, units = 0.0f;
     SeqRows s{};
     for (int i = 0; i < B; i += QLM_WAVE) {
         s = seq_rows(a.bt, min(i + lane, B - 1));
         if (i + lane >= B) s.n = 0;
         if (s.n > 0) {
             const float keys = (float)min(s.ctx + seen_rows(a, s), a.slots);
-            cost += (float)tiles_of(s.n, a.lg, MT) * keys;
+            const float tiles = (float)tiles_of(s.n, a.lg, MT);
+            cost += tiles * keys;
+            units += tiles;
             longest = fmaxf(longest, keys);
         }
     }
-    const float share = wave_sum(cost) / (float)a.target;
-    it.len = uni(min((int)fminf(share, (float)(1 << 29)) / 32 * 32 + 32, 1 << 29));
-    it.len = max(it.len, wave_max(longest) <= (float)a.alone ? a.alone : a.least);
-    it.len = uni(it.len);
+    cost = wave_sum(cost);
+    longest = wave_max(longest);
+    float share = cost / (float)a.target;
+    if (MT <= 16 && longest * wave_sum(units) > 1.5f * cost) share *= kUneven;
+    int len = uni(min((int)fminf(share, (float)(1 << 29)) / 32 * 32 + 32, 1 << 29));
+    len = uni(max(len, longest <= (float)a.alone ? a.alone : a.least));
     int before = 0, rec = 0;
     for (int i = 0; i < B; i += QLM_WAVE) {
         if (B > QLM_WAVE) {
             s = seq_rows(a.bt, min(i + lane, B - 1));
             if (i + lane >= B) s.n = 0;
         }
-        int items = 0, recs = 0;
+        int items = 0, recs = 0, keys = 0;
         if (s.n > 0) {
-            const int keys = min(s.ctx + seen_rows(a, s), a.slots);
-            const int nch = (keys - 1) / it.len + 1;
+            keys = min(s.ctx + seen_rows(a, s), a.slots);
+            const int nch = (keys - 1) / len + 1;
             items = tiles_of(s.n, a.lg, MT) * nch;
             recs = nch > 1 ? items : 0;
         }
@@ -145,6 +156,7 @@ __device__ __forceinline__ bool find_item(const PaArgs& a, int want, Item& it) {
             it.sq = SeqRows{of(s.first), of(s.n), of(s.ctx)};
             const int mine = want - before - of(ic - items);
             const int tiles = tiles_of(it.sq.n, a.lg, MT), nch = of(items) / tiles;
+            it.len = ((of(keys) + nch - 1) / nch + 31) / 32 * 32;  // all about as long
             it.chunk = mine % nch;
             it.tile = tiles - 1 - mine / nch;
             it.rec = rec + of(rc - recs) + mine - it.chunk;
@@ -1340,14 +1352,15 @@ PaPlan plan_of(int rows, int B, int G, int n_kv, int hd, long long slots) {
     // about the rows of a sequence
     const long long per = ((long long)rows * G + B - 1) / B;
     p.mt = per <= 8 ? 8 : per <= 16 ? 16 : 64;
-    const int wanted = p.mt <= 16 ? 512 : 256;  // a CU holds one workgroup of either
-    p.target = std::max(1, wanted / n_kv);
+    p.target = std::max(1, 256 / n_kv);  // a CU holds one workgroup
     const long long units = ((long long)rows * G) / p.mt + B;
-    p.items = (int)(units + p.target + 8);  // (8: what fp32 sums may be off by)
+    const long long most = p.mt <= 16 ? p.target + p.target / 2 + 1 : p.target;  // items but those
     p.alone = p.mt <= 16 ? 1024 : 128;
     p.least = p.mt <= 16 ? 256 : 128;
     p.join = slots > p.alone;
-    if (p.join) p.rec_rows = (2 * p.target + 16) * n_kv * p.mt;
+    // (8: what fp32 sums may be off by)
+    p.items = (int)std::min(units + most + 8, units * (p.join ? (slots - 1) / p.least + 1 : 1));
+    if (p.join) p.rec_rows = (int)(2 * most + 16) * n_kv * p.mt;
     const size_t rec = (size_t)p.rec_rows * (hd + 4) * sizeof(float);
     p.desc_at = rec;
     p.bytes = p.join ? rec + (size_t)rows * n_kv * sizeof(int2) : 0;
