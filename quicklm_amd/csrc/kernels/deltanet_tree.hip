@@ -28,7 +28,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct TreeArgs {
     const float* proj;
-    const float* conv;  // [B, 3, 3 H d]
+    const float* conv;  // [B, 3, 3 H d], read, or advanced (commit)
     const float* wt;    // [4, 3 H d]
     const float* A_log;
     const float* dt_bias;
@@ -164,6 +164,20 @@ __device__ __forceinline__ void put_head(const TreeArgs& a, int row, int h, bool
     const float sn = 1.0f / sqrtf(wave_sum(fmaf(o0, o0, o1 * o1)) / (float)kD + 1e-6f);
     to[0] = live ? (o0 * sn) * a.norm_w[lane] * silu_f(z0) : 0.0f;
     to[64] = live ? (o1 * sn) * a.norm_w[lane + 64] * silu_f(z1) : 0.0f;
+}
+
+// A channel of a sequence's ring (cs): the last three of (the ring's three, the
+// path's T inputs), put where position ctx_len + accepted expects them.
+template <typename F>
+__device__ __forceinline__ void advance_ring(const TreeArgs& a, float* cs, int C, int ctx, int T,
+                                             int ch, F row_of) {
+    float x[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j)  // place T + j of that line
+        x[j] = T + j >= 3 ? a.proj[(size_t)row_of(T + j - 3) * a.ldp + ch]
+                          : cs[(size_t)((ctx % 3 + T + j) % 3) * C];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) cs[(size_t)((ctx % 3 + T + j) % 3) * C] = x[j];
 }
 
 template <int TM, int NC, bool COMMIT>
@@ -469,6 +483,13 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                 for (int i = 0; i < 4; ++i) at[(size_t)i * kD] = x[i];
             }
         }
+        if constexpr (NC == 8) {  // nobody else reads these channels of the ring
+            static_assert(3 * kD <= kThreads, "a thread a channel");
+            const int own = (tid / kD) * HD + h * kD + tid % kD;
+            if (tid < 3 * kD)
+                advance_ring(a, const_cast<float*>(cs) + own, C, sq.ctx, T, own,
+                             [&](int i) { return sh.row[i]; });
+        }
         return;
     }
     // ---- outputs: the state's part, and what the nodes above have added ----
@@ -622,10 +643,9 @@ __global__ __launch_bounds__(kNormThreads) void k_dn_tree_norm(TreeArgs a) {
     }
 }
 
-// The rings' advance: the last three of (the ring's three, the path's inputs),
-// put where position ctx_len + accepted expects them. After k_dn_tree, whose
-// workgroups all read the old ring.
-__global__ __launch_bounds__(kThreads) void k_dn_tree_ring(TreeArgs a, float* conv) {
+// The rings' advance where a head's columns are several workgroups': after
+// k_dn_tree, whose workgroups all read the old ring.
+__global__ __launch_bounds__(kThreads) void k_dn_tree_ring(TreeArgs a) {
     const int b = blockIdx.y, C = 3 * a.H * kD;
     const SeqRows sq = seq_rows(a.bt, b);
     int p;
@@ -633,17 +653,11 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree_ring(TreeArgs a, float* co
     if (T == 0) return;
     int row[3];
 #pragma unroll
-    for (int j = 0; j < 3; ++j) row[j] = T + j >= 3 ? sq.first + __shfl(p, max(T + j - 3, 0)) : -1;
-    const int ch = blockIdx.x * kThreads + threadIdx.x, ctx = sq.ctx % 3;
-    if (ch >= C) return;
-    float* cs = conv + (size_t)b * 3 * C + ch;
-    float x[3];
-#pragma unroll
-    for (int j = 0; j < 3; ++j)  // place T + j of that line
-        x[j] = row[j] >= 0 ? a.proj[(size_t)row[j] * a.ldp + ch]
-                           : cs[(size_t)((ctx + T + j) % 3) * C];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) cs[(size_t)((ctx + T + j) % 3) * C] = x[j];
+    for (int j = 0; j < 3; ++j) row[j] = sq.first + __shfl(p, max(T + j - 3, 0));
+    const int ch = blockIdx.x * kThreads + threadIdx.x;
+    if (ch < C)
+        advance_ring(a, const_cast<float*>(a.conv) + (size_t)b * 3 * C + ch, C, sq.ctx, T, ch,
+                     [&](int i) { return row[i - T + 3]; });
 }
 
 template <int TM, int NC, bool COMMIT>
@@ -739,9 +753,9 @@ extern "C" int qlm_deltanet_tree_commit(const float* proj, int ldp, const qlm_ro
                      nullptr, path,     accepted, ldp, 0, H, ld_path, 0, *batch};
     hipStream_t st = as_stream(stream);
     const int r = launch_nodes<true>(a, st);
-    if (r != QLM_OK) return r;
+    if (r != QLM_OK || columns_of((long long)H * batch->B) == 8) return r;
     hipLaunchKernelGGL(k_dn_tree_ring, dim3((3 * H * d + kThreads - 1) / kThreads, batch->B),
-                       dim3(kThreads), 0, st, a, conv_state);
+                       dim3(kThreads), 0, st, a);
     return qlm_launch_status();
 }
 
