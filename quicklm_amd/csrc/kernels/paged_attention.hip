@@ -365,15 +365,16 @@ __device__ __forceinline__ void request_rows(const PaArgs& a, const Item& it, in
     }
 }
 
-// What the rows see, and their queries' terms.
+// What the rows see, and their queries' terms. parent: of the sequence's row `lane`,
+// requested ahead of the keys (loads come back in order).
 template <int HD, int RT, bool PACK, Math M>
-__device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r0,
+__device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r0, int parent,
                                           const Queries<HD, RT>& Q, Rows<HD, RT, PACK, M>& R) {
     using T = Rows<HD, RT, PACK, M>;
-    const int lane = threadIdx.x & (QLM_WAVE - 1), n = lane & 15;
+    const int n = threadIdx.x & 15;
     const int total = it.sq.n << a.lg;
     unsigned long long mine = 0;
-    if (a.bt.parent) mine = tree_line(tree_parent(a.bt, it.sq, lane));
+    if (a.bt.parent) mine = tree_line(parent);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int tok = min(r0 + 16 * t + (PACK ? n & 7 : n), total - 1) >> a.lg;
@@ -945,6 +946,7 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
             fetch_group<HD, F32>(a, a.pg.v, gr[h], g, slot_of(j) + 16 * h, to + (NH + h) * GRP);
         }
     };
+    const int parent = a.bt.parent ? tree_parent(a.bt, it.sq, lane) : 0;
     Group gr[3][NH];  // of blocks j, j + 1 and j + 2
 #pragma unroll
     for (int j = 0; j < 3; ++j) groups(j, gr[j]);
@@ -956,7 +958,7 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
     if (mine > 1) fetch(1, gr[1]);
     __builtin_amdgcn_sched_barrier(0);
     Rows<HD, 1, PACK, M> R;
-    take_rows<HD, 1, PACK, M>(a, it, r0, Q, R);
+    take_rows<HD, 1, PACK, M>(a, it, r0, parent, Q, R);
     int staged = -1, raised = -1;  // the block that is there, and the last one begun again
     float x[1][P::XN];
     for (int j = 0;;) {
@@ -1132,6 +1134,7 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
                     *reinterpret_cast<u32x2*>(to + p * kPlane) = w[p];
             }
     };
+    const int parent = a.bt.parent ? tree_parent(a.bt, it.sq, lane) : 0;
     Group gr[2] = {group(0), group(1)};
     const int w0 = uni(r0 + 16 * RT * wave);  // this wave's first row
     Queries<HD, RT> Q;
@@ -1140,7 +1143,7 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
     fetch(0, gr[0]);
     __builtin_amdgcn_sched_barrier(0);
     Rows<HD, RT, false, M> R;
-    take_rows<HD, RT, false, M>(a, it, w0, Q, R);
+    take_rows<HD, RT, false, M>(a, it, w0, parent, Q, R);
     // what all of this wave's rows see without a mask, and all they can see
     const int wave_end = uni(
         w0 < total ? min(keys_end(a, it.sq, (min(w0 + 16 * RT, total) - 1) >> a.lg), k1) : 0);
