@@ -17,6 +17,11 @@
 // columns. Products run on the fp32 matrix cores. Logarithms of the decays are
 // summed in 64 bits along each line: a ratio of two products far below the fp32
 // range is as good as any other.
+//
+// Bound by the phases that wait for each other, of which a workgroup a CU overlaps
+// none: 16 trees of up to 64 nodes, 16 heads, take 46 us, a quarter of that the
+// state's products; their 36 MB alone would take 8. One tree of 16 nodes 13 us, 16
+// accepted paths' commit 17.
 
 #include "paged.hpp"
 
@@ -670,8 +675,8 @@ int launch_tree(const TreeArgs& a, hipStream_t st) {
 
 // Column tiles of a workgroup: the fewest that need no more workgroups than CUs,
 // since all of a head repeat its convolutions and its nodes' products (16 heads,
-// trees of 64, us with 1, 2, 4 and 8: 2 sequences 28, 29, 34, 45; 4 49, 31, 36, 46;
-// 8 93, 56, 39, 47; 16 181, 106, 72, 50).
+// trees of 64, us with 1, 2, 4 and 8: 2 sequences 27, 27, 33, 44; 4 50, 30, 35, 44;
+// 8 94, 56, 39, 46; 16 182, 106, 73, 50).
 int columns_of(long long heads) {
     return heads > 128 ? 8 : heads > 64 ? 4 : heads > 32 ? 2 : 1;
 }

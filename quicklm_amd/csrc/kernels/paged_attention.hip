@@ -37,6 +37,12 @@
 // and finds its own; a launch has room for as many as there can be. A unit of
 // more than one chunk leaves records [m, l, O] that k_pa_join merges; the others
 // write their outputs.
+//
+// Measured with 16 / 4 heads of 128, bf16: 64 single tokens after 256 to 8192 slots
+// 109 us, bound by HBM (5.1 TB/s); 2048 rows after 2048 148 us, bound by the matrix
+// cores (1050 TFLOP/s of bf16 products, half of their cycles in the key loop); 8 trees of 64
+// nodes after 4032 65 us, of which 13 are the start and the join; one token after
+// 600 11 us, latency.
 
 #include <algorithm>
 
