@@ -18,6 +18,7 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kAppendThreads = 256;
+constexpr int kScalarAxes = 4;  // axes whose positions are read ahead
 
 struct AppendArgs {
     const float* qkv;
@@ -34,8 +35,9 @@ struct AppendArgs {
 // Groups of HD / 4 lanes take K heads each of the row blockIdx.x, four elements a
 // lane: query heads first, then keys, then values. Few rows: K = 1, a workgroup
 // for each few heads. Many: K = 3, all requested before the row's sequence is
-// looked up, which three heads then share (2048 rows of 16 + 2 x 4 heads of 128
-// into a bf16 cache, 46 MB: 21.9 us with K = 1, 14.9 with 3; of 512 9.4 and 9.3).
+// looked up, which three heads then share (16 + 2 x 4 heads of 128 into a bf16
+// cache, K = 1 and 3: 340 rows 5.2 and 6.1 us, 600 7.2 and 7.0, 2048 15.8 and 12.2,
+// 46 MB at 3.7 TB/s).
 template <int HD, typename KV, int K>
 __global__ __launch_bounds__(kAppendThreads) void k_paged_append(AppendArgs a) {
     constexpr int LPH = HD / 4, HPB = kAppendThreads / LPH;  // lanes a head, heads at once
@@ -43,6 +45,22 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append(AppendArgs a) {
     const int grp = threadIdx.x / LPH, l = threadIdx.x % LPH, e0 = 4 * l;
     const int row = blockIdx.x, n_kv = a.pg.n_kv, heads = a.n_q + 2 * n_kv;
     const float* xr = a.qkv + (size_t)row * a.ldqkv;
+    // vector loads come back in order: what leads to the angles is asked for ahead of
+    // the row, or through the scalar cache
+    const int half = a.rot / 2;
+    const int start0 = a.bt.row_start[min((int)(threadIdx.x & (QLM_WAVE - 1)), a.bt.B)];
+    // (and none of them under a branch, behind which the compiler waits for all that
+    // the shortest way there has asked for: something else is read instead)
+    const bool has_axis = a.positions && a.pair_axis && half > 0;
+    const int* const axes = has_axis ? a.pair_axis : a.bt.row_start;
+    int pair[4], axis[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = max(min(e0 + j, a.rot - 1), 0);
+        pair[j] = e < half ? e : e - half;
+        axis[j] = axes[has_axis ? pair[j] : 0];
+    }
+    __builtin_amdgcn_sched_barrier(0);
     f32x4u v[K], gn[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -51,14 +69,26 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append(AppendArgs a) {
         const size_t at = hc < a.n_q ? (size_t)hc * a.q_stride
                                      : (size_t)a.n_q * a.q_stride + (size_t)(hc - a.n_q) * HD;
         v[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4u*>(xr + at + e0));
-        const float* gain = hc < a.n_q ? a.qn : hc < a.n_q + n_kv ? a.kn : nullptr;
-        gn[k] = f32x4u{0.0f, 0.0f, 0.0f, 0.0f};
-        if (gain) gn[k] = *reinterpret_cast<const f32x4u*>(gain + e0);
     }
-
-    const int b = seq_of_row(a.bt, row);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int hc = min((int)(blockIdx.y * K + k) * HPB + grp, heads - 1);
+        const float* gain = hc < a.n_q ? a.qn : a.kn;
+        gn[k] = *reinterpret_cast<const f32x4u*>((gain ? gain : xr) + e0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    int at_axis[kScalarAxes];
+    if (a.positions) {
+#pragma unroll
+        for (int x = 0; x < kScalarAxes; ++x)
+            at_axis[x] = uniform_load(a.positions, (size_t)min(x, a.n_axes - 1) * a.ld_pos + row);
+    }
+    const int b = __builtin_amdgcn_readfirstlane(seq_of_row(a.bt, row, start0));
     if (b < 0) return;  // the whole workgroup
-    const SeqRows sq = seq_rows(a.bt, b);
+    const int first = min(max(uniform_load(a.bt.row_start, b), 0), a.bt.rows);
+    const int end = min(max(uniform_load(a.bt.row_start, b + 1), 0), a.bt.rows);
+    const int ctx = min(max(uniform_load(a.bt.ctx_len, b), 0), 1 << 30);
+    const SeqRows sq{first, max(end - first, 0), ctx};
     const int i = row - sq.first;
     if (i < 0 || i >= sq.n) return;
     const int slot_page = page_of(a.pg, b, sq.ctx + i);
@@ -73,27 +103,38 @@ __global__ __launch_bounds__(kAppendThreads) void k_paged_append(AppendArgs a) {
         depth = __popcll(mine) - 1;
     }
     // the angles of this lane's elements, the same for every head
-    const int half = a.rot / 2;
-    float c4[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (e0 < a.rot) {
+    float c4[4], s4[4];
+    if (half > 0) {
+        int pos[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pos[j] = sq.ctx + depth;
+        if (a.positions) {
+            bool there[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                axis[j] = has_axis ? axis[j] : 0;
+                there[j] = axis[j] >= 0 && axis[j] < a.n_axes;
+                pos[j] = at_axis[0];
+#pragma unroll
+                for (int x = 1; x < kScalarAxes; ++x) pos[j] = axis[j] == x ? at_axis[x] : pos[j];
+            }
+            if (a.n_axes > kScalarAxes) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    pos[j] = a.positions[(size_t)(there[j] ? axis[j] : 0) * a.ld_pos + row];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pos[j] = there[j] ? pos[j] : -1;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int e = e0 + j;
-            if (e >= a.rot) break;
-            const int pair = e < half ? e : e - half;
-            int pos = sq.ctx + depth, axis = 0;
-            if (a.positions) {
-                if (a.pair_axis) axis = a.pair_axis[pair];
-                const bool there = axis >= 0 && axis < a.n_axes;
-                pos = a.positions[(size_t)(there ? axis : 0) * a.ld_pos + row];
-                if (!there) pos = -1;
-            }
-            c4[j] = s4[j] = NAN;  // no angle
-            if (pos >= 0 && pos < a.n_pos) {
-                c4[j] = a.cos_tab[(size_t)pos * half + pair];
-                s4[j] = a.sin_tab[(size_t)pos * half + pair];
-            }
+            const size_t at = (size_t)min(max(pos[j], 0), a.n_pos - 1) * half + pair[j];
+            c4[j] = a.cos_tab[at];
+            s4[j] = a.sin_tab[at];
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (pos[j] < 0 || pos[j] >= a.n_pos) c4[j] = s4[j] = NAN;  // no angle
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {

@@ -20,17 +20,29 @@ __device__ __forceinline__ SeqRows seq_rows(const qlm_row_batch& bt, int b) {
 }
 
 // The sequence of row r: the last b < B with row_start[b] <= r, or -1 for a row
-// that no sequence owns. The whole wave takes part.
-__device__ __forceinline__ int seq_of_row(const qlm_row_batch& bt, int r) {
+// that no sequence owns. The whole wave takes part. start0: row_start[min(lane, B)].
+__device__ __forceinline__ int seq_of_row(const qlm_row_batch& bt, int r, int start0) {
     const int lane = threadIdx.x & (QLM_WAVE - 1);
     int count = 0;  // entries of row_start[0..B] that are <= r
     for (int i = 0; i <= bt.B; i += QLM_WAVE) {
-        const int e = bt.row_start[min(i + lane, bt.B)];
+        const int e = i ? bt.row_start[min(i + lane, bt.B)] : start0;
         const int c = __popcll(__ballot(i + lane <= bt.B && max(e, 0) <= r));
         count += c;
         if (c < QLM_WAVE) break;
     }
     return count > 0 && count <= bt.B ? count - 1 : -1;
+}
+
+__device__ __forceinline__ int seq_of_row(const qlm_row_batch& bt, int r) {
+    return seq_of_row(bt, r, bt.row_start[min((int)(threadIdx.x & (QLM_WAVE - 1)), bt.B)]);
+}
+
+// p[i], i the same in all lanes, through the scalar cache: memory that the launch
+// does not write.
+__device__ __forceinline__ int uniform_load(const int* p, size_t i) {
+    const auto* q = reinterpret_cast<const __attribute__((address_space(4))) int*>(
+        reinterpret_cast<uintptr_t>(p));
+    return q[i];
 }
 
 // The tree over a sequence's first QLM_TREE_MAX rows, one row a lane: the line

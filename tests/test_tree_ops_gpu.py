@@ -133,6 +133,15 @@ def test_append(hip, rng, hd, bf16, n_q, n_kv, gated, rot, axes, norm):
     check_append(rows, pages, got, pools, inp, n_q, gated, rot)
 
 
+@pytest.mark.parametrize("axes", [4, 5, 9])
+def test_append_many_axes(hip, rng, axes):
+    say(f"append axes={axes}")
+    rows = Rows(hip, [5, 2], [3, 40])
+    pages = Pages(hip, rng, [8, 42], 1, 128, 16, True, filled=[3, 40])
+    got, pools, inp = run_append(hip, rng, rows, pages, 2, False, 64, axes)
+    check_append(rows, pages, got, pools, inp, 2, False, 64)
+
+
 @pytest.mark.parametrize("page", [16, 64, 256])
 def test_append_trees(hip, rng, page):
     """Positions are the context and the depth; rows outside the tree (padding,
