@@ -213,10 +213,7 @@ struct Group {
 __device__ __forceinline__ Group group_at(const PaArgs& a, int b, int slot, int end, int lgp) {
     const int i = slot >> lgp;
     const bool in = slot < end && i < a.pg.ld_table;
-    // a scalar load: of the constant address space
-    const auto* table = reinterpret_cast<const __attribute__((address_space(4))) int*>(
-        reinterpret_cast<uintptr_t>(a.pg.table));
-    const int p = table[(size_t)b * a.pg.ld_table + (in ? i : 0)];
+    const int p = uniform_load(a.pg.table, (size_t)b * a.pg.ld_table + (in ? i : 0));
     Group g;
     g.valid = uni(in && (unsigned)p < (unsigned)a.pg.n_pages ? min(end - slot, 16) : 0);
     g.page = uni(g.valid > 0 ? p : 0);
