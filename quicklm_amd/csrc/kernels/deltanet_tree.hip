@@ -66,20 +66,12 @@ struct TreeShared {
     int bad;              // >= 0: outputs that did not come out finite
 };
 
-// x / (1 + exp(-x)) to four roundings: v_exp_f32 of the product with log2 e, whose
-// own rounding error is put back, v_rcp_f32 and a Newton step, instead of expf
-// and a division (half the conv's instructions). Below -80 the exponential
-// stays at exp(80): what is left is less than 1e-32.
-__device__ __forceinline__ float silu_fast(float x) {
-    constexpr float kLog2e = 1.44269502e0f, kLn2 = 0.693147182f;
-    const float c = fmaxf(x, -80.0f), hi = c * -kLog2e;
-    const float lo = fmaf(c, -1.92596303e-8f, fmaf(c, -kLog2e, -hi));
-    float e = __builtin_amdgcn_exp2f(hi);
-    e = fmaf(e * kLn2, lo, e);
-    const float d = 1.0f + e;
-    float r = __builtin_amdgcn_rcpf(d);
-    r = fmaf(fmaf(-d, r, 1.0f), r, r);
-    return x * r;
+// SiLU of a convolution's sum (silu_f's expf and division were half of the
+// convolutions' instructions). Below kDeepGate 0, less than 2e-33 off; of -inf, as
+// silu_f has it, NaN.
+__device__ __forceinline__ float silu_conv(float x) {
+    const float y = silu_fast(x);
+    return x < kDeepGate ? x * 0.0f : y;
 }
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
@@ -334,7 +326,7 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                     float acc = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc = fmaf(x[i][j], w4[j], acc);
-                    y[i0 + i] = 2 * (i0 + i) + hf < T ? silu_fast(acc) : 0.0f;
+                    y[i0 + i] = 2 * (i0 + i) + hf < T ? silu_conv(acc) : 0.0f;
                 }
             } else {
 #pragma unroll
@@ -349,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             acc = fmaf(sh.w[tp.y][vc], vw[1], acc);
             acc = fmaf(sh.w[tp.z][vc], vw[2], acc);
             acc = fmaf(sh.w[tp.w][vc], vw[3], acc);
-            yv[j] = i < T ? silu_fast(acc) : 0.0f;
+            yv[j] = i < T ? silu_conv(acc) : 0.0f;
         }
         __syncthreads();
 #pragma unroll
@@ -604,7 +596,7 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
                                             : cs[(size_t)(tp - TM) * C + vch];
                     acc = fmaf(x, a.wt[(size_t)e * C + vch], acc);
                 }
-                const float w = sh.beta[u] * (silu_fast(acc) - sum);
+                const float w = sh.beta[u] * (silu_conv(acc) - sum);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[e] = fmaf(sh.k[u][8 * i8 + e] * sh.sk[u], w, s[e]);
             }

@@ -1,0 +1,67 @@
+"""Edges of the paged attention and of the DeltaNet mixer over trees: scores and
+convolutions at the ends of fp32's range, whatever lies in slots that nobody sees,
+contexts that are cut and joined, and every form that a call can take. Against
+the definitions in 64 bits, or against the framework's row-by-row mixer where that
+is what the operators promise; tolerances are those of test_tree_ops_gpu.py."""
+
+import numpy as np
+import pytest
+
+from tests.test_tree_ops_gpu import (DN_TOL, buf, check_attention, check_tree, dn_inputs,
+                                     run_attention, run_tree)
+from tests.tree_util import Pages, Rows, deltanet_ref, lines, random_tree
+from tests.util import say
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- DeltaNet: convolutions at the ends of the range ------------------------------
+
+
+def prefill(hip, inp, T, H, ctx):
+    """Outputs, state and ring that the framework's row-by-row mixer leaves."""
+    d = {k: buf(hip, v) for k, v in inp.items()}
+    out = buf(hip, np.zeros((T, H * 128), np.float32))
+    hip.call("qlm_deltanet_prefill", d["proj"], inp["proj"].shape[1], T, d["conv"], d["conv_w"],
+             d["A_log"], d["dt"], d["norm"], d["state"], ctx, out, H * 128, H, 128, None)
+    return (out.to_numpy((T, H * 128), np.float32),
+            d["state"].to_numpy(inp["state"].shape, np.float32),
+            d["conv"].to_numpy(inp["conv"].shape, np.float32))
+
+
+def commit_chain(hip, rows, inp, T, H):
+    path = np.full((1, 64), -1, np.int32)
+    path[0, :T] = np.arange(T)
+    d = {k: buf(hip, v) for k, v in inp.items()}
+    hip.call("qlm_deltanet_tree_commit", d["proj"], inp["proj"].shape[1], rows.c, buf(hip, path),
+             64, buf(hip, np.array([T], np.int32)), d["conv"], d["conv_w"], d["A_log"], d["dt"],
+             d["state"], H, 128, None)
+    return (d["state"].to_numpy(inp["state"].shape, np.float32),
+            d["conv"].to_numpy(inp["conv"].shape, np.float32))
+
+
+def sums_of(rng, rows, H, part, values):
+    """Inputs whose convolution of channel 5 of head 0 of `part` is values[i] at
+    node i."""
+    inp = dn_inputs(rng, rows, H, 1)
+    ch = "qkv".index(part) * H * 128 + 5
+    inp["conv_w"][:, ch] = [0, 0, 0, 1]
+    for i, x in values.items():
+        inp["proj"][i, ch] = x
+    return inp
+
+
+@pytest.mark.parametrize("H", [1, 140])
+@pytest.mark.parametrize("part", ["q", "k", "v"])
+@pytest.mark.parametrize("value", [2.5e38, 1e30, -1e25, -1e36, -2.5e38])
+def test_deltanet_large_convolutions(hip, rng, H, part, value):
+    """SiLU of a sum far from 0 is the sum or 0, as the row-by-row mixer has it."""
+    T, ctx = 7, 5
+    say(f"deltanet conv {part} = {value} H={H}")
+    rows = Rows(hip, [T], [ctx])
+    inp = sums_of(rng, rows, H, part, {2: value})
+    want, _, _ = prefill(hip, inp, T, H, ctx)
+    assert np.isfinite(want).all()
+    got = run_tree(hip, rows, inp, H)
+    for a, b in zip(got.reshape(T, H, 128), want.reshape(T, H, 128)):
+        assert (np.abs(a - b).max(1) <= 2 * DN_TOL * np.abs(b).max(1)).all()
