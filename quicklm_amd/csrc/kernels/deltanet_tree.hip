@@ -351,7 +351,10 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
             if (v_on) sh.w[vg + j * VG][vc] = yv[j];
     }
     __syncthreads();
-    // ---- norms: four threads a node ----
+    // ---- norms: four threads a node. Vectors are normalised in their products, but
+    // those so long that a product of two might leave the range at once (an infinite
+    // length leaves 0) ----
+    constexpr float kShort = 1e-15f;
     static_assert(kThreads / 4 >= QLM_TREE_MAX, "every node");
     if (const int i = tid / 4; i < TM) {
         float s0 = 0.0f, s1 = 0.0f;
@@ -368,9 +371,20 @@ __global__ __launch_bounds__(kThreads) void k_dn_tree(TreeArgs a) {
         }
         s0 = group_sum<4>(s0);
         s1 = group_sum<4>(s1);
+        s0 = 1.0f / sqrtf(s0 + 1e-6f);
+        s1 = 1.0f / sqrtf(s1 + 1e-6f);
+        if (s0 < kShort || s1 < kShort) {
+            auto shorten = [&](float* x, float& by) {
+                if (!(by < kShort)) return;
+                for (int e = tid & 3; e < kD; e += 4) x[e] *= by;
+                by = 1.0f;
+            };
+            shorten(sh.q[i], s0);
+            shorten(sh.k[i], s1);
+        }
         if ((tid & 3) == 0) {
-            sh.sq[i] = 1.0f / sqrtf(s0 + 1e-6f);
-            sh.sk[i] = 1.0f / sqrtf(s1 + 1e-6f);
+            sh.sq[i] = s0;
+            sh.sk[i] = s1;
         }
     }
     __syncthreads();

@@ -65,3 +65,24 @@ def test_deltanet_large_convolutions(hip, rng, H, part, value):
     got = run_tree(hip, rows, inp, H)
     for a, b in zip(got.reshape(T, H, 128), want.reshape(T, H, 128)):
         assert (np.abs(a - b).max(1) <= 2 * DN_TOL * np.abs(b).max(1)).all()
+
+
+@pytest.mark.parametrize("H", [1, 140])
+@pytest.mark.parametrize("part", ["q", "k"])
+def test_deltanet_vectors_whose_squares_leave_the_range(hip, rng, H, part):
+    """Their l2 norm is infinite: the row-by-row mixer's vector is 0 then, and the
+    state goes on."""
+    T, ctx = 9, 4
+    say(f"deltanet large {part} H={H}")
+    rows = Rows(hip, [T], [ctx])
+    inp = sums_of(rng, rows, H, part, {2: 1e25, 4: 3e22, 5: 1e18, 7: 2e38})
+    inp["state"][0, 0, 5] *= 1e3  # (1e25 times it times 1e18 is past the range too)
+    want, state, conv = prefill(hip, inp, T, H, ctx)
+    assert np.isfinite(want).all() and np.isfinite(state).all()
+    got = run_tree(hip, rows, inp, H)
+    for a, b in zip(got.reshape(T, H, 128), want.reshape(T, H, 128)):
+        assert (np.abs(a - b).max(1) <= 2 * DN_TOL * np.abs(b).max(1)).all()
+    got, ring = commit_chain(hip, rows, inp, T, H)
+    err = np.abs(got - state).max((0, 2, 3))
+    assert (err <= 2 * DN_TOL * np.abs(state).max((0, 2, 3))).all()
+    assert np.array_equal(ring, conv)
