@@ -263,6 +263,10 @@ template <typename T>
 __device__ __forceinline__ T lds_read(uint32_t at) {
     return *(__attribute__((address_space(3))) const T*)(uintptr_t)at;
 }
+template <typename T>
+__device__ __forceinline__ void lds_write(uint32_t at, T v) {
+    *(__attribute__((address_space(3))) T*)(uintptr_t)at = v;
+}
 
 // N floats (four, eight) as three bf16 terms each (24 bits: exact). What a term
 // leaves is x - h, exact: one product with -1 and its sum with x (v_dot2_f32_bf16)
@@ -342,6 +346,7 @@ struct Rows {
     int high[RT];         // bits of the relative score that moves it: kRise, at first any
     int lim[RT];  // slots below this one are seen; -1: a row outside the tree
     unsigned long long line[RT];  // new rows seen beside those
+    unsigned long long unseen;    // new rows that no row sees, the same in all lanes
 };
 
 // Query rows r0 + 16 t + n of the unit (r: its token and head): requested here.
@@ -377,7 +382,11 @@ __device__ __forceinline__ void take_rows(const PaArgs& a, const Item& it, int r
     const int n = threadIdx.x & 15;
     const int total = it.sq.n << a.lg;
     unsigned long long mine = 0;
-    if (a.bt.parent) mine = tree_line(parent);
+    R.unseen = 0;
+    if (a.bt.parent) {
+        mine = tree_line(parent);
+        R.unseen = __ballot((int)(threadIdx.x & (QLM_WAVE - 1)) < it.sq.n && mine == 0);
+    }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int tok = min(r0 + 16 * t + (PACK ? n & 7 : n), total - 1) >> a.lg;
@@ -428,13 +437,38 @@ __device__ __forceinline__ void fresh(uint32_t& x) {
     if constexpr (HD > 128) asm volatile("" : "+v"(x));
 }
 
+// Zeros over the values of new rows that no row sees, of the part from slot k0 on
+// at vp. A padding row's slot is never written, and a probability of 0 times a NaN
+// that happens to lie there would be one. Waves that share the part all write
+// these zeros, each before it reads them.
+template <int HD, Math M>
+__device__ __forceinline__ void clear_unseen(unsigned long long unseen, const char* vp, int k0,
+                                             int ctx) {
+    using L = Lay<HD, M == kF32>;
+    constexpr int KEYS = Part<M != kBf16>::KEYS;
+    const int r0 = k0 - ctx;  // the part's first slot as a new row
+    if (unseen == 0 || r0 <= -KEYS || r0 >= QLM_TREE_MAX) return;
+    unsigned left = (unsigned)(r0 < 0 ? unseen << -r0 : unseen >> r0) & (0xffffffffu >> (32 - KEYS));
+    uint32_t at = lds_at(vp) + (threadIdx.x & (QLM_WAVE - 1)) * 4, zero = 0u;
+    asm volatile("" : "+v"(at), "+v"(zero));  // (not held over the loop either)
+    for (; left; left &= left - 1) {
+        const uint32_t row = at + (__ffs((int)left) - 1) * L::ROW;
+#pragma unroll
+        for (int p = 0; p < (M == kSplit ? 3 : 1); ++p)
+#pragma unroll
+            for (int e = 0; e < L::ROW; e += 4 * QLM_WAVE)
+                lds_write(row + p * kPlane + e, zero);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
 // Scores of a part of the keys, from slot k0 on, relative to the references, of
-// keys that a row does not see -inf: x[t][4 h + i] of key 16 h + 4 qd + i. kp:
-// its K groups in LDS. `all`: every row sees every key of it.
+// keys that a row does not see -inf: x[t][4 h + i] of key 16 h + 4 qd + i. kp, vp:
+// its K and V groups in LDS. `all`: every row sees every key of it.
 template <int HD, int RT, bool PACK, Math M>
-__device__ __forceinline__ void scores(const Rows<HD, RT, PACK, M>& R, const char* kp, int k0,
-                                       int ctx, int valid0, int valid1, bool all,
-                                       float (&x)[RT][Part<M != kBf16>::XN]) {
+__device__ __forceinline__ void scores(const Rows<HD, RT, PACK, M>& R, const char* kp,
+                                       const char* vp, int k0, int ctx, int valid0, int valid1,
+                                       bool all, float (&x)[RT][Part<M != kBf16>::XN]) {
     using T = Rows<HD, RT, PACK, M>;
     using L = Lay<HD, M == kF32>;
     constexpr int NH = Part<M != kBf16>::NH, XN = Part<M != kBf16>::XN;
@@ -516,6 +550,7 @@ __device__ __forceinline__ void scores(const Rows<HD, RT, PACK, M>& R, const cha
         }
     if (all) return;
     asm volatile("");  // (a branch, not selections that every part would compute)
+    clear_unseen<HD, M>(R.unseen, vp, k0, ctx);
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -979,7 +1014,7 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
             }
             const int va = gr[0][0].valid, vb = gr[0][NH - 1].valid;
             const bool all = s0 + P::KEYS <= it.sq.ctx && va == 16 && vb == 16;
-            scores<HD, 1, PACK, M>(R, at, s0, it.sq.ctx, va, vb, all, x);
+            scores<HD, 1, PACK, M>(R, at, at + NH * GRP, s0, it.sq.ctx, va, vb, all, x);
             move = raised != j && too_high(R, x);
             if (move) break;
             accumulate<HD, 1, PACK, M>(R, x, at + NH * GRP);
@@ -1184,7 +1219,7 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
                 }
             const bool all = s0 + P::KEYS <= free_end && va == 16 && vb == 16;
             const char* kp = lds + (F32 ? 0 : (j & 1) * 2 * S::POOL) + h * NH * GRP;
-            scores<HD, RT, false, M>(R, kp, s0, it.sq.ctx, va, vb, all, x);
+            scores<HD, RT, false, M>(R, kp, kp + S::POOL, s0, it.sq.ctx, va, vb, all, x);
             move = raised != i && too_high(R, x);
             if (move) break;
             accumulate<HD, RT, false, M>(R, x, kp + S::POOL);

@@ -86,3 +86,33 @@ def test_deltanet_vectors_whose_squares_leave_the_range(hip, rng, H, part):
     err = np.abs(got - state).max((0, 2, 3))
     assert (err <= 2 * DN_TOL * np.abs(state).max((0, 2, 3))).all()
     assert np.array_equal(ring, conv)
+
+
+# ---- attention: whatever lies in slots that nobody sees ----------------------------
+
+
+@pytest.mark.parametrize("hd,bf16", [(128, True), (128, False), (256, True), (256, False)])
+@pytest.mark.parametrize("n_q,n_kv,nodes,ctx", [
+    (1, 1, 7, 0), (2, 2, 9, 1500), (8, 1, 30, 77), (8, 2, 15, 1200), (4, 2, 64, 0), (4, 2, 64, 700)])
+@pytest.mark.parametrize("what", [np.nan, -np.inf])
+def test_attention_padding_leaves_no_trace(hip, rng, hd, bf16, n_q, n_kv, nodes, ctx, what):
+    """Padding nodes' slots are never written. The same bits come out whatever
+    they hold, so nothing is computed a second time on their account."""
+    say(f"attention padding of {what} hd={hd} bf16={bf16} {n_q}/{n_kv} nodes={nodes} ctx={ctx}")
+    n, at = [nodes, 1, nodes], [ctx, 5, ctx // 2]
+    parents = [random_tree(rng, nodes, padding=nodes // 4), [-1], random_tree(rng, nodes)]
+    parents[2][nodes // 2] = nodes  # no node, and those below it
+    rows = Rows(hip, n, at, parents)
+    pages = Pages(hip, rng, [a + c for a, c in zip(n, at)], n_kv, hd, 16, bf16)
+    unseen = [pages.at(b, c + i) for b, _, k, c, ls in rows.seqs() for i in range(k)
+              if ls[i] is None]
+    q = rng.standard_normal((rows.rows, n_q * hd)).astype(np.float32)
+    out = []
+    for x in (0.0, what):
+        for p, i in unseen:
+            pages.k[0, p, :, i] = pages.v[0, p, :, i] = x
+        pages.upload(hip)
+        got = run_attention(hip, rng, rows, pages, n_q, q=q)
+        check_attention(rows, pages, *got, n_q)
+        out.append(got[0])
+    assert np.array_equal(*out)
