@@ -464,9 +464,10 @@ __device__ __forceinline__ void clear_unseen(unsigned long long unseen, const ch
 
 // Scores of a part of the keys, from slot k0 on, relative to the references, of
 // keys that a row does not see -inf: x[t][4 h + i] of key 16 h + 4 qd + i. kp, vp:
-// its K and V groups in LDS. `all`: every row sees every key of it.
+// its K and V groups in LDS. `all`: every row sees every key of it. False: no row
+// sees any.
 template <int HD, int RT, bool PACK, Math M>
-__device__ __forceinline__ void scores(const Rows<HD, RT, PACK, M>& R, const char* kp,
+__device__ __forceinline__ bool scores(const Rows<HD, RT, PACK, M>& R, const char* kp,
                                        const char* vp, int k0, int ctx, int valid0, int valid1,
                                        bool all, float (&x)[RT][Part<M != kBf16>::XN]) {
     using T = Rows<HD, RT, PACK, M>;
@@ -548,9 +549,10 @@ __device__ __forceinline__ void scores(const Rows<HD, RT, PACK, M>& R, const cha
             x[t][j] = s[j / 4][t][j % 4];
             if constexpr (PACK && M == kBf16) x[t][j] = fold8(x[t][j]);
         }
-    if (all) return;
+    if (all) return true;
     asm volatile("");  // (a branch, not selections that every part would compute)
     clear_unseen<HD, M>(R.unseen, vp, k0, ctx);
+    bool any = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -560,7 +562,9 @@ __device__ __forceinline__ void scores(const Rows<HD, RT, PACK, M>& R, const cha
             if (row >= 0 && row < QLM_TREE_MAX) sees |= (R.line[t] >> row) & 1ull;
             sees &= in < (j < 4 ? valid0 : valid1);
             x[t][j] = sees ? x[t][j] : -INFINITY;
+            any |= sees;
         }
+    return __builtin_expect(__ballot(any) != 0, 1);
 }
 
 // Whether some score is too far above its row's reference.
@@ -769,34 +773,41 @@ __device__ void row_in_fp32(const PaArgs& a, int b, const SeqRows& sq, int i, in
     }
     bool any = false;
     const int end = line ? min(sq.ctx + (a.bt.parent ? seen_rows(a, sq) : i + 1), a.slots) : 0;
-    for (int s = 0; s < end; ++s) {
-        if (a.bt.parent && s >= sq.ctx && !(line >> (s - sq.ctx) & 1ull)) continue;
-        const int page = page_of(a.pg, b, s);
-        if (page < 0) continue;
-        any = true;
-        const size_t at = slot_at(a.pg, page, g, s) + lane;
-        float x = 0.0f, v[E];
+    const int size = a.pg.page_size;
+    // 64 pages' numbers at a time: those that are not there cost nothing else
+    for (int p0 = 0; p0 * (long long)size < end; p0 += QLM_WAVE) {
+        const int mine = page_of(a.pg, b, (p0 + lane) * size);
+        for (unsigned long long left = __ballot(mine >= 0); left; left &= left - 1) {
+            const int w = __ffsll((long long)left) - 1, s0 = (p0 + w) * size;
+            const int page = __builtin_amdgcn_readlane(mine, w);
+            for (int s = s0; s < min(s0 + size, end); ++s) {
+                if (a.bt.parent && s >= sq.ctx && !(line >> (s - sq.ctx) & 1ull)) continue;
+                any = true;
+                const size_t at = slot_at(a.pg, page, g, s) + lane;
+                float x = 0.0f, v[E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            float k;
-            if constexpr (sizeof(KV) == 4) {
-                k = reinterpret_cast<const float*>(a.pg.k)[at + 64 * j];
-                v[j] = reinterpret_cast<const float*>(a.pg.v)[at + 64 * j];
-            } else {
-                k = bf16_to_f32(reinterpret_cast<const uint16_t*>(a.pg.k)[at + 64 * j]);
-                v[j] = bf16_to_f32(reinterpret_cast<const uint16_t*>(a.pg.v)[at + 64 * j]);
+                for (int j = 0; j < E; ++j) {
+                    float k;
+                    if constexpr (sizeof(KV) == 4) {
+                        k = reinterpret_cast<const float*>(a.pg.k)[at + 64 * j];
+                        v[j] = reinterpret_cast<const float*>(a.pg.v)[at + 64 * j];
+                    } else {
+                        k = bf16_to_f32(reinterpret_cast<const uint16_t*>(a.pg.k)[at + 64 * j]);
+                        v[j] = bf16_to_f32(reinterpret_cast<const uint16_t*>(a.pg.v)[at + 64 * j]);
+                    }
+                    x = fmaf(q[j], k, x);
+                }
+                x = wave_sum(x);
+                const float top = fmaxf(m, x), ref = top == -INFINITY ? 0.0f : top;
+                const float f = exp2f(m - ref), p = exp2f(x - ref);
+                l = fmaf(l, f, p);
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    // a key of no weight leaves no trace of its value
+                    o[j] = p == 0.0f ? o[j] * f : fmaf(p, v[j], o[j] * f);
+                m = top;
             }
-            x = fmaf(q[j], k, x);
         }
-        x = wave_sum(x);
-        const float top = fmaxf(m, x), ref = top == -INFINITY ? 0.0f : top;
-        const float f = exp2f(m - ref), p = exp2f(x - ref);
-        l = fmaf(l, f, p);
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-            // a key of no weight leaves no trace of its value
-            o[j] = p == 0.0f ? o[j] * f : fmaf(p, v[j], o[j] * f);
-        m = top;
     }
 #pragma unroll
     for (int j = 0; j < E; ++j) o[j] = any ? o[j] / l : 0.0f;
@@ -1014,10 +1025,11 @@ __global__ __launch_bounds__((FewShape<HD, F32>::NW * QLM_WAVE)) void k_pa_few(P
             }
             const int va = gr[0][0].valid, vb = gr[0][NH - 1].valid;
             const bool all = s0 + P::KEYS <= it.sq.ctx && va == 16 && vb == 16;
-            scores<HD, 1, PACK, M>(R, at, at + NH * GRP, s0, it.sq.ctx, va, vb, all, x);
-            move = raised != j && too_high(R, x);
-            if (move) break;
-            accumulate<HD, 1, PACK, M>(R, x, at + NH * GRP);
+            if (scores<HD, 1, PACK, M>(R, at, at + NH * GRP, s0, it.sq.ctx, va, vb, all, x)) {
+                move = raised != j && too_high(R, x);
+                if (move) break;
+                accumulate<HD, 1, PACK, M>(R, x, at + NH * GRP);
+            }
             // the block is read: its place takes the next but one
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (j + 2 < mine) fetch(j + 2, gr[2]);
@@ -1219,10 +1231,11 @@ __global__ __launch_bounds__(512, 2) void k_pa_tile(PaArgs a) {
                 }
             const bool all = s0 + P::KEYS <= free_end && va == 16 && vb == 16;
             const char* kp = lds + (F32 ? 0 : (j & 1) * 2 * S::POOL) + h * NH * GRP;
-            scores<HD, RT, false, M>(R, kp, kp + S::POOL, s0, it.sq.ctx, va, vb, all, x);
-            move = raised != i && too_high(R, x);
-            if (move) break;
-            accumulate<HD, RT, false, M>(R, x, kp + S::POOL);
+            if (scores<HD, RT, false, M>(R, kp, kp + S::POOL, s0, it.sq.ctx, va, vb, all, x)) {
+                move = raised != i && too_high(R, x);
+                if (move) break;
+                accumulate<HD, RT, false, M>(R, x, kp + S::POOL);
+            }
         }
         if (!move) break;
         raise(R, x);

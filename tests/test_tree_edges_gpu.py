@@ -4,10 +4,12 @@ contexts that are cut and joined, and every form that a call can take. Against
 the definitions in 64 bits, or against the framework's row-by-row mixer where that
 is what the operators promise; tolerances are those of test_tree_ops_gpu.py."""
 
+import time
+
 import numpy as np
 import pytest
 
-from tests.test_tree_ops_gpu import (DN_TOL, buf, check_attention, check_tree, dn_inputs,
+from tests.test_tree_ops_gpu import (DN_TOL, FILL, buf, check_attention, check_tree, dn_inputs,
                                      run_attention, run_tree)
 from tests.tree_util import Pages, Rows, deltanet_ref, lines, random_tree
 from tests.util import say
@@ -116,3 +118,34 @@ def test_attention_padding_leaves_no_trace(hip, rng, hd, bf16, n_q, n_kv, nodes,
         check_attention(rows, pages, *got, n_q)
         out.append(got[0])
     assert np.array_equal(*out)
+
+
+@pytest.mark.parametrize("hd,bf16", [(128, True), (256, False)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_of_rows_without_a_page_is_no_slower(hip, rng, hd, bf16, n):
+    """Sequences that only fill a batch up, their tables without a page and their
+    lengths whatever they were: zeros, and sooner than if the pages were there."""
+    B, ctx = 16, 8000
+    say(f"attention without pages hd={hd} bf16={bf16} n={n}")
+    rows = Rows(hip, [n] * B, [ctx] * B)
+    pages = Pages(hip, rng, [ctx + n], 2, hd, 64, bf16)
+    pages.table = np.repeat(pages.table, B, 0)  # (one context for all)
+    pages.upload(hip)
+    q = buf(hip, rng.standard_normal((rows.rows, 4 * hd)).astype(np.float32))
+    out = buf(hip, np.full((rows.rows, 4 * hd), FILL, np.float32))
+    size = hip.lib().qlm_paged_attention_workspace_bytes(rows.rows, B, 4, 2, hd, pages.ld * 64)
+    work, took = hip.DeviceBuffer(size), []
+    for table in (pages.table, np.full_like(pages.table, -1)):
+        pages.dt.upload(table)
+        times = []
+        for _ in range(6):
+            hip.sync()
+            t = time.perf_counter()
+            hip.call("qlm_paged_attention", q, 4 * hd, rows.c, pages.c, None, 0, 0, out, 4 * hd, 4,
+                     work, size, None)
+            hip.sync()
+            times.append(time.perf_counter() - t)
+        took.append(min(times))
+    assert (out.to_numpy((rows.rows, 4 * hd), np.float32) == 0).all()
+    say(f"  {took[0] * 1e6:.0f} us, without pages {took[1] * 1e6:.0f}")
+    assert took[1] <= 1.5 * took[0]
