@@ -138,7 +138,8 @@ __device__ __forceinline__ bool find_item(const PaArgs& a, int want, Item& it) {
     longest = wave_max(longest);
     float share = cost / (float)a.target;
     if (MT <= 16 && longest * wave_sum(units) > 1.5f * cost) share *= kUneven;
-    int len = uni(min((int)fminf(share, (float)(1 << 29)) / 32 * 32 + 32, 1 << 29));
+    // (no context is longer than 2^30: what `target` has no room for stays uncut)
+    int len = uni(min((int)fminf(share, (float)(1 << 30)) / 32 * 32 + 32, 1 << 30));
     len = uni(max(len, longest <= (float)a.alone ? a.alone : a.least));
     int before = 0, rec = 0;
     for (int i = 0; i < B; i += QLM_WAVE) {
