@@ -149,3 +149,143 @@ def test_attention_of_rows_without_a_page_is_no_slower(hip, rng, hd, bf16, n):
     assert (out.to_numpy((rows.rows, 4 * hd), np.float32) == 0).all()
     say(f"  {took[0] * 1e6:.0f} us, without pages {took[1] * 1e6:.0f}")
     assert took[1] <= 1.5 * took[0]
+
+
+# ---- attention: scores that are next to nothing ------------------------------------
+
+
+@pytest.mark.parametrize("hd,bf16", [(128, True), (128, False), (256, True), (256, False)])
+@pytest.mark.parametrize("n,n_q", [(1, 1), (2, 8), (70, 1)])
+def test_attention_scores_that_round_to_minus_zero(hip, rng, hd, bf16, n, n_q):
+    """Blocks of keys whose scores are products below the subnormal numbers,
+    negative: they weigh exp(0), beside blocks that weigh otherwise."""
+    say(f"attention scores of -0 hd={hd} bf16={bf16} n={n} n_q={n_q}")
+    ctx = 300
+    rows = Rows(hip, [n], [ctx])
+    pages = Pages(hip, rng, [ctx + n], 1, hd, 16, bf16)
+    half = hd // 2
+    for s in range(ctx + n):
+        p, at = pages.at(0, s)
+        if s // 32 % 4 in (0, 3):
+            pages.k[0, p, 0, at, :half] = -2.0 ** -90
+            pages.k[0, p, 0, at, half:] = 0
+        else:
+            pages.k[0, p, 0, at, :half] = 0
+    pages.upload(hip)
+    q = np.abs(rng.standard_normal((n, n_q * hd))).astype(np.float32)
+    q.reshape(n, n_q, 2, half)[:, :, 0] *= 2.0 ** -80
+    check_attention(rows, pages, *run_attention(hip, rng, rows, pages, n_q, q=q), n_q)
+
+
+# ---- attention: contexts that are cut and joined -----------------------------------
+
+
+CUT = {
+    # one longer than the mean by far, one without rows or keys among them
+    "uneven": ([40, 1100, 5000, 2500, 0], [1, 1, 1, 1, 1]),
+    "even": ([2100, 2100, 2100], [1, 1, 1]),
+    "with rows of none": ([1300, 4000, 9, 3000], [1, 0, 1, 1]),
+    "one": ([9000], [1]),
+}
+
+
+@pytest.mark.parametrize("hd,bf16", [(128, True), (128, False), (256, True), (256, False)])
+@pytest.mark.parametrize("n_q,n_kv,rows_each", [(2, 2, 1), (4, 1, 2), (4, 1, 4), (16, 2, 2)])
+@pytest.mark.parametrize("what", CUT)
+def test_attention_cut_contexts(hip, rng, hd, bf16, n_q, n_kv, rows_each, what):
+    """Units of 8 and of 16 rows."""
+    say(f"attention cut {what} hd={hd} bf16={bf16} {n_q}/{n_kv} rows={rows_each}")
+    ctx, n = CUT[what]
+    n = [k * rows_each for k in n]
+    rows = Rows(hip, n, ctx, before=1, behind=1)
+    pages = Pages(hip, rng, [a + c for a, c in zip(n, ctx)], n_kv, hd, 64, bf16)
+    check_attention(rows, pages, *run_attention(hip, rng, rows, pages, n_q, gated=True), n_q)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("n_q,n_kv,ctx", [(16, 16, [5000, 300, 9000, 40]), (24, 24, [4000, 3900]),
+                                          (24, 12, [100, 7000, 2000]), (260, 260, [1500, 700])])
+def test_attention_cut_contexts_of_many_heads(hip, rng, bf16, n_q, n_kv, ctx):
+    """Few pieces a head: longer than the shortest that a context is cut into, and
+    as many as the batch's lengths ask for."""
+    say(f"attention cut {n_q}/{n_kv} bf16={bf16}")
+    rows = Rows(hip, [1] * len(ctx), ctx)
+    pages = Pages(hip, rng, [c + 1 for c in ctx], n_kv, 128, 128, bf16)
+    check_attention(rows, pages, *run_attention(hip, rng, rows, pages, n_q), n_q)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("n_q,rows_each", [(1, 1), (8, 2), (4, 20)])
+def test_attention_many_sequences_some_of_them_cut(hip, rng, bf16, n_q, rows_each):
+    """More sequences than a wave has lanes, whose records begin in the first
+    round over them and go on in the later ones."""
+    B = 150
+    say(f"attention many cut bf16={bf16} n_q={n_q} rows={rows_each}")
+    ctx = [int(x) for x in rng.integers(0, 90, B)]
+    for b, c in ((3, 1500), (60, 1100), (64, 2600), (65, 1300), (127, 1700), (128, 2000), (149, 1400)):
+        ctx[b] = c
+    n = [rows_each * int(x > 0.2) for x in rng.random(B)]
+    for b in (3, 64, 128, 149):
+        n[b] = rows_each
+    rows = Rows(hip, n, ctx, behind=1)
+    pages = Pages(hip, rng, [a + c for a, c in zip(n, ctx)], 1, 128, 32, bf16)
+    check_attention(rows, pages, *run_attention(hip, rng, rows, pages, n_q), n_q)
+
+
+@pytest.mark.parametrize("hd,bf16", [(128, True), (128, False), (256, True), (256, False)])
+@pytest.mark.parametrize("n_q,n_kv", [(2, 2), (4, 1), (8, 1)])
+def test_attention_prompts_and_single_tokens_together(hip, rng, hd, bf16, n_q, n_kv):
+    """Prompts of several tiles beside tokens whose contexts are cut."""
+    say(f"attention mixed hd={hd} bf16={bf16} {n_q}/{n_kv}")
+    n, ctx = [150, 1, 1, 0, 90, 1], [0, 3000, 1500, 40, 700, 130]
+    rows = Rows(hip, n, ctx, behind=1)
+    pages = Pages(hip, rng, [a + c for a, c in zip(n, ctx)], n_kv, hd, 128, bf16)
+    check_attention(rows, pages, *run_attention(hip, rng, rows, pages, n_q, gated=True), n_q)
+
+
+def test_attention_a_long_context(hip, rng):
+    say("attention ctx=40000")
+    rows = Rows(hip, [1, 3], [40000, 17])
+    pages = Pages(hip, rng, [40001, 20], 1, 128, 256, True)
+    check_attention(rows, pages, *run_attention(hip, rng, rows, pages, 4), 4)
+
+
+# ---- DeltaNet: every form ------------------------------------------------------------
+
+
+# (rows of a call, and so the nodes that a workgroup has room for; heads of all
+# its sequences, and so the columns of one)
+@pytest.mark.parametrize("H,B", [(2, 1), (20, 2), (80, 1), (70, 2)])
+@pytest.mark.parametrize("n", [14, 30, 50])
+@pytest.mark.parametrize("strong", [False, True])
+def test_deltanet_every_form(hip, rng, H, B, n, strong):
+    """Trees of 2 to n nodes, and their longest lines' commit."""
+    say(f"deltanet forms H={H} B={B} n={n} strong={strong}")
+    sizes = [n] if B == 1 else [n - n // 3, n // 3]
+    ctx = [int(x) for x in rng.integers(0, 9, B)]
+    parents = [random_tree(rng, k, reach=2) for k in sizes]
+    parents[0] = [-1] + [i - 1 if i < sizes[0] - 3 else int(rng.integers(0, i))
+                         for i in range(1, sizes[0])]
+    rows = Rows(hip, sizes, ctx, parents)
+    inp = dn_inputs(rng, rows, H, B, strong=strong)
+    check_tree(rows, inp, H, run_tree(hip, rows, inp, H))
+    path, paths = np.full((B, 64), -1, np.int32), []
+    for b in range(B):
+        paths.append(max(lines(parents[b], sizes[b]), key=len))
+        path[b, :len(paths[b])] = paths[b]
+    d = {k: buf(hip, v) for k, v in inp.items()}
+    hip.call("qlm_deltanet_tree_commit", d["proj"], inp["proj"].shape[1], rows.c, buf(hip, path),
+             64, buf(hip, np.array([len(p) for p in paths], np.int32)), d["conv"], d["conv_w"],
+             d["A_log"], d["dt"], d["state"], H, 128, None)
+    state = d["state"].to_numpy(inp["state"].shape, np.float32)
+    conv = d["conv"].to_numpy(inp["conv"].shape, np.float32)
+    for b in range(B):
+        # (the lines of the path's own rows: no other state is needed)
+        ref = deltanet_ref(rows, b, [p if p is not None and set(p) <= set(paths[b]) else None
+                                     for p in lines(parents[b], sizes[b])], inp["proj"],
+                           inp["conv"][b], inp["conv_w"], inp["A_log"], inp["dt"],
+                           inp["state"][b], H, rows.start[b], ctx[b])
+        S, _, line, _ = ref[paths[b][-1]]
+        assert np.abs(state[b] - S).max() <= DN_TOL * np.abs(S).max()
+        for j in range(3):
+            assert np.array_equal(conv[b, (ctx[b] + len(paths[b]) + j) % 3], line[j])
