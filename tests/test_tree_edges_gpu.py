@@ -90,6 +90,25 @@ def test_deltanet_vectors_whose_squares_leave_the_range(hip, rng, H, part):
     assert np.array_equal(ring, conv)
 
 
+@pytest.mark.parametrize("H,B", [(1, 2), (40, 2), (70, 2)])
+@pytest.mark.parametrize("nodes", [14, 40])
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+def test_deltanet_padding_leaves_no_trace(hip, rng, H, B, nodes, what):
+    """The same bits come out whatever a padding node's row of proj holds."""
+    say(f"deltanet padding of {what} H={H} nodes={nodes}")
+    parents = [random_tree(rng, nodes, padding=nodes // 4), random_tree(rng, nodes)]
+    parents[1][nodes // 2] = nodes  # no node, and those below it
+    rows = Rows(hip, [nodes] * B, [3, 7], parents)
+    inp = dn_inputs(rng, rows, H, B)
+    unseen = [f + i for _, f, n, _, ls in rows.seqs() for i in range(n) if ls[i] is None]
+    out = []
+    for x in (0.0, what):
+        inp["proj"][unseen] = x
+        out.append(run_tree(hip, rows, inp, H))
+        check_tree(rows, inp, H, out[-1])
+    assert np.array_equal(*out)
+
+
 # ---- attention: whatever lies in slots that nobody sees ----------------------------
 
 
