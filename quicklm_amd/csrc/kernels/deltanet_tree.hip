@@ -24,6 +24,7 @@
 // accepted paths' commit 17.
 
 #include "paged.hpp"
+#include "silu.hpp"
 
 namespace {
 

@@ -31,6 +31,7 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "silu.hpp"
 
 namespace {
 
