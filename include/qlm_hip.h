@@ -577,7 +577,7 @@ typedef struct qlm_row_batch {
  * table[b * ld_table + s / page_size]. Slots from ld_table * page_size on, and
  * those of a page number outside 0..n_pages-1, are not there: not written, and
  * seen by no row. What lies in slots that no row sees is never used, NaN
- * included. dtype 0 = fp32, 1 = bf16 (rounded to nearest even when written);
+ * included, and costs nothing. dtype 0 = fp32, 1 = bf16 (rounded to nearest even when written);
  * hd 128 or 256; k, v 16-byte aligned. */
 typedef struct qlm_kv_pages {
     void* k;
@@ -622,8 +622,12 @@ int qlm_paged_append(const float* qkv, int ldqkv, const float* q_norm, const flo
  * arithmetic throughout: products run on the bf16 matrix cores, queries,
  * probabilities and fp32 keys and values split exactly into three bf16 terms, or
  * on the fp32 ones; results that do not come out finite are computed again
- * without the keys that a row does not see. Single
- * tokens, trees, prompts and mixtures take the same call; a long context is
+ * without the keys that a row does not see, about half a microsecond a key: so
+ * are those of rows beside one whose values hold a NaN or an infinity.
+ * Single tokens, trees, prompts and mixtures take the same call (in units of 8, 16
+ * or 64 pairs of a row and a query head by B and rows alone: tokens beside a long
+ * prompt, or rows and sequences that are only room, are slower than calls of
+ * their own); a long context is
  * split over the GPU and joined, by lengths that are read on the device, so
  * the sums' order depends on the batch's lengths. work: device scratch of
  * qlm_paged_attention_workspace_bytes(rows, B, n_q, n_kv, hd, slots) bytes, slots
@@ -657,7 +661,8 @@ int qlm_tree_commit(const int* tokens, const int* picks, const qlm_row_batch* ba
  * convolution, recurrence and output as if its line's rows alone had followed
  * the sequence's state [B, H, d, d] and conv ring [B, 3, 3*H*d] (oldest tap row =
  * ctx_len[b] % 3), neither of which is changed. Rows past a sequence's first
- * QLM_TREE_MAX are outside, without a parent array too. proj, out as
+ * QLM_TREE_MAX are outside, without a parent array too (prompts go to
+ * qlm_deltanet_prefill_chunked, a sequence a call). proj, out as
  * qlm_deltanet_prefill's (out must not overlap proj), within 1e-4 of it
  * (reassociated fp32). d = 128. work:
  * device scratch of qlm_deltanet_tree_workspace_bytes(rows, H, d) bytes (0 for

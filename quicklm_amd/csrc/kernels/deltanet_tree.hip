@@ -20,8 +20,8 @@
 //
 // Bound by the phases that wait for each other, of which a workgroup a CU overlaps
 // none: 16 trees of up to 64 nodes, 16 heads, take 46 us, a quarter of that the
-// state's products; their 36 MB alone would take 8. One tree of 16 nodes 13 us, 16
-// accepted paths' commit 17.
+// state's products; their 36 MB alone would take 8. One tree of 16 nodes 14 us, 16
+// accepted paths' commit 16.
 
 #include "paged.hpp"
 #include "silu.hpp"
@@ -701,7 +701,10 @@ int launch_columns(const TreeArgs& a, hipStream_t st) {
 // LDS for 64 nodes leaves a CU one workgroup, for 16 it has room for four. No
 // sequence has more nodes than the call has rows; where that does not bound
 // them and 16 are likely to do (the accepted path of a tree; short trees on
-// average), sequences of up to 16 have a launch of their own.
+// average), sequences of up to 16 have a launch of their own. What that gives and
+// costs (16 heads, us with it and without): 16 trees of 16 18 and 20; of up to 36, 18
+// on average, 47 and 33, since the larger ones' workgroups then begin later; of up
+// to 64, 27 on average, which the rule leaves in one launch, 59 and 46.
 template <bool COMMIT>
 int launch_nodes(TreeArgs a, hipStream_t st) {
     if (a.bt.rows <= 16) return launch_columns<16, COMMIT>(a, st);

@@ -36,8 +36,8 @@ struct AppendArgs {
 // lane: query heads first, then keys, then values. Few rows: K = 1, a workgroup
 // for each few heads. Many: K = 3, all requested before the row's sequence is
 // looked up, which three heads then share (16 + 2 x 4 heads of 128 into a bf16
-// cache, K = 1 and 3: 340 rows 5.2 and 6.1 us, 600 7.2 and 7.0, 2048 15.8 and 12.2,
-// 46 MB at 3.7 TB/s).
+// cache, one axis, K = 1 and 3: 340 rows 5.2 and 6.1 us, 600 7.2 and 7.0, 2048 15.8
+// and 12.2, 46 MB at 3.7 TB/s; positions of three axes 12.8).
 template <int HD, typename KV, int K>
 __global__ __launch_bounds__(kAppendThreads) void k_paged_append(AppendArgs a) {
     constexpr int LPH = HD / 4, HPB = kAppendThreads / LPH;  // lanes a head, heads at once

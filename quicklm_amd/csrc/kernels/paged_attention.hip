@@ -38,11 +38,12 @@
 // more than one chunk leaves records [m, l, O] that k_pa_join merges; the others
 // write their outputs.
 //
-// Measured with 16 / 4 heads of 128, bf16: 64 single tokens after 256 to 8192 slots
-// 109 us, bound by HBM (5.1 TB/s); 2048 rows after 2048 148 us, bound by the matrix
-// cores (1050 TFLOP/s of bf16 products, half of their cycles in the key loop); 8 trees of 64
-// nodes after 4032 65 us, of which 13 are the start and the join; one token after
-// 600 11 us, latency.
+// Measured with 16 / 4 heads of 128, bf16, calls one after the other: 64 single
+// tokens after 256 to 8192 slots 107 us, HBM (5.2 TB/s; 5.1 when something else has
+// been read in between, 6.1 for 64 after 32768, 4.3 GB); 2048 rows after 2048 148 us,
+// matrix cores (1050 TFLOP/s of bf16 products, half of their cycles in the key
+// loop); 8 trees of 64 nodes after 4032 62, 74 with the keys out of HBM, of which 13
+// are the start and the join; one token after 600 11 us, latency.
 
 #include <algorithm>
 
@@ -112,7 +113,10 @@ __device__ __forceinline__ int wave_scan(int v) {
 // single tokens after 4096 slots 99 us (16 / 4 heads of 128, bf16), in twice as
 // many 104; one after 32768 26 and 36. Where the longest is well above the mean
 // one item a CU leaves most of them waiting for it: half as many items again, 64
-// after 256 to 8192 slots 108 us, 126 without, 120 with twice as many.
+// after 256 to 8192 slots 108 us, 121 without, 120 with twice as many; 16 after up to
+// 30000 110 and 135, 8 51 and 62 (128 after up to 4000, where the rounds of items
+// come out otherwise, 121 and 116). All equally long and cut like that: 64 after
+// 4096 104 for 99, one after 32768 33 for 26.
 constexpr float kUneven = 2.0f / 3.0f;
 
 // Item `want` of a kv head, counted over the sequences: the longest prompts'
@@ -449,7 +453,8 @@ __device__ __forceinline__ void clear_unseen(unsigned long long unseen, const ch
     constexpr int KEYS = Part<M != kBf16>::KEYS;
     const int r0 = k0 - ctx;  // the part's first slot as a new row
     if (unseen == 0 || r0 <= -KEYS || r0 >= QLM_TREE_MAX) return;
-    unsigned left = (unsigned)(r0 < 0 ? unseen << -r0 : unseen >> r0) & (0xffffffffu >> (32 - KEYS));
+    unsigned left = (unsigned)(r0 < 0 ? unseen << -r0 : unseen >> r0);
+    left &= 0xffffffffu >> (32 - KEYS);
     uint32_t at = lds_at(vp) + (threadIdx.x & (QLM_WAVE - 1)) * 4, zero = 0u;
     asm volatile("" : "+v"(at), "+v"(zero));  // (not held over the loop either)
     for (; left; left &= left - 1) {
@@ -752,7 +757,9 @@ __device__ __forceinline__ void accumulate(Rows<HD, RT, PACK, M>& R,
 
 // Head h of row i of a sequence in fp32, key after key, by a whole wave: for
 // results that did not come out finite. What a row does not see is not
-// touched here, so that only its own keys and values can make it NaN.
+// touched here, so that only its own keys and values can make it NaN. About half a
+// microsecond a key, a wave's rows in turn: one token after 4000 slots 2.7 ms, 8 trees
+// of 64 after 4032 5.8, a prompt of 2048 rows after 2048 42.
 template <int HD, typename KV>
 __device__ void row_in_fp32(const PaArgs& a, int b, const SeqRows& sq, int i, int h,
                             float (&o)[HD / QLM_WAVE]) {
@@ -1410,6 +1417,12 @@ PaPlan plan_of(int rows, int B, int G, int n_kv, int hd, long long slots) {
     p.target = std::max(1, 256 / n_kv);  // a CU holds one workgroup
     const long long units = ((long long)rows * G) / p.mt + B;
     const long long most = p.mt <= 16 ? p.target + p.target / 2 + 1 : p.target;  // items but those
+    // Cutting costs the join's launch. Single tokens, whole up to 1024 slots and up to
+    // 512: one after 1000 14.8 and 13.4 us, 16 15.5 and 14.9, but 64 26.0 and 29.3 (up
+    // to 256: 64 after 500 20.7 for 17.3; up to 2048: one after 2000 22.0 for 13.4).
+    // Pieces of 256 slots at least, 512 and 128: one after 1500 13.4, 15.0 and 13.1,
+    // after 16000 18.7, 17.1 and 19.4. Tiles have work enough in 128: 5 trees of 33 in
+    // fp32 35, with 256 44, with 512 65; the bf16 cases within 2 of each other.
     p.alone = p.mt <= 16 ? 1024 : 128;
     p.least = p.mt <= 16 ? 256 : 128;
     p.join = slots > p.alone;
@@ -1451,6 +1464,10 @@ int launch_attention(const PaArgs& a, const PaPlan& p, hipStream_t st) {
         hipLaunchKernelGGL((k_pa_tile<HD, F32>), grid, tile, 0, st, a);
     const int rc = qlm_launch_status();
     if (rc != QLM_OK || !p.join) return rc;
+    // The join: one token after 4000, 16 tasks of 16 records, 14.0 us with four waves a
+    // task, 16.8 with one; 4 trees of 64, 4096 tasks, 36.8 and 29.9 (2 of them, 2048,
+    // 23.4 and 20.9). Many tasks in 8192 waves: 2048 rows after 2048 148.6, a task a wave
+    // 151.3; 8192 tasks a wave each 62.8, four a wave 65.1.
     const int tasks = a.bt.rows * a.n_q;
     if (tasks <= 2048) {
         hipLaunchKernelGGL((k_pa_join<HD, KV, 4>), dim3(tasks), dim3(kJoinThreads), 0, st, a, p.mt,
