@@ -470,8 +470,8 @@ __device__ __forceinline__ void clear_unseen(unsigned long long unseen, const ch
 
 // Scores of a part of the keys, from slot k0 on, relative to the references, of
 // keys that a row does not see -inf: x[t][4 h + i] of key 16 h + 4 qd + i. kp, vp:
-// its K and V groups in LDS. `all`: every row sees every key of it. False: no row
-// sees any.
+// its K and V groups in LDS. `all`: every row sees every key of it. False: none of its
+// slots is there.
 template <int HD, int RT, bool PACK, Math M>
 __device__ __forceinline__ bool scores(const Rows<HD, RT, PACK, M>& R, const char* kp,
                                        const char* vp, int k0, int ctx, int valid0, int valid1,
@@ -557,8 +557,8 @@ __device__ __forceinline__ bool scores(const Rows<HD, RT, PACK, M>& R, const cha
         }
     if (all) return true;
     asm volatile("");  // (a branch, not selections that every part would compute)
+    if ((valid0 | valid1) == 0) return false;
     clear_unseen<HD, M>(R.unseen, vp, k0, ctx);
-    bool any = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -568,9 +568,8 @@ __device__ __forceinline__ bool scores(const Rows<HD, RT, PACK, M>& R, const cha
             if (row >= 0 && row < QLM_TREE_MAX) sees |= (R.line[t] >> row) & 1ull;
             sees &= in < (j < 4 ? valid0 : valid1);
             x[t][j] = sees ? x[t][j] : -INFINITY;
-            any |= sees;
         }
-    return __builtin_expect(__ballot(any) != 0, 1);
+    return true;
 }
 
 // Whether some score is too far above its row's reference.
